@@ -579,6 +579,103 @@ int terra_swin_weight_grad(const void* dy, const void* x, float* dw, int dtype, 
 int terra_swin_gelu_bwd(const void* dout, const void* h, void* dh, int dtype, int64_t rows,
                         int features, float* column_sums, void* stream);
 
+/* ---- regularised training: dropout, and the end of a half-block --------------
+ *
+ * The dropout mask of these entry points is drawn from a counter-based
+ * generator and never stored: Philox4x32-10 with the 64-bit seed as its key and
+ * the counter (column >> 3, row, 0, stream_id).  Its four words are eight 16-bit
+ * draws for the chunk's eight columns, low half first; an element is dropped (its
+ * value is 0) where its draw is below t = round(p * 65536), and the others are
+ * scaled by 65536 / (65536 - t).  So the mask depends on the seed, the stream and
+ * the element's row and column alone, a backward call with the same ones sees the
+ * same mask, and p is rounded to 2^-16.  `seed`: a 64-bit integer in device memory
+ * (8-byte aligned; may be NULL where t is 0), read when the kernel runs, so that a
+ * replayed graph takes the seed that is there then.  Calls that must not share a
+ * mask take other seeds or other stream ids.  0 <= p <= 1; rows < 2^31.
+ */
+
+/* y = dropout(x) for x [rows, columns] with row stride x_stride (elements), y
+ * packed; f32, bf16 or f16; y may be x itself (packed rows).  The backward is
+ * the same call on the output's gradient.  columns < 2^24. */
+int terra_swin_dropout(const void* x, void* y, int dtype, int64_t rows, int64_t columns, int64_t x_stride,
+                       double p, const void* seed, uint32_t stream_id, void* stream);
+
+/* a = dropout(GELU(h)) (erf form) for packed h [rows, columns], in fp32 and
+ * rounded once; a may be h itself.  Stands between fc1 and fc2 of the MLP
+ * (models/mlp.py:162-168). */
+int terra_swin_gelu_dropout(const void* h, void* a, int dtype, int64_t rows, int64_t columns,
+                            double p, const void* seed, uint32_t stream_id, void* stream);
+
+/* Its backward: dh = keep * da * (Phi(h) + h phi(h)), rounded once, and, where
+ * column_sums (fp32 [columns]) is not NULL, the sums of dh over the rows (fc1's
+ * bias gradient), written, not added, in an order that the sizes fix.  The sums
+ * need a workspace of terra_swin_gelu_dropout_workspace fp32 values (a negative
+ * result is a status).  dh may be da or h itself. */
+int terra_swin_gelu_dropout_workspace(int64_t rows, int64_t columns);
+int terra_swin_gelu_dropout_bwd(const void* da, const void* h, void* dh, int dtype, int64_t rows, int64_t columns,
+                                double p, const void* seed, uint32_t stream_id,
+                                float* column_sums, float* workspace, void* stream);
+
+/* Norms of terra_swin_residual_norm. */
+enum terra_norm {
+  TERRA_NORM_NONE = 0,
+  TERRA_NORM_LAYER = 1, /* (v - mean) * rsqrt(var + eps) * weight + bias   */
+  TERRA_NORM_RMS = 2    /* v * rsqrt(mean(v^2) + eps) * weight + bias      */
+};
+
+/* Description of the end of a half-block over `rows` token rows:
+ *   n = post_norm(h),  m = dropout(n),  y = residual_scale * x + gate * m,
+ *   z = next_norm(y)   (of the y that is not yet rounded)
+ * h: h_dtype, row stride h_stride; x: x_dtype, row stride x_stride (elements);
+ * y like x and z in h_dtype, packed.  x_dtype is h_dtype, or f32 for bf16 / f16
+ * h (the fp32 stream of an autocast run).  gate_rows: 0 (no gate), 1 (gate fp32
+ * [C]), or B (gate fp32 [B, C], a row for each rows / B consecutive rows).
+ * windows != 0: h holds the window tokens of `geom`, [B_, N, C] in the order of
+ * terra_swin_partition, rows is geom's B * H * W, and a row's branch is the
+ * window token that window_reverse and the inverse roll bring to it; rows that no
+ * emitted window holds have m = 0.  The dropout row is the row of x.
+ * channels <= 8192. */
+typedef struct terra_swin_residual_norm_desc {
+  int64_t rows;
+  int64_t h_stride, x_stride;
+  int64_t gate_rows;
+  double p;              /* dropout probability                  */
+  int32_t channels;
+  int32_t h_dtype, x_dtype;
+  int32_t post_norm, next_norm; /* enum terra_norm              */
+  float post_eps, next_eps;
+  float residual_scale;
+  uint32_t stream_id;
+  int32_t windows;
+  terra_swin_geom geom;
+} terra_swin_residual_norm_desc;
+
+/* Parameters fp32 [C], or NULL for weights of 1 and biases of 0; z may be NULL
+ * without a next norm.  Outputs overlap nothing.
+ * Stands where the reference reverses the windows and adds the residual
+ *           models/utils.py:41-45, models/transformer.py:246, 296-298
+ *           models/mlp.py:168-171
+ */
+int terra_swin_residual_norm(const void* h, const void* x, void* y, void* z,
+                             const terra_swin_residual_norm_desc* desc,
+                             const float* post_weight, const float* post_bias, const float* gate,
+                             const float* next_weight, const float* next_bias,
+                             const void* seed, void* stream);
+
+/* Its backward, from the packed gradients of y and z (either may be NULL: zero):
+ * dh and dx (packed; dh in h's order, its rows that no row of x reads are left as
+ * they were), and the parameters' gradients, fp32, written, not added, each of
+ * which may be NULL; the sums over rows are taken in an order that the sizes fix.
+ * workspace: terra_swin_residual_norm_workspace fp32 values (a negative result
+ * is a status), needed where a parameter's gradient is asked for. */
+int terra_swin_residual_norm_workspace(const terra_swin_residual_norm_desc* desc);
+int terra_swin_residual_norm_bwd(const void* h, const void* x, const void* dy, const void* dz, void* dh, void* dx,
+                                 const terra_swin_residual_norm_desc* desc,
+                                 const float* post_weight, const float* post_bias, const float* gate,
+                                 const float* next_weight, const void* seed,
+                                 float* dpost_weight, float* dpost_bias, float* dgate,
+                                 float* dnext_weight, float* dnext_bias, float* workspace, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -71,6 +71,13 @@ EXPORTED_SYMBOLS = (
     "terra_swin_block_f32_train",
     "terra_swin_linear_short",
     "terra_swin_weight_grad_slices",
+    "terra_swin_dropout",
+    "terra_swin_gelu_dropout",
+    "terra_swin_gelu_dropout_workspace",
+    "terra_swin_gelu_dropout_bwd",
+    "terra_swin_residual_norm",
+    "terra_swin_residual_norm_workspace",
+    "terra_swin_residual_norm_bwd",
 )
 
 
@@ -163,6 +170,34 @@ class SwinMlpDesc(ctypes.Structure):
         ("hidden", ctypes.c_int32),
         ("layernorm", ctypes.c_int32),
         ("ln_eps", ctypes.c_float),
+    ]
+
+
+NORM_NONE = 0
+NORM_LAYER = 1
+NORM_RMS = 2
+
+
+class ResidualNormDesc(ctypes.Structure):
+    """Mirror of ``terra_swin_residual_norm_desc``."""
+
+    _fields_ = [
+        ("rows", ctypes.c_int64),
+        ("h_stride", ctypes.c_int64),
+        ("x_stride", ctypes.c_int64),
+        ("gate_rows", ctypes.c_int64),
+        ("p", ctypes.c_double),
+        ("channels", ctypes.c_int32),
+        ("h_dtype", ctypes.c_int32),
+        ("x_dtype", ctypes.c_int32),
+        ("post_norm", ctypes.c_int32),
+        ("next_norm", ctypes.c_int32),
+        ("post_eps", ctypes.c_float),
+        ("next_eps", ctypes.c_float),
+        ("residual_scale", ctypes.c_float),
+        ("stream_id", ctypes.c_uint32),
+        ("windows", ctypes.c_int32),
+        ("geom", SwinGeom),
     ]
 
 
@@ -268,6 +303,21 @@ def load() -> ctypes.CDLL:
                                                 ctypes.c_int, vp]
         lib.terra_swin_weight_grad.restype = ctypes.c_int
         lib.terra_swin_weight_grad.argtypes = [vp, vp, vp, ctypes.c_int, i64, ctypes.c_int, ctypes.c_int, vp, vp]
+        f64, u32 = ctypes.c_double, ctypes.c_uint32
+        lib.terra_swin_dropout.restype = ctypes.c_int
+        lib.terra_swin_dropout.argtypes = [vp, vp, ctypes.c_int, i64, i64, i64, f64, vp, u32, vp]
+        lib.terra_swin_gelu_dropout.restype = ctypes.c_int
+        lib.terra_swin_gelu_dropout.argtypes = [vp, vp, ctypes.c_int, i64, i64, f64, vp, u32, vp]
+        lib.terra_swin_gelu_dropout_workspace.restype = ctypes.c_int
+        lib.terra_swin_gelu_dropout_workspace.argtypes = [i64, i64]
+        lib.terra_swin_gelu_dropout_bwd.restype = ctypes.c_int
+        lib.terra_swin_gelu_dropout_bwd.argtypes = [vp, vp, vp, ctypes.c_int, i64, i64, f64, vp, u32, vp, vp, vp]
+        lib.terra_swin_residual_norm.restype = ctypes.c_int
+        lib.terra_swin_residual_norm.argtypes = [vp] * 4 + [ctypes.POINTER(ResidualNormDesc)] + [vp] * 7
+        lib.terra_swin_residual_norm_workspace.restype = ctypes.c_int
+        lib.terra_swin_residual_norm_workspace.argtypes = [ctypes.POINTER(ResidualNormDesc)]
+        lib.terra_swin_residual_norm_bwd.restype = ctypes.c_int
+        lib.terra_swin_residual_norm_bwd.argtypes = [vp] * 6 + [ctypes.POINTER(ResidualNormDesc)] + [vp] * 12
         version = lib.terra_abi_version()
         if version != ABI_VERSION:
             raise RuntimeError(f"terra_amd: {LIB_PATH} has ABI version {version}, expected {ABI_VERSION}; rebuild it")

@@ -21,9 +21,10 @@ from __future__ import annotations
 from typing import Optional, Tuple, Union
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from . import kernels
-from .kernels import ShiftMask, WindowGeometry, WindowMask
+from .kernels import Norm, ShiftMask, WindowGeometry, WindowMask
 
 MaskArg = Union[None, torch.Tensor, ShiftMask, WindowMask]
 
@@ -646,3 +647,109 @@ def attention_half(x: torch.Tensor, geom: WindowGeometry, norm: torch.nn.LayerNo
     q, k, v, proj = attn.q_linear, attn.k_linear, attn.v_linear, attn.proj
     return _AttentionHalf.apply(x, norm.weight, norm.bias, q.weight, k.weight, v.weight, q.bias, k.bias, v.bias,
                                 proj.weight, proj.bias, attn._table(), geom, norm.eps, attn.num_heads, attn.scale, mask, fused)
+
+
+class _Dropout(torch.autograd.Function):
+    """kernels.dropout; the backward draws the mask again from the seed."""
+
+    @staticmethod
+    def forward(ctx, x, p, seed, stream):
+        ctx.p, ctx.stream = p, stream
+        ctx.save_for_backward(seed)
+        return kernels.dropout(x, p, seed, stream)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        return kernels.dropout(dy.contiguous(), ctx.p, ctx.saved_tensors[0], ctx.stream), None, None, None
+
+
+def _seed(x: torch.Tensor, p: float, seed: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
+    return kernels.dropout_seed(x.device) if seed is None and p > 0 else seed
+
+
+def dropout(x: torch.Tensor, p: float, seed: Optional[torch.Tensor] = None, stream: int = 0) -> torch.Tensor:
+    """:func:`kernels.dropout` with a gradient.  ``seed`` None draws one from
+    torch's generator on x's device."""
+    seed = _seed(x, p, seed)
+    if _needs_grad(x):
+        return _Dropout.apply(x, p, seed, stream)
+    return kernels.dropout(x, p, seed, stream)
+
+
+class _GeluDropout(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, h, p, seed, stream, bias_sums):
+        ctx.p, ctx.stream, ctx.bias_sums = p, stream, bias_sums
+        ctx.save_for_backward(h, seed)
+        return kernels.gelu_dropout(h, p, seed, stream)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, da):
+        h, seed = ctx.saved_tensors
+        dh = kernels.gelu_dropout_backward(da.contiguous(), h, ctx.p, seed, ctx.stream,
+                                           column_sums=ctx.bias_sums is not None)
+        if ctx.bias_sums is not None:
+            dh, ctx.bias_sums.sums = dh
+        return dh, None, None, None, None
+
+
+def gelu_dropout(h: torch.Tensor, p: float, seed: Optional[torch.Tensor] = None, stream: int = 0,
+                 bias_sums: Optional[ColumnSumLink] = None) -> torch.Tensor:
+    """:func:`kernels.gelu_dropout` with a gradient.  ``seed`` None draws one
+    from torch's generator.  ``bias_sums``: the :class:`ColumnSumLink` of the
+    :func:`linear` that produced ``h``, whose bias gradient the backward sums."""
+    seed, h = _seed(h, p, seed), h.contiguous()
+    if _needs_grad(h):
+        return _GeluDropout.apply(h, p, seed, stream, bias_sums)
+    return kernels.gelu_dropout(h, p, seed, stream)
+
+
+class _ResidualNorm(torch.autograd.Function):
+    """kernels.residual_norm; the backward keeps h, x and the parameters and
+    recomputes the norms and the mask."""
+
+    @staticmethod
+    def forward(ctx, h, x, post_w, post_b, gate, next_w, next_b, post, nxt, geom, residual_scale, p, seed, stream):
+        ctx.cfg = (post, nxt, geom, residual_scale, p, stream)
+        ctx.save_for_backward(h, x, post_w, post_b, gate, next_w, next_b, seed)
+        ctx.set_materialize_grads(False)
+        return kernels.residual_norm(h, x, _norm(post, post_w, post_b), gate, _norm(nxt, next_w, next_b), geom,
+                                     residual_scale, p, seed, stream)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy, dz=None):
+        h, x, post_w, post_b, gate, next_w, next_b, seed = ctx.saved_tensors
+        post, nxt, geom, residual_scale, p, stream = ctx.cfg
+        packed = lambda g: None if g is None else g.contiguous()  # noqa: E731
+        g = kernels.residual_norm_backward(h, x, packed(dy), packed(dz), _norm(post, post_w, post_b), gate,
+                                           _norm(nxt, next_w, next_b), geom, residual_scale, p, seed, stream,
+                                           needs=ctx.needs_input_grad[2:7])
+        cast = lambda t, q: None if t is None else t.to(q.dtype)  # noqa: E731
+        return (g.dh, g.dx, *(cast(t, q) for t, q in zip(g[2:], (post_w, post_b, gate, next_w, next_b))),
+                *(None,) * 7)
+
+
+def _norm(kind: Optional[Tuple[float, bool]], weight, bias) -> Optional[Norm]:
+    return None if kind is None else Norm(weight, bias, *kind)
+
+
+def residual_norm(h: torch.Tensor, x: torch.Tensor, post_norm: Optional[Norm] = None,
+                  gate: Optional[torch.Tensor] = None, next_norm: Optional[Norm] = None,
+                  geom: Optional[WindowGeometry] = None, residual_scale: float = 1.0, p: float = 0.0,
+                  seed: Optional[torch.Tensor] = None, stream: int = 0):
+    """:func:`kernels.residual_norm` with gradients for h, x, the gate and the
+    norms' parameters.  ``seed`` None draws one from torch's generator.  An x of
+    a type that the kernel does not take beside h's is promoted first, as
+    ``x + h`` would be."""
+    seed = _seed(h, p, seed)
+    if x.dtype != h.dtype and x.dtype != torch.float32:
+        x = x.to(torch.promote_types(x.dtype, h.dtype))
+    params = [None if n is None else getattr(n, name) for n in (post_norm, next_norm) for name in ("weight", "bias")]
+    if _needs_grad(h, x, gate, *params):
+        kinds = [None if n is None else (n.eps, n.rms) for n in (post_norm, next_norm)]
+        return _ResidualNorm.apply(h, x, params[0], params[1], gate, params[2], params[3], *kinds, geom, residual_scale, p,
+                                   seed, stream)
+    return kernels.residual_norm(h, x, post_norm, gate, next_norm, geom, residual_scale, p, seed, stream)

@@ -1,0 +1,350 @@
+// Forward of the end of a half-block (residual_norm.h): the branch's
+// post-norm, dropout, gate, scaled residual and the next half-block's norm in
+// one pass.  Bound by memory: h and x read once, y and z written once.
+#include "residual_norm.h"
+
+namespace terra {
+namespace {
+
+template <int DTH, int DTX, int kG, int kK, bool kVec>
+__global__ __launch_bounds__(tail_threads(kG)) void tail_kernel(const TailArgs a) {
+  constexpr int kGroups = tail_threads(kG) / kG;
+  constexpr int kHB = ChunkElt<DTH>::kBytes, kXB = ChunkElt<DTX>::kBytes;
+  __shared__ typename RowSum<kG>::Shared s_red;
+  const int lane = threadIdx.x % kG, group = threadIdx.x / kG, C = a.C;
+  RowSum<kG> sum(&s_red);
+  // A lane's columns never change: their parameters stay in registers.
+  float pw[kK][kChunkCols], pb[kK][kChunkCols], gate[kK][kChunkCols], nw[kK][kChunkCols], nb[kK][kChunkCols];
+#pragma unroll
+  for (int k = 0; k < kK; ++k) {
+    const int col = (lane + kG * k) * kChunkCols;
+    load_params<kVec>(a.pw, 1.f, col, C, pw[k]);
+    load_params<kVec>(a.pb, 0.f, col, C, pb[k]);
+    load_params<kVec>(a.gate_rows == 1 ? a.gate : nullptr, 1.f, col, C, gate[k]);
+    load_params<kVec>(a.nw, 1.f, col, C, nw[k]);
+    load_params<kVec>(a.nb, 0.f, col, C, nb[k]);
+  }
+  const uint64_t seed = a.drop.threshold > 0 ? *a.drop.seed : 0;
+  for (uint32_t base = blockIdx.x * kGroups; base < a.rows; base += gridDim.x * kGroups) {
+    const uint32_t row = base + group;
+    const bool live = row < a.rows;
+    const uint32_t r = live ? row : a.rows - 1;  // a row past the end re-reads the last one
+    const int64_t src = a.windows ? a.map.source(r) : (int64_t)r;
+    const bool has = src >= 0;
+    const uint8_t* hp = a.h + (has ? src : 0) * a.h_row_bytes;
+    const uint8_t* xp = a.x + (int64_t)r * a.x_row_bytes;
+    RowChunk<DTH> hq[kK];
+    RowChunk<DTX> xq[kK];
+#pragma unroll
+    for (int k = 0; k < kK; ++k) {
+      const int col = (lane + kG * k) * kChunkCols;
+      hq[k] = load_chunk<DTH, kVec>(hp, col, C, col < C);
+      xq[k] = load_chunk<DTX, kVec>(xp, col, C, col < C);
+      if (a.gate_rows > 1) load_params<kVec>(a.gate + (int64_t)(r / a.per_sample) * C, 1.f, col, C, gate[k]);
+    }
+    float v[kK][kChunkCols];
+#pragma unroll
+    for (int k = 0; k < kK; ++k) {
+      const int col = (lane + kG * k) * kChunkCols;
+      unpack<DTH, kVec>(hq[k], v[k], col, C, has && col < C);
+    }
+    if (a.post != TERRA_NORM_NONE) normalise<kG, kK, kVec>(v, a.post, a.post_eps, a.inv_c, lane, C, sum);
+    const uint32_t live_rows = min(a.rows - base, (uint32_t)kGroups);
+    const __amdgpu_buffer_rsrc_t y_out = buffer_rsrc(a.y + (int64_t)base * C * kXB, live_rows * (uint32_t)(C * kXB));
+#pragma unroll
+    for (int k = 0; k < kK; ++k) {
+      const int col = (lane + kG * k) * kChunkCols;
+      float xv[kChunkCols];
+      unpack<DTX, kVec>(xq[k], xv, col, C, col < C);
+#pragma unroll
+      for (int j = 0; j < kChunkCols; ++j) v[k][j] = has ? fmaf(v[k][j], pw[k][j], pb[k][j]) : 0.f;
+      if (a.drop.threshold > 0) {
+        const ChunkDraws d = chunk_draws(seed, (uint32_t)(lane + kG * k), r, a.drop.stream);
+#pragma unroll
+        for (int j = 0; j < kChunkCols; ++j) v[k][j] = kept(d, j, a.drop.threshold) ? v[k][j] * a.drop.scale : 0.f;
+      }
+#pragma unroll
+      for (int j = 0; j < kChunkCols; ++j) v[k][j] = fmaf(a.alpha, xv[j], gate[k][j] * v[k][j]);
+      if (live && col < C) store_chunk<DTX, kVec>(v[k], y_out, (uint32_t)(group * C + col) * kXB, col, C);
+    }
+    if (a.next != TERRA_NORM_NONE) {
+      normalise<kG, kK, kVec>(v, a.next, a.next_eps, a.inv_c, lane, C, sum);
+      const __amdgpu_buffer_rsrc_t z_out = buffer_rsrc(a.z + (int64_t)base * C * kHB, live_rows * (uint32_t)(C * kHB));
+#pragma unroll
+      for (int k = 0; k < kK; ++k) {
+        const int col = (lane + kG * k) * kChunkCols;
+#pragma unroll
+        for (int j = 0; j < kChunkCols; ++j) v[k][j] = fmaf(v[k][j], nw[k][j], nb[k][j]);
+        if (live && col < C) store_chunk<DTH, kVec>(v[k], z_out, (uint32_t)(group * C + col) * kHB, col, C);
+      }
+    }
+  }
+}
+
+template <int DTH, int DTX, int kG, int kK>
+void launch(const TailArgs& a, bool vec, hipStream_t s) {
+  constexpr uint32_t kGroups = tail_threads(kG) / kG;
+  // Workgroups stay for several rows each, so that the parameters' loads are paid once.
+  const uint32_t need = (a.rows + kGroups - 1) / kGroups, most = 2048;
+  const uint32_t blocks = need < most ? need : most;
+  if (vec) tail_kernel<DTH, DTX, kG, kK, true><<<blocks, tail_threads(kG), 0, s>>>(a);
+  else tail_kernel<DTH, DTX, kG, kK, false><<<blocks, tail_threads(kG), 0, s>>>(a);
+}
+
+template <int DTH, int DTX>
+void dispatch(const TailArgs& a, bool vec, hipStream_t s) {
+  const TailShape t = tail_shape(a.C);
+  switch (t.lanes * 10 + t.chunks) {
+    case 161: return launch<DTH, DTX, 16, 1>(a, vec, s);
+    case 321: return launch<DTH, DTX, 32, 1>(a, vec, s);
+    case 641: return launch<DTH, DTX, 64, 1>(a, vec, s);
+    case 642: return launch<DTH, DTX, 64, 2>(a, vec, s);
+    case 2561: return launch<DTH, DTX, 256, 1>(a, vec, s);
+    case 2562: return launch<DTH, DTX, 256, 2>(a, vec, s);
+    default: return launch<DTH, DTX, 512, 2>(a, vec, s);
+  }
+}
+
+// A tensor of the call: how far it reaches, for the overlap checks.
+struct Span {
+  const void* p;
+  int64_t bytes;
+  const char* name;
+};
+
+int check_spans(std::initializer_list<Span> in, std::initializer_list<Span> out) {
+  for (const Span* o = out.begin(); o != out.end(); ++o) {
+    if (o->p == nullptr) continue;
+    auto meets = [&](const Span& s) {
+      const uintptr_t a = (uintptr_t)o->p, b = (uintptr_t)s.p;
+      return s.p != nullptr && s.bytes > 0 && o->bytes > 0 && a < b + (uintptr_t)s.bytes && b < a + (uintptr_t)o->bytes;
+    };
+    for (const Span& s : in)
+      if (meets(s)) return fail(TERRA_ERR_SHAPE, "%s must not overlap %s", o->name, s.name);
+    for (const Span* q = out.begin(); q != o; ++q)
+      if (meets(*q)) return fail(TERRA_ERR_SHAPE, "%s must not overlap %s", o->name, q->name);
+  }
+  return TERRA_OK;
+}
+
+// Checks the descriptor; fills the sizes of `a`.  h_rows: rows of h.
+int prepare(const terra_swin_residual_norm_desc* d, TailArgs* a, bool* vec, int64_t* h_rows) {
+  if (d == nullptr) return fail(TERRA_ERR_NULL, "desc is NULL");
+  const int h = d->h_dtype, x = d->x_dtype;
+  const bool half = h == TERRA_DTYPE_BF16 || h == TERRA_DTYPE_F16;
+  if (!((half && (x == h || x == TERRA_DTYPE_F32)) || (h == TERRA_DTYPE_F32 && x == TERRA_DTYPE_F32)))
+    return fail(TERRA_ERR_DTYPE, "h is bf16, f16 or f32 and x of h's dtype or f32 (got %d and %d)", h, x);
+  if (d->rows < 0 || d->channels <= 0) return fail(TERRA_ERR_SHAPE, "rows must be >= 0 and channels > 0");
+  if (d->channels > kTailMaxChannels)
+    return fail(TERRA_ERR_UNSUPPORTED, "rows of up to %d channels (got %d)", kTailMaxChannels, d->channels);
+  if (d->rows >= (1ll << 31)) return fail(TERRA_ERR_SHAPE, "%lld rows: at most 2^31 - 1", (long long)d->rows);
+  for (int kind : {d->post_norm, d->next_norm})
+    if (kind != TERRA_NORM_NONE && kind != TERRA_NORM_LAYER && kind != TERRA_NORM_RMS)
+      return fail(TERRA_ERR_SHAPE, "unknown norm %d", kind);
+  if (d->gate_rows < 0 || d->gate_rows >= (1ll << 31) || (d->gate_rows > 1 && d->rows % d->gate_rows != 0))
+    return fail(TERRA_ERR_SHAPE, "%lld rows are not a whole number for each of %lld gate rows", (long long)d->rows,
+                (long long)d->gate_rows);
+  if (d->h_stride < d->channels || d->x_stride < d->channels)
+    return fail(TERRA_ERR_SHAPE, "a row stride is below the %d channels", d->channels);
+  a->rows = (uint32_t)d->rows;
+  a->C = d->channels;
+  a->post = d->post_norm;
+  a->next = d->next_norm;
+  a->post_eps = d->post_eps;
+  a->next_eps = d->next_eps;
+  a->alpha = d->residual_scale;
+  a->inv_c = 1.f / (float)d->channels;
+  // As many gate rows as rows are one each, whatever their number; the count fits 32 bits as the rows do.
+  a->gate_rows = d->rows > 0 ? (int32_t)d->gate_rows : 0;
+  a->per_sample = a->gate_rows > 1 ? (uint32_t)(d->rows / d->gate_rows) : a->rows;
+  a->h_row_bytes = d->h_stride * dtype_size(h);
+  a->x_row_bytes = d->x_stride * dtype_size(x);
+  *vec = d->channels % kChunkCols == 0 && a->h_row_bytes % 16 == 0 && a->x_row_bytes % 16 == 0;
+  *h_rows = d->rows;
+  a->windows = d->windows;
+  if (d->windows && d->rows > 0) {
+    const terra_swin_geom& q = d->geom;
+    GeomDims dims;
+    const int st = validate_geom(&q, &dims);
+    if (st != TERRA_OK) return st;
+    if (q.channels != d->channels || (int64_t)q.batch * q.height * q.width != d->rows)
+      return fail(TERRA_ERR_SHAPE, "the geometry's grid is not the %lld rows of %d channels", (long long)d->rows, d->channels);
+    *h_rows = (int64_t)q.batch * dims.nWe * q.window * q.window;
+    if (dims.Hp >= (1ll << 31) || dims.Wp >= (1ll << 31) || dims.nWe >= (1ll << 31))
+      return fail(TERRA_ERR_SHAPE, "the window frame is too large");
+    WindowMap& m = a->map;
+    m.Hp = (int32_t)dims.Hp;
+    m.Wp = (int32_t)dims.Wp;
+    m.shift_h = q.shift_h;
+    m.shift_w = q.shift_w;
+    m.pad_top = q.pad_top;
+    m.pad_left = q.pad_left;
+    m.row_begin = q.win_row_begin;
+    m.rows = (int32_t)dims.rows;
+    m.cols = (int32_t)dims.nWw;
+    m.ws = q.window;
+    m.valid_begin = q.valid_begin;
+    m.valid_end = q.valid_end > 0 ? q.valid_end : 0;
+    m.fd_W = FastDiv((uint32_t)q.width);
+    m.fd_H = FastDiv((uint32_t)q.height);
+    m.fd_ws = FastDiv((uint32_t)q.window);
+  }
+  return TERRA_OK;
+}
+
+// Alignment of a tensor's or a parameter's pointer; NULL where it may be left out.
+int check_pointer(const void* p, int elt, const char* name, bool needed, bool* vec) {
+  if (p == nullptr) return needed ? fail(TERRA_ERR_NULL, "%s is NULL", name) : TERRA_OK;
+  if ((uintptr_t)p % (uintptr_t)elt != 0) return fail(TERRA_ERR_ALIGN, "%s is not aligned to its elements", name);
+  if ((uintptr_t)p % 16 != 0) *vec = false;
+  return TERRA_OK;
+}
+
+int64_t span_bytes(int64_t rows, int64_t row_bytes, int64_t packed) { return rows > 0 ? (rows - 1) * row_bytes + packed : 0; }
+
+int launched(const char* what) {
+  const hipError_t e = hipGetLastError();
+  return e == hipSuccess ? TERRA_OK : fail(TERRA_ERR_LAUNCH, "%s launch failed: %s", what, hipGetErrorString(e));
+}
+
+}  // namespace
+}  // namespace terra
+
+using namespace terra;
+
+#define TERRA_TRY(call)                    \
+  do {                                     \
+    const int st_ = (call);                \
+    if (st_ != TERRA_OK) return st_;       \
+  } while (0)
+
+extern "C" int terra_swin_residual_norm(const void* h, const void* x, void* y, void* z,
+                                        const terra_swin_residual_norm_desc* desc,
+                                        const float* post_weight, const float* post_bias, const float* gate,
+                                        const float* next_weight, const float* next_bias,
+                                        const void* seed, void* stream) {
+  clear_error();
+  TailArgs a = {};
+  bool vec = false;
+  int64_t h_rows = 0;
+  TERRA_TRY(prepare(desc, &a, &vec, &h_rows));
+  TERRA_TRY(dropout_args(desc->p, seed, desc->stream_id, &a.drop));
+  if (a.rows == 0) return TERRA_OK;
+  const int he = dtype_size(desc->h_dtype), xe = dtype_size(desc->x_dtype);
+  TERRA_TRY(check_pointer(h, he, "h", true, &vec));
+  TERRA_TRY(check_pointer(x, xe, "x", true, &vec));
+  TERRA_TRY(check_pointer(y, xe, "y", true, &vec));
+  TERRA_TRY(check_pointer(z, he, "z", a.next != TERRA_NORM_NONE, &vec));
+  TERRA_TRY(check_pointer(gate, 4, "gate", a.gate_rows > 0, &vec));
+  for (const float* p : {post_weight, post_bias, next_weight, next_bias})
+    TERRA_TRY(check_pointer(p, 4, "a norm's parameter", false, &vec));
+  const int64_t C = a.C;
+  if (a.next == TERRA_NORM_NONE) z = nullptr;
+  TERRA_TRY(check_spans({{h, span_bytes(h_rows, a.h_row_bytes, C * he), "h"}, {x, span_bytes(a.rows, a.x_row_bytes, C * xe), "x"}},
+                        {{y, a.rows * C * xe, "y"}, {z, a.rows * C * he, "z"}}));
+  a.h = (const uint8_t*)h;
+  a.x = (const uint8_t*)x;
+  a.y = (uint8_t*)y;
+  a.z = (uint8_t*)z;
+  if (a.post != TERRA_NORM_NONE) a.pw = post_weight, a.pb = post_bias;
+  if (a.next != TERRA_NORM_NONE) a.nw = next_weight, a.nb = next_bias;
+  a.gate = gate;
+  hipStream_t s = (hipStream_t)stream;
+  const int hd = desc->h_dtype, xd = desc->x_dtype;
+  if (hd == TERRA_DTYPE_F32) dispatch<TERRA_DTYPE_F32, TERRA_DTYPE_F32>(a, vec, s);
+  else if (hd == TERRA_DTYPE_BF16 && xd == TERRA_DTYPE_BF16) dispatch<TERRA_DTYPE_BF16, TERRA_DTYPE_BF16>(a, vec, s);
+  else if (hd == TERRA_DTYPE_BF16) dispatch<TERRA_DTYPE_BF16, TERRA_DTYPE_F32>(a, vec, s);
+  else if (xd == TERRA_DTYPE_F16) dispatch<TERRA_DTYPE_F16, TERRA_DTYPE_F16>(a, vec, s);
+  else dispatch<TERRA_DTYPE_F16, TERRA_DTYPE_F32>(a, vec, s);
+  return launched("terra_swin_residual_norm");
+}
+
+// fp32 values: the workgroups' sums of four vectors, then the gate's units
+// where a sample has several.  At most 1024 workgroups and twice as many units,
+// fewer where rows are wide: the count fits an int.
+extern "C" int terra_swin_residual_norm_workspace(const terra_swin_residual_norm_desc* desc) {
+  clear_error();
+  TailArgs a = {};
+  bool vec = false;
+  int64_t h_rows = 0;
+  TERRA_TRY(prepare(desc, &a, &vec, &h_rows));
+  if (a.rows == 0) return 0;
+  const TailBwdPlan p = tail_bwd_plan(a.rows, a.C, a.gate_rows);
+  return (int)(p.blocks * 4 * a.C + (a.gate_rows > 0 && p.slabs > 1 ? p.units * a.C : 0));
+}
+
+extern "C" int terra_swin_residual_norm_bwd(const void* h, const void* x, const void* dy, const void* dz, void* dh, void* dx,
+                                            const terra_swin_residual_norm_desc* desc,
+                                            const float* post_weight, const float* post_bias, const float* gate,
+                                            const float* next_weight, const void* seed,
+                                            float* dpost_weight, float* dpost_bias, float* dgate,
+                                            float* dnext_weight, float* dnext_bias, float* workspace, void* stream) {
+  clear_error();
+  TailArgs a = {};
+  bool vec = false;
+  int64_t h_rows = 0;
+  TERRA_TRY(prepare(desc, &a, &vec, &h_rows));
+  TERRA_TRY(dropout_args(desc->p, seed, desc->stream_id, &a.drop));
+  const int he = dtype_size(desc->h_dtype), xe = dtype_size(desc->x_dtype);
+  bool ignored = false;
+  for (const float* p : {(const float*)dpost_weight, (const float*)dpost_bias, (const float*)dgate,
+                         (const float*)dnext_weight, (const float*)dnext_bias, (const float*)workspace})
+    TERRA_TRY(check_pointer(p, 4, "a parameter's gradient or the workspace", false, &ignored));
+  if (a.post == TERRA_NORM_NONE && (dpost_weight != nullptr || dpost_bias != nullptr))
+    return fail(TERRA_ERR_SHAPE, "gradients of a post-norm that the call has not");
+  if (a.next == TERRA_NORM_NONE && (dz != nullptr || dnext_weight != nullptr || dnext_bias != nullptr))
+    return fail(TERRA_ERR_SHAPE, "gradients of a next norm that the call has not");
+  if (dgate != nullptr && desc->gate_rows == 0) return fail(TERRA_ERR_SHAPE, "the gradient of a gate that the call has not");
+  hipStream_t s = (hipStream_t)stream;
+  SumJobs jobs = {};
+  jobs.C = a.C;
+  int n = 0;
+  if (a.rows == 0) {  // sums of no rows
+    for (float* p : {dpost_weight, dpost_bias, dnext_weight, dnext_bias})
+      if (p != nullptr) jobs.job[n++] = {p, p, 0, 0, 1};
+    if (dgate != nullptr) jobs.job[n++] = {dgate, dgate, 0, 0, (int32_t)desc->gate_rows};
+    if (n > 0) launch_sums(jobs, n, s);
+    return launched("terra_swin_residual_norm_bwd");
+  }
+  TERRA_TRY(check_pointer(h, he, "h", true, &vec));
+  TERRA_TRY(check_pointer(x, xe, "x", true, &vec));
+  TERRA_TRY(check_pointer(dy, xe, "dy", false, &vec));
+  TERRA_TRY(check_pointer(dz, he, "dz", false, &vec));
+  TERRA_TRY(check_pointer(dh, he, "dh", true, &vec));
+  TERRA_TRY(check_pointer(dx, xe, "dx", true, &vec));
+  TERRA_TRY(check_pointer(gate, 4, "gate", a.gate_rows > 0, &vec));
+  for (const float* p : {post_weight, post_bias, next_weight})
+    TERRA_TRY(check_pointer(p, 4, "a norm's parameter", false, &vec));
+  const bool sums = dpost_weight != nullptr || dpost_bias != nullptr || dnext_weight != nullptr || dnext_bias != nullptr;
+  if ((sums || dgate != nullptr) && workspace == nullptr) return fail(TERRA_ERR_NULL, "parameter gradients need a workspace");
+  const int64_t C = a.C;
+  TERRA_TRY(check_spans({{h, span_bytes(h_rows, a.h_row_bytes, C * he), "h"}, {x, span_bytes(a.rows, a.x_row_bytes, C * xe), "x"},
+                         {dy, a.rows * C * xe, "dy"}, {dz, a.rows * C * he, "dz"}},
+                        {{dh, h_rows * C * he, "dh"}, {dx, a.rows * C * xe, "dx"}}));
+  a.h = (const uint8_t*)h;
+  a.x = (const uint8_t*)x;
+  a.dy = (const uint8_t*)dy;
+  a.dz = (const uint8_t*)dz;
+  a.dh = (uint8_t*)dh;
+  a.dx = (uint8_t*)dx;
+  if (a.post != TERRA_NORM_NONE) a.pw = post_weight, a.pb = post_bias;
+  if (a.next != TERRA_NORM_NONE) a.nw = next_weight;
+  a.gate = gate;
+  const TailBwdPlan p = tail_bwd_plan(a.rows, a.C, a.gate_rows);
+  a.slabs = p.slabs;
+  a.slab_rows = p.slab_rows;
+  a.units = p.units;
+  a.partial = sums ? workspace : nullptr;
+  // One slab a sample: the unit's sums are the gate's gradient itself.
+  const bool direct = dgate != nullptr && p.slabs == 1;
+  float* units = workspace + (int64_t)p.blocks * 4 * C;
+  a.gate_partial = dgate == nullptr ? nullptr : (direct ? dgate : units);
+  TERRA_TRY(launch_tail_bwd(desc->h_dtype, desc->x_dtype, &a, p, vec, s));
+  float* dst[4] = {dpost_weight, dpost_bias, dnext_weight, dnext_bias};
+  for (int i = 0; i < 4; ++i)
+    if (dst[i] != nullptr) jobs.job[n++] = {workspace + i * C, dst[i], 4 * C, (int32_t)p.blocks, 1};
+  if (dgate != nullptr && !direct)
+    jobs.job[n++] = {units, dgate, C, (int32_t)p.slabs, a.gate_rows > 1 ? a.gate_rows : 1};
+  if (n > 0) launch_sums(jobs, n, s);
+  return launched("terra_swin_residual_norm_bwd");
+}

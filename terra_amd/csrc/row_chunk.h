@@ -1,0 +1,310 @@
+// Rows in chunks of eight columns, shared by the dropout and residual-norm
+// kernels: loads, stores, the dropout mask of a chunk, and sums over the lanes
+// that hold a row.
+//
+// A chunk is the unit of the dropout mask (one Philox call gives its eight
+// 16-bit draws) and of memory access (16 bytes in 16-bit types, two times 16
+// in fp32).  kVec: rows of whole, 16-byte aligned chunks; otherwise the eight
+// columns are accessed one by one and those from C on are absent.
+#pragma once
+
+#include "common.h"
+
+namespace terra {
+namespace {
+
+constexpr int kChunkCols = 8;
+
+template <int DT> struct ChunkElt { static constexpr int kBytes = 2; };
+template <> struct ChunkElt<TERRA_DTYPE_F32> { static constexpr int kBytes = 4; };
+
+template <int DT>
+struct RowChunk {
+  static constexpr int kWords = ChunkElt<DT>::kBytes / 2;
+  stream_u32x4 q[kWords];
+};
+
+// The chunk at columns [col, col + 8) of the row at `row`, whose addresses are
+// valid whatever `present` says; a chunk that is not present reads the row's
+// first one, and what was read is discarded by unpack (no branch: a load under
+// one gets a wait of its own at the join).
+template <int DT, bool kVec>
+__device__ __forceinline__ RowChunk<DT> load_chunk(const uint8_t* row, int col, int C, bool present) {
+  constexpr int kB = ChunkElt<DT>::kBytes;
+  RowChunk<DT> r;
+  if constexpr (kVec) {
+    const stream_u32x4* p = reinterpret_cast<const stream_u32x4*>(row + (present ? (int64_t)col * kB : 0));
+#pragma unroll
+    for (int i = 0; i < RowChunk<DT>::kWords; ++i) r.q[i] = __builtin_nontemporal_load(p + i);
+  } else {
+#pragma unroll
+    for (int j = 0; j < kChunkCols; ++j) {
+      const int c = present && col + j < C ? col + j : 0;
+      if constexpr (kB == 4) {
+        r.q[j >> 2][j & 3] = reinterpret_cast<const uint32_t*>(row)[c];
+      } else {
+        const uint32_t v = reinterpret_cast<const uint16_t*>(row)[c];
+        if (j & 1) r.q[0][j >> 1] |= v << 16;
+        else r.q[0][j >> 1] = v;
+      }
+    }
+  }
+  return r;
+}
+
+// The chunk's values in fp32; zeros where it is not present and, without
+// kVec, from column C on.
+template <int DT, bool kVec>
+__device__ __forceinline__ void unpack(const RowChunk<DT>& r, float (&f)[kChunkCols], int col, int C, bool present) {
+#pragma unroll
+  for (int j = 0; j < kChunkCols; ++j) {
+    float v;
+    if constexpr (DT == TERRA_DTYPE_F32) {
+      v = __uint_as_float(r.q[j >> 2][j & 3]);
+    } else {
+      const uint32_t w = r.q[0][j >> 1];
+      if constexpr (DT == TERRA_DTYPE_BF16) v = __uint_as_float(j & 1 ? w & 0xffff0000u : w << 16);
+      else v = __half2float(__ushort_as_half((uint16_t)(j & 1 ? w >> 16 : w & 0xffffu)));
+    }
+    f[j] = present && (kVec || col + j < C) ? v : 0.f;
+  }
+}
+
+typedef __bf16 chunk_bf16x2 __attribute__((ext_vector_type(2)));
+
+// Two fp32 values rounded once, to nearest even, into one word of a 16-bit type.
+template <int DT>
+__device__ __forceinline__ uint32_t pack2(float a, float b) {
+  if constexpr (DT == TERRA_DTYPE_BF16) {
+    chunk_bf16x2 v;
+    v[0] = (__bf16)a;
+    v[1] = (__bf16)b;
+    return __builtin_bit_cast(uint32_t, v);
+  } else {
+    return (uint32_t)__half_as_ushort(__float2half_rn(a)) | ((uint32_t)__half_as_ushort(__float2half_rn(b)) << 16);
+  }
+}
+
+// Stores the chunk's values at byte offset `off` (its first column) of the
+// descriptor's range, rounded once to DT; the caller checks that it is present.
+template <int DT, bool kVec>
+__device__ __forceinline__ void store_chunk(const float (&f)[kChunkCols], __amdgpu_buffer_rsrc_t out, uint32_t off,
+                                            int col, int C) {
+  if constexpr (kVec) {
+    if constexpr (DT == TERRA_DTYPE_F32) {
+      stream_store_sc1(stream_u32x4{__float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]),
+                                    __float_as_uint(f[3])}, out, off);
+      stream_store_sc1(stream_u32x4{__float_as_uint(f[4]), __float_as_uint(f[5]), __float_as_uint(f[6]),
+                                    __float_as_uint(f[7])}, out, off + 16);
+    } else {
+      stream_store_sc1(stream_u32x4{pack2<DT>(f[0], f[1]), pack2<DT>(f[2], f[3]), pack2<DT>(f[4], f[5]),
+                                    pack2<DT>(f[6], f[7])}, out, off);
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < kChunkCols; ++j) {
+      if (col + j >= C) break;
+      if constexpr (DT == TERRA_DTYPE_F32) stream_store_sc1(__float_as_uint(f[j]), out, off + 4 * j);
+      else stream_store_sc1((uint16_t)pack2<DT>(f[j], 0.f), out, off + 2 * j);
+    }
+  }
+}
+
+// The chunk's values stored at its columns of the row at `row`, rounded once.
+template <int DT, bool kVec>
+__device__ __forceinline__ void store_row(const float (&f)[kChunkCols], uint8_t* row, int col, int C) {
+  if constexpr (kVec) {
+    stream_u32x4* p = reinterpret_cast<stream_u32x4*>(row + (int64_t)col * ChunkElt<DT>::kBytes);
+    if constexpr (DT == TERRA_DTYPE_F32) {
+      __builtin_nontemporal_store(stream_u32x4{__float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]),
+                                               __float_as_uint(f[3])}, p);
+      __builtin_nontemporal_store(stream_u32x4{__float_as_uint(f[4]), __float_as_uint(f[5]), __float_as_uint(f[6]),
+                                               __float_as_uint(f[7])}, p + 1);
+    } else {
+      __builtin_nontemporal_store(stream_u32x4{pack2<DT>(f[0], f[1]), pack2<DT>(f[2], f[3]), pack2<DT>(f[4], f[5]),
+                                               pack2<DT>(f[6], f[7])}, p);
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < kChunkCols; ++j) {
+      if (col + j >= C) break;
+      if constexpr (DT == TERRA_DTYPE_F32) reinterpret_cast<float*>(row)[col + j] = f[j];
+      else reinterpret_cast<uint16_t*>(row)[col + j] = (uint16_t)pack2<DT>(f[j], 0.f);
+    }
+  }
+}
+
+// ---- the dropout mask --------------------------------------------------------
+// Philox4x32-10 (Salmon, Moraes, Dror, Shaw, "Parallel random numbers: as easy
+// as 1, 2, 3", SC 2011): ten rounds of two 32x32 -> 64-bit products over a
+// 128-bit counter under a 64-bit key.  Counter = (column >> 3, row, 0, stream),
+// key = the seed; the four result words are the draws of the chunk's eight
+// columns, 16 bits each, low half first.  A draw below `threshold` =
+// round(p 65536) drops its element, so p is kept to 2^-17, and the scale of
+// the kept ones, 65536 / (65536 - threshold), makes the expectation exact.
+// 16 bits a draw rather than 32 halve the generator's work, which is as long
+// as the memory traffic of a 16-bit element otherwise.
+struct DropoutArgs {
+  const uint64_t* seed;
+  uint32_t threshold;  // 0: nothing is dropped (seed not read); 65536: everything
+  float scale;         // of the kept elements
+  uint32_t stream;
+};
+
+struct ChunkDraws {
+  uint32_t w[4];
+};
+
+__device__ __forceinline__ ChunkDraws chunk_draws(uint64_t seed, uint32_t chunk, uint32_t row, uint32_t stream) {
+  uint32_t c0 = chunk, c1 = row, c2 = 0, c3 = stream;
+  uint32_t k0 = (uint32_t)seed, k1 = (uint32_t)(seed >> 32);
+#pragma unroll
+  for (int i = 0; i < 10; ++i) {
+    const uint64_t a = (uint64_t)c0 * 0xD2511F53u, b = (uint64_t)c2 * 0xCD9E8D57u;
+    c0 = (uint32_t)(b >> 32) ^ c1 ^ k0;
+    c1 = (uint32_t)b;
+    c2 = (uint32_t)(a >> 32) ^ c3 ^ k1;
+    c3 = (uint32_t)a;
+    k0 += 0x9E3779B9u;
+    k1 += 0xBB67AE85u;
+  }
+  return {{c0, c1, c2, c3}};
+}
+
+__device__ __forceinline__ bool kept(const ChunkDraws& d, int j, uint32_t threshold) {
+  return (j & 1 ? d.w[j >> 1] >> 16 : d.w[j >> 1] & 0xffffu) >= threshold;
+}
+
+// ---- sums over the lanes of a row ---------------------------------------------
+// Sum over the kL aligned lanes of a wave (kL = 16, 32 or 64); every lane ends
+// with the same bits, since each step adds the same two values on both sides.
+template <int kL>
+__device__ __forceinline__ float lanes_sum(float v) {
+  v = row16_sum(v);
+  if constexpr (kL >= 32) {
+    const uint32_t b = __float_as_uint(v);
+    const auto p = __builtin_amdgcn_permlane16_swap(b, b, false, false);
+    v = __uint_as_float(p[0]) + __uint_as_float(p[1]);
+  }
+  if constexpr (kL >= 64) {
+    const uint32_t b = __float_as_uint(v);
+    const auto p = __builtin_amdgcn_permlane32_swap(b, b, false, false);
+    v = __uint_as_float(p[0]) + __uint_as_float(p[1]);
+  }
+  return v;
+}
+
+// Sums over the kG lanes of a row: of a part of a wave (kG <= 64), or of the
+// whole workgroup (kG = its threads), whose waves meet in LDS.  Two slots take
+// turns, so one barrier a sum is enough: a wave writes a slot again only after
+// the barrier of the sum in between, which every wave reaches after it has
+// read that slot.
+template <int kG>
+struct RowSum {
+  static constexpr int kWaves = kG > 64 ? kG / 64 : 1;
+  struct Shared { float part[kG > 64 ? 2 : 1][kWaves][2]; };
+  Shared* s;
+  int turn = 0;
+
+  __device__ __forceinline__ explicit RowSum(Shared* shared) : s(shared) {}
+
+  __device__ __forceinline__ void two(float& a, float& b) {
+    if constexpr (kG <= 64) {
+      a = lanes_sum<kG>(a);
+      b = lanes_sum<kG>(b);
+    } else {
+      a = lanes_sum<64>(a);
+      b = lanes_sum<64>(b);
+      if ((threadIdx.x & 63) == 0) {
+        s->part[turn][threadIdx.x >> 6][0] = a;
+        s->part[turn][threadIdx.x >> 6][1] = b;
+      }
+      lds_sync();
+      a = b = 0.f;
+#pragma unroll
+      for (int w = 0; w < kWaves; ++w) {
+        a += s->part[turn][w][0];
+        b += s->part[turn][w][1];
+      }
+      turn ^= 1;
+    }
+  }
+  __device__ __forceinline__ float one(float a) {
+    if constexpr (kG <= 64) return lanes_sum<kG>(a);
+    float b = 0.f;
+    two(a, b);
+    return a;
+  }
+  // A workgroup barrier that waits for LDS only: loads of rows ahead stay in flight.
+  static __device__ __forceinline__ void lds_sync() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
+};
+
+// ---- column sums in two levels -------------------------------------------------
+// Adds up partial sums of the workgroups of an earlier launch, in an order
+// that the sizes alone fix: dst[b][c] = sum over i < count of
+// src[(b * count + i) * src_stride + c].
+struct SumJob {
+  const float* src;
+  float* dst;
+  int64_t src_stride;
+  int32_t count;
+  int32_t batch;
+};
+constexpr int kMaxSumJobs = 5;
+struct SumJobs {
+  SumJob job[kMaxSumJobs];
+  int32_t C;
+};
+
+constexpr int kSumThreads = 1024;
+constexpr int kSumCols = 64;
+
+// One workgroup for 64 columns of one row of one job: its 16 waves take every
+// 16th partial each.  (static: each source file that sums has its own copy)
+static __global__ __launch_bounds__(kSumThreads) void sum_partials_kernel(const SumJobs jobs) {
+  const SumJob j = jobs.job[blockIdx.y];
+  __shared__ double s[kSumThreads / 64][kSumCols];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int c = blockIdx.x * kSumCols + lane;
+  for (int b = blockIdx.z; b < j.batch; b += gridDim.z) {
+    double sum = 0.0;
+    const float* src = j.src + (int64_t)b * j.count * j.src_stride + (c < jobs.C ? c : 0);
+    int i = wave;
+    for (; i + 48 < j.count; i += 64) {
+      const float v0 = src[(int64_t)i * j.src_stride], v1 = src[(int64_t)(i + 16) * j.src_stride];
+      const float v2 = src[(int64_t)(i + 32) * j.src_stride], v3 = src[(int64_t)(i + 48) * j.src_stride];
+      sum += ((double)v0 + (double)v1) + ((double)v2 + (double)v3);
+    }
+    for (; i < j.count; i += 16) sum += (double)src[(int64_t)i * j.src_stride];
+    s[wave][lane] = sum;
+    __syncthreads();
+    if (wave == 0 && c < jobs.C) {
+      for (int w = 1; w < kSumThreads / 64; ++w) sum += s[w][lane];
+      j.dst[(int64_t)b * jobs.C + c] = (float)sum;
+    }
+    __syncthreads();
+  }
+}
+
+// Launches the jobs with a destination (count of them in `n`).
+inline void launch_sums(const SumJobs& jobs, int n, hipStream_t s) {
+  int batch = 1;
+  for (int i = 0; i < n; ++i) batch = jobs.job[i].batch > batch ? jobs.job[i].batch : batch;
+  const dim3 grid((unsigned)((jobs.C + kSumCols - 1) / kSumCols), (unsigned)n, (unsigned)(batch < 1024 ? batch : 1024));
+  sum_partials_kernel<<<grid, kSumThreads, 0, s>>>(jobs);
+}
+
+// Whether dropout with these arguments is valid; fills `d`.
+inline int dropout_args(double p, const void* seed, uint32_t stream, DropoutArgs* d) {
+  if (!(p >= 0.0 && p <= 1.0)) return fail(TERRA_ERR_SHAPE, "the dropout probability must be in [0, 1] (got %g)", p);
+  d->threshold = (uint32_t)(p * 65536.0 + 0.5);
+  d->scale = d->threshold < 65536u ? (float)(65536.0 / (65536.0 - (double)d->threshold)) : 0.f;
+  d->stream = stream;
+  d->seed = (const uint64_t*)seed;
+  if (d->threshold > 0 && seed == nullptr) return fail(TERRA_ERR_NULL, "dropout needs a seed");
+  if (((uintptr_t)seed & 7u) != 0) return fail(TERRA_ERR_ALIGN, "the seed must be 8-byte aligned");
+  return TERRA_OK;
+}
+
+}  // namespace
+}  // namespace terra

@@ -11,7 +11,7 @@ import ctypes
 import weakref
 from collections import OrderedDict
 from dataclasses import dataclass
-from typing import Optional, Sequence, Tuple, Union
+from typing import NamedTuple, Optional, Sequence, Tuple, Union
 
 import torch
 
@@ -1264,3 +1264,314 @@ class _MlpLaunch(_Launch):
         self.ptrs = (_ptr(params[0]), _ptr(params[1]), _ptr(fc1_weight), _ptr(params[2]), _ptr(fc2_weight),
                      _ptr(params[3]))
         self.fn, self.name = _lib.load().terra_swin_mlp_fwd, "terra_swin_mlp_fwd"
+
+
+# ---- regularised training: dropout, and the end of a half-block ---------------
+
+_FLOATS = (torch.float32, torch.bfloat16, torch.float16)
+
+
+def dropout_seed(device: Union[str, torch.device, None] = None,
+                 generator: Optional[torch.Generator] = None) -> torch.Tensor:
+    """A seed for the dropout kernels: one int64 drawn on ``device`` (default:
+    the current one) from torch's generator, so ``torch.manual_seed`` fixes it, and in a captured
+    graph every replay draws a new one."""
+    return torch.empty(1, dtype=torch.int64, device="cuda" if device is None else device).random_(generator=generator)
+
+
+def _dropout_args(x: torch.Tensor, p: float, seed: Optional[torch.Tensor], stream: int) -> Tuple[float, int]:
+    p, stream = float(p), int(stream)
+    if not 0.0 <= p <= 1.0:
+        raise ValueError(f"the dropout probability must be in [0, 1] (got {p})")
+    if not 0 <= stream < 1 << 32:
+        raise ValueError(f"stream must be in [0, 2^32) (got {stream})")
+    if seed is None:
+        if p > 0.0:
+            raise ValueError("dropout with p > 0 needs a seed (see dropout_seed)")
+    elif seed.dtype != torch.int64 or seed.numel() != 1 or seed.device != x.device:
+        raise ValueError(f"seed must be one int64 value on {x.device} (got {seed.dtype}, {seed.numel()} values on "
+                         f"{seed.device})")
+    return p, stream
+
+
+def _token_rows(t: torch.Tensor, name: str) -> Tuple[int, int, int]:
+    """(rows, C, row stride) of t [..., C]: unit channel stride and one stride
+    over all leading dimensions (packed rows, or column blocks of wider ones)."""
+    if t.dim() < 1:
+        raise ValueError(f"{name} must be [..., C], got a scalar")
+    C = t.shape[-1]
+    rows = t.numel() // C if C else 0
+    if t.is_contiguous() or rows == 0:
+        return rows, C, C
+    step, stride = 1, None
+    for n, s in zip(reversed(t.shape[:-1]), reversed(t.stride()[:-1])):
+        if n == 1:
+            continue
+        if stride is None:
+            stride = s
+        elif s != stride * step:
+            stride = -1
+            break
+        step *= n
+    if stride is None:
+        stride = C
+    if (C > 1 and t.stride(-1) != 1) or stride < C:
+        raise ValueError(f"{name} must have unit channel stride and one row stride of at least {C} (strides {t.stride()})")
+    return rows, C, stride
+
+
+def _same(out: Optional[torch.Tensor], like: torch.Tensor) -> torch.Tensor:
+    """``out``, checked, or a new packed tensor like ``like``."""
+    if out is None:
+        return torch.empty(like.shape, dtype=like.dtype, device=like.device)
+    if out.shape != like.shape or out.dtype != like.dtype or not out.is_contiguous() or out.device != like.device:
+        raise ValueError(f"out must be a contiguous {like.dtype} tensor of shape {tuple(like.shape)} on {like.device}")
+    return out
+
+
+def dropout(x: torch.Tensor, p: float, seed: Optional[torch.Tensor], stream: int = 0,
+            out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Dropout of ``x`` [..., C] (fp32, bf16 or fp16): kept elements times
+    1 / (1 - p), dropped ones 0, the mask drawn from a counter-based generator
+    in the kernel and never stored.  It depends on ``seed`` (an int64 on the
+    device, see :func:`dropout_seed`), ``stream`` (the call site: calls that
+    share a seed take streams of their own) and the element's row and column;
+    the backward is the same call on the output's gradient.  ``p`` is rounded
+    to a multiple of 2^-16, and the scale is that of the rounded one.
+    ``out`` may be ``x``."""
+    dev = _require_device(x)
+    code = _dtype_code(x, _FLOATS)
+    p, stream = _dropout_args(x, p, seed, stream)
+    rows, C, stride = _token_rows(x, "x")
+    out = _same(out, x)
+    if rows == 0:
+        return out
+    with torch.cuda.device(dev):
+        st = _lib.load().terra_swin_dropout(_ptr(x), _ptr(out), code, rows, C, stride, p, _ptr(seed), stream, _stream(dev))
+    _lib.check(st, "terra_swin_dropout")
+    return out
+
+
+def gelu_dropout(h: torch.Tensor, p: float, seed: Optional[torch.Tensor], stream: int = 0,
+                 out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """``dropout(GELU(h))`` (erf form, models/mlp.py:165) of a contiguous ``h``
+    [..., features] in one pass, rounded once; the mask as :func:`dropout`'s.
+    ``out`` may be ``h``."""
+    dev = _require_device(h)
+    code = _dtype_code(h, _FLOATS)
+    p, stream = _dropout_args(h, p, seed, stream)
+    if h.dim() < 1 or not h.is_contiguous():
+        raise ValueError("h must be a contiguous [..., features] tensor")
+    out = _same(out, h)
+    if h.numel() == 0:
+        return out
+    C = h.shape[-1]
+    with torch.cuda.device(dev):
+        st = _lib.load().terra_swin_gelu_dropout(_ptr(h), _ptr(out), code, h.numel() // C, C, p, _ptr(seed), stream,
+                                                 _stream(dev))
+    _lib.check(st, "terra_swin_gelu_dropout")
+    return out
+
+
+def gelu_dropout_backward(dout: torch.Tensor, h: torch.Tensor, p: float, seed: Optional[torch.Tensor], stream: int = 0,
+                          column_sums: bool = False, out: Optional[torch.Tensor] = None):
+    """The gradient of :func:`gelu_dropout` at ``h`` for the output gradient
+    ``dout`` (like h): ``keep * dout * (Phi(h) + h phi(h))``, rounded once, with
+    the mask drawn again.  With ``column_sums`` also its sums over the rows
+    (fp32 [features], the bias gradient of the Linear that produced ``h``),
+    before the rounding and in an order that the sizes fix: ``(dh, sums)``.
+    ``out`` may be ``dout`` or ``h``."""
+    dev = _require_device(dout, h)
+    code = _dtype_code(h, _FLOATS)
+    p, stream = _dropout_args(h, p, seed, stream)
+    if dout.shape != h.shape or dout.dtype != h.dtype:
+        raise ValueError(f"dout {tuple(dout.shape)} {dout.dtype} must match h {tuple(h.shape)} {h.dtype}")
+    if h.dim() < 1 or not (dout.is_contiguous() and h.is_contiguous()):
+        raise ValueError("dout and h must be contiguous [..., features] tensors")
+    out = _same(out, h)
+    C = h.shape[-1]
+    if h.numel() == 0:
+        return (out, torch.zeros(C, dtype=torch.float32, device=dev)) if column_sums else out
+    lib, rows = _lib.load(), h.numel() // C
+    sums = work = None
+    if column_sums:
+        sums = torch.empty(C, dtype=torch.float32, device=dev)
+        work = torch.empty(_size(lib.terra_swin_gelu_dropout_workspace(rows, C), "terra_swin_gelu_dropout_workspace"),
+                           dtype=torch.float32, device=dev)
+    with torch.cuda.device(dev):
+        st = lib.terra_swin_gelu_dropout_bwd(_ptr(dout), _ptr(h), _ptr(out), code, rows, C, p, _ptr(seed), stream,
+                                             _ptr(sums), _ptr(work), _stream(dev))
+    _lib.check(st, "terra_swin_gelu_dropout_bwd")
+    return (out, sums) if column_sums else out
+
+
+def _size(n: int, what: str) -> int:
+    """A workspace size, or the error that a negative one is."""
+    if n < 0:
+        _lib.check(int(n), what)
+    return int(n)
+
+
+@dataclass(frozen=True, eq=False)
+class Norm:
+    """A norm over the channels for :func:`residual_norm`: LayerNorm, or with
+    ``rms`` the RMS norm ``v / sqrt(mean(v^2) + eps)``; affine [C] weight and
+    bias, either None (1, 0)."""
+
+    weight: Optional[torch.Tensor] = None
+    bias: Optional[torch.Tensor] = None
+    eps: float = 1e-5
+    rms: bool = False
+
+    @staticmethod
+    def of(module: Optional[torch.nn.Module]) -> Optional["Norm"]:
+        """The norm that an nn.LayerNorm or nn.RMSNorm over one dimension is."""
+        if module is None:
+            return None
+        if type(module) is torch.nn.LayerNorm and len(module.normalized_shape) == 1:
+            return Norm(module.weight, module.bias, module.eps)
+        if type(module) is torch.nn.RMSNorm and len(module.normalized_shape) == 1:
+            # eps None is the machine epsilon of the type that torch normalises in
+            eps = torch.finfo(torch.float32).eps if module.eps is None else module.eps
+            return Norm(module.weight, None, eps, rms=True)
+        raise TypeError(f"expected an nn.LayerNorm or nn.RMSNorm over the channels, got {module!r}")
+
+
+class ResidualNormGrads(NamedTuple):
+    """What :func:`residual_norm_backward` gives; None where there is none."""
+
+    dh: torch.Tensor
+    dx: torch.Tensor
+    dpost_weight: Optional[torch.Tensor]
+    dpost_bias: Optional[torch.Tensor]
+    dgate: Optional[torch.Tensor]
+    dnext_weight: Optional[torch.Tensor]
+    dnext_bias: Optional[torch.Tensor]
+
+
+class _Tail:
+    """The checked arguments of a residual_norm call: descriptor, parameters
+    as the kernels read them (fp32), and what its outputs look like."""
+
+    def __init__(self, h, x, post_norm, gate, next_norm, geom, residual_scale, p, seed, stream):
+        self.dev = dev = _require_device(h, x)
+        d = _lib.ResidualNormDesc()
+        d.h_dtype, d.x_dtype = _dtype_code(h, _FLOATS), _dtype_code(x, _FLOATS)
+        if x.dtype not in (h.dtype, torch.float32):
+            raise TypeError(f"x must be {h.dtype} like h, or float32 (got {x.dtype})")
+        d.p, d.stream_id = _dropout_args(h, p, seed, stream)
+        rows, C, d.x_stride = _token_rows(x, "x")
+        h_rows, hc, d.h_stride = _token_rows(h, "h")
+        if hc != C or C == 0:
+            raise ValueError(f"h {tuple(h.shape)} and x {tuple(x.shape)} must have the same channels, at least one")
+        if geom is None:
+            if h.shape != x.shape:
+                raise ValueError(f"h {tuple(h.shape)} must have x's shape {tuple(x.shape)} (or a geometry)")
+        else:
+            tokens = geom.batch * geom.height * geom.width
+            if geom.channels != C or rows != tokens or x.shape[0] != geom.batch:
+                raise ValueError(f"x {tuple(x.shape)} is not the geometry's grid "
+                                 f"{(geom.batch, geom.height, geom.width, geom.channels)}")
+            if h_rows != geom.num_windows * geom.window ** 2:
+                raise ValueError(f"h {tuple(h.shape)} is not the geometry's {geom.num_windows} windows of "
+                                 f"{geom.window ** 2} tokens")
+            d.windows, d.geom = 1, geom.to_c()
+            # Every window token is some row's branch: nothing of dh is left unwritten.
+            self.covered = h_rows == tokens and geom.valid is None and not any(geom.pad)
+        d.rows, d.channels, d.residual_scale = rows, C, float(residual_scale)
+        self.desc, self.seed, self.geom, self.rows, self.C = d, seed, geom, rows, C
+        self.params = []
+
+        def param(t, name, shape):
+            if t is None:
+                self.params.append(None)
+                return
+            _require_device(x, t)
+            if tuple(t.shape) != shape:
+                raise ValueError(f"{name} must be {list(shape)}, got {list(t.shape)}")
+            self.params.append(t.detach().to(torch.float32).contiguous())
+
+        for which, n in (("post", post_norm), ("next", next_norm)):
+            if n is not None:
+                setattr(d, which + "_norm", _lib.NORM_RMS if n.rms else _lib.NORM_LAYER)
+                setattr(d, which + "_eps", float(n.eps))
+            param(None if n is None else n.weight, f"{which}_norm's weight", (C,))
+            param(None if n is None else n.bias, f"{which}_norm's bias", (C,))
+        if gate is not None and gate.dim() == 2:
+            param(gate, "gate", (x.shape[0] if x.dim() > 1 else 1, C))
+            d.gate_rows = gate.shape[0]
+        else:
+            param(gate, "gate", (C,))
+            d.gate_rows = int(gate is not None)
+
+    def pointers(self):
+        """post weight, post bias, gate, next weight, next bias."""
+        pw, pb, nw, nb, gate = self.params
+        return _ptr(pw), _ptr(pb), _ptr(gate), _ptr(nw), _ptr(nb)
+
+
+def residual_norm(h: torch.Tensor, x: torch.Tensor, post_norm: Optional[Norm] = None,
+                  gate: Optional[torch.Tensor] = None, next_norm: Optional[Norm] = None,
+                  geom: Optional[WindowGeometry] = None, residual_scale: float = 1.0, p: float = 0.0,
+                  seed: Optional[torch.Tensor] = None, stream: int = 0):
+    """The end of a half-block in one pass over the token rows:
+
+        y = residual_scale * x + gate * dropout(post_norm(h)),   z = next_norm(y)
+
+    h: the branch's output [..., C]; x: the residual stream, of h's shape and
+    dtype, or fp32 for a bf16 / fp16 h (autocast).  ``gate``: [C] (a layer
+    scale) or [B, C] for x [B, ..., C] (a gate of each sample's own, or
+    stochastic depth: a drawn 0 or 1 / keep for each sample).  ``geom``: h is in window order
+    [B_, N, C] and x the grid [B, H, W, C] (or [B, H * W, C]); the window
+    reverse and the inverse roll are part of the read, and rows that no emitted
+    window holds get no branch (as :func:`swin_reverse`).  ``p``, ``seed``,
+    ``stream``: dropout as :func:`dropout` over the rows of x.
+
+    Returns y, in x's shape and dtype, or with ``next_norm`` (y, z), z in h's
+    dtype and from the y that is not yet rounded.  C <= 8192; h and x may be
+    column blocks of wider rows."""
+    t = _Tail(h, x, post_norm, gate, next_norm, geom, residual_scale, p, seed, stream)
+    y = torch.empty(x.shape, dtype=x.dtype, device=t.dev)
+    z = torch.empty(x.shape, dtype=h.dtype, device=t.dev) if next_norm is not None else None
+    if t.rows > 0:
+        with torch.cuda.device(t.dev):
+            st = _lib.load().terra_swin_residual_norm(_ptr(h), _ptr(x), _ptr(y), _ptr(z), ctypes.byref(t.desc),
+                                                      *t.pointers(), _ptr(seed), _stream(t.dev))
+        _lib.check(st, "terra_swin_residual_norm")
+    return y if z is None else (y, z)
+
+
+def residual_norm_backward(h: torch.Tensor, x: torch.Tensor, dy: Optional[torch.Tensor], dz: Optional[torch.Tensor],
+                           post_norm: Optional[Norm] = None, gate: Optional[torch.Tensor] = None,
+                           next_norm: Optional[Norm] = None, geom: Optional[WindowGeometry] = None,
+                           residual_scale: float = 1.0, p: float = 0.0, seed: Optional[torch.Tensor] = None,
+                           stream: int = 0, needs: Sequence[bool] = (True,) * 5) -> ResidualNormGrads:
+    """Gradients of :func:`residual_norm` (the same arguments) for the
+    gradients ``dy`` of y and ``dz`` of z (contiguous, in y's and z's shape and
+    dtype; either may be None), everything recomputed from h and x.  ``needs``:
+    which of the five parameter gradients (in the order of
+    :class:`ResidualNormGrads`) are taken where the parameter is there; they
+    are fp32, the sums over rows in an order that the sizes fix."""
+    t = _Tail(h, x, post_norm, gate, next_norm, geom, residual_scale, p, seed, stream)
+    for name, g, like in (("dy", dy, x), ("dz", dz, h)):
+        if g is not None:
+            _require_device(x, g)
+            if g.shape != x.shape or g.dtype != like.dtype or not g.is_contiguous():
+                raise ValueError(f"{name} must be a contiguous {like.dtype} tensor of shape {tuple(x.shape)}")
+    if dz is not None and next_norm is None:
+        raise ValueError("dz without a next_norm")
+    empty = torch.empty if geom is None or t.covered else torch.zeros
+    dh = empty(h.shape, dtype=h.dtype, device=t.dev)
+    dx = torch.empty(x.shape, dtype=x.dtype, device=t.dev)
+    pw, pb, nw, nb, g = t.params
+    grads = [torch.empty(q.shape, dtype=torch.float32, device=t.dev) if q is not None and need else None
+             for q, need in zip((pw, pb, g, nw, nb), needs)]
+    lib, work = _lib.load(), None
+    if any(q is not None for q in grads):
+        work = torch.empty(_size(lib.terra_swin_residual_norm_workspace(ctypes.byref(t.desc)),
+                                 "terra_swin_residual_norm_workspace"), dtype=torch.float32, device=t.dev)
+    with torch.cuda.device(t.dev):
+        st = lib.terra_swin_residual_norm_bwd(_ptr(h), _ptr(x), _ptr(dy), _ptr(dz), _ptr(dh), _ptr(dx), ctypes.byref(t.desc),
+                                              *t.pointers()[:4], _ptr(seed), *map(_ptr, grads), _ptr(work), _stream(t.dev))
+    _lib.check(st, "terra_swin_residual_norm_bwd")
+    return ResidualNormGrads(dh, dx, *grads)
