@@ -708,32 +708,30 @@ def gelu_dropout(h: torch.Tensor, p: float, seed: Optional[torch.Tensor] = None,
 
 class _ResidualNorm(torch.autograd.Function):
     """kernels.residual_norm; the backward keeps h, x and the parameters and
-    recomputes the norms and the mask."""
+    recomputes the norms and the mask.  The call's checked arguments go from
+    the forward to the backward, which on small inputs is bound by the host."""
 
     @staticmethod
-    def forward(ctx, h, x, post_w, post_b, gate, next_w, next_b, post, nxt, geom, residual_scale, p, seed, stream):
-        ctx.cfg = (post, nxt, geom, residual_scale, p, stream)
+    def forward(ctx, h, x, post_w, post_b, gate, next_w, next_b, seed, tail, norms):
+        ctx.tail, ctx.norms = tail, norms
         ctx.save_for_backward(h, x, post_w, post_b, gate, next_w, next_b, seed)
         ctx.set_materialize_grads(False)
-        return kernels.residual_norm(h, x, _norm(post, post_w, post_b), gate, _norm(nxt, next_w, next_b), geom,
-                                     residual_scale, p, seed, stream)
+        return tail.forward(h, x, tail.params(norms[0], gate, norms[1]), seed)
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dy, dz=None):
         h, x, post_w, post_b, gate, next_w, next_b, seed = ctx.saved_tensors
-        post, nxt, geom, residual_scale, p, stream = ctx.cfg
-        packed = lambda g: None if g is None else g.contiguous()  # noqa: E731
-        g = kernels.residual_norm_backward(h, x, packed(dy), packed(dz), _norm(post, post_w, post_b), gate,
-                                           _norm(nxt, next_w, next_b), geom, residual_scale, p, seed, stream,
-                                           needs=ctx.needs_input_grad[2:7])
-        cast = lambda t, q: None if t is None else t.to(q.dtype)  # noqa: E731
-        return (g.dh, g.dx, *(cast(t, q) for t, q in zip(g[2:], (post_w, post_b, gate, next_w, next_b))),
-                *(None,) * 7)
-
-
-def _norm(kind: Optional[Tuple[float, bool]], weight, bias) -> Optional[Norm]:
-    return None if kind is None else Norm(weight, bias, *kind)
+        if dy is not None and not dy.is_contiguous():
+            dy = dy.contiguous()
+        if dz is not None and not dz.is_contiguous():
+            dz = dz.contiguous()
+        post, nxt = ctx.norms
+        ps = ctx.tail.params(None if post is None else Norm(post_w, post_b), gate,
+                             None if nxt is None else Norm(next_w, next_b))
+        g = ctx.tail.backward(h, x, dy, dz, ps, seed, ctx.needs_input_grad[2:7])
+        return (g.dh, g.dx, *(t if t is None or t.dtype == q.dtype else t.to(q.dtype)
+                              for t, q in zip(g[2:], (post_w, post_b, gate, next_w, next_b))), None, None, None)
 
 
 def residual_norm(h: torch.Tensor, x: torch.Tensor, post_norm: Optional[Norm] = None,
@@ -747,9 +745,9 @@ def residual_norm(h: torch.Tensor, x: torch.Tensor, post_norm: Optional[Norm] = 
     seed = _seed(h, p, seed)
     if x.dtype != h.dtype and x.dtype != torch.float32:
         x = x.to(torch.promote_types(x.dtype, h.dtype))
-    params = [None if n is None else getattr(n, name) for n in (post_norm, next_norm) for name in ("weight", "bias")]
+    params = [t for n in (post_norm, next_norm) for t in ((None, None) if n is None else (n.weight, n.bias))]
     if _needs_grad(h, x, gate, *params):
-        kinds = [None if n is None else (n.eps, n.rms) for n in (post_norm, next_norm)]
-        return _ResidualNorm.apply(h, x, params[0], params[1], gate, params[2], params[3], *kinds, geom, residual_scale, p,
-                                   seed, stream)
+        tail = kernels._Tail(h, x, post_norm, gate, next_norm, geom, residual_scale, p, seed, stream)
+        return _ResidualNorm.apply(h, x, params[0], params[1], gate, params[2], params[3], seed, tail,
+                                   (post_norm, next_norm))
     return kernels.residual_norm(h, x, post_norm, gate, next_norm, geom, residual_scale, p, seed, stream)

@@ -1271,6 +1271,22 @@ class _MlpLaunch(_Launch):
 _FLOATS = (torch.float32, torch.bfloat16, torch.float16)
 
 
+def _enqueue(name: str, dev: torch.device, *args) -> None:
+    """Calls an entry point of the library on dev's current stream.  These
+    operators are short enough on small inputs for the host to set their pace, so
+    the device is switched only where another one is current, and the stream's
+    handle is read directly (a torch.cuda.device block and a Stream object
+    cost 7 us a call, of 11 for a small dropout)."""
+    fn = getattr(_lib.load(), name)
+    if dev.index == torch._C._cuda_getDevice():
+        st = fn(*args, torch._C._cuda_getCurrentRawStream(dev.index))
+    else:
+        with torch.cuda.device(dev):
+            st = fn(*args, torch._C._cuda_getCurrentRawStream(dev.index))
+    if st != 0:
+        _lib.check(st, name)
+
+
 def dropout_seed(device: Union[str, torch.device, None] = None,
                  generator: Optional[torch.Generator] = None) -> torch.Tensor:
     """A seed for the dropout kernels: one int64 drawn on ``device`` (default:
@@ -1346,9 +1362,7 @@ def dropout(x: torch.Tensor, p: float, seed: Optional[torch.Tensor], stream: int
     out = _same(out, x)
     if rows == 0:
         return out
-    with torch.cuda.device(dev):
-        st = _lib.load().terra_swin_dropout(_ptr(x), _ptr(out), code, rows, C, stride, p, _ptr(seed), stream, _stream(dev))
-    _lib.check(st, "terra_swin_dropout")
+    _enqueue("terra_swin_dropout", dev, x.data_ptr(), out.data_ptr(), code, rows, C, stride, p, _ptr(seed), stream)
     return out
 
 
@@ -1366,10 +1380,7 @@ def gelu_dropout(h: torch.Tensor, p: float, seed: Optional[torch.Tensor], stream
     if h.numel() == 0:
         return out
     C = h.shape[-1]
-    with torch.cuda.device(dev):
-        st = _lib.load().terra_swin_gelu_dropout(_ptr(h), _ptr(out), code, h.numel() // C, C, p, _ptr(seed), stream,
-                                                 _stream(dev))
-    _lib.check(st, "terra_swin_gelu_dropout")
+    _enqueue("terra_swin_gelu_dropout", dev, h.data_ptr(), out.data_ptr(), code, h.numel() // C, C, p, _ptr(seed), stream)
     return out
 
 
@@ -1398,10 +1409,8 @@ def gelu_dropout_backward(dout: torch.Tensor, h: torch.Tensor, p: float, seed: O
         sums = torch.empty(C, dtype=torch.float32, device=dev)
         work = torch.empty(_size(lib.terra_swin_gelu_dropout_workspace(rows, C), "terra_swin_gelu_dropout_workspace"),
                            dtype=torch.float32, device=dev)
-    with torch.cuda.device(dev):
-        st = lib.terra_swin_gelu_dropout_bwd(_ptr(dout), _ptr(h), _ptr(out), code, rows, C, p, _ptr(seed), stream,
-                                             _ptr(sums), _ptr(work), _stream(dev))
-    _lib.check(st, "terra_swin_gelu_dropout_bwd")
+    _enqueue("terra_swin_gelu_dropout_bwd", dev, dout.data_ptr(), h.data_ptr(), out.data_ptr(), code, rows, C, p, _ptr(seed),
+             stream, _ptr(sums), _ptr(work))
     return (out, sums) if column_sums else out
 
 
@@ -1450,20 +1459,23 @@ class ResidualNormGrads(NamedTuple):
 
 
 class _Tail:
-    """The checked arguments of a residual_norm call: descriptor, parameters
-    as the kernels read them (fp32), and what its outputs look like."""
+    """The checked arguments of a residual_norm call but the tensors: the
+    descriptor, and what its outputs look like."""
+
+    __slots__ = ("dev", "desc", "rows", "C", "covered", "geom")
 
     def __init__(self, h, x, post_norm, gate, next_norm, geom, residual_scale, p, seed, stream):
-        self.dev = dev = _require_device(h, x)
-        d = _lib.ResidualNormDesc()
+        self.dev = _require_device(h, x)
+        self.desc = d = _lib.ResidualNormDesc()
         d.h_dtype, d.x_dtype = _dtype_code(h, _FLOATS), _dtype_code(x, _FLOATS)
-        if x.dtype not in (h.dtype, torch.float32):
+        if x.dtype != h.dtype and x.dtype != torch.float32:
             raise TypeError(f"x must be {h.dtype} like h, or float32 (got {x.dtype})")
         d.p, d.stream_id = _dropout_args(h, p, seed, stream)
         rows, C, d.x_stride = _token_rows(x, "x")
         h_rows, hc, d.h_stride = _token_rows(h, "h")
         if hc != C or C == 0:
             raise ValueError(f"h {tuple(h.shape)} and x {tuple(x.shape)} must have the same channels, at least one")
+        self.covered, self.geom = True, geom
         if geom is None:
             if h.shape != x.shape:
                 raise ValueError(f"h {tuple(h.shape)} must have x's shape {tuple(x.shape)} (or a geometry)")
@@ -1476,38 +1488,62 @@ class _Tail:
                 raise ValueError(f"h {tuple(h.shape)} is not the geometry's {geom.num_windows} windows of "
                                  f"{geom.window ** 2} tokens")
             d.windows, d.geom = 1, geom.to_c()
-            # Every window token is some row's branch: nothing of dh is left unwritten.
+            # Whether every window token is some row's branch, so that all of dh is written.
             self.covered = h_rows == tokens and geom.valid is None and not any(geom.pad)
         d.rows, d.channels, d.residual_scale = rows, C, float(residual_scale)
-        self.desc, self.seed, self.geom, self.rows, self.C = d, seed, geom, rows, C
-        self.params = []
+        self.rows, self.C = rows, C
+        if post_norm is not None:
+            d.post_norm, d.post_eps = (_lib.NORM_RMS if post_norm.rms else _lib.NORM_LAYER), float(post_norm.eps)
+        if next_norm is not None:
+            d.next_norm, d.next_eps = (_lib.NORM_RMS if next_norm.rms else _lib.NORM_LAYER), float(next_norm.eps)
+        if gate is not None:
+            if gate.dim() == 2 and x.dim() > 1 and gate.shape[0] != x.shape[0]:
+                raise ValueError(f"gate must be [{C}] or [{x.shape[0]}, {C}], got {list(gate.shape)}")
+            d.gate_rows = gate.shape[0] if gate.dim() == 2 else 1
 
-        def param(t, name, shape):
-            if t is None:
-                self.params.append(None)
-                return
-            _require_device(x, t)
-            if tuple(t.shape) != shape:
-                raise ValueError(f"{name} must be {list(shape)}, got {list(t.shape)}")
-            self.params.append(t.detach().to(torch.float32).contiguous())
+    def params(self, post_norm, gate, next_norm):
+        """post weight, post bias, gate, next weight, next bias as the kernels
+        read them: fp32, contiguous, checked (None where absent)."""
+        ps, C = [], self.C
+        for name, t in (("post_norm's weight", None if post_norm is None else post_norm.weight),
+                        ("post_norm's bias", None if post_norm is None else post_norm.bias), ("gate", gate),
+                        ("next_norm's weight", None if next_norm is None else next_norm.weight),
+                        ("next_norm's bias", None if next_norm is None else next_norm.bias)):
+            if t is not None:
+                if t.shape[-1:] != (C,) or t.dim() != 1 and (name != "gate" or t.dim() != 2):
+                    raise ValueError(f"{name} must have {C} channels, got {list(t.shape)}")
+                if t.device != self.dev:
+                    raise ValueError(f"tensors on different devices: {self.dev} and {t.device}")
+                if t.dtype != torch.float32 or not t.is_contiguous():
+                    t = t.detach().to(torch.float32).contiguous()
+            ps.append(t)
+        return ps
 
-        for which, n in (("post", post_norm), ("next", next_norm)):
-            if n is not None:
-                setattr(d, which + "_norm", _lib.NORM_RMS if n.rms else _lib.NORM_LAYER)
-                setattr(d, which + "_eps", float(n.eps))
-            param(None if n is None else n.weight, f"{which}_norm's weight", (C,))
-            param(None if n is None else n.bias, f"{which}_norm's bias", (C,))
-        if gate is not None and gate.dim() == 2:
-            param(gate, "gate", (x.shape[0] if x.dim() > 1 else 1, C))
-            d.gate_rows = gate.shape[0]
-        else:
-            param(gate, "gate", (C,))
-            d.gate_rows = int(gate is not None)
+    def forward(self, h, x, ps, seed):
+        y = torch.empty(x.shape, dtype=x.dtype, device=self.dev)
+        z = torch.empty(x.shape, dtype=h.dtype, device=self.dev) if self.desc.next_norm else None
+        if self.rows > 0:
+            _enqueue("terra_swin_residual_norm", self.dev, h.data_ptr(), x.data_ptr(), y.data_ptr(), _ptr(z),
+                     ctypes.byref(self.desc), *map(_ptr, ps), _ptr(seed))
+        return y if z is None else (y, z)
 
-    def pointers(self):
-        """post weight, post bias, gate, next weight, next bias."""
-        pw, pb, nw, nb, gate = self.params
-        return _ptr(pw), _ptr(pb), _ptr(gate), _ptr(nw), _ptr(nb)
+    def backward(self, h, x, dy, dz, ps, seed, needs) -> "ResidualNormGrads":
+        dev = self.dev
+        dh = (torch.empty if self.covered else torch.zeros)(h.shape, dtype=h.dtype, device=dev)
+        dx = torch.empty(x.shape, dtype=x.dtype, device=dev)
+        want = [t is not None and need for t, need in zip(ps, needs)]
+        grads, work, vectors = [None] * 5, None, sum(want)
+        if vectors:
+            if want[2] and ps[2].dim() == 2:
+                grads[2] = torch.empty(ps[2].shape, dtype=torch.float32, device=dev)
+                vectors -= 1
+            rows = iter(torch.empty((vectors, self.C), dtype=torch.float32, device=dev).unbind(0))
+            grads = [g if g is not None or not w else next(rows) for g, w in zip(grads, want)]
+            n = _lib.load().terra_swin_residual_norm_workspace(ctypes.byref(self.desc))
+            work = torch.empty(_size(n, "terra_swin_residual_norm_workspace"), dtype=torch.float32, device=dev)
+        _enqueue("terra_swin_residual_norm_bwd", dev, h.data_ptr(), x.data_ptr(), _ptr(dy), _ptr(dz), dh.data_ptr(),
+                 dx.data_ptr(), ctypes.byref(self.desc), *map(_ptr, ps[:4]), _ptr(seed), *map(_ptr, grads), _ptr(work))
+        return ResidualNormGrads(dh, dx, *grads)
 
 
 def residual_norm(h: torch.Tensor, x: torch.Tensor, post_norm: Optional[Norm] = None,
@@ -1521,24 +1557,17 @@ def residual_norm(h: torch.Tensor, x: torch.Tensor, post_norm: Optional[Norm] = 
     h: the branch's output [..., C]; x: the residual stream, of h's shape and
     dtype, or fp32 for a bf16 / fp16 h (autocast).  ``gate``: [C] (a layer
     scale) or [B, C] for x [B, ..., C] (a gate of each sample's own, or
-    stochastic depth: a drawn 0 or 1 / keep for each sample).  ``geom``: h is in window order
-    [B_, N, C] and x the grid [B, H, W, C] (or [B, H * W, C]); the window
-    reverse and the inverse roll are part of the read, and rows that no emitted
-    window holds get no branch (as :func:`swin_reverse`).  ``p``, ``seed``,
-    ``stream``: dropout as :func:`dropout` over the rows of x.
+    stochastic depth: a drawn 0 or 1 / keep for each sample).  ``geom``: h is in
+    window order [B_, N, C] and x the grid [B, H, W, C] (or [B, H * W, C]); the
+    window reverse and the inverse roll are part of the read, and rows that no
+    emitted window holds get no branch (as :func:`swin_reverse`).  ``p``,
+    ``seed``, ``stream``: dropout as :func:`dropout` over the rows of x.
 
     Returns y, in x's shape and dtype, or with ``next_norm`` (y, z), z in h's
     dtype and from the y that is not yet rounded.  C <= 8192; h and x may be
     column blocks of wider rows."""
     t = _Tail(h, x, post_norm, gate, next_norm, geom, residual_scale, p, seed, stream)
-    y = torch.empty(x.shape, dtype=x.dtype, device=t.dev)
-    z = torch.empty(x.shape, dtype=h.dtype, device=t.dev) if next_norm is not None else None
-    if t.rows > 0:
-        with torch.cuda.device(t.dev):
-            st = _lib.load().terra_swin_residual_norm(_ptr(h), _ptr(x), _ptr(y), _ptr(z), ctypes.byref(t.desc),
-                                                      *t.pointers(), _ptr(seed), _stream(t.dev))
-        _lib.check(st, "terra_swin_residual_norm")
-    return y if z is None else (y, z)
+    return t.forward(h, x, t.params(post_norm, gate, next_norm), seed)
 
 
 def residual_norm_backward(h: torch.Tensor, x: torch.Tensor, dy: Optional[torch.Tensor], dz: Optional[torch.Tensor],
@@ -1560,18 +1589,4 @@ def residual_norm_backward(h: torch.Tensor, x: torch.Tensor, dy: Optional[torch.
                 raise ValueError(f"{name} must be a contiguous {like.dtype} tensor of shape {tuple(x.shape)}")
     if dz is not None and next_norm is None:
         raise ValueError("dz without a next_norm")
-    empty = torch.empty if geom is None or t.covered else torch.zeros
-    dh = empty(h.shape, dtype=h.dtype, device=t.dev)
-    dx = torch.empty(x.shape, dtype=x.dtype, device=t.dev)
-    pw, pb, nw, nb, g = t.params
-    grads = [torch.empty(q.shape, dtype=torch.float32, device=t.dev) if q is not None and need else None
-             for q, need in zip((pw, pb, g, nw, nb), needs)]
-    lib, work = _lib.load(), None
-    if any(q is not None for q in grads):
-        work = torch.empty(_size(lib.terra_swin_residual_norm_workspace(ctypes.byref(t.desc)),
-                                 "terra_swin_residual_norm_workspace"), dtype=torch.float32, device=t.dev)
-    with torch.cuda.device(t.dev):
-        st = lib.terra_swin_residual_norm_bwd(_ptr(h), _ptr(x), _ptr(dy), _ptr(dz), _ptr(dh), _ptr(dx), ctypes.byref(t.desc),
-                                              *t.pointers()[:4], _ptr(seed), *map(_ptr, grads), _ptr(work), _stream(t.dev))
-    _lib.check(st, "terra_swin_residual_norm_bwd")
-    return ResidualNormGrads(dh, dx, *grads)
+    return t.backward(h, x, dy, dz, t.params(post_norm, gate, next_norm), seed, needs)
