@@ -85,8 +85,11 @@ __global__ __launch_bounds__(kDropThreads) void drop_kernel(const DropParams a) 
           buffer_rsrc(a.out + (int64_t)base * a.row_bytes + strip, (uint32_t)(left < 0x7fffffff ? left : 0x7fffffff));
       if (!present || (uint32_t)tr >= live) continue;
       float f[kChunkCols], g[kChunkCols];
-      unpack<DT, kVec>(v[i], f, col, a.C, true);
-      if constexpr (kBwd) unpack<DT, kVec>(hv[i], g, col, a.C, true);
+#pragma unroll
+      for (int j = 0; j < kChunkCols; ++j) {
+        f[j] = chunk_value<DT>(v[i], j);
+        if constexpr (kBwd) g[j] = chunk_value<DT>(hv[i], j);
+      }
 #pragma unroll
       for (int j = 0; j < kChunkCols; ++j) f[j] = drop_value<kOp>(f[j], kBwd ? g[j] : 0.f);
       if (a.drop.threshold > 0) {

@@ -51,6 +51,7 @@ struct TailArgs {
   const float *pw, *pb, *gate, *nw, *nb;  // NULL: 1 (weights, gate) or 0 (biases)
   float* partial;       // backward: [gridDim.x][4][C], the workgroups' sums for pw, pb, nw, nb
   float* gate_partial;  // backward: [units][C]
+  int32_t branch_sums;  // backward: pw's, pb's or the gate's gradient is asked for
   DropoutArgs drop;
   uint32_t rows, per_sample;        // per_sample: rows that share a row of the gate
   int64_t h_row_bytes, x_row_bytes; // of h and x; the other tensors' rows are packed
@@ -67,17 +68,165 @@ struct TailShape {
   int32_t lanes, chunks;  // per row, per lane
 };
 
-// Fewest lanes that hold the row with one chunk each up to a wave; then two
-// chunks a lane, then a workgroup for each row.
+// Where a lane's values stand: value j of its chunk k is column base(k, j / 4) + j % 4.
+// With a 16-bit x the chunk is eight columns in a row (16 bytes a load).  An fp32 x
+// is accessed 16 bytes, four columns, a lane, neighbouring lanes side by
+// side, and the chunk is two such pieces kG lanes apart: eight columns in a row would
+// be two loads of every other 16 bytes, each line fetched, and worse, written,
+// in two halves (524288 x 192, bf16 h and fp32 x, forward: 365 us against FWDMIX).
+template <int kG, int kK, int kP>
+struct RowLanes {
+  static_assert(kP == 8 || kP == 4, "columns a lane holds side by side");
+  int lane, C;
+  __device__ __forceinline__ int base(int k, int half) const {
+    return kP == 8 ? (lane + kG * k) * 8 + 4 * half : (lane + kG * (2 * k + half)) * 4;
+  }
+  template <bool kVec>
+  __device__ __forceinline__ bool has(int k, int j) const { return base(k, j >> 2) + (kVec ? 0 : (j & 3)) < C; }
+
+  // The lane's chunk k of the row at `row`, whose addresses are valid; absent columns read column 0.
+  template <int DT, bool kVec>
+  __device__ __forceinline__ RowChunk<DT> load(const uint8_t* row, int k) const {
+    constexpr int kB = ChunkElt<DT>::kBytes;
+    RowChunk<DT> r;
+    if constexpr (kVec && (kB == 4 || kP == 4)) {
+#pragma unroll
+      for (int q = 0; q < 2; ++q) {
+        const int col = base(k, q);
+        const uint8_t* p = row + (col < C ? (int64_t)col * kB : 0);
+        if constexpr (kB == 4) {
+          r.q[q] = __builtin_nontemporal_load(reinterpret_cast<const stream_u32x4*>(p));
+        } else {
+          const stream_u32x2 v = __builtin_nontemporal_load(reinterpret_cast<const stream_u32x2*>(p));
+          r.q[0][2 * q] = v[0];
+          r.q[0][2 * q + 1] = v[1];
+        }
+      }
+    } else if constexpr (kVec) {
+      const int col = base(k, 0);
+      r.q[0] = __builtin_nontemporal_load(reinterpret_cast<const stream_u32x4*>(row + (col < C ? (int64_t)col * kB : 0)));
+    } else {
+#pragma unroll
+      for (int j = 0; j < kChunkCols; ++j) {
+        const int at = base(k, j >> 2) + (j & 3), c = at < C ? at : 0;
+        if constexpr (kB == 4) {
+          r.q[j >> 2][j & 3] = reinterpret_cast<const uint32_t*>(row)[c];
+        } else {
+          const uint32_t v = reinterpret_cast<const uint16_t*>(row)[c];
+          r.q[0][j >> 1] = j & 1 ? r.q[0][j >> 1] | (v << 16) : v;
+        }
+      }
+    }
+    return r;
+  }
+
+  // Its values in fp32, zeros in absent columns and where the row is not there.
+  template <int DT, bool kVec>
+  __device__ __forceinline__ void values(const RowChunk<DT>& r, int k, bool there, float (&f)[kChunkCols]) const {
+#pragma unroll
+    for (int j = 0; j < kChunkCols; ++j) {
+      const float v = chunk_value<DT>(r, j);
+      f[j] = there && has<kVec>(k, j) ? v : 0.f;
+    }
+  }
+
+  // Stores chunk k, rounded once, into the row that begins `off` bytes into the descriptor's range.
+  template <int DT, bool kVec>
+  __device__ __forceinline__ void store(const float (&f)[kChunkCols], __amdgpu_buffer_rsrc_t out, uint32_t off, int k) const {
+    constexpr uint32_t kB = ChunkElt<DT>::kBytes;
+    if constexpr (kVec && kB == 2 && kP == 8) {
+      const int col = base(k, 0);
+      if (col < C)
+        stream_store_sc1(stream_u32x4{pack2<DT>(f[0], f[1]), pack2<DT>(f[2], f[3]), pack2<DT>(f[4], f[5]),
+                                      pack2<DT>(f[6], f[7])}, out, off + (uint32_t)col * kB);
+    } else if constexpr (kVec) {
+#pragma unroll
+      for (int q = 0; q < 2; ++q) {
+        const int col = base(k, q);
+        if (col >= C) continue;
+        if constexpr (kB == 4)
+          stream_store_sc1(stream_u32x4{__float_as_uint(f[4 * q]), __float_as_uint(f[4 * q + 1]), __float_as_uint(f[4 * q + 2]),
+                                        __float_as_uint(f[4 * q + 3])}, out, off + (uint32_t)col * kB);
+        else
+          stream_store_sc1(stream_u32x2{pack2<DT>(f[4 * q], f[4 * q + 1]), pack2<DT>(f[4 * q + 2], f[4 * q + 3])}, out,
+                           off + (uint32_t)col * kB);
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < kChunkCols; ++j) {
+        const int col = base(k, j >> 2) + (j & 3);
+        if (col >= C) continue;
+        if constexpr (kB == 4) stream_store_sc1(__float_as_uint(f[j]), out, off + (uint32_t)col * kB);
+        else stream_store_sc1((uint16_t)pack2<DT>(f[j], 0.f), out, off + (uint32_t)col * kB);
+      }
+    }
+  }
+
+  // The same into the row at `row`, a place of each row's own.
+  template <int DT, bool kVec>
+  __device__ __forceinline__ void store(const float (&f)[kChunkCols], uint8_t* row, int k) const {
+    constexpr int kB = ChunkElt<DT>::kBytes;
+    if constexpr (kVec && kB == 2 && kP == 8) {
+      const int col = base(k, 0);
+      if (col < C)
+        __builtin_nontemporal_store(stream_u32x4{pack2<DT>(f[0], f[1]), pack2<DT>(f[2], f[3]), pack2<DT>(f[4], f[5]),
+                                                 pack2<DT>(f[6], f[7])},
+                                    reinterpret_cast<stream_u32x4*>(row + (int64_t)col * kB));
+    } else if constexpr (kVec) {
+#pragma unroll
+      for (int q = 0; q < 2; ++q) {
+        const int col = base(k, q);
+        if (col >= C) continue;
+        if constexpr (kB == 4)
+          __builtin_nontemporal_store(stream_u32x4{__float_as_uint(f[4 * q]), __float_as_uint(f[4 * q + 1]),
+                                                   __float_as_uint(f[4 * q + 2]), __float_as_uint(f[4 * q + 3])},
+                                      reinterpret_cast<stream_u32x4*>(row + (int64_t)col * kB));
+        else
+          __builtin_nontemporal_store(stream_u32x2{pack2<DT>(f[4 * q], f[4 * q + 1]), pack2<DT>(f[4 * q + 2], f[4 * q + 3])},
+                                      reinterpret_cast<stream_u32x2*>(row + (int64_t)col * kB));
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < kChunkCols; ++j) {
+        const int col = base(k, j >> 2) + (j & 3);
+        if (col >= C) continue;
+        if constexpr (kB == 4) reinterpret_cast<float*>(row)[col] = f[j];
+        else reinterpret_cast<uint16_t*>(row)[col] = (uint16_t)pack2<DT>(f[j], 0.f);
+      }
+    }
+  }
+
+  // The draws of chunk k's eight values.  Where a chunk is two pieces, lanes 2i
+  // and 2i + 1 hold the halves of two chunks of the mask: the even lane
+  // draws the first, the odd one the second, and they swap halves.
+  __device__ __forceinline__ ChunkDraws draws(uint64_t seed, int k, uint32_t row, uint32_t stream) const {
+    if constexpr (kP == 8) {
+      return chunk_draws(seed, (uint32_t)(lane + kG * k), row, stream);
+    } else {
+      const bool odd = lane & 1;
+      const ChunkDraws d = chunk_draws(seed, (uint32_t)((lane >> 1) + kG * k + (odd ? kG / 2 : 0)), row, stream);
+      const uint32_t r0 = lane_xor1(odd ? d.w[0] : d.w[2]), r1 = lane_xor1(odd ? d.w[1] : d.w[3]);
+      return {{odd ? r0 : d.w[0], odd ? r1 : d.w[1], odd ? d.w[2] : r0, odd ? d.w[3] : r1}};
+    }
+  }
+};
+
+// The fewest idle lanes of one to three chunks a lane, and among those the most chunks: what a row costs beside its
+// values (addresses, sums over lanes, row tests) is paid once for all chunks of a lane.  From 129 chunks on a
+// workgroup holds the row.
 inline TailShape tail_shape(int C) {
   const int n = (C + kChunkCols - 1) / kChunkCols;
-  if (n <= 16) return {16, 1};
-  if (n <= 32) return {32, 1};
-  if (n <= 64) return {64, 1};
-  if (n <= 128) return {64, 2};
-  if (n <= 256) return {256, 1};
-  if (n <= 512) return {256, 2};
-  return {512, 2};
+  if (n > 512) return {512, 2};
+  if (n > 256) return {256, 2};
+  if (n > 128) return {256, 1};
+  TailShape best = {64, 2};
+  for (int k = 1; k <= 3; ++k)
+    for (int g = 8; g <= 64; g *= 2) {
+      if (g * k < n || (k == 3 && g == 64)) continue;
+      if (g * k <= best.lanes * best.chunks) best = {g, k};
+      break;
+    }
+  return best;
 }
 constexpr int kTailMaxChannels = 8192;
 
@@ -85,9 +234,9 @@ constexpr int tail_threads(int lanes) { return lanes > 256 ? lanes : 256; }
 
 // The statistics of a normalised row held as kK chunks a lane: v becomes
 // (v - mean) r (zero in absent columns), r is returned.
-template <int kG, int kK, bool kVec>
-__device__ __forceinline__ float normalise(float (&v)[kK][kChunkCols], int kind, float eps, float inv_c, int lane, int C,
-                                           RowSum<kG>& sum) {
+template <int kG, int kK, int kP, bool kVec>
+__device__ __forceinline__ float normalise(float (&v)[kK][kChunkCols], int kind, float eps, float inv_c,
+                                           const RowLanes<kG, kK, kP>& at, RowSum<kG>& sum) {
   if (kind == TERRA_NORM_LAYER) {
     float s = 0.f;
 #pragma unroll
@@ -96,11 +245,9 @@ __device__ __forceinline__ float normalise(float (&v)[kK][kChunkCols], int kind,
       for (int j = 0; j < kChunkCols; ++j) s += v[k][j];
     const float mean = sum.one(s) * inv_c;
 #pragma unroll
-    for (int k = 0; k < kK; ++k) {
-      const int col = (lane + kG * k) * kChunkCols;
+    for (int k = 0; k < kK; ++k)
 #pragma unroll
-      for (int j = 0; j < kChunkCols; ++j) v[k][j] = col + (kVec ? 0 : j) < C ? v[k][j] - mean : 0.f;
-    }
+      for (int j = 0; j < kChunkCols; ++j) v[k][j] = at.template has<kVec>(k, j) ? v[k][j] - mean : 0.f;
   }
   float q = 0.f;
 #pragma unroll
@@ -115,24 +262,87 @@ __device__ __forceinline__ float normalise(float (&v)[kK][kChunkCols], int kind,
   return r;
 }
 
-// Eight parameters of a chunk in fp32, `none` where the pointer is NULL and 0
-// in absent columns.
-template <bool kVec>
-__device__ __forceinline__ void load_params(const float* p, float none, int col, int C, float (&f)[kChunkCols]) {
-#pragma unroll
-  for (int j = 0; j < kChunkCols; ++j) f[j] = col + (kVec ? 0 : j) < C ? none : 0.f;
-  if (p == nullptr) return;
-  if constexpr (kVec) {
-    if (col < C) {
-      const float4 a = *reinterpret_cast<const float4*>(p + col), b = *reinterpret_cast<const float4*>(p + col + 4);
-      f[0] = a.x, f[1] = a.y, f[2] = a.z, f[3] = a.w, f[4] = b.x, f[5] = b.y, f[6] = b.z, f[7] = b.w;
-    }
-  } else {
-#pragma unroll
-    for (int j = 0; j < kChunkCols; ++j)
-      if (col + j < C) f[j] = p[col + j];
+// f<DTH, DTX, lanes, chunks>(...) for the shape at run time (inside a function
+// template over DTH and DTX).
+#define TERRA_TAIL_SHAPES(f, shape, ...)                                            \
+  switch ((shape).lanes * 10 + (shape).chunks) {                                    \
+    case 81: return f<DTH, DTX, 8, 1>(__VA_ARGS__);                                 \
+    case 82: return f<DTH, DTX, 8, 2>(__VA_ARGS__);                                 \
+    case 83: return f<DTH, DTX, 8, 3>(__VA_ARGS__);                                 \
+    case 162: return f<DTH, DTX, 16, 2>(__VA_ARGS__);                               \
+    case 163: return f<DTH, DTX, 16, 3>(__VA_ARGS__);                               \
+    case 322: return f<DTH, DTX, 32, 2>(__VA_ARGS__);                               \
+    case 323: return f<DTH, DTX, 32, 3>(__VA_ARGS__);                               \
+    case 642: return f<DTH, DTX, 64, 2>(__VA_ARGS__);                               \
+    case 2561: return f<DTH, DTX, 256, 1>(__VA_ARGS__);                             \
+    case 2562: return f<DTH, DTX, 256, 2>(__VA_ARGS__);                             \
+    default: return f<DTH, DTX, 512, 2>(__VA_ARGS__);                               \
   }
+
+// A parameter, `none` where the pointer is NULL.
+__device__ __forceinline__ float param_at(const float* p, float none, int c) { return p == nullptr ? none : p[c]; }
+
+// The branch's affine map with the gate and the dropout scale in it:
+//   gate * s * (nhat w + b) = nhat gw + gb
+__device__ __forceinline__ void branch_params(const TailArgs& a, const float* gate, int c, float& gw, float& gb) {
+  const float g = param_at(gate, 1.f, c) * (a.drop.threshold > 0 ? a.drop.scale : 1.f);
+  gw = g * param_at(a.pw, 1.f, c);
+  gb = g * param_at(a.pb, 0.f, c);
 }
+
+// Per-column parameters of a row's lanes: in LDS where rows share a workgroup
+// (kG <= 64), else, each lane's columns being its own, in registers.
+template <int kN, int kG, int kK, int kP>
+struct ColumnParams {
+  static constexpr bool kLds = kG <= 64;
+  static constexpr int kCols = kG * kK * kChunkCols, kThreads = tail_threads(kG);
+  struct Shared { __attribute__((aligned(16))) float v[kLds ? kN : 1][kLds ? kCols : 4]; };
+  Shared* s;
+  float r[kLds ? 1 : kN][kLds ? 1 : kK][kChunkCols];
+
+  __device__ __forceinline__ explicit ColumnParams(Shared* shared) : s(shared) {}
+
+  // f(column, out[kN]) for every column below C; 0 in absent ones.  With LDS the caller adds the barriers.
+  template <typename F>
+  __device__ __forceinline__ void fill(const RowLanes<kG, kK, kP>& at, F f) {
+    const int C = at.C;
+    if constexpr (kLds) {
+      for (int c = threadIdx.x; c < kCols; c += kThreads) {
+        float v[kN] = {};
+        if (c < C) f(c, v);
+#pragma unroll
+        for (int i = 0; i < kN; ++i) s->v[i][c] = v[i];
+      }
+    } else {
+#pragma unroll
+      for (int k = 0; k < kK; ++k)
+#pragma unroll
+        for (int j = 0; j < kChunkCols; ++j) {
+          const int c = at.base(k, j >> 2) + (j & 3);
+          float v[kN] = {};
+          if (c < C) f(c, v);
+#pragma unroll
+          for (int i = 0; i < kN; ++i) r[i][k][j] = v[i];
+        }
+    }
+  }
+  // At the top of a loop over rows: the parameters are read from LDS in each
+  // turn.  The compiler would otherwise hold all of them in registers over the
+  // loop, and the waves for which there is then no room are worth more.
+  __device__ __forceinline__ void stay() const {
+    if constexpr (kLds) asm volatile("" ::: "memory");
+  }
+  __device__ __forceinline__ void get(int i, int k, const RowLanes<kG, kK, kP>& at, float (&f)[kChunkCols]) const {
+    if constexpr (kLds) {
+      const float4 lo = *reinterpret_cast<const float4*>(&s->v[i][at.base(k, 0)]);
+      const float4 hi = *reinterpret_cast<const float4*>(&s->v[i][at.base(k, 1)]);
+      f[0] = lo.x, f[1] = lo.y, f[2] = lo.z, f[3] = lo.w, f[4] = hi.x, f[5] = hi.y, f[6] = hi.z, f[7] = hi.w;
+    } else {
+#pragma unroll
+      for (int j = 0; j < kChunkCols; ++j) f[j] = r[i][k][j];
+    }
+  }
+};
 
 }  // namespace
 

@@ -10,22 +10,23 @@ template <int DTH, int DTX, int kG, int kK, bool kVec>
 __global__ __launch_bounds__(tail_threads(kG)) void tail_kernel(const TailArgs a) {
   constexpr int kGroups = tail_threads(kG) / kG;
   constexpr int kHB = ChunkElt<DTH>::kBytes, kXB = ChunkElt<DTX>::kBytes;
+  constexpr int kP = DTX == TERRA_DTYPE_F32 ? 4 : 8;
+  using Params = ColumnParams<4, kG, kK, kP>;
   __shared__ typename RowSum<kG>::Shared s_red;
-  const int lane = threadIdx.x % kG, group = threadIdx.x / kG, C = a.C;
+  __shared__ typename Params::Shared s_par;
+  const int group = threadIdx.x / kG, C = a.C;
+  const RowLanes<kG, kK, kP> at = {(int)(threadIdx.x % kG), C};
   RowSum<kG> sum(&s_red);
-  // A lane's columns never change: their parameters stay in registers.
-  float pw[kK][kChunkCols], pb[kK][kChunkCols], gate[kK][kChunkCols], nw[kK][kChunkCols], nb[kK][kChunkCols];
-#pragma unroll
-  for (int k = 0; k < kK; ++k) {
-    const int col = (lane + kG * k) * kChunkCols;
-    load_params<kVec>(a.pw, 1.f, col, C, pw[k]);
-    load_params<kVec>(a.pb, 0.f, col, C, pb[k]);
-    load_params<kVec>(a.gate_rows == 1 ? a.gate : nullptr, 1.f, col, C, gate[k]);
-    load_params<kVec>(a.nw, 1.f, col, C, nw[k]);
-    load_params<kVec>(a.nb, 0.f, col, C, nb[k]);
-  }
+  Params par(&s_par);  // gw, gb (branch_params), nw, nb
+  par.fill(at, [&](int c, float (&v)[4]) {
+    branch_params(a, a.gate_rows == 1 ? a.gate : nullptr, c, v[0], v[1]);
+    v[2] = param_at(a.nw, 1.f, c);
+    v[3] = param_at(a.nb, 0.f, c);
+  });
+  if constexpr (Params::kLds) __syncthreads();
   const uint64_t seed = a.drop.threshold > 0 ? *a.drop.seed : 0;
   for (uint32_t base = blockIdx.x * kGroups; base < a.rows; base += gridDim.x * kGroups) {
+    par.stay();
     const uint32_t row = base + group;
     const bool live = row < a.rows;
     const uint32_t r = live ? row : a.rows - 1;  // a row past the end re-reads the last one
@@ -37,45 +38,54 @@ __global__ __launch_bounds__(tail_threads(kG)) void tail_kernel(const TailArgs a
     RowChunk<DTX> xq[kK];
 #pragma unroll
     for (int k = 0; k < kK; ++k) {
-      const int col = (lane + kG * k) * kChunkCols;
-      hq[k] = load_chunk<DTH, kVec>(hp, col, C, col < C);
-      xq[k] = load_chunk<DTX, kVec>(xp, col, C, col < C);
-      if (a.gate_rows > 1) load_params<kVec>(a.gate + (int64_t)(r / a.per_sample) * C, 1.f, col, C, gate[k]);
+      hq[k] = at.template load<DTH, kVec>(hp, k);
+      xq[k] = at.template load<DTX, kVec>(xp, k);
     }
     float v[kK][kChunkCols];
 #pragma unroll
     for (int k = 0; k < kK; ++k) {
-      const int col = (lane + kG * k) * kChunkCols;
-      unpack<DTH, kVec>(hq[k], v[k], col, C, has && col < C);
+      at.template values<DTH, kVec>(hq[k], k, has, v[k]);
     }
-    if (a.post != TERRA_NORM_NONE) normalise<kG, kK, kVec>(v, a.post, a.post_eps, a.inv_c, lane, C, sum);
+    if (a.post != TERRA_NORM_NONE) normalise<kG, kK, kP, kVec>(v, a.post, a.post_eps, a.inv_c, at, sum);
     const uint32_t live_rows = min(a.rows - base, (uint32_t)kGroups);
     const __amdgpu_buffer_rsrc_t y_out = buffer_rsrc(a.y + (int64_t)base * C * kXB, live_rows * (uint32_t)(C * kXB));
 #pragma unroll
     for (int k = 0; k < kK; ++k) {
-      const int col = (lane + kG * k) * kChunkCols;
-      float xv[kChunkCols];
-      unpack<DTX, kVec>(xq[k], xv, col, C, col < C);
+      float gw[kChunkCols], gb[kChunkCols], xv[kChunkCols];
+      par.get(0, k, at, gw);
+      par.get(1, k, at, gb);
+      if (a.gate_rows > 1) {  // this row's sample's gate
+        const float* gate = a.gate + (int64_t)(r / a.per_sample) * C;
 #pragma unroll
-      for (int j = 0; j < kChunkCols; ++j) v[k][j] = has ? fmaf(v[k][j], pw[k][j], pb[k][j]) : 0.f;
+        for (int j = 0; j < kChunkCols; ++j) {
+          const float g = at.template has<kVec>(k, j) ? gate[at.base(k, j >> 2) + (j & 3)] : 0.f;
+          gw[j] *= g;
+          gb[j] *= g;
+        }
+      }
+      at.template values<DTX, kVec>(xq[k], k, true, xv);
+#pragma unroll
+      for (int j = 0; j < kChunkCols; ++j) v[k][j] = has ? fmaf(v[k][j], gw[j], gb[j]) : 0.f;
       if (a.drop.threshold > 0) {
-        const ChunkDraws d = chunk_draws(seed, (uint32_t)(lane + kG * k), r, a.drop.stream);
+        const ChunkDraws d = at.draws(seed, k, r, a.drop.stream);
 #pragma unroll
-        for (int j = 0; j < kChunkCols; ++j) v[k][j] = kept(d, j, a.drop.threshold) ? v[k][j] * a.drop.scale : 0.f;
+        for (int j = 0; j < kChunkCols; ++j) v[k][j] = kept(d, j, a.drop.threshold) ? v[k][j] : 0.f;
       }
 #pragma unroll
-      for (int j = 0; j < kChunkCols; ++j) v[k][j] = fmaf(a.alpha, xv[j], gate[k][j] * v[k][j]);
-      if (live && col < C) store_chunk<DTX, kVec>(v[k], y_out, (uint32_t)(group * C + col) * kXB, col, C);
+      for (int j = 0; j < kChunkCols; ++j) v[k][j] = fmaf(a.alpha, xv[j], v[k][j]);
+      if (live) at.template store<DTX, kVec>(v[k], y_out, (uint32_t)(group * C) * kXB, k);
     }
     if (a.next != TERRA_NORM_NONE) {
-      normalise<kG, kK, kVec>(v, a.next, a.next_eps, a.inv_c, lane, C, sum);
+      normalise<kG, kK, kP, kVec>(v, a.next, a.next_eps, a.inv_c, at, sum);
       const __amdgpu_buffer_rsrc_t z_out = buffer_rsrc(a.z + (int64_t)base * C * kHB, live_rows * (uint32_t)(C * kHB));
 #pragma unroll
       for (int k = 0; k < kK; ++k) {
-        const int col = (lane + kG * k) * kChunkCols;
+        float w[kChunkCols], b[kChunkCols];
+        par.get(2, k, at, w);
+        par.get(3, k, at, b);
 #pragma unroll
-        for (int j = 0; j < kChunkCols; ++j) v[k][j] = fmaf(v[k][j], nw[k][j], nb[k][j]);
-        if (live && col < C) store_chunk<DTH, kVec>(v[k], z_out, (uint32_t)(group * C + col) * kHB, col, C);
+        for (int j = 0; j < kChunkCols; ++j) v[k][j] = fmaf(v[k][j], w[j], b[j]);
+        if (live) at.template store<DTH, kVec>(v[k], z_out, (uint32_t)(group * C) * kHB, k);
       }
     }
   }
@@ -93,16 +103,7 @@ void launch(const TailArgs& a, bool vec, hipStream_t s) {
 
 template <int DTH, int DTX>
 void dispatch(const TailArgs& a, bool vec, hipStream_t s) {
-  const TailShape t = tail_shape(a.C);
-  switch (t.lanes * 10 + t.chunks) {
-    case 161: return launch<DTH, DTX, 16, 1>(a, vec, s);
-    case 321: return launch<DTH, DTX, 32, 1>(a, vec, s);
-    case 641: return launch<DTH, DTX, 64, 1>(a, vec, s);
-    case 642: return launch<DTH, DTX, 64, 2>(a, vec, s);
-    case 2561: return launch<DTH, DTX, 256, 1>(a, vec, s);
-    case 2562: return launch<DTH, DTX, 256, 2>(a, vec, s);
-    default: return launch<DTH, DTX, 512, 2>(a, vec, s);
-  }
+  TERRA_TAIL_SHAPES(launch, tail_shape(a.C), a, vec, s);
 }
 
 // A tensor of the call: how far it reaches, for the overlap checks.
@@ -335,6 +336,7 @@ extern "C" int terra_swin_residual_norm_bwd(const void* h, const void* x, const 
   a.slab_rows = p.slab_rows;
   a.units = p.units;
   a.partial = sums ? workspace : nullptr;
+  a.branch_sums = dpost_weight != nullptr || dpost_bias != nullptr || dgate != nullptr;
   // One slab a sample: the unit's sums are the gate's gradient itself.
   const bool direct = dgate != nullptr && p.slabs == 1;
   float* units = workspace + (int64_t)p.blocks * 4 * C;

@@ -1,21 +1,25 @@
 // Backward of the end of a half-block (residual_norm.h), from the gradients
 // of y and z.  No statistic, mask or intermediate of the forward is kept: each
-// row is recomputed from h and x in registers, and then
+// row is recomputed from h and x in registers, and then, with gw = gate s w1
+// and gb = gate s b1 (branch_params),
 //
+//   y  = alpha x + keep (nhat gw + gb)
 //   g  = dz w2,  dY = dy + r2 (g - mean g - yhat mean(g yhat)),  dx = alpha dY
-//   dgate += dY m,  dn = keep s gate dY
-//   u  = dn w1,  dh = r1 (u - mean u - nhat mean(u nhat))
-//   dw2 += dz yhat,  db2 += dz,  dw1 += dn nhat,  db1 += dn
+//   t  = keep dY,  u = t gw,  dh = r1 (u - mean u - nhat mean(u nhat))
+//   dw2 = sum dz yhat,  db2 = sum dz
 //
-// (an RMS norm has no mean g and mean u term; without a norm dY = dy, dh = dn).
+// (an RMS norm has no mean g and mean u term; without a norm dY = dy, dh = u).
+// The branch's three parameter gradients are two sums over the rows that share
+// a gate, A = s sum t nhat and B = s sum t:
+//   dgate = w1 A + b1 B,  dw1 = sum over gates of gate A,  db1 = ... gate B
+// which spares the rows' loop a sum, the value m and a product per element.
 // Bound by memory: h, x, dy, dz read once, dh and dx written once.
 //
 // Sums over rows: a unit is up to slab_rows consecutive rows of one sample,
 // workgroups take units in grid strides, and each lane keeps the sums of its
-// columns in registers over all of them; the gate's are written out unit by
-// unit, since its row changes with the sample.  A second launch adds the
-// workgroups' sums (sum_partials_kernel): no atomics, an order that the sizes
-// fix.
+// columns in registers; A and B leave them unit by unit, since the gate changes
+// with the sample.  A second launch adds the workgroups' sums
+// (sum_partials_kernel): no atomics, an order that the sizes fix.
 #include "residual_norm.h"
 
 namespace terra {
@@ -25,79 +29,80 @@ template <int DTH, int DTX, int kG, int kK, bool kVec>
 __global__ __launch_bounds__(tail_threads(kG)) void tail_bwd_kernel(const TailArgs a) {
   constexpr int kThreads = tail_threads(kG), kGroups = kThreads / kG, kCols = kG * kK * kChunkCols;
   constexpr int kHB = ChunkElt<DTH>::kBytes, kXB = ChunkElt<DTX>::kBytes;
-  // w1, b1, gate, w2 of the lane's columns: in LDS where several rows share a
-  // workgroup, in registers where each lane's columns are its own.
-  constexpr bool kLds = kG <= 64;
+  constexpr int kP = DTX == TERRA_DTYPE_F32 ? 4 : 8;
+  using Params = ColumnParams<3, kG, kK, kP>;
   __shared__ typename RowSum<kG>::Shared s_red;
-  __shared__ __attribute__((aligned(16))) float s_par[kLds ? 4 : 1][kLds ? kCols : 1];
+  __shared__ typename Params::Shared s_par;
   __shared__ __attribute__((aligned(16))) float s_acc[kGroups > 1 ? kGroups * kCols : 1];
-  float r_par[4][kLds ? 1 : kK][kChunkCols];
-  const int lane = threadIdx.x % kG, group = threadIdx.x / kG, C = a.C;
+  const int group = threadIdx.x / kG, C = a.C;
+  const RowLanes<kG, kK, kP> at = {(int)(threadIdx.x % kG), C};
   RowSum<kG> sum(&s_red);
-
-  auto stage = [&](int which, const float* p, float none) {
-    if constexpr (kLds) {
-      for (int c = threadIdx.x; c < kCols; c += kThreads) s_par[which][c] = c >= C ? 0.f : (p == nullptr ? none : p[c]);
-    } else {
-#pragma unroll
-      for (int k = 0; k < kK; ++k) load_params<kVec>(p, none, (lane + kG * k) * kChunkCols, C, r_par[which][k]);
-    }
+  Params par(&s_par);  // gw, gb, w2
+  auto stage = [&](const float* gate) {
+    par.fill(at, [&](int c, float (&v)[3]) {
+      branch_params(a, gate, c, v[0], v[1]);
+      v[2] = param_at(a.nw, 1.f, c);
+    });
   };
-  auto param = [&](int which, int k, float (&f)[kChunkCols]) {
-    if constexpr (kLds) {
-      const float4* p = reinterpret_cast<const float4*>(&s_par[which][(lane + kG * k) * kChunkCols]);
-      const float4 lo = p[0], hi = p[1];
-      f[0] = lo.x, f[1] = lo.y, f[2] = lo.z, f[3] = lo.w, f[4] = hi.x, f[5] = hi.y, f[6] = hi.z, f[7] = hi.w;
-    } else {
-#pragma unroll
-      for (int j = 0; j < kChunkCols; ++j) f[j] = r_par[which][k][j];
-    }
-  };
-  stage(0, a.pw, 1.f);
-  stage(1, a.pb, 0.f);
-  stage(2, a.gate_rows == 1 ? a.gate : nullptr, 1.f);
-  stage(3, a.nw, 1.f);
-  __syncthreads();
+  stage(a.gate_rows == 1 ? a.gate : nullptr);
+  if constexpr (Params::kLds) __syncthreads();
   const uint64_t seed = a.drop.threshold > 0 ? *a.drop.seed : 0;
 
-  float acc_pw[kK][kChunkCols] = {}, acc_pb[kK][kChunkCols] = {}, acc_gate[kK][kChunkCols] = {};
-  float acc_nw[kK][kChunkCols] = {}, acc_nb[kK][kChunkCols] = {};
-  // The workgroup's sums of one vector: over its row groups, then to dst [C].
-  auto flush = [&](float (&acc)[kK][kChunkCols], float* dst) {
+  float acc_a[kK][kChunkCols] = {}, acc_b[kK][kChunkCols] = {}, acc_nw[kK][kChunkCols] = {}, acc_nb[kK][kChunkCols] = {};
+  // The workgroup's sums of two vectors over its row groups, given to f(column, sum, other).
+  constexpr int kOwn = (kCols + kThreads - 1) / kThreads;
+  auto flush = [&](float (&p)[kK][kChunkCols], float (&q)[kK][kChunkCols], auto f) {
     if constexpr (kGroups > 1) {
+      float own[2][kOwn];
 #pragma unroll
-      for (int k = 0; k < kK; ++k)
+      for (int which = 0; which < 2; ++which) {
 #pragma unroll
-        for (int j = 0; j < kChunkCols; ++j) s_acc[group * kCols + (lane + kG * k) * kChunkCols + j] = acc[k][j];
-      __syncthreads();
-      for (int c = threadIdx.x; c < C; c += kThreads) {
-        float t = 0.f;
+        for (int k = 0; k < kK; ++k) {
+          const float* v = which == 0 ? p[k] : q[k];
+          *reinterpret_cast<float4*>(&s_acc[group * kCols + at.base(k, 0)]) = make_float4(v[0], v[1], v[2], v[3]);
+          *reinterpret_cast<float4*>(&s_acc[group * kCols + at.base(k, 1)]) = make_float4(v[4], v[5], v[6], v[7]);
+        }
+        __syncthreads();
 #pragma unroll
-        for (int g = 0; g < kGroups; ++g) t += s_acc[g * kCols + c];
-        dst[c] = t;
+        for (int i = 0; i < kOwn; ++i) {
+          const int c = threadIdx.x + i * kThreads;
+          float t = 0.f;
+          if (c < kCols)
+#pragma unroll
+            for (int g = 0; g < kGroups; ++g) t += s_acc[g * kCols + c];
+          own[which][i] = t;
+        }
+        __syncthreads();
       }
-      __syncthreads();
+#pragma unroll
+      for (int i = 0; i < kOwn; ++i) {
+        const int c = threadIdx.x + i * kThreads;
+        if (c < C) f(c, own[0][i], own[1][i]);
+      }
     } else {
 #pragma unroll
       for (int k = 0; k < kK; ++k)
 #pragma unroll
         for (int j = 0; j < kChunkCols; ++j) {
-          const int c = (lane + kG * k) * kChunkCols + j;
-          if (c < C) dst[c] = acc[k][j];
+          const int c = at.base(k, j >> 2) + (j & 3);
+          if (c < C) f(c, p[k][j], q[k][j]);
         }
     }
   };
+  float* const mine = a.partial != nullptr ? a.partial + (int64_t)blockIdx.x * 4 * C : nullptr;
 
   for (uint32_t unit = blockIdx.x; unit < a.units; unit += gridDim.x) {
     const uint32_t sample = unit / a.slabs, slab = unit % a.slabs;
     const uint32_t begin = sample * a.per_sample + slab * a.slab_rows;
     const uint32_t end = min(begin + a.slab_rows, (sample + 1) * a.per_sample);
+    const float* const gate = a.gate_rows > 0 ? a.gate + (int64_t)sample * C : nullptr;
     if (a.gate_rows > 1) {
-      __syncthreads();
-      stage(2, a.gate + (int64_t)sample * C, 1.f);
-      __syncthreads();
+      if constexpr (Params::kLds) __syncthreads();
+      stage(gate);
+      if constexpr (Params::kLds) __syncthreads();
     }
     for (uint32_t base = begin; base < end; base += kGroups) {
+      par.stay();
       const uint32_t row = base + group;
       const bool live = row < end;
       const uint32_t r = live ? row : end - 1;  // a row past the end re-reads the unit's last one
@@ -111,158 +116,157 @@ __global__ __launch_bounds__(tail_threads(kG)) void tail_bwd_kernel(const TailAr
       const uint8_t* dzp = a.dz != nullptr ? a.dz + (int64_t)r * C * kHB : hp;
 #pragma unroll
       for (int k = 0; k < kK; ++k) {
-        const int col = (lane + kG * k) * kChunkCols;
-        const bool in = col < C;
-        hq[k] = load_chunk<DTH, kVec>(hp, col, C, in);
-        xq[k] = load_chunk<DTX, kVec>(xp, col, C, in);
-        dyq[k] = load_chunk<DTX, kVec>(dyp, col, C, in);
-        dzq[k] = load_chunk<DTH, kVec>(dzp, col, C, in);
+        hq[k] = at.template load<DTH, kVec>(hp, k);
+        xq[k] = at.template load<DTX, kVec>(xp, k);
+        dzq[k] = at.template load<DTH, kVec>(dzp, k);
+        dyq[k] = at.template load<DTX, kVec>(dyp, k);
       }
-      // The forward: nhat in nv, m, and yhat in yv.
-      float nv[kK][kChunkCols], m[kK][kChunkCols], yv[kK][kChunkCols];
+      // The forward: nhat in nv, y in yv.
+      float nv[kK][kChunkCols], yv[kK][kChunkCols], dv[kK][kChunkCols];
       ChunkDraws draws[kK];
 #pragma unroll
       for (int k = 0; k < kK; ++k) {
-        const int col = (lane + kG * k) * kChunkCols;
-        unpack<DTH, kVec>(hq[k], nv[k], col, C, has && col < C);
+        at.template values<DTH, kVec>(hq[k], k, has, nv[k]);
       }
-      float r1 = 1.f, r2 = 1.f;
-      if (a.post != TERRA_NORM_NONE) r1 = normalise<kG, kK, kVec>(nv, a.post, a.post_eps, a.inv_c, lane, C, sum);
-#pragma unroll
-      for (int k = 0; k < kK; ++k) {
-        const int col = (lane + kG * k) * kChunkCols;
-        float w[kChunkCols], b[kChunkCols], g[kChunkCols], xv[kChunkCols];
-        param(0, k, w);
-        param(1, k, b);
-        param(2, k, g);
-        unpack<DTX, kVec>(xq[k], xv, col, C, col < C);
-#pragma unroll
-        for (int j = 0; j < kChunkCols; ++j) m[k][j] = has ? fmaf(nv[k][j], w[j], b[j]) : 0.f;
-        if (a.drop.threshold > 0) {
-          draws[k] = chunk_draws(seed, (uint32_t)(lane + kG * k), r, a.drop.stream);
-#pragma unroll
-          for (int j = 0; j < kChunkCols; ++j) m[k][j] = kept(draws[k], j, a.drop.threshold) ? m[k][j] * a.drop.scale : 0.f;
-        }
-#pragma unroll
-        for (int j = 0; j < kChunkCols; ++j) yv[k][j] = fmaf(a.alpha, xv[j], g[j] * m[k][j]);
-      }
-      // dY in dv.
-      float dv[kK][kChunkCols];
-#pragma unroll
-      for (int k = 0; k < kK; ++k) {
-        const int col = (lane + kG * k) * kChunkCols;
-        unpack<DTX, kVec>(dyq[k], dv[k], col, C, a.dy != nullptr && col < C);
-      }
-      if (a.next != TERRA_NORM_NONE && a.dz != nullptr) {
-        r2 = normalise<kG, kK, kVec>(yv, a.next, a.next_eps, a.inv_c, lane, C, sum);
-        float s0 = 0.f, s1 = 0.f;
-        float gv[kK][kChunkCols];
+      float r1 = 1.f;
+      if (a.post != TERRA_NORM_NONE) r1 = normalise<kG, kK, kP, kVec>(nv, a.post, a.post_eps, a.inv_c, at, sum);
+      if (a.drop.threshold > 0)
 #pragma unroll
         for (int k = 0; k < kK; ++k) {
-          const int col = (lane + kG * k) * kChunkCols;
+          draws[k] = at.draws(seed, k, r, a.drop.stream);
+          // NaN and infinities of the branch stay out of A where they are dropped.
+          if (a.post == TERRA_NORM_NONE)
+#pragma unroll
+            for (int j = 0; j < kChunkCols; ++j) nv[k][j] = kept(draws[k], j, a.drop.threshold) ? nv[k][j] : 0.f;
+        }
+      if (a.next != TERRA_NORM_NONE && a.dz != nullptr) {
+#pragma unroll
+        for (int k = 0; k < kK; ++k) {
+          float gw[kChunkCols], gb[kChunkCols], xv[kChunkCols];
+          par.get(0, k, at, gw);
+          par.get(1, k, at, gb);
+          at.template values<DTX, kVec>(xq[k], k, true, xv);
+#pragma unroll
+          for (int j = 0; j < kChunkCols; ++j) yv[k][j] = has ? fmaf(nv[k][j], gw[j], gb[j]) : 0.f;
+          if (a.drop.threshold > 0)
+#pragma unroll
+            for (int j = 0; j < kChunkCols; ++j) yv[k][j] = kept(draws[k], j, a.drop.threshold) ? yv[k][j] : 0.f;
+#pragma unroll
+          for (int j = 0; j < kChunkCols; ++j) yv[k][j] = fmaf(a.alpha, xv[j], yv[k][j]);
+        }
+        const float r2 = normalise<kG, kK, kP, kVec>(yv, a.next, a.next_eps, a.inv_c, at, sum);
+        float s0 = 0.f, s1 = 0.f;
+#pragma unroll
+        for (int k = 0; k < kK; ++k) {
           float w[kChunkCols];
-          param(3, k, w);
-          unpack<DTH, kVec>(dzq[k], gv[k], col, C, live && col < C);
+          par.get(2, k, at, w);
+          at.template values<DTH, kVec>(dzq[k], k, true, dv[k]);
+          if (live)
+#pragma unroll
+            for (int j = 0; j < kChunkCols; ++j) {
+              acc_nw[k][j] = fmaf(dv[k][j], yv[k][j], acc_nw[k][j]);
+              acc_nb[k][j] += dv[k][j];
+            }
 #pragma unroll
           for (int j = 0; j < kChunkCols; ++j) {
-            if (live) acc_nw[k][j] = fmaf(gv[k][j], yv[k][j], acc_nw[k][j]);
-            acc_nb[k][j] += gv[k][j];
-            gv[k][j] *= w[j];
-            s0 += gv[k][j];
-            s1 = fmaf(gv[k][j], yv[k][j], s1);
+            dv[k][j] *= w[j];
+            s0 += dv[k][j];
+            s1 = fmaf(dv[k][j], yv[k][j], s1);
           }
         }
         sum.two(s0, s1);
         s0 = a.next == TERRA_NORM_LAYER ? s0 * a.inv_c : 0.f;
         s1 *= a.inv_c;
 #pragma unroll
-        for (int k = 0; k < kK; ++k)
+        for (int k = 0; k < kK; ++k) {
+          float dyv[kChunkCols];
+          at.template values<DTX, kVec>(dyq[k], k, a.dy != nullptr, dyv);
 #pragma unroll
-          for (int j = 0; j < kChunkCols; ++j) dv[k][j] += r2 * (gv[k][j] - s0 - yv[k][j] * s1);
-      }
-      // dx, the gate's gradient, and dn in dv.
-      const __amdgpu_buffer_rsrc_t dx_out =
-          buffer_rsrc(a.dx + (int64_t)base * C * kXB, min(end - base, (uint32_t)kGroups) * (uint32_t)(C * kXB));
-#pragma unroll
-      for (int k = 0; k < kK; ++k) {
-        const int col = (lane + kG * k) * kChunkCols;
-        float g[kChunkCols], dxv[kChunkCols];
-        param(2, k, g);
-#pragma unroll
-        for (int j = 0; j < kChunkCols; ++j) dxv[j] = a.alpha * dv[k][j];
-        if (live && col < C) store_chunk<DTX, kVec>(dxv, dx_out, (uint32_t)(group * C + col) * kXB, col, C);
-#pragma unroll
-        for (int j = 0; j < kChunkCols; ++j) {
-          if (live && has) acc_gate[k][j] = fmaf(dv[k][j], m[k][j], acc_gate[k][j]);
-          dv[k][j] *= g[j];
+          for (int j = 0; j < kChunkCols; ++j) dv[k][j] = fmaf(r2, fmaf(-yv[k][j], s1, dv[k][j] - s0), dyv[j]);
         }
-        if (a.drop.threshold > 0)
-#pragma unroll
-          for (int j = 0; j < kChunkCols; ++j)
-            dv[k][j] = kept(draws[k], j, a.drop.threshold) ? dv[k][j] * a.drop.scale : 0.f;
-      }
-      if (a.post != TERRA_NORM_NONE) {
-        float s0 = 0.f, s1 = 0.f;
+      } else {
 #pragma unroll
         for (int k = 0; k < kK; ++k) {
-          float w[kChunkCols];
-          param(0, k, w);
+          at.template values<DTX, kVec>(dyq[k], k, a.dy != nullptr, dv[k]);
+        }
+      }
+      // dv is dY: dx, then t, A and B, then u in dv.
+      const __amdgpu_buffer_rsrc_t dx_out =
+          buffer_rsrc(a.dx + (int64_t)base * C * kXB, min(end - base, (uint32_t)kGroups) * (uint32_t)(C * kXB));
+      float s0 = 0.f, s1 = 0.f;
+#pragma unroll
+      for (int k = 0; k < kK; ++k) {
+        float out[kChunkCols], gw[kChunkCols];
+#pragma unroll
+        for (int j = 0; j < kChunkCols; ++j) out[j] = a.alpha * dv[k][j];
+        if (live) at.template store<DTX, kVec>(out, dx_out, (uint32_t)(group * C) * kXB, k);
+        if (a.drop.threshold > 0)
+#pragma unroll
+          for (int j = 0; j < kChunkCols; ++j) dv[k][j] = kept(draws[k], j, a.drop.threshold) ? dv[k][j] : 0.f;
+        if (live && has)
 #pragma unroll
           for (int j = 0; j < kChunkCols; ++j) {
-            if (live && has) {
-              acc_pw[k][j] = fmaf(dv[k][j], nv[k][j], acc_pw[k][j]);
-              acc_pb[k][j] += dv[k][j];
-            }
-            dv[k][j] *= w[j];
-            s0 += dv[k][j];
-            s1 = fmaf(dv[k][j], nv[k][j], s1);
+            acc_a[k][j] = fmaf(dv[k][j], nv[k][j], acc_a[k][j]);
+            acc_b[k][j] += dv[k][j];
           }
+        par.get(0, k, at, gw);
+#pragma unroll
+        for (int j = 0; j < kChunkCols; ++j) {
+          dv[k][j] *= gw[j];
+          s0 += dv[k][j];
+          s1 = fmaf(dv[k][j], nv[k][j], s1);
         }
+      }
+      if (a.post != TERRA_NORM_NONE) {
         sum.two(s0, s1);
         s0 = a.post == TERRA_NORM_LAYER ? s0 * a.inv_c : 0.f;
         s1 *= a.inv_c;
 #pragma unroll
         for (int k = 0; k < kK; ++k)
 #pragma unroll
-          for (int j = 0; j < kChunkCols; ++j) dv[k][j] = r1 * (dv[k][j] - s0 - nv[k][j] * s1);
+          for (int j = 0; j < kChunkCols; ++j) dv[k][j] = r1 * fmaf(-nv[k][j], s1, dv[k][j] - s0);
       }
       // In window order each row has a place of its own: a descriptor for it
-      // would not be uniform over the wave's rows, so these bounds are the row's.
+      // would not be uniform over the wave's rows.
       if (a.windows) {
 #pragma unroll
         for (int k = 0; k < kK; ++k) {
-          const int col = (lane + kG * k) * kChunkCols;
-          if (live && has && col < C) store_row<DTH, kVec>(dv[k], a.dh + src * C * kHB, col, C);
+          if (live && has) at.template store<DTH, kVec>(dv[k], a.dh + src * C * kHB, k);
         }
       } else {
         const __amdgpu_buffer_rsrc_t dh_out =
             buffer_rsrc(a.dh + (int64_t)base * C * kHB, min(end - base, (uint32_t)kGroups) * (uint32_t)(C * kHB));
 #pragma unroll
         for (int k = 0; k < kK; ++k) {
-          const int col = (lane + kG * k) * kChunkCols;
-          if (live && col < C) store_chunk<DTH, kVec>(dv[k], dh_out, (uint32_t)(group * C + col) * kHB, col, C);
+          if (live) at.template store<DTH, kVec>(dv[k], dh_out, (uint32_t)(group * C) * kHB, k);
         }
       }
     }
-    if (a.gate_partial != nullptr) {
-      flush(acc_gate, a.gate_partial + (int64_t)unit * C);
+    if (a.branch_sums) {
+      const float scale = a.drop.threshold > 0 ? a.drop.scale : 1.f;
+      const bool first = unit == blockIdx.x;
+      flush(acc_a, acc_b, [&](int c, float sa, float sb) {
+        sa *= scale;
+        sb *= scale;
+        if (a.gate_partial != nullptr)
+          a.gate_partial[(int64_t)unit * C + c] = fmaf(param_at(a.pw, 1.f, c), sa, param_at(a.pb, 0.f, c) * sb);
+        if (mine != nullptr) {
+          const float g = param_at(gate, 1.f, c);
+          mine[c] = fmaf(g, sa, first ? 0.f : mine[c]);
+          mine[C + c] = fmaf(g, sb, first ? 0.f : mine[C + c]);
+        }
+      });
 #pragma unroll
       for (int k = 0; k < kK; ++k)
 #pragma unroll
-        for (int j = 0; j < kChunkCols; ++j) acc_gate[k][j] = 0.f;
+        for (int j = 0; j < kChunkCols; ++j) acc_a[k][j] = acc_b[k][j] = 0.f;
     }
   }
-  if (a.partial != nullptr) {
-    float* dst = a.partial + (int64_t)blockIdx.x * 4 * C;
-    if (a.post != TERRA_NORM_NONE) {
-      flush(acc_pw, dst);
-      flush(acc_pb, dst + C);
-    }
-    if (a.next != TERRA_NORM_NONE) {
-      flush(acc_nw, dst + 2 * (int64_t)C);
-      flush(acc_nb, dst + 3 * (int64_t)C);
-    }
-  }
+  if (mine != nullptr && a.next != TERRA_NORM_NONE)
+    flush(acc_nw, acc_nb, [&](int c, float sw, float sb) {
+      mine[2 * C + c] = sw;
+      mine[3 * C + c] = sb;
+    });
 }
 
 template <int DTH, int DTX, int kG, int kK>
@@ -273,15 +277,7 @@ void launch(const TailArgs& a, const TailBwdPlan& p, bool vec, hipStream_t s) {
 
 template <int DTH, int DTX>
 void dispatch(const TailArgs& a, const TailBwdPlan& p, bool vec, hipStream_t s) {
-  switch (p.shape.lanes * 10 + p.shape.chunks) {
-    case 161: return launch<DTH, DTX, 16, 1>(a, p, vec, s);
-    case 321: return launch<DTH, DTX, 32, 1>(a, p, vec, s);
-    case 641: return launch<DTH, DTX, 64, 1>(a, p, vec, s);
-    case 642: return launch<DTH, DTX, 64, 2>(a, p, vec, s);
-    case 2561: return launch<DTH, DTX, 256, 1>(a, p, vec, s);
-    case 2562: return launch<DTH, DTX, 256, 2>(a, p, vec, s);
-    default: return launch<DTH, DTX, 512, 2>(a, p, vec, s);
-  }
+  TERRA_TAIL_SHAPES(launch, p.shape, a, p, vec, s);
 }
 
 }  // namespace

@@ -52,22 +52,13 @@ __device__ __forceinline__ RowChunk<DT> load_chunk(const uint8_t* row, int col, 
   return r;
 }
 
-// The chunk's values in fp32; zeros where it is not present and, without
-// kVec, from column C on.
-template <int DT, bool kVec>
-__device__ __forceinline__ void unpack(const RowChunk<DT>& r, float (&f)[kChunkCols], int col, int C, bool present) {
-#pragma unroll
-  for (int j = 0; j < kChunkCols; ++j) {
-    float v;
-    if constexpr (DT == TERRA_DTYPE_F32) {
-      v = __uint_as_float(r.q[j >> 2][j & 3]);
-    } else {
-      const uint32_t w = r.q[0][j >> 1];
-      if constexpr (DT == TERRA_DTYPE_BF16) v = __uint_as_float(j & 1 ? w & 0xffff0000u : w << 16);
-      else v = __half2float(__ushort_as_half((uint16_t)(j & 1 ? w >> 16 : w & 0xffffu)));
-    }
-    f[j] = present && (kVec || col + j < C) ? v : 0.f;
-  }
+// Value j of a chunk in fp32.
+template <int DT>
+__device__ __forceinline__ float chunk_value(const RowChunk<DT>& r, int j) {
+  if constexpr (DT == TERRA_DTYPE_F32) return __uint_as_float(r.q[j >> 2][j & 3]);
+  const uint32_t w = r.q[0][j >> 1];
+  if constexpr (DT == TERRA_DTYPE_BF16) return __uint_as_float(j & 1 ? w & 0xffff0000u : w << 16);
+  return __half2float(__ushort_as_half((uint16_t)(j & 1 ? w >> 16 : w & 0xffffu)));
 }
 
 typedef __bf16 chunk_bf16x2 __attribute__((ext_vector_type(2)));
@@ -106,30 +97,6 @@ __device__ __forceinline__ void store_chunk(const float (&f)[kChunkCols], __amdg
       if (col + j >= C) break;
       if constexpr (DT == TERRA_DTYPE_F32) stream_store_sc1(__float_as_uint(f[j]), out, off + 4 * j);
       else stream_store_sc1((uint16_t)pack2<DT>(f[j], 0.f), out, off + 2 * j);
-    }
-  }
-}
-
-// The chunk's values stored at its columns of the row at `row`, rounded once.
-template <int DT, bool kVec>
-__device__ __forceinline__ void store_row(const float (&f)[kChunkCols], uint8_t* row, int col, int C) {
-  if constexpr (kVec) {
-    stream_u32x4* p = reinterpret_cast<stream_u32x4*>(row + (int64_t)col * ChunkElt<DT>::kBytes);
-    if constexpr (DT == TERRA_DTYPE_F32) {
-      __builtin_nontemporal_store(stream_u32x4{__float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]),
-                                               __float_as_uint(f[3])}, p);
-      __builtin_nontemporal_store(stream_u32x4{__float_as_uint(f[4]), __float_as_uint(f[5]), __float_as_uint(f[6]),
-                                               __float_as_uint(f[7])}, p + 1);
-    } else {
-      __builtin_nontemporal_store(stream_u32x4{pack2<DT>(f[0], f[1]), pack2<DT>(f[2], f[3]), pack2<DT>(f[4], f[5]),
-                                               pack2<DT>(f[6], f[7])}, p);
-    }
-  } else {
-#pragma unroll
-    for (int j = 0; j < kChunkCols; ++j) {
-      if (col + j >= C) break;
-      if constexpr (DT == TERRA_DTYPE_F32) reinterpret_cast<float*>(row)[col + j] = f[j];
-      else reinterpret_cast<uint16_t*>(row)[col + j] = (uint16_t)pack2<DT>(f[j], 0.f);
     }
   }
 }
@@ -175,11 +142,17 @@ __device__ __forceinline__ bool kept(const ChunkDraws& d, int j, uint32_t thresh
   return (j & 1 ? d.w[j >> 1] >> 16 : d.w[j >> 1] & 0xffffu) >= threshold;
 }
 
+// The value of the neighbouring lane l ^ 1 (quad permute [1, 0, 3, 2]).
+__device__ __forceinline__ uint32_t lane_xor1(uint32_t v) {
+  return (uint32_t)__builtin_amdgcn_mov_dpp((int)v, 0xb1, 0xf, 0xf, false);
+}
+
 // ---- sums over the lanes of a row ---------------------------------------------
-// Sum over the kL aligned lanes of a wave (kL = 16, 32 or 64); every lane ends
+// Sum over the kL aligned lanes of a wave (kL = 8, 16, 32 or 64); every lane ends
 // with the same bits, since each step adds the same two values on both sides.
 template <int kL>
 __device__ __forceinline__ float lanes_sum(float v) {
+  if constexpr (kL == 8) return group8_sum(v);
   v = row16_sum(v);
   if constexpr (kL >= 32) {
     const uint32_t b = __float_as_uint(v);
@@ -257,32 +230,39 @@ struct SumJobs {
 };
 
 constexpr int kSumThreads = 1024;
-constexpr int kSumCols = 64;
+constexpr int kSumCols = 16;
+constexpr int kSumParts = kSumThreads / kSumCols;
 
-// One workgroup for 64 columns of one row of one job: its 16 waves take every
-// 16th partial each.  (static: each source file that sums has its own copy)
+// One workgroup for 16 columns of one row of one job: 64 adders take every
+// 64th partial each, in fp64.  (static: each source file that sums has its own
+// copy.)  Few columns a workgroup, so that a vector of some hundred columns
+// still has tens of workgroups to wait for the partials' loads.
 static __global__ __launch_bounds__(kSumThreads) void sum_partials_kernel(const SumJobs jobs) {
   const SumJob j = jobs.job[blockIdx.y];
-  __shared__ double s[kSumThreads / 64][kSumCols];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  __shared__ double s[kSumParts][kSumCols];
+  const int lane = threadIdx.x % kSumCols, part = threadIdx.x / kSumCols;
   const int c = blockIdx.x * kSumCols + lane;
   for (int b = blockIdx.z; b < j.batch; b += gridDim.z) {
     double sum = 0.0;
     const float* src = j.src + (int64_t)b * j.count * j.src_stride + (c < jobs.C ? c : 0);
-    int i = wave;
-    for (; i + 48 < j.count; i += 64) {
-      const float v0 = src[(int64_t)i * j.src_stride], v1 = src[(int64_t)(i + 16) * j.src_stride];
-      const float v2 = src[(int64_t)(i + 32) * j.src_stride], v3 = src[(int64_t)(i + 48) * j.src_stride];
-      sum += ((double)v0 + (double)v1) + ((double)v2 + (double)v3);
+    constexpr int kAhead = 8;
+    for (int i = part; i < j.count; i += kAhead * kSumParts) {
+      float v[kAhead];
+#pragma unroll
+      for (int u = 0; u < kAhead; ++u) {
+        const int at = i + u * kSumParts;
+        v[u] = src[(int64_t)(at < j.count ? at : i) * j.src_stride];
+      }
+#pragma unroll
+      for (int u = 0; u < kAhead; ++u) sum += i + u * kSumParts < j.count ? (double)v[u] : 0.0;
     }
-    for (; i < j.count; i += 16) sum += (double)src[(int64_t)i * j.src_stride];
-    s[wave][lane] = sum;
+    s[part][lane] = sum;
     __syncthreads();
-    if (wave == 0 && c < jobs.C) {
-      for (int w = 1; w < kSumThreads / 64; ++w) sum += s[w][lane];
-      j.dst[(int64_t)b * jobs.C + c] = (float)sum;
+    for (int half = kSumParts / 2; half > 0; half /= 2) {
+      if (part < half) s[part][lane] = sum += s[part + half][lane];
+      __syncthreads();
     }
-    __syncthreads();
+    if (part == 0 && c < jobs.C) j.dst[(int64_t)b * jobs.C + c] = (float)sum;
   }
 }
 

@@ -89,8 +89,9 @@ class Case:
         gs = torch.autograd.grad(outs, list(v.values()), [self.dy.double()] + ([] if z is None else [self.dz.double()]))
         return y.detach(), None if z is None else z.detach(), dict(zip(v, gs))
 
-    def check(self, dev):
-        y, z, g = self.run(dev)
+    def check(self, dev, got=None):
+        """The kernels' results (of ``got``: those of an equal call) against the oracle's."""
+        y, z, g = self.run(dev) if got is None else got
         assert y.shape == self.grid and y.dtype == self.dts[1]
         yr, zr, gr = self.oracle()
         C, R = self.C, self.x.numel() // self.C
@@ -227,23 +228,24 @@ def test_bitwise_the_same_each_time(dev):
         assert all(torch.equal(a, b) for a, b in zip(g, g2))
 
 
+@pytest.mark.parametrize("dts", TYPES)
 @pytest.mark.parametrize("C", [96, 100])
-def test_strides_and_alignment(dev, C):
-    c = Case((37, C), (BF16, BF16), p=0.1, seed=8)
-    y, z, g = c.check(dev)
+@pytest.mark.parametrize("extra", [8, 9])
+def test_strides_and_alignment(dev, C, extra, dts):
+    """Column blocks of wider rows, on the 16-byte grid (C = 96, 8 more) and off
+    it: each against the oracle, and those of one kind the same bit for bit."""
+    c = Case((37, C), dts, p=0.1, seed=8)
+    packed = c.check(dev)
     t, kw = c.args(dev)
-    wide = torch.zeros(37, 2 * C + 9, dtype=BF16, device=dev)
+    first = {C % 8 == 0: packed}
     for lo in (0, 8, 5):
-        h = wide.clone()[:, lo:lo + C].copy_(t["h"])
-        x = wide.clone()[:, lo:lo + C].copy_(t["x"])
-        out = kernels.residual_norm(h, x, **kw)
-        grads = kernels.residual_norm_backward(h, x, t["dy"], t["dz"], **kw)
-        if lo != 5:  # the same code path; off the 16-byte grid the sums keep their order too
-            assert torch.equal(out[0], y) and torch.equal(out[1], z)
-            assert all(torch.equal(a, b) for a, b in zip(grads, g))
-        else:
-            assert (out[0].float() - y.float()).abs().max() <= 2 ** -7 * y.float().abs().max()
-            assert (grads.dh.float() - g.dh.float()).abs().max() <= 2 ** -7 * g.dh.float().abs().max()
+        h, x = (torch.zeros(37, 2 * C + extra, dtype=d, device=dev)[:, lo:lo + C].copy_(t[n]) for n, d in zip("hx", dts))
+        got = (*kernels.residual_norm(h, x, **kw), kernels.residual_norm_backward(h, x, t["dy"], t["dz"], **kw))
+        c.check(dev, got)
+        same = first.setdefault(all(v.stride(0) * v.element_size() % 16 == 0 and v.data_ptr() % 16 == 0 for v in (h, x))
+                                and C % 8 == 0, got)
+        assert torch.equal(got[0], same[0]) and torch.equal(got[1], same[1])
+        assert all(torch.equal(a, b) for a, b in zip(got[2], same[2]))
 
 
 @pytest.mark.parametrize("gate", [None, "channel", "sample"])
