@@ -59,7 +59,7 @@ struct TailArgs {
   float post_eps, next_eps, alpha, inv_c;
   int32_t gate_rows;                // 0: none, 1: one for all, B: one for each sample
   int32_t windows;                  // h is in window order
-  uint32_t slabs, slab_rows, units; // backward: see there
+  uint32_t slabs, units;            // backward: see there
   WindowMap map;
 };
 
@@ -212,16 +212,16 @@ struct RowLanes {
 };
 
 // The fewest idle lanes of one to three chunks a lane, and among those the most chunks: what a row costs beside its
-// values (addresses, sums over lanes, row tests) is paid once for all chunks of a lane.  From 129 chunks on a
-// workgroup holds the row.
-inline TailShape tail_shape(int C) {
+// values (addresses, sums over lanes, row tests) is paid once for all chunks of a lane.  Rows in 16-byte pieces take
+// 16 lanes at least: with 8 a 16-bit h is read in runs of 64 bytes.  From 129 chunks on a workgroup holds the row.
+inline TailShape tail_shape(int C, bool pieces) {
   const int n = (C + kChunkCols - 1) / kChunkCols;
   if (n > 512) return {512, 2};
   if (n > 256) return {256, 2};
   if (n > 128) return {256, 1};
   TailShape best = {64, 2};
   for (int k = 1; k <= 3; ++k)
-    for (int g = 8; g <= 64; g *= 2) {
+    for (int g = pieces ? 16 : 8; g <= 64; g *= 2) {
       if (g * k < n || (k == 3 && g == 64)) continue;
       if (g * k <= best.lanes * best.chunks) best = {g, k};
       break;
@@ -269,6 +269,7 @@ __device__ __forceinline__ float normalise(float (&v)[kK][kChunkCols], int kind,
     case 81: return f<DTH, DTX, 8, 1>(__VA_ARGS__);                                 \
     case 82: return f<DTH, DTX, 8, 2>(__VA_ARGS__);                                 \
     case 83: return f<DTH, DTX, 8, 3>(__VA_ARGS__);                                 \
+    case 161: return f<DTH, DTX, 16, 1>(__VA_ARGS__);                               \
     case 162: return f<DTH, DTX, 16, 2>(__VA_ARGS__);                               \
     case 163: return f<DTH, DTX, 16, 3>(__VA_ARGS__);                               \
     case 322: return f<DTH, DTX, 32, 2>(__VA_ARGS__);                               \
@@ -349,9 +350,9 @@ struct ColumnParams {
 // The backward's launch, by the types of h and x (residual_norm_bwd.hip).
 struct TailBwdPlan {
   TailShape shape;
-  uint32_t slabs, slab_rows, units, blocks;
+  uint32_t slabs, units, blocks;
 };
-TailBwdPlan tail_bwd_plan(uint32_t rows, int C, int gate_rows);
+TailBwdPlan tail_bwd_plan(uint32_t rows, int C, int gate_rows, bool pieces);
 int launch_tail_bwd(int h_dtype, int x_dtype, const void* args, const TailBwdPlan& plan, bool vec, hipStream_t s);
 
 }  // namespace terra

@@ -18,33 +18,48 @@ __global__ __launch_bounds__(tail_threads(kG)) void tail_kernel(const TailArgs a
   const RowLanes<kG, kK, kP> at = {(int)(threadIdx.x % kG), C};
   RowSum<kG> sum(&s_red);
   Params par(&s_par);  // gw, gb (branch_params), nw, nb
+  const uint64_t seed = a.drop.threshold > 0 ? *a.drop.seed : 0;
+  // A row's chunks of h and x; a row past the end re-reads the last one.
+  struct Row {
+    uint32_t r;
+    bool has;
+    RowChunk<DTH> h[kK];
+    RowChunk<DTX> x[kK];
+  };
+  auto fetch = [&](uint32_t base) {
+    Row q;
+    const uint32_t row = base + group;
+    q.r = row < a.rows ? row : a.rows - 1;
+    const int64_t src = a.windows ? a.map.source(q.r) : (int64_t)q.r;
+    q.has = src >= 0;
+    const uint8_t* hp = a.h + (q.has ? src : 0) * a.h_row_bytes;
+    const uint8_t* xp = a.x + (int64_t)q.r * a.x_row_bytes;
+#pragma unroll
+    for (int k = 0; k < kK; ++k) {
+      q.h[k] = at.template load<DTH, kVec>(hp, k);
+      q.x[k] = at.template load<DTX, kVec>(xp, k);
+    }
+    return q;
+  };
+  const uint32_t step = gridDim.x * kGroups;
+  uint32_t base = blockIdx.x * kGroups;
+  Row ahead = fetch(base);
   par.fill(at, [&](int c, float (&v)[4]) {
     branch_params(a, a.gate_rows == 1 ? a.gate : nullptr, c, v[0], v[1]);
     v[2] = param_at(a.nw, 1.f, c);
     v[3] = param_at(a.nb, 0.f, c);
   });
-  if constexpr (Params::kLds) __syncthreads();
-  const uint64_t seed = a.drop.threshold > 0 ? *a.drop.seed : 0;
-  for (uint32_t base = blockIdx.x * kGroups; base < a.rows; base += gridDim.x * kGroups) {
+  if constexpr (Params::kLds) RowSum<kG>::lds_sync();
+  for (; base < a.rows; base += step) {
     par.stay();
-    const uint32_t row = base + group;
-    const bool live = row < a.rows;
-    const uint32_t r = live ? row : a.rows - 1;  // a row past the end re-reads the last one
-    const int64_t src = a.windows ? a.map.source(r) : (int64_t)r;
-    const bool has = src >= 0;
-    const uint8_t* hp = a.h + (has ? src : 0) * a.h_row_bytes;
-    const uint8_t* xp = a.x + (int64_t)r * a.x_row_bytes;
-    RowChunk<DTH> hq[kK];
-    RowChunk<DTX> xq[kK];
-#pragma unroll
-    for (int k = 0; k < kK; ++k) {
-      hq[k] = at.template load<DTH, kVec>(hp, k);
-      xq[k] = at.template load<DTX, kVec>(xp, k);
-    }
+    const Row q = ahead;
+    if (base + step < a.rows) ahead = fetch(base + step);
+    const uint32_t r = q.r;
+    const bool live = base + group < a.rows, has = q.has;
     float v[kK][kChunkCols];
 #pragma unroll
     for (int k = 0; k < kK; ++k) {
-      at.template values<DTH, kVec>(hq[k], k, has, v[k]);
+      at.template values<DTH, kVec>(q.h[k], k, has, v[k]);
     }
     if (a.post != TERRA_NORM_NONE) normalise<kG, kK, kP, kVec>(v, a.post, a.post_eps, a.inv_c, at, sum);
     const uint32_t live_rows = min(a.rows - base, (uint32_t)kGroups);
@@ -63,7 +78,7 @@ __global__ __launch_bounds__(tail_threads(kG)) void tail_kernel(const TailArgs a
           gb[j] *= g;
         }
       }
-      at.template values<DTX, kVec>(xq[k], k, true, xv);
+      at.template values<DTX, kVec>(q.x[k], k, true, xv);
 #pragma unroll
       for (int j = 0; j < kChunkCols; ++j) v[k][j] = has ? fmaf(v[k][j], gw[j], gb[j]) : 0.f;
       if (a.drop.threshold > 0) {
@@ -94,16 +109,20 @@ __global__ __launch_bounds__(tail_threads(kG)) void tail_kernel(const TailArgs a
 template <int DTH, int DTX, int kG, int kK>
 void launch(const TailArgs& a, bool vec, hipStream_t s) {
   constexpr uint32_t kGroups = tail_threads(kG) / kG;
-  // Workgroups stay for several rows each, so that the parameters' loads are paid once.
-  const uint32_t need = (a.rows + kGroups - 1) / kGroups, most = 2048;
-  const uint32_t blocks = need < most ? need : most;
+  // Row groups of a workgroup: few, so that workgroups that load and such that
+  // compute are always side by side (2048 that stay for all rows: TAILSTAY us at
+  // 524288 x 192 bf16, one group each TAILONE), but enough for the parameters, 16 C
+  // bytes a workgroup, to be a small part of what it reads.
+  constexpr uint32_t kTurns = kG > 64 ? 16 : (kG > 16 ? kG / 16 : 1);
+  const uint32_t need = (a.rows + kGroups - 1) / kGroups;
+  const uint32_t blocks = (need + kTurns - 1) / kTurns;
   if (vec) tail_kernel<DTH, DTX, kG, kK, true><<<blocks, tail_threads(kG), 0, s>>>(a);
   else tail_kernel<DTH, DTX, kG, kK, false><<<blocks, tail_threads(kG), 0, s>>>(a);
 }
 
 template <int DTH, int DTX>
 void dispatch(const TailArgs& a, bool vec, hipStream_t s) {
-  TERRA_TAIL_SHAPES(launch, tail_shape(a.C), a, vec, s);
+  TERRA_TAIL_SHAPES(launch, tail_shape(a.C, DTX == TERRA_DTYPE_F32), a, vec, s);
 }
 
 // A tensor of the call: how far it reaches, for the overlap checks.
@@ -270,7 +289,7 @@ extern "C" int terra_swin_residual_norm_workspace(const terra_swin_residual_norm
   int64_t h_rows = 0;
   TERRA_TRY(prepare(desc, &a, &vec, &h_rows));
   if (a.rows == 0) return 0;
-  const TailBwdPlan p = tail_bwd_plan(a.rows, a.C, a.gate_rows);
+  const TailBwdPlan p = tail_bwd_plan(a.rows, a.C, a.gate_rows, desc->x_dtype == TERRA_DTYPE_F32);
   return (int)(p.blocks * 4 * a.C + (a.gate_rows > 0 && p.slabs > 1 ? p.units * a.C : 0));
 }
 
@@ -331,9 +350,8 @@ extern "C" int terra_swin_residual_norm_bwd(const void* h, const void* x, const 
   if (a.post != TERRA_NORM_NONE) a.pw = post_weight, a.pb = post_bias;
   if (a.next != TERRA_NORM_NONE) a.nw = next_weight;
   a.gate = gate;
-  const TailBwdPlan p = tail_bwd_plan(a.rows, a.C, a.gate_rows);
+  const TailBwdPlan p = tail_bwd_plan(a.rows, a.C, a.gate_rows, desc->x_dtype == TERRA_DTYPE_F32);
   a.slabs = p.slabs;
-  a.slab_rows = p.slab_rows;
   a.units = p.units;
   a.partial = sums ? workspace : nullptr;
   a.branch_sums = dpost_weight != nullptr || dpost_bias != nullptr || dgate != nullptr;

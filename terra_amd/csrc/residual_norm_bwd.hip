@@ -15,9 +15,10 @@
 // which spares the rows' loop a sum, the value m and a product per element.
 // Bound by memory: h, x, dy, dz read once, dh and dx written once.
 //
-// Sums over rows: a unit is up to slab_rows consecutive rows of one sample,
-// workgroups take units in grid strides, and each lane keeps the sums of its
-// columns in registers; A and B leave them unit by unit, since the gate changes
+// Sums over rows: a unit is every slabs-th group of rows of one sample (so
+// that workgroups side by side read rows side by side; with a run of rows each,
+// 156672 x 1024 bf16 took RUNS us), workgroups take units in grid strides, and
+// each lane keeps the sums of its columns in registers; A and B leave them unit by unit, since the gate changes
 // with the sample.  A second launch adds the workgroups' sums
 // (sum_partials_kernel): no atomics, an order that the sizes fix.
 #include "residual_norm.h"
@@ -93,19 +94,18 @@ __global__ __launch_bounds__(tail_threads(kG)) void tail_bwd_kernel(const TailAr
 
   for (uint32_t unit = blockIdx.x; unit < a.units; unit += gridDim.x) {
     const uint32_t sample = unit / a.slabs, slab = unit % a.slabs;
-    const uint32_t begin = sample * a.per_sample + slab * a.slab_rows;
-    const uint32_t end = min(begin + a.slab_rows, (sample + 1) * a.per_sample);
+    const uint32_t end = (sample + 1) * a.per_sample;
     const float* const gate = a.gate_rows > 0 ? a.gate + (int64_t)sample * C : nullptr;
     if (a.gate_rows > 1) {
       if constexpr (Params::kLds) __syncthreads();
       stage(gate);
       if constexpr (Params::kLds) __syncthreads();
     }
-    for (uint32_t base = begin; base < end; base += kGroups) {
+    for (uint32_t base = sample * a.per_sample + slab * kGroups; base < end; base += a.slabs * kGroups) {
       par.stay();
       const uint32_t row = base + group;
       const bool live = row < end;
-      const uint32_t r = live ? row : end - 1;  // a row past the end re-reads the unit's last one
+      const uint32_t r = live ? row : end - 1;  // a row past the end re-reads the sample's last one
       const int64_t src = a.windows ? a.map.source(r) : (int64_t)r;
       const bool has = src >= 0;
       RowChunk<DTH> hq[kK], dzq[kK];
@@ -284,18 +284,16 @@ void dispatch(const TailArgs& a, const TailBwdPlan& p, bool vec, hipStream_t s) 
 
 // Workgroups: what fits the 256 compute units at once; slabs of the rows of a
 // sample so that every workgroup has a unit, and rows enough for its groups.
-TailBwdPlan tail_bwd_plan(uint32_t rows, int C, int gate_rows) {
+TailBwdPlan tail_bwd_plan(uint32_t rows, int C, int gate_rows, bool pieces) {
   TailBwdPlan p;
-  p.shape = tail_shape(C);
+  p.shape = tail_shape(C, pieces);
   const uint32_t groups = (uint32_t)(tail_threads(p.shape.lanes) / p.shape.lanes);
   const uint32_t most = p.shape.lanes > 256 ? 256u : (p.shape.chunks > 1 ? 512u : 1024u);
   const uint32_t samples = gate_rows > 1 ? (uint32_t)gate_rows : 1u, per = rows / samples;
   uint32_t slabs = (most + samples - 1) / samples;
   const uint32_t useful = (per + groups - 1) / groups;
   if (slabs > useful) slabs = useful;
-  p.slab_rows = (per + slabs - 1) / slabs;
-  p.slab_rows = (p.slab_rows + groups - 1) / groups * groups;
-  p.slabs = (per + p.slab_rows - 1) / p.slab_rows;
+  p.slabs = slabs;
   p.units = p.slabs * samples;
   p.blocks = p.units < most ? p.units : most;
   return p;
