@@ -17,7 +17,8 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 SOURCES = ("abi.hip", "window_copy.hip", "window_attention.hip", "window_attention_bwd.hip", "swin_block.hip",
            "swin_mlp.hip", "linear.hip", "mlp_backward.hip", "weight_grad.hip", "linear_short.hip", "block_f32.hip",
-           "dropout.hip", "residual_norm.hip", "residual_norm_bwd.hip")
+           "dropout.hip", "residual_norm.hip", "residual_norm_f32_f32.hip", "residual_norm_bf16_bf16.hip",
+           "residual_norm_bf16_f32.hip", "residual_norm_f16_f16.hip", "residual_norm_f16_f32.hip")
 ARCH = "gfx950"
 
 HIPCC_FLAGS = [

@@ -1,5 +1,5 @@
-// The end of a half-block, row by row of C channels (residual_norm.hip holds
-// the forward, residual_norm_bwd.hip the backward):
+// The end of a half-block, row by row of C channels (residual_norm_fwd.h and
+// residual_norm_bwd.h hold the kernels, residual_norm.hip the entry points):
 //
 //   n = post_norm(h)          LayerNorm, RMS norm or nothing, with affine
 //   m = keep s n              dropout (row_chunk.h)
@@ -45,6 +45,21 @@ struct WindowMap {
   }
 };
 
+// What a launch has.  The first three are template parameters of the kernels:
+// tested at run time they cost the rows' loops a register copy of every value
+// that either side of a test may hold (a backward of 156672 x 1024 bf16: MOVS
+// instead of SPEC us).
+enum TailFlags : uint32_t {
+  kTailPost = 1,       // a post-norm
+  kTailNext = 2,       // a next norm (backward: whose gradient is given)
+  kTailDrop = 4,
+  kTailFeatures = 7,
+  kTailAtRunTime = 8,  // as a template parameter: the first three are the call's flags
+  kTailPostLayer = 16, kTailNextLayer = 32,  // the norm is a LayerNorm
+  kTailWindows = 64,   // h is in window order
+  kTailDy = 128,       // backward: the gradient of y is given
+};
+
 struct TailArgs {
   const uint8_t *h, *x, *dy, *dz;   // dy, dz: backward, either may be NULL (zero)
   uint8_t *y, *z, *dh, *dx;
@@ -55,13 +70,18 @@ struct TailArgs {
   DropoutArgs drop;
   uint32_t rows, per_sample;        // per_sample: rows that share a row of the gate
   int64_t h_row_bytes, x_row_bytes; // of h and x; the other tensors' rows are packed
-  int32_t C, post, next;            // post, next: enum terra_norm
+  int32_t C;
+  uint32_t flags;                   // TailFlags
   float post_eps, next_eps, alpha, inv_c;
   int32_t gate_rows;                // 0: none, 1: one for all, B: one for each sample
-  int32_t windows;                  // h is in window order
   uint32_t slabs, units;            // backward: see there
   WindowMap map;
 };
+
+template <int kF>
+__device__ __forceinline__ bool tail_has(const TailArgs& a, uint32_t feature) {
+  return (kF == kTailAtRunTime ? a.flags : (uint32_t)kF) & feature;
+}
 
 // How the lanes hold a row: kG lanes with kK chunks each.
 struct TailShape {
@@ -121,13 +141,22 @@ struct RowLanes {
   }
 
   // Its values in fp32, zeros in absent columns and where the row is not there.
+  // all: (uniform) no lane of the launch has either, which spares the selects.
   template <int DT, bool kVec>
-  __device__ __forceinline__ void values(const RowChunk<DT>& r, int k, bool there, float (&f)[kChunkCols]) const {
+  __device__ __forceinline__ void values(RowChunk<DT> r, int k, bool there, bool all, float (&f)[kChunkCols]) const {
+    if (!kVec || !all) {
 #pragma unroll
-    for (int j = 0; j < kChunkCols; ++j) {
-      const float v = chunk_value<DT>(r, j);
-      f[j] = there && has<kVec>(k, j) ? v : 0.f;
+      for (int i = 0; i < RowChunk<DT>::kWords; ++i)
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+          const int j = ChunkElt<DT>::kBytes == 4 ? 4 * i + w : 2 * w;
+          uint32_t v = there && has<kVec>(k, j) ? r.q[i][w] : 0u;
+          if constexpr (!kVec && ChunkElt<DT>::kBytes == 2) v = has<false>(k, j + 1) ? v : v & 0xffffu;
+          r.q[i][w] = v;
+        }
     }
+#pragma unroll
+    for (int j = 0; j < kChunkCols; ++j) f[j] = chunk_value<DT>(r, j);
   }
 
   // Stores chunk k, rounded once, into the row that begins `off` bytes into the descriptor's range.
@@ -199,7 +228,9 @@ struct RowLanes {
   // The draws of chunk k's eight values.  Where a chunk is two pieces, lanes 2i
   // and 2i + 1 hold the halves of two chunks of the mask: the even lane
   // draws the first, the odd one the second, and they swap halves.
-  __device__ __forceinline__ ChunkDraws draws(uint64_t seed, int k, uint32_t row, uint32_t stream) const {
+  // Without dropout they are never below the threshold.
+  __device__ __forceinline__ ChunkDraws draws(bool drop, uint64_t seed, int k, uint32_t row, uint32_t stream) const {
+    if (!drop) return {{~0u, ~0u, ~0u, ~0u}};
     if constexpr (kP == 8) {
       return chunk_draws(seed, (uint32_t)(lane + kG * k), row, stream);
     } else {
@@ -211,23 +242,28 @@ struct RowLanes {
   }
 };
 
-// The fewest idle lanes of one to three chunks a lane, and among those the most chunks: what a row costs beside its
-// values (addresses, sums over lanes, row tests) is paid once for all chunks of a lane.  Rows in 16-byte pieces take
-// 16 lanes at least: with 8 a 16-bit h is read in runs of 64 bytes.  From 129 chunks on a workgroup holds the row.
-inline TailShape tail_shape(int C, bool pieces) {
+// Few idle lanes, and the most chunks a lane that leave room for waves to run
+// side by side: what a row costs beside its values (addresses, sums over lanes,
+// row tests) is paid once for all chunks of a lane.  most: three chunks, but two
+// in the backward of an fp32 x, whose registers then hold two waves a SIMD
+// (524288 x 192, bf16 h: 347 us, with three 693).  Eight lanes a row only where
+// columns stand eight by eight: as 16-byte pieces of fp32 they would read a
+// 16-bit h in runs of 64 bytes.  From 129 chunks on a workgroup holds the row.
+inline TailShape tail_shape(int C, bool pieces, int most) {
   const int n = (C + kChunkCols - 1) / kChunkCols;
   if (n > 512) return {512, 2};
-  if (n > 256) return {256, 2};
+  if (n > 256) return {512, 1};
   if (n > 128) return {256, 1};
-  TailShape best = {64, 2};
-  for (int k = 1; k <= 3; ++k)
-    for (int g = pieces ? 16 : 8; g <= 64; g *= 2) {
-      if (g * k < n || (k == 3 && g == 64)) continue;
-      if (g * k <= best.lanes * best.chunks) best = {g, k};
-      break;
-    }
-  return best;
+  if (n <= 16) return {16, 1};
+  if (n <= 24 && most == 3 && !pieces) return {8, 3};
+  if (n <= 32) return {16, 2};
+  if (n <= 48 && most == 3) return {16, 3};
+  if (n <= 64) return {32, 2};
+  if (n <= 96 && most == 3) return {32, 3};
+  return {64, 2};
 }
+inline bool tail_pieces(int x_dtype) { return x_dtype == TERRA_DTYPE_F32; }
+inline int tail_bwd_most(int x_dtype) { return x_dtype == TERRA_DTYPE_F32 ? 2 : 3; }
 constexpr int kTailMaxChannels = 8192;
 
 constexpr int tail_threads(int lanes) { return lanes > 256 ? lanes : 256; }
@@ -235,20 +271,21 @@ constexpr int tail_threads(int lanes) { return lanes > 256 ? lanes : 256; }
 // The statistics of a normalised row held as kK chunks a lane: v becomes
 // (v - mean) r (zero in absent columns), r is returned.
 template <int kG, int kK, int kP, bool kVec>
-__device__ __forceinline__ float normalise(float (&v)[kK][kChunkCols], int kind, float eps, float inv_c,
+__device__ __forceinline__ float normalise(float (&v)[kK][kChunkCols], bool layer, float eps, float inv_c,
                                            const RowLanes<kG, kK, kP>& at, RowSum<kG>& sum) {
-  if (kind == TERRA_NORM_LAYER) {
+  float mean = 0.f;
+  if (layer) {
     float s = 0.f;
 #pragma unroll
     for (int k = 0; k < kK; ++k)
 #pragma unroll
       for (int j = 0; j < kChunkCols; ++j) s += v[k][j];
-    const float mean = sum.one(s) * inv_c;
-#pragma unroll
-    for (int k = 0; k < kK; ++k)
-#pragma unroll
-      for (int j = 0; j < kChunkCols; ++j) v[k][j] = at.template has<kVec>(k, j) ? v[k][j] - mean : 0.f;
+    mean = sum.one(s) * inv_c;
   }
+#pragma unroll
+  for (int k = 0; k < kK; ++k)
+#pragma unroll
+    for (int j = 0; j < kChunkCols; ++j) v[k][j] -= at.template has<kVec>(k, j) ? mean : 0.f;  // kVec: one select for four
   float q = 0.f;
 #pragma unroll
   for (int k = 0; k < kK; ++k)
@@ -262,40 +299,23 @@ __device__ __forceinline__ float normalise(float (&v)[kK][kChunkCols], int kind,
   return r;
 }
 
-// f<DTH, DTX, lanes, chunks>(...) for the shape at run time (inside a function
-// template over DTH and DTX).
-#define TERRA_TAIL_SHAPES(f, shape, ...)                                            \
-  switch ((shape).lanes * 10 + (shape).chunks) {                                    \
-    case 81: return f<DTH, DTX, 8, 1>(__VA_ARGS__);                                 \
-    case 82: return f<DTH, DTX, 8, 2>(__VA_ARGS__);                                 \
-    case 83: return f<DTH, DTX, 8, 3>(__VA_ARGS__);                                 \
-    case 161: return f<DTH, DTX, 16, 1>(__VA_ARGS__);                               \
-    case 162: return f<DTH, DTX, 16, 2>(__VA_ARGS__);                               \
-    case 163: return f<DTH, DTX, 16, 3>(__VA_ARGS__);                               \
-    case 322: return f<DTH, DTX, 32, 2>(__VA_ARGS__);                               \
-    case 323: return f<DTH, DTX, 32, 3>(__VA_ARGS__);                               \
-    case 642: return f<DTH, DTX, 64, 2>(__VA_ARGS__);                               \
-    case 2561: return f<DTH, DTX, 256, 1>(__VA_ARGS__);                             \
-    case 2562: return f<DTH, DTX, 256, 2>(__VA_ARGS__);                             \
-    default: return f<DTH, DTX, 512, 2>(__VA_ARGS__);                               \
-  }
-
 // A parameter, `none` where the pointer is NULL.
 __device__ __forceinline__ float param_at(const float* p, float none, int c) { return p == nullptr ? none : p[c]; }
 
 // The branch's affine map with the gate and the dropout scale in it:
 //   gate * s * (nhat w + b) = nhat gw + gb
 __device__ __forceinline__ void branch_params(const TailArgs& a, const float* gate, int c, float& gw, float& gb) {
-  const float g = param_at(gate, 1.f, c) * (a.drop.threshold > 0 ? a.drop.scale : 1.f);
+  const float g = param_at(gate, 1.f, c) * a.drop.scale;
   gw = g * param_at(a.pw, 1.f, c);
   gb = g * param_at(a.pb, 0.f, c);
 }
 
 // Per-column parameters of a row's lanes: in LDS where rows share a workgroup
-// (kG <= 64), else, each lane's columns being its own, in registers.
+// (kG <= 64), else, each lane's columns being its own, in registers, but for the
+// backward of the widest rows, which has none left.
 template <int kN, int kG, int kK, int kP>
 struct ColumnParams {
-  static constexpr bool kLds = kG <= 64;
+  static constexpr bool kLds = kG <= 64 || (kN == 3 && kK > 1);
   static constexpr int kCols = kG * kK * kChunkCols, kThreads = tail_threads(kG);
   struct Shared { __attribute__((aligned(16))) float v[kLds ? kN : 1][kLds ? kCols : 4]; };
   Shared* s;
@@ -345,14 +365,51 @@ struct ColumnParams {
   }
 };
 
+// Calls f<DTH, DTX, lanes, chunks, kVec, features>(...) for the call's shape and
+// features: those of aligned rows each have kernels of their own, other rows one for all.
+#define TERRA_TAIL_FEATURES(f, g, k, features, vec, ...)                                                      \
+  if (!(vec)) return f<DTH, DTX, g, k, false, kTailAtRunTime>(__VA_ARGS__);                                   \
+  switch ((features) & kTailFeatures) {                                                                       \
+    case 0: return f<DTH, DTX, g, k, true, 0>(__VA_ARGS__);                                                   \
+    case 1: return f<DTH, DTX, g, k, true, 1>(__VA_ARGS__);                                                   \
+    case 2: return f<DTH, DTX, g, k, true, 2>(__VA_ARGS__);                                                   \
+    case 3: return f<DTH, DTX, g, k, true, 3>(__VA_ARGS__);                                                   \
+    case 4: return f<DTH, DTX, g, k, true, 4>(__VA_ARGS__);                                                   \
+    case 5: return f<DTH, DTX, g, k, true, 5>(__VA_ARGS__);                                                   \
+    case 6: return f<DTH, DTX, g, k, true, 6>(__VA_ARGS__);                                                   \
+    default: return f<DTH, DTX, g, k, true, 7>(__VA_ARGS__);                                                  \
+  }
+#define TERRA_TAIL_SHAPES(f, shape, most, features, vec, ...)                                                 \
+  if constexpr ((most) == 3) {                                                                                \
+    if constexpr (DTX != TERRA_DTYPE_F32)                                                                     \
+      if ((shape).lanes == 8) { TERRA_TAIL_FEATURES(f, 8, 3, features, vec, __VA_ARGS__) }                    \
+    if ((shape).chunks == 3 && (shape).lanes == 16) { TERRA_TAIL_FEATURES(f, 16, 3, features, vec, __VA_ARGS__) } \
+    if ((shape).chunks == 3) { TERRA_TAIL_FEATURES(f, 32, 3, features, vec, __VA_ARGS__) }                    \
+  }                                                                                                           \
+  switch ((shape).lanes * 10 + (shape).chunks) {                                                              \
+    case 161: { TERRA_TAIL_FEATURES(f, 16, 1, features, vec, __VA_ARGS__) }                                   \
+    case 162: { TERRA_TAIL_FEATURES(f, 16, 2, features, vec, __VA_ARGS__) }                                   \
+    case 322: { TERRA_TAIL_FEATURES(f, 32, 2, features, vec, __VA_ARGS__) }                                   \
+    case 642: { TERRA_TAIL_FEATURES(f, 64, 2, features, vec, __VA_ARGS__) }                                   \
+    case 2561: { TERRA_TAIL_FEATURES(f, 256, 1, features, vec, __VA_ARGS__) }                                 \
+    case 5121: { TERRA_TAIL_FEATURES(f, 512, 1, features, vec, __VA_ARGS__) }                                 \
+    default: { TERRA_TAIL_FEATURES(f, 512, 2, features, vec, __VA_ARGS__) }                                   \
+  }
+
 }  // namespace
 
-// The backward's launch, by the types of h and x (residual_norm_bwd.hip).
+// The backward's grid, by the sizes of the call (residual_norm.hip).
 struct TailBwdPlan {
   TailShape shape;
   uint32_t slabs, units, blocks;
 };
-TailBwdPlan tail_bwd_plan(uint32_t rows, int C, int gate_rows, bool pieces);
-int launch_tail_bwd(int h_dtype, int x_dtype, const void* args, const TailBwdPlan& plan, bool vec, hipStream_t s);
+
+// The kernels' launches by the types of h and x, each with a source file of its
+// own; `args` is a TailArgs.
+#define TERRA_TAIL_TYPES(X) X(f32, f32) X(bf16, bf16) X(bf16, f32) X(f16, f16) X(f16, f32)
+#define TERRA_TAIL_DECLARE(h, x)                                \
+  void tail_fwd_##h##_##x(const void* args, bool vec, hipStream_t s); \
+  void tail_bwd_##h##_##x(const void* args, const TailBwdPlan& plan, bool vec, hipStream_t s);
+TERRA_TAIL_TYPES(TERRA_TAIL_DECLARE)
 
 }  // namespace terra

@@ -1,129 +1,9 @@
-// Forward of the end of a half-block (residual_norm.h): the branch's
-// post-norm, dropout, gate, scaled residual and the next half-block's norm in
-// one pass.  Bound by memory: h and x read once, y and z written once.
+// Entry points of the end of a half-block (residual_norm.h): argument checks,
+// the backward's grid and workspace, and the choice of kernels by type.
 #include "residual_norm.h"
 
 namespace terra {
 namespace {
-
-template <int DTH, int DTX, int kG, int kK, bool kVec>
-__global__ __launch_bounds__(tail_threads(kG)) void tail_kernel(const TailArgs a) {
-  constexpr int kGroups = tail_threads(kG) / kG;
-  constexpr int kHB = ChunkElt<DTH>::kBytes, kXB = ChunkElt<DTX>::kBytes;
-  constexpr int kP = DTX == TERRA_DTYPE_F32 ? 4 : 8;
-  using Params = ColumnParams<4, kG, kK, kP>;
-  __shared__ typename RowSum<kG>::Shared s_red;
-  __shared__ typename Params::Shared s_par;
-  const int group = threadIdx.x / kG, C = a.C;
-  const RowLanes<kG, kK, kP> at = {(int)(threadIdx.x % kG), C};
-  RowSum<kG> sum(&s_red);
-  Params par(&s_par);  // gw, gb (branch_params), nw, nb
-  const uint64_t seed = a.drop.threshold > 0 ? *a.drop.seed : 0;
-  // A row's chunks of h and x; a row past the end re-reads the last one.
-  struct Row {
-    uint32_t r;
-    bool has;
-    RowChunk<DTH> h[kK];
-    RowChunk<DTX> x[kK];
-  };
-  auto fetch = [&](uint32_t base) {
-    Row q;
-    const uint32_t row = base + group;
-    q.r = row < a.rows ? row : a.rows - 1;
-    const int64_t src = a.windows ? a.map.source(q.r) : (int64_t)q.r;
-    q.has = src >= 0;
-    const uint8_t* hp = a.h + (q.has ? src : 0) * a.h_row_bytes;
-    const uint8_t* xp = a.x + (int64_t)q.r * a.x_row_bytes;
-#pragma unroll
-    for (int k = 0; k < kK; ++k) {
-      q.h[k] = at.template load<DTH, kVec>(hp, k);
-      q.x[k] = at.template load<DTX, kVec>(xp, k);
-    }
-    return q;
-  };
-  const uint32_t step = gridDim.x * kGroups;
-  uint32_t base = blockIdx.x * kGroups;
-  Row ahead = fetch(base);
-  par.fill(at, [&](int c, float (&v)[4]) {
-    branch_params(a, a.gate_rows == 1 ? a.gate : nullptr, c, v[0], v[1]);
-    v[2] = param_at(a.nw, 1.f, c);
-    v[3] = param_at(a.nb, 0.f, c);
-  });
-  if constexpr (Params::kLds) RowSum<kG>::lds_sync();
-  for (; base < a.rows; base += step) {
-    par.stay();
-    const Row q = ahead;
-    if (base + step < a.rows) ahead = fetch(base + step);
-    const uint32_t r = q.r;
-    const bool live = base + group < a.rows, has = q.has;
-    float v[kK][kChunkCols];
-#pragma unroll
-    for (int k = 0; k < kK; ++k) {
-      at.template values<DTH, kVec>(q.h[k], k, has, v[k]);
-    }
-    if (a.post != TERRA_NORM_NONE) normalise<kG, kK, kP, kVec>(v, a.post, a.post_eps, a.inv_c, at, sum);
-    const uint32_t live_rows = min(a.rows - base, (uint32_t)kGroups);
-    const __amdgpu_buffer_rsrc_t y_out = buffer_rsrc(a.y + (int64_t)base * C * kXB, live_rows * (uint32_t)(C * kXB));
-#pragma unroll
-    for (int k = 0; k < kK; ++k) {
-      float gw[kChunkCols], gb[kChunkCols], xv[kChunkCols];
-      par.get(0, k, at, gw);
-      par.get(1, k, at, gb);
-      if (a.gate_rows > 1) {  // this row's sample's gate
-        const float* gate = a.gate + (int64_t)(r / a.per_sample) * C;
-#pragma unroll
-        for (int j = 0; j < kChunkCols; ++j) {
-          const float g = at.template has<kVec>(k, j) ? gate[at.base(k, j >> 2) + (j & 3)] : 0.f;
-          gw[j] *= g;
-          gb[j] *= g;
-        }
-      }
-      at.template values<DTX, kVec>(q.x[k], k, true, xv);
-#pragma unroll
-      for (int j = 0; j < kChunkCols; ++j) v[k][j] = has ? fmaf(v[k][j], gw[j], gb[j]) : 0.f;
-      if (a.drop.threshold > 0) {
-        const ChunkDraws d = at.draws(seed, k, r, a.drop.stream);
-#pragma unroll
-        for (int j = 0; j < kChunkCols; ++j) v[k][j] = kept(d, j, a.drop.threshold) ? v[k][j] : 0.f;
-      }
-#pragma unroll
-      for (int j = 0; j < kChunkCols; ++j) v[k][j] = fmaf(a.alpha, xv[j], v[k][j]);
-      if (live) at.template store<DTX, kVec>(v[k], y_out, (uint32_t)(group * C) * kXB, k);
-    }
-    if (a.next != TERRA_NORM_NONE) {
-      normalise<kG, kK, kP, kVec>(v, a.next, a.next_eps, a.inv_c, at, sum);
-      const __amdgpu_buffer_rsrc_t z_out = buffer_rsrc(a.z + (int64_t)base * C * kHB, live_rows * (uint32_t)(C * kHB));
-#pragma unroll
-      for (int k = 0; k < kK; ++k) {
-        float w[kChunkCols], b[kChunkCols];
-        par.get(2, k, at, w);
-        par.get(3, k, at, b);
-#pragma unroll
-        for (int j = 0; j < kChunkCols; ++j) v[k][j] = fmaf(v[k][j], w[j], b[j]);
-        if (live) at.template store<DTH, kVec>(v[k], z_out, (uint32_t)(group * C) * kHB, k);
-      }
-    }
-  }
-}
-
-template <int DTH, int DTX, int kG, int kK>
-void launch(const TailArgs& a, bool vec, hipStream_t s) {
-  constexpr uint32_t kGroups = tail_threads(kG) / kG;
-  // Row groups of a workgroup: few, so that workgroups that load and such that
-  // compute are always side by side (2048 that stay for all rows: TAILSTAY us at
-  // 524288 x 192 bf16, one group each TAILONE), but enough for the parameters, 16 C
-  // bytes a workgroup, to be a small part of what it reads.
-  constexpr uint32_t kTurns = kG > 64 ? 16 : (kG > 16 ? kG / 16 : 1);
-  const uint32_t need = (a.rows + kGroups - 1) / kGroups;
-  const uint32_t blocks = (need + kTurns - 1) / kTurns;
-  if (vec) tail_kernel<DTH, DTX, kG, kK, true><<<blocks, tail_threads(kG), 0, s>>>(a);
-  else tail_kernel<DTH, DTX, kG, kK, false><<<blocks, tail_threads(kG), 0, s>>>(a);
-}
-
-template <int DTH, int DTX>
-void dispatch(const TailArgs& a, bool vec, hipStream_t s) {
-  TERRA_TAIL_SHAPES(launch, tail_shape(a.C, DTX == TERRA_DTYPE_F32), a, vec, s);
-}
 
 // A tensor of the call: how far it reaches, for the overlap checks.
 struct Span {
@@ -168,8 +48,8 @@ int prepare(const terra_swin_residual_norm_desc* d, TailArgs* a, bool* vec, int6
     return fail(TERRA_ERR_SHAPE, "a row stride is below the %d channels", d->channels);
   a->rows = (uint32_t)d->rows;
   a->C = d->channels;
-  a->post = d->post_norm;
-  a->next = d->next_norm;
+  a->flags = (d->post_norm != TERRA_NORM_NONE ? kTailPost : 0u) | (d->post_norm == TERRA_NORM_LAYER ? kTailPostLayer : 0u) |
+             (d->next_norm != TERRA_NORM_NONE ? kTailNext : 0u) | (d->next_norm == TERRA_NORM_LAYER ? kTailNextLayer : 0u);
   a->post_eps = d->post_eps;
   a->next_eps = d->next_eps;
   a->alpha = d->residual_scale;
@@ -181,8 +61,8 @@ int prepare(const terra_swin_residual_norm_desc* d, TailArgs* a, bool* vec, int6
   a->x_row_bytes = d->x_stride * dtype_size(x);
   *vec = d->channels % kChunkCols == 0 && a->h_row_bytes % 16 == 0 && a->x_row_bytes % 16 == 0;
   *h_rows = d->rows;
-  a->windows = d->windows;
   if (d->windows && d->rows > 0) {
+    a->flags |= kTailWindows;
     const terra_swin_geom& q = d->geom;
     GeomDims dims;
     const int st = validate_geom(&q, &dims);
@@ -210,6 +90,39 @@ int prepare(const terra_swin_residual_norm_desc* d, TailArgs* a, bool* vec, int6
     m.fd_ws = FastDiv((uint32_t)q.window);
   }
   return TERRA_OK;
+}
+
+// Workgroups: what fits the 256 compute units at once; slabs of the rows of a
+// sample so that every workgroup has a unit, and rows enough for its groups.
+TailBwdPlan tail_bwd_plan(uint32_t rows, int C, int gate_rows, int x_dtype) {
+  TailBwdPlan p;
+  p.shape = tail_shape(C, tail_pieces(x_dtype), tail_bwd_most(x_dtype));
+  const uint32_t groups = (uint32_t)(tail_threads(p.shape.lanes) / p.shape.lanes);
+  const uint32_t most = p.shape.lanes > 256 ? 512u / (uint32_t)p.shape.chunks : (p.shape.chunks > 1 ? 512u : 1024u);
+  const uint32_t samples = gate_rows > 1 ? (uint32_t)gate_rows : 1u, per = rows / samples;
+  uint32_t slabs = (most + samples - 1) / samples;
+  const uint32_t useful = (per + groups - 1) / groups;
+  if (slabs > useful) slabs = useful;
+  p.slabs = slabs;
+  p.units = p.slabs * samples;
+  p.blocks = p.units < most ? p.units : most;
+  return p;
+}
+
+// f of the launches for the call's types.
+#define TERRA_TAIL_LAUNCHES(h, x)                                                                    \
+  struct Launch_##h##_##x {                                                                          \
+    static void fwd(const void* a, bool vec, hipStream_t s) { tail_fwd_##h##_##x(a, vec, s); }       \
+    static void bwd(const void* a, const TailBwdPlan& p, bool vec, hipStream_t s) { tail_bwd_##h##_##x(a, p, vec, s); } \
+  };
+TERRA_TAIL_TYPES(TERRA_TAIL_LAUNCHES)
+
+template <typename F>
+void by_type(const terra_swin_residual_norm_desc* d, F f) {
+  const bool f32 = d->x_dtype == TERRA_DTYPE_F32;
+  if (d->h_dtype == TERRA_DTYPE_F32) f(Launch_f32_f32{});
+  else if (d->h_dtype == TERRA_DTYPE_BF16) f32 ? f(Launch_bf16_f32{}) : f(Launch_bf16_bf16{});
+  else f32 ? f(Launch_f16_f32{}) : f(Launch_f16_f16{});
 }
 
 // Alignment of a tensor's or a parameter's pointer; NULL where it may be left out.
@@ -249,33 +162,29 @@ extern "C" int terra_swin_residual_norm(const void* h, const void* x, void* y, v
   int64_t h_rows = 0;
   TERRA_TRY(prepare(desc, &a, &vec, &h_rows));
   TERRA_TRY(dropout_args(desc->p, seed, desc->stream_id, &a.drop));
+  if (a.drop.threshold > 0) a.flags |= kTailDrop;
   if (a.rows == 0) return TERRA_OK;
   const int he = dtype_size(desc->h_dtype), xe = dtype_size(desc->x_dtype);
   TERRA_TRY(check_pointer(h, he, "h", true, &vec));
   TERRA_TRY(check_pointer(x, xe, "x", true, &vec));
   TERRA_TRY(check_pointer(y, xe, "y", true, &vec));
-  TERRA_TRY(check_pointer(z, he, "z", a.next != TERRA_NORM_NONE, &vec));
+  TERRA_TRY(check_pointer(z, he, "z", (a.flags & kTailNext) != 0, &vec));
   TERRA_TRY(check_pointer(gate, 4, "gate", a.gate_rows > 0, &vec));
   for (const float* p : {post_weight, post_bias, next_weight, next_bias})
     TERRA_TRY(check_pointer(p, 4, "a norm's parameter", false, &vec));
   const int64_t C = a.C;
-  if (a.next == TERRA_NORM_NONE) z = nullptr;
+  if ((a.flags & kTailNext) == 0) z = nullptr;
   TERRA_TRY(check_spans({{h, span_bytes(h_rows, a.h_row_bytes, C * he), "h"}, {x, span_bytes(a.rows, a.x_row_bytes, C * xe), "x"}},
                         {{y, a.rows * C * xe, "y"}, {z, a.rows * C * he, "z"}}));
   a.h = (const uint8_t*)h;
   a.x = (const uint8_t*)x;
   a.y = (uint8_t*)y;
   a.z = (uint8_t*)z;
-  if (a.post != TERRA_NORM_NONE) a.pw = post_weight, a.pb = post_bias;
-  if (a.next != TERRA_NORM_NONE) a.nw = next_weight, a.nb = next_bias;
+  if ((a.flags & kTailPost) != 0) a.pw = post_weight, a.pb = post_bias;
+  if ((a.flags & kTailNext) != 0) a.nw = next_weight, a.nb = next_bias;
   a.gate = gate;
   hipStream_t s = (hipStream_t)stream;
-  const int hd = desc->h_dtype, xd = desc->x_dtype;
-  if (hd == TERRA_DTYPE_F32) dispatch<TERRA_DTYPE_F32, TERRA_DTYPE_F32>(a, vec, s);
-  else if (hd == TERRA_DTYPE_BF16 && xd == TERRA_DTYPE_BF16) dispatch<TERRA_DTYPE_BF16, TERRA_DTYPE_BF16>(a, vec, s);
-  else if (hd == TERRA_DTYPE_BF16) dispatch<TERRA_DTYPE_BF16, TERRA_DTYPE_F32>(a, vec, s);
-  else if (xd == TERRA_DTYPE_F16) dispatch<TERRA_DTYPE_F16, TERRA_DTYPE_F16>(a, vec, s);
-  else dispatch<TERRA_DTYPE_F16, TERRA_DTYPE_F32>(a, vec, s);
+  by_type(desc, [&](auto t) { t.fwd(&a, vec, s); });
   return launched("terra_swin_residual_norm");
 }
 
@@ -289,7 +198,7 @@ extern "C" int terra_swin_residual_norm_workspace(const terra_swin_residual_norm
   int64_t h_rows = 0;
   TERRA_TRY(prepare(desc, &a, &vec, &h_rows));
   if (a.rows == 0) return 0;
-  const TailBwdPlan p = tail_bwd_plan(a.rows, a.C, a.gate_rows, desc->x_dtype == TERRA_DTYPE_F32);
+  const TailBwdPlan p = tail_bwd_plan(a.rows, a.C, a.gate_rows, desc->x_dtype);
   return (int)(p.blocks * 4 * a.C + (a.gate_rows > 0 && p.slabs > 1 ? p.units * a.C : 0));
 }
 
@@ -305,14 +214,15 @@ extern "C" int terra_swin_residual_norm_bwd(const void* h, const void* x, const 
   int64_t h_rows = 0;
   TERRA_TRY(prepare(desc, &a, &vec, &h_rows));
   TERRA_TRY(dropout_args(desc->p, seed, desc->stream_id, &a.drop));
+  if (a.drop.threshold > 0) a.flags |= kTailDrop;
   const int he = dtype_size(desc->h_dtype), xe = dtype_size(desc->x_dtype);
   bool ignored = false;
   for (const float* p : {(const float*)dpost_weight, (const float*)dpost_bias, (const float*)dgate,
                          (const float*)dnext_weight, (const float*)dnext_bias, (const float*)workspace})
     TERRA_TRY(check_pointer(p, 4, "a parameter's gradient or the workspace", false, &ignored));
-  if (a.post == TERRA_NORM_NONE && (dpost_weight != nullptr || dpost_bias != nullptr))
+  if ((a.flags & kTailPost) == 0 && (dpost_weight != nullptr || dpost_bias != nullptr))
     return fail(TERRA_ERR_SHAPE, "gradients of a post-norm that the call has not");
-  if (a.next == TERRA_NORM_NONE && (dz != nullptr || dnext_weight != nullptr || dnext_bias != nullptr))
+  if ((a.flags & kTailNext) == 0 && (dz != nullptr || dnext_weight != nullptr || dnext_bias != nullptr))
     return fail(TERRA_ERR_SHAPE, "gradients of a next norm that the call has not");
   if (dgate != nullptr && desc->gate_rows == 0) return fail(TERRA_ERR_SHAPE, "the gradient of a gate that the call has not");
   hipStream_t s = (hipStream_t)stream;
@@ -347,10 +257,12 @@ extern "C" int terra_swin_residual_norm_bwd(const void* h, const void* x, const 
   a.dz = (const uint8_t*)dz;
   a.dh = (uint8_t*)dh;
   a.dx = (uint8_t*)dx;
-  if (a.post != TERRA_NORM_NONE) a.pw = post_weight, a.pb = post_bias;
-  if (a.next != TERRA_NORM_NONE) a.nw = next_weight;
+  if ((a.flags & kTailPost) != 0) a.pw = post_weight, a.pb = post_bias;
+  if ((a.flags & kTailNext) != 0) a.nw = next_weight;
+  if (dz == nullptr) a.flags &= ~kTailNext;
+  if (dy != nullptr) a.flags |= kTailDy;
   a.gate = gate;
-  const TailBwdPlan p = tail_bwd_plan(a.rows, a.C, a.gate_rows, desc->x_dtype == TERRA_DTYPE_F32);
+  const TailBwdPlan p = tail_bwd_plan(a.rows, a.C, a.gate_rows, desc->x_dtype);
   a.slabs = p.slabs;
   a.units = p.units;
   a.partial = sums ? workspace : nullptr;
@@ -359,7 +271,7 @@ extern "C" int terra_swin_residual_norm_bwd(const void* h, const void* x, const 
   const bool direct = dgate != nullptr && p.slabs == 1;
   float* units = workspace + (int64_t)p.blocks * 4 * C;
   a.gate_partial = dgate == nullptr ? nullptr : (direct ? dgate : units);
-  TERRA_TRY(launch_tail_bwd(desc->h_dtype, desc->x_dtype, &a, p, vec, s));
+  by_type(desc, [&](auto t) { t.bwd(&a, p, vec, s); });
   float* dst[4] = {dpost_weight, dpost_bias, dnext_weight, dnext_bias};
   for (int i = 0; i < 4; ++i)
     if (dst[i] != nullptr) jobs.job[n++] = {workspace + i * C, dst[i], 4 * C, (int32_t)p.blocks, 1};

@@ -21,13 +21,15 @@
 // each lane keeps the sums of its columns in registers; A and B leave them unit by unit, since the gate changes
 // with the sample.  A second launch adds the workgroups' sums
 // (sum_partials_kernel): no atomics, an order that the sizes fix.
+#pragma once
+
 #include "residual_norm.h"
 
 namespace terra {
 namespace {
 
-template <int DTH, int DTX, int kG, int kK, bool kVec>
-__global__ __launch_bounds__(tail_threads(kG)) void tail_bwd_kernel(const TailArgs a) {
+template <int DTH, int DTX, int kG, int kK, bool kVec, int kF>
+__global__ __launch_bounds__(tail_threads(kG), kG == 512 && kK == 1 ? 4 : (kK == 3 ? 2 : 1)) void tail_bwd_kernel(const TailArgs a) {
   constexpr int kThreads = tail_threads(kG), kGroups = kThreads / kG, kCols = kG * kK * kChunkCols;
   constexpr int kHB = ChunkElt<DTH>::kBytes, kXB = ChunkElt<DTX>::kBytes;
   constexpr int kP = DTX == TERRA_DTYPE_F32 ? 4 : 8;
@@ -38,6 +40,7 @@ __global__ __launch_bounds__(tail_threads(kG)) void tail_bwd_kernel(const TailAr
   const int group = threadIdx.x / kG, C = a.C;
   const RowLanes<kG, kK, kP> at = {(int)(threadIdx.x % kG), C};
   RowSum<kG> sum(&s_red);
+  const bool full = C == kG * kK * kChunkCols;  // every lane has columns
   Params par(&s_par);  // gw, gb, w2
   auto stage = [&](const float* gate) {
     par.fill(at, [&](int c, float (&v)[3]) {
@@ -47,7 +50,7 @@ __global__ __launch_bounds__(tail_threads(kG)) void tail_bwd_kernel(const TailAr
   };
   stage(a.gate_rows == 1 ? a.gate : nullptr);
   if constexpr (Params::kLds) __syncthreads();
-  const uint64_t seed = a.drop.threshold > 0 ? *a.drop.seed : 0;
+  const uint64_t seed = tail_has<kF>(a, kTailDrop) ? *a.drop.seed : 0;
 
   float acc_a[kK][kChunkCols] = {}, acc_b[kK][kChunkCols] = {}, acc_nw[kK][kChunkCols] = {}, acc_nb[kK][kChunkCols] = {};
   // The workgroup's sums of two vectors over its row groups, given to f(column, sum, other).
@@ -106,14 +109,14 @@ __global__ __launch_bounds__(tail_threads(kG)) void tail_bwd_kernel(const TailAr
       const uint32_t row = base + group;
       const bool live = row < end;
       const uint32_t r = live ? row : end - 1;  // a row past the end re-reads the sample's last one
-      const int64_t src = a.windows ? a.map.source(r) : (int64_t)r;
+      const int64_t src = a.flags & kTailWindows ? a.map.source(r) : (int64_t)r;
       const bool has = src >= 0;
       RowChunk<DTH> hq[kK], dzq[kK];
       RowChunk<DTX> xq[kK], dyq[kK];
       const uint8_t* hp = a.h + (has ? src : 0) * a.h_row_bytes;
       const uint8_t* xp = a.x + (int64_t)r * a.x_row_bytes;
-      const uint8_t* dyp = a.dy != nullptr ? a.dy + (int64_t)r * C * kXB : xp;
-      const uint8_t* dzp = a.dz != nullptr ? a.dz + (int64_t)r * C * kHB : hp;
+      const uint8_t* dyp = a.flags & kTailDy ? a.dy + (int64_t)r * C * kXB : xp;
+      const uint8_t* dzp = tail_has<kF>(a, kTailNext) ? a.dz + (int64_t)r * C * kHB : hp;
 #pragma unroll
       for (int k = 0; k < kK; ++k) {
         hq[k] = at.template load<DTH, kVec>(hp, k);
@@ -126,41 +129,35 @@ __global__ __launch_bounds__(tail_threads(kG)) void tail_bwd_kernel(const TailAr
       ChunkDraws draws[kK];
 #pragma unroll
       for (int k = 0; k < kK; ++k) {
-        at.template values<DTH, kVec>(hq[k], k, has, nv[k]);
+        at.template values<DTH, kVec>(hq[k], k, has, full && !(a.flags & kTailWindows), nv[k]);
       }
       float r1 = 1.f;
-      if (a.post != TERRA_NORM_NONE) r1 = normalise<kG, kK, kP, kVec>(nv, a.post, a.post_eps, a.inv_c, at, sum);
-      if (a.drop.threshold > 0)
+      if (tail_has<kF>(a, kTailPost)) r1 = normalise<kG, kK, kP, kVec>(nv, a.flags & kTailPostLayer, a.post_eps, a.inv_c, at, sum);
 #pragma unroll
-        for (int k = 0; k < kK; ++k) {
-          draws[k] = at.draws(seed, k, r, a.drop.stream);
-          // NaN and infinities of the branch stay out of A where they are dropped.
-          if (a.post == TERRA_NORM_NONE)
+      for (int k = 0; k < kK; ++k) draws[k] = at.draws(tail_has<kF>(a, kTailDrop), seed, k, r, a.drop.stream);
+      if (!tail_has<kF>(a, kTailPost) && tail_has<kF>(a, kTailDrop))  // NaN and infinities of the branch stay out of A where they are dropped
 #pragma unroll
-            for (int j = 0; j < kChunkCols; ++j) nv[k][j] = kept(draws[k], j, a.drop.threshold) ? nv[k][j] : 0.f;
-        }
-      if (a.next != TERRA_NORM_NONE && a.dz != nullptr) {
+        for (int k = 0; k < kK; ++k)
+#pragma unroll
+          for (int j = 0; j < kChunkCols; ++j) nv[k][j] = kept(draws[k], j, a.drop.threshold) ? nv[k][j] : 0.f;
+      if (tail_has<kF>(a, kTailNext)) {
 #pragma unroll
         for (int k = 0; k < kK; ++k) {
           float gw[kChunkCols], gb[kChunkCols], xv[kChunkCols];
           par.get(0, k, at, gw);
           par.get(1, k, at, gb);
-          at.template values<DTX, kVec>(xq[k], k, true, xv);
+          at.template values<DTX, kVec>(xq[k], k, true, full, xv);
 #pragma unroll
-          for (int j = 0; j < kChunkCols; ++j) yv[k][j] = has ? fmaf(nv[k][j], gw[j], gb[j]) : 0.f;
-          if (a.drop.threshold > 0)
-#pragma unroll
-            for (int j = 0; j < kChunkCols; ++j) yv[k][j] = kept(draws[k], j, a.drop.threshold) ? yv[k][j] : 0.f;
-#pragma unroll
-          for (int j = 0; j < kChunkCols; ++j) yv[k][j] = fmaf(a.alpha, xv[j], yv[k][j]);
+          for (int j = 0; j < kChunkCols; ++j)
+            yv[k][j] = fmaf(a.alpha, xv[j], has && kept(draws[k], j, a.drop.threshold) ? fmaf(nv[k][j], gw[j], gb[j]) : 0.f);
         }
-        const float r2 = normalise<kG, kK, kP, kVec>(yv, a.next, a.next_eps, a.inv_c, at, sum);
+        const float r2 = normalise<kG, kK, kP, kVec>(yv, a.flags & kTailNextLayer, a.next_eps, a.inv_c, at, sum);
         float s0 = 0.f, s1 = 0.f;
 #pragma unroll
         for (int k = 0; k < kK; ++k) {
           float w[kChunkCols];
           par.get(2, k, at, w);
-          at.template values<DTH, kVec>(dzq[k], k, true, dv[k]);
+          at.template values<DTH, kVec>(dzq[k], k, true, full, dv[k]);
           if (live)
 #pragma unroll
             for (int j = 0; j < kChunkCols; ++j) {
@@ -175,19 +172,25 @@ __global__ __launch_bounds__(tail_threads(kG)) void tail_bwd_kernel(const TailAr
           }
         }
         sum.two(s0, s1);
-        s0 = a.next == TERRA_NORM_LAYER ? s0 * a.inv_c : 0.f;
-        s1 *= a.inv_c;
+        s0 = a.flags & kTailNextLayer ? r2 * (s0 * a.inv_c) : 0.f;
+        s1 = r2 * (s1 * a.inv_c);
 #pragma unroll
         for (int k = 0; k < kK; ++k) {
           float dyv[kChunkCols];
-          at.template values<DTX, kVec>(dyq[k], k, a.dy != nullptr, dyv);
+          at.template values<DTX, kVec>(dyq[k], k, true, full, dyv);
+          if (!(a.flags & kTailDy))
 #pragma unroll
-          for (int j = 0; j < kChunkCols; ++j) dv[k][j] = fmaf(r2, fmaf(-yv[k][j], s1, dv[k][j] - s0), dyv[j]);
+            for (int j = 0; j < kChunkCols; ++j) dyv[j] = 0.f;
+#pragma unroll
+          for (int j = 0; j < kChunkCols; ++j) dv[k][j] = fmaf(r2, dv[k][j], fmaf(-s1, yv[k][j], dyv[j] - s0));
         }
       } else {
 #pragma unroll
         for (int k = 0; k < kK; ++k) {
-          at.template values<DTX, kVec>(dyq[k], k, a.dy != nullptr, dv[k]);
+          at.template values<DTX, kVec>(dyq[k], k, true, full, dv[k]);
+          if (!(a.flags & kTailDy))
+#pragma unroll
+            for (int j = 0; j < kChunkCols; ++j) dv[k][j] = 0.f;
         }
       }
       // dv is dY: dx, then t, A and B, then u in dv.
@@ -200,9 +203,8 @@ __global__ __launch_bounds__(tail_threads(kG)) void tail_bwd_kernel(const TailAr
 #pragma unroll
         for (int j = 0; j < kChunkCols; ++j) out[j] = a.alpha * dv[k][j];
         if (live) at.template store<DTX, kVec>(out, dx_out, (uint32_t)(group * C) * kXB, k);
-        if (a.drop.threshold > 0)
 #pragma unroll
-          for (int j = 0; j < kChunkCols; ++j) dv[k][j] = kept(draws[k], j, a.drop.threshold) ? dv[k][j] : 0.f;
+        for (int j = 0; j < kChunkCols; ++j) dv[k][j] = kept(draws[k], j, a.drop.threshold) ? dv[k][j] : 0.f;
         if (live && has)
 #pragma unroll
           for (int j = 0; j < kChunkCols; ++j) {
@@ -217,18 +219,18 @@ __global__ __launch_bounds__(tail_threads(kG)) void tail_bwd_kernel(const TailAr
           s1 = fmaf(dv[k][j], nv[k][j], s1);
         }
       }
-      if (a.post != TERRA_NORM_NONE) {
+      if (tail_has<kF>(a, kTailPost)) {
         sum.two(s0, s1);
-        s0 = a.post == TERRA_NORM_LAYER ? s0 * a.inv_c : 0.f;
-        s1 *= a.inv_c;
+        s0 = a.flags & kTailPostLayer ? r1 * (s0 * a.inv_c) : 0.f;
+        s1 = r1 * (s1 * a.inv_c);
 #pragma unroll
         for (int k = 0; k < kK; ++k)
 #pragma unroll
-          for (int j = 0; j < kChunkCols; ++j) dv[k][j] = r1 * fmaf(-nv[k][j], s1, dv[k][j] - s0);
+          for (int j = 0; j < kChunkCols; ++j) dv[k][j] = fmaf(r1, dv[k][j], fmaf(-s1, nv[k][j], -s0));
       }
       // In window order each row has a place of its own: a descriptor for it
       // would not be uniform over the wave's rows.
-      if (a.windows) {
+      if (a.flags & kTailWindows) {
 #pragma unroll
         for (int k = 0; k < kK; ++k) {
           if (live && has) at.template store<DTH, kVec>(dv[k], a.dh + src * C * kHB, k);
@@ -243,11 +245,10 @@ __global__ __launch_bounds__(tail_threads(kG)) void tail_bwd_kernel(const TailAr
       }
     }
     if (a.branch_sums) {
-      const float scale = a.drop.threshold > 0 ? a.drop.scale : 1.f;
       const bool first = unit == blockIdx.x;
       flush(acc_a, acc_b, [&](int c, float sa, float sb) {
-        sa *= scale;
-        sb *= scale;
+        sa *= a.drop.scale;
+        sb *= a.drop.scale;
         if (a.gate_partial != nullptr)
           a.gate_partial[(int64_t)unit * C + c] = fmaf(param_at(a.pw, 1.f, c), sa, param_at(a.pb, 0.f, c) * sb);
         if (mine != nullptr) {
@@ -262,51 +263,22 @@ __global__ __launch_bounds__(tail_threads(kG)) void tail_bwd_kernel(const TailAr
         for (int j = 0; j < kChunkCols; ++j) acc_a[k][j] = acc_b[k][j] = 0.f;
     }
   }
-  if (mine != nullptr && a.next != TERRA_NORM_NONE)
+  if (mine != nullptr)
     flush(acc_nw, acc_nb, [&](int c, float sw, float sb) {
       mine[2 * C + c] = sw;
       mine[3 * C + c] = sb;
     });
 }
 
-template <int DTH, int DTX, int kG, int kK>
-void launch(const TailArgs& a, const TailBwdPlan& p, bool vec, hipStream_t s) {
-  if (vec) tail_bwd_kernel<DTH, DTX, kG, kK, true><<<p.blocks, tail_threads(kG), 0, s>>>(a);
-  else tail_bwd_kernel<DTH, DTX, kG, kK, false><<<p.blocks, tail_threads(kG), 0, s>>>(a);
+template <int DTH, int DTX, int kG, int kK, bool kVec, int kF>
+void launch_bwd(const TailArgs& a, const TailBwdPlan& p, hipStream_t s) {
+  tail_bwd_kernel<DTH, DTX, kG, kK, kVec, kF><<<p.blocks, tail_threads(kG), 0, s>>>(a);
 }
 
 template <int DTH, int DTX>
-void dispatch(const TailArgs& a, const TailBwdPlan& p, bool vec, hipStream_t s) {
-  TERRA_TAIL_SHAPES(launch, p.shape, a, p, vec, s);
+void dispatch_bwd(const TailArgs& a, const TailBwdPlan& p, bool vec, hipStream_t s) {
+  TERRA_TAIL_SHAPES(launch_bwd, p.shape, (DTX == TERRA_DTYPE_F32 ? 2 : 3), a.flags, vec, a, p, s)
 }
 
 }  // namespace
-
-// Workgroups: what fits the 256 compute units at once; slabs of the rows of a
-// sample so that every workgroup has a unit, and rows enough for its groups.
-TailBwdPlan tail_bwd_plan(uint32_t rows, int C, int gate_rows, bool pieces) {
-  TailBwdPlan p;
-  p.shape = tail_shape(C, pieces);
-  const uint32_t groups = (uint32_t)(tail_threads(p.shape.lanes) / p.shape.lanes);
-  const uint32_t most = p.shape.lanes > 256 ? 256u : (p.shape.chunks > 1 ? 512u : 1024u);
-  const uint32_t samples = gate_rows > 1 ? (uint32_t)gate_rows : 1u, per = rows / samples;
-  uint32_t slabs = (most + samples - 1) / samples;
-  const uint32_t useful = (per + groups - 1) / groups;
-  if (slabs > useful) slabs = useful;
-  p.slabs = slabs;
-  p.units = p.slabs * samples;
-  p.blocks = p.units < most ? p.units : most;
-  return p;
-}
-
-int launch_tail_bwd(int h_dtype, int x_dtype, const void* args, const TailBwdPlan& plan, bool vec, hipStream_t s) {
-  const TailArgs& a = *static_cast<const TailArgs*>(args);
-  if (h_dtype == TERRA_DTYPE_F32) dispatch<TERRA_DTYPE_F32, TERRA_DTYPE_F32>(a, plan, vec, s);
-  else if (h_dtype == TERRA_DTYPE_BF16 && x_dtype == TERRA_DTYPE_BF16) dispatch<TERRA_DTYPE_BF16, TERRA_DTYPE_BF16>(a, plan, vec, s);
-  else if (h_dtype == TERRA_DTYPE_BF16) dispatch<TERRA_DTYPE_BF16, TERRA_DTYPE_F32>(a, plan, vec, s);
-  else if (x_dtype == TERRA_DTYPE_F16) dispatch<TERRA_DTYPE_F16, TERRA_DTYPE_F16>(a, plan, vec, s);
-  else dispatch<TERRA_DTYPE_F16, TERRA_DTYPE_F32>(a, plan, vec, s);
-  return TERRA_OK;
-}
-
 }  // namespace terra

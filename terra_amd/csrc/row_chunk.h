@@ -114,7 +114,7 @@ __device__ __forceinline__ void store_chunk(const float (&f)[kChunkCols], __amdg
 struct DropoutArgs {
   const uint64_t* seed;
   uint32_t threshold;  // 0: nothing is dropped (seed not read); 65536: everything
-  float scale;         // of the kept elements
+  float scale;         // of the kept elements (1 without dropout)
   uint32_t stream;
 };
 
@@ -193,12 +193,9 @@ struct RowSum {
         s->part[turn][threadIdx.x >> 6][1] = b;
       }
       lds_sync();
-      a = b = 0.f;
-#pragma unroll
-      for (int w = 0; w < kWaves; ++w) {
-        a += s->part[turn][w][0];
-        b += s->part[turn][w][1];
-      }
+      const float* p = s->part[turn][threadIdx.x % kWaves];  // one wave's sums a lane, then over those lanes
+      a = waves_sum(p[0]);
+      b = waves_sum(p[1]);
       turn ^= 1;
     }
   }
@@ -207,6 +204,12 @@ struct RowSum {
     float b = 0.f;
     two(a, b);
     return a;
+  }
+  static __device__ __forceinline__ float waves_sum(float v) {
+    static_assert(kG <= 64 || kWaves == 4 || kWaves == 8, "waves of a row");
+    if constexpr (kWaves == 8) return group8_sum(v);
+    v += dpp_move<0xb1>(v);
+    return v + dpp_move<0x4e>(v);
   }
   // A workgroup barrier that waits for LDS only: loads of rows ahead stay in flight.
   static __device__ __forceinline__ void lds_sync() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
