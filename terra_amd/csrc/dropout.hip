@@ -38,14 +38,46 @@ struct DropParams {
   int32_t T, R;
 };
 
-// Phi(h) by erfc, which keeps its relative precision for h << 0.
-__device__ __forceinline__ float normal_cdf(float h) { return 0.5f * erfcf(-0.70710678118654752f * h); }
+// Phi(h) and, up to 1 / sqrt(2 pi), phi(h).  With a = |h| and e = exp(-a^2 / 2),
+// Phi(-a) = e G(a), where G(a) = erfcx(a / sqrt 2) / 2 falls smoothly from 1/2 like
+// 1 / a: a polynomial of degree 8 in u = 1 / (1 + 0.3 a) without a constant term,
+// fitted to the least largest relative error over 0 <= a <= 14 (1.5e-7; in fp32
+// 4.4e-7 relative for h < 0, 1.7e-7 absolute), so the tail keeps its relative
+// precision.  About 20 instructions, of which exp2 and the reciprocal go to the
+// transcendental unit; erfcf and expf took three times as many.
+__device__ __forceinline__ void normal_parts(float h, float& cdf, float& e) {
+  const float a = fabsf(h);
+  const float u = __builtin_amdgcn_rcpf(fmaf(0.3f, a, 1.f));
+  e = __builtin_amdgcn_exp2f(-0.72134752044448170f * (h * h));
+  float p = 0.0356753467f;
+  p = fmaf(p, u, -0.157205686f);
+  p = fmaf(p, u, 0.20635832f);
+  p = fmaf(p, u, -0.0536883323f);
+  p = fmaf(p, u, 0.128564218f);
+  p = fmaf(p, u, 0.0999126806f);
+  p = fmaf(p, u, 0.120754089f);
+  p = fmaf(p, u, 0.11962929f);
+  const float q = p * u * e;
+  cdf = h > 0.f ? 1.f - q : q;
+}
+
+__device__ __forceinline__ float gelu_factor(float h) {
+  float cdf, e;
+  normal_parts(h, cdf, e);
+  return cdf;
+}
+
+__device__ __forceinline__ float gelu_slope_of(float h) {
+  float cdf, e;
+  normal_parts(h, cdf, e);
+  return fmaf(0.39894228040143268f * h, e, cdf);
+}
 
 template <int kOp>
 __device__ __forceinline__ float drop_value(float v, float h) {
   if constexpr (kOp == kDropout) return v;
-  else if constexpr (kOp == kGeluFwd) return v * normal_cdf(v);
-  else return v * (normal_cdf(h) + h * (0.39894228040143268f * expf(-0.5f * h * h)));
+  else if constexpr (kOp == kGeluFwd) return v * gelu_factor(v);
+  else return v * gelu_slope_of(h);
 }
 
 template <int kOp, int DT, bool kVec>
