@@ -10,8 +10,12 @@
 // A dropped element is 0 whatever its value was.  Each value is computed in
 // fp32 and rounded once.
 //
-// Layout: a thread owns one chunk column and steps through rows, so column
-// sums stay in its registers; a workgroup is T chunk columns by R rows.
+// Layout: a thread owns eight columns and steps through rows, so column sums
+// stay in its registers; a workgroup is T such threads by R rows.
+//
+// Bound by memory: 2 values an element moved, 3 in the backward.  524288 x 768:
+// dropout bf16 271 us and fp32 (262144 rows) 275, GELU 318, backward 410, with
+// column sums 479; a large copy moves the same bytes in 310, 310, 310, 465, 465.
 #include "gelu.h"
 #include "row_chunk.h"
 
@@ -73,23 +77,76 @@ __device__ __forceinline__ float gelu_slope_of(float h) {
   return fmaf(0.39894228040143268f * h, e, cdf);
 }
 
+// What an element is multiplied by, without the mask: s, s Phi(h), or s times the slope at h.
 template <int kOp>
-__device__ __forceinline__ float drop_value(float v, float h) {
-  if constexpr (kOp == kDropout) return v;
-  else if constexpr (kOp == kGeluFwd) return v * gelu_factor(v);
-  else return v * gelu_slope_of(h);
+__device__ __forceinline__ float drop_factor(float h, float scale) {
+  if constexpr (kOp == kDropout) return scale;
+  else if constexpr (kOp == kGeluFwd) return gelu_factor(h) * scale;
+  else return gelu_slope_of(h) * scale;
 }
 
-template <int kOp, int DT, bool kVec>
+// The same by table for a bf16 h: one of 2^16 values, of which those with
+// 2^-12 <= |h| < 16 are read from an fp32 table that the workgroup fills with
+// drop_factor (gelu.h's layout); beyond 16 the last entries are the limits (1
+// and 0, exp(-127) being 0 in fp32), and a wave with a smaller value, an infinity or
+// a NaN computes its chunk.  For the forward, which is bound by instructions
+// without it (524288 x 768: 318 us against 390); the backward reads a third more and is as fast without (492 against 495).
+template <int kOp>
+__device__ __forceinline__ void table_factors(const stream_u32x4& h, const uint8_t* table, float scale, float (&f)[kChunkCols]) {
+  u16x2 dmax = {0, 0};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) slope_pair(h[i], table, dmax, f[2 * i], f[2 * i + 1]);
+  const uint32_t dm = dmax.x > dmax.y ? dmax.x : dmax.y;
+  if (__builtin_amdgcn_ballot_w64(dm >= kSlopeRare) != 0)
+#pragma unroll
+    for (int j = 0; j < kChunkCols; ++j)
+      f[j] = drop_factor<kOp>(__uint_as_float(j & 1 ? h[j >> 1] & 0xffff0000u : h[j >> 1] << 16), scale);
+}
+
+template <int kOp, int DT, bool kVec, bool kTable>
 __global__ __launch_bounds__(kDropThreads) void drop_kernel(const DropParams a) {
   constexpr int kB = ChunkElt<DT>::kBytes;
   constexpr bool kBwd = kOp >= kGeluBwd;
   constexpr bool kSum = kOp == kGeluBwdSum;
   __shared__ float s_sum[kSum ? kDropThreads * kChunkCols : 1];
+  static_assert(!kTable || (kVec && DT == TERRA_DTYPE_BF16 && kOp == kGeluFwd), "the table is of bf16 values");
+  __shared__ __attribute__((aligned(16))) float s_table[kTable ? 2 * kSlopeTabSpan : 4];
+  if constexpr (kTable) {
+    for (int e = threadIdx.x; e < 2 * kSlopeTabSpan; e += blockDim.x) {
+      const uint32_t bits = e < kSlopeTabSpan ? kSlopeTabLo + e : 0x8000u + kSlopeTabLo + (e - kSlopeTabSpan);
+      s_table[e] = drop_factor<kOp>(__uint_as_float(bits << 16), a.drop.scale);
+    }
+    __syncthreads();
+  }
   const int tc = threadIdx.x % a.T, tr = threadIdx.x / a.T;
-  const int chunk = blockIdx.y * a.T + tc, col = chunk * kChunkCols;
-  const bool present = tr < a.R && col < a.C;
-  const int64_t strip = (int64_t)blockIdx.y * a.T * kChunkCols * kB;  // bytes before this strip of columns
+  const int strip_col = blockIdx.y * a.T * kChunkCols;
+  const int64_t strip = (int64_t)strip_col * kB;  // bytes before this strip of columns
+  // The thread's columns: c[0] .. c[0] + 3 and c[1] .. c[1] + 3 of the strip (see row_chunk.h).
+  const int c[2] = {kB == 2 ? tc * 8 : tc * 4, kB == 2 ? tc * 8 + 4 : (tc + a.T) * 4};
+  const int width = a.C - strip_col;  // columns from the strip's first one on
+  const bool present = tr < a.R && c[0] < width;
+  auto load = [&](const uint8_t* row) {
+    RowChunk<DT> r;
+    if constexpr (kVec) {
+#pragma unroll
+      for (int q = 0; q < RowChunk<DT>::kWords; ++q)
+        r.q[q] = __builtin_nontemporal_load(
+            reinterpret_cast<const stream_u32x4*>(row + (present && c[q] < width ? strip + c[q] * kB : 0)));
+    } else {
+#pragma unroll
+      for (int j = 0; j < kChunkCols; ++j) {
+        const int at = c[j >> 2] + (j & 3);
+        const int64_t col = present && at < width ? strip_col + at : 0;
+        if constexpr (kB == 4) {
+          r.q[j >> 2][j & 3] = reinterpret_cast<const uint32_t*>(row)[col];
+        } else {
+          const uint32_t v = reinterpret_cast<const uint16_t*>(row)[col];
+          r.q[0][j >> 1] = j & 1 ? r.q[0][j >> 1] | (v << 16) : v;
+        }
+      }
+    }
+    return r;
+  };
   const uint64_t seed = a.drop.threshold > 0 ? *a.drop.seed : 0;
   float acc[kSum ? kChunkCols : 1];
   if constexpr (kSum)
@@ -103,8 +160,8 @@ __global__ __launch_bounds__(kDropThreads) void drop_kernel(const DropParams a) 
     for (int i = 0; i < kDropRows; ++i) {
       const uint64_t row = r0 + (uint64_t)(i * a.R + tr);
       const int64_t r = row < a.rows ? (int64_t)row : (int64_t)a.rows - 1;  // a row past the end re-reads the last one
-      v[i] = load_chunk<DT, kVec>(a.in + r * a.in_row_bytes, col, a.C, present);
-      if constexpr (kBwd) hv[i] = load_chunk<DT, kVec>(a.h + r * a.row_bytes, col, a.C, present);
+      v[i] = load(a.in + r * a.in_row_bytes);
+      if constexpr (kBwd) hv[i] = load(a.h + r * a.row_bytes);
     }
 #pragma unroll
     for (int i = 0; i < kDropRows; ++i) {
@@ -116,43 +173,71 @@ __global__ __launch_bounds__(kDropThreads) void drop_kernel(const DropParams a) 
       const __amdgpu_buffer_rsrc_t out =
           buffer_rsrc(a.out + (int64_t)base * a.row_bytes + strip, (uint32_t)(left < 0x7fffffff ? left : 0x7fffffff));
       if (!present || (uint32_t)tr >= live) continue;
-      float f[kChunkCols], g[kChunkCols];
+      float f[kChunkCols], w[kChunkCols];
+      const RowChunk<DT>& at = kBwd ? hv[i] : v[i];  // where the factor is taken
+      if constexpr (kTable) {
+        table_factors<kOp>(at.q[0], reinterpret_cast<const uint8_t*>(s_table), a.drop.scale, w);
+      } else {
 #pragma unroll
-      for (int j = 0; j < kChunkCols; ++j) {
-        f[j] = chunk_value<DT>(v[i], j);
-        if constexpr (kBwd) g[j] = chunk_value<DT>(hv[i], j);
+        for (int j = 0; j < kChunkCols; ++j) w[j] = drop_factor<kOp>(chunk_value<DT>(at, j), a.drop.scale);
       }
 #pragma unroll
-      for (int j = 0; j < kChunkCols; ++j) f[j] = drop_value<kOp>(f[j], kBwd ? g[j] : 0.f);
+      for (int j = 0; j < kChunkCols; ++j) f[j] = chunk_value<DT>(v[i], j) * w[j];
       if (a.drop.threshold > 0) {
-        const ChunkDraws d = chunk_draws(seed, (uint32_t)chunk, (uint32_t)base + (uint32_t)tr, a.drop.stream);
+        const uint32_t row = (uint32_t)base + (uint32_t)tr, first = (uint32_t)((strip_col + c[0]) / kChunkCols);
+        const ChunkDraws d = kB == 2 ? chunk_draws(seed, first, row, a.drop.stream)
+                                     : half_draws(seed, tc & 1, first, first + a.T / 2, row, a.drop.stream);
 #pragma unroll
-        for (int j = 0; j < kChunkCols; ++j) f[j] = kept(d, j, a.drop.threshold) ? f[j] * a.drop.scale : 0.f;
+        for (int j = 0; j < kChunkCols; ++j) f[j] = kept(d, j, a.drop.threshold) ? f[j] : 0.f;
       }
       if constexpr (kSum)
 #pragma unroll
         for (int j = 0; j < kChunkCols; ++j) acc[j] += f[j];
-      store_chunk<DT, kVec>(f, out, (uint32_t)((int64_t)tr * a.row_bytes) + (uint32_t)(tc * kChunkCols * kB), col, a.C);
+      const uint32_t off = (uint32_t)((int64_t)tr * a.row_bytes);
+      if constexpr (kVec && kB == 2) {
+        stream_store_sc1(stream_u32x4{pack2<DT>(f[0], f[1]), pack2<DT>(f[2], f[3]), pack2<DT>(f[4], f[5]),
+                                      pack2<DT>(f[6], f[7])}, out, off + (uint32_t)(c[0] * kB));
+      } else if constexpr (kVec) {
+#pragma unroll
+        for (int q = 0; q < 2; ++q)
+          if (c[q] < width)
+            stream_store_sc1(stream_u32x4{__float_as_uint(f[4 * q]), __float_as_uint(f[4 * q + 1]),
+                                          __float_as_uint(f[4 * q + 2]), __float_as_uint(f[4 * q + 3])}, out,
+                             off + (uint32_t)(c[q] * kB));
+      } else {
+#pragma unroll
+        for (int j = 0; j < kChunkCols; ++j) {
+          const int at = c[j >> 2] + (j & 3);
+          if (at >= width) continue;
+          if constexpr (kB == 4) stream_store_sc1(__float_as_uint(f[j]), out, off + (uint32_t)(at * kB));
+          else stream_store_sc1((uint16_t)pack2<DT>(f[j], 0.f), out, off + (uint32_t)(at * kB));
+        }
+      }
     }
   }
   if constexpr (kSum) {
-    const int width = a.T * kChunkCols;
+    const int cols = a.T * kChunkCols;  // of the strip
     if (tr < a.R)
 #pragma unroll
-      for (int j = 0; j < kChunkCols; ++j) s_sum[tr * width + tc * kChunkCols + j] = acc[j];
+      for (int j = 0; j < kChunkCols; ++j) s_sum[tr * cols + c[j >> 2] + (j & 3)] = acc[j];
     __syncthreads();
-    for (int c = threadIdx.x; c < width; c += blockDim.x) {
-      const int out_col = blockIdx.y * width + c;
-      if (out_col >= a.C) break;
+    for (int at = threadIdx.x; at < cols && at < width; at += blockDim.x) {
       float sum = 0.f;
-      for (int r = 0; r < a.R; ++r) sum += s_sum[r * width + c];
-      a.partial[(int64_t)blockIdx.x * a.C + out_col] = sum;
+      for (int r = 0; r < a.R; ++r) sum += s_sum[r * cols + at];
+      a.partial[(int64_t)blockIdx.x * a.C + strip_col + at] = sum;
     }
   }
 }
 
-// Workgroups that sum columns: about eight for each of the 256 compute units.
-constexpr int kSumBlocks = 2048;
+// Workgroups that stay for many rows: those that sum columns, whose number is
+// also that of the partial sums to write and to add (524288 x 768 bf16: 479 us
+// with 1024, 486 with 2048, 513 with 4096, 570 with 768; without sums, a
+// workgroup for every four rows a thread, 410), and those that fill a table (309
+// with 2048, 329 with 1024).
+constexpr int kSumBlocks = 1024, kTableBlocks = 2048;
+
+// Elements from which the forward's table pays (50176 x 512: 22.8 us, without it 33.9; 8192 x 512 7.2 and 6.9).
+constexpr int64_t kTableElements = 1ll << 22;
 
 struct DropPlan {
   int32_t T, R, strips;
@@ -160,32 +245,45 @@ struct DropPlan {
 };
 
 // T chunk columns by R rows of threads; column strips where a row has more chunks than a workgroup threads.
-DropPlan drop_plan(int64_t rows, int C, bool sums) {
+DropPlan drop_plan(int64_t rows, int C, bool pieces, int64_t stay) {
   DropPlan p;
   const int chunks = (C - 1) / kChunkCols + 1;
   p.strips = (chunks - 1) / kDropThreads + 1;
   p.T = (chunks - 1) / p.strips + 1;
+  p.T += pieces ? p.T & 1 : 0;  // lanes of a row in pairs
   p.R = kDropThreads / p.T;
   const int64_t per_block = (int64_t)p.R * kDropRows;
   p.blocks = (rows + per_block - 1) / per_block;
-  const int64_t most = sums ? (kSumBlocks + p.strips - 1) / p.strips : (1ll << 22);  // a grid dimension holds fewer than 2^32 threads
+  // without a number, what a grid dimension of fewer than 2^32 threads holds
+  const int64_t most = stay > 0 ? (stay + p.strips - 1) / p.strips : (1ll << 22);
   if (p.blocks > most) p.blocks = most;
   return p;
 }
 
+// Whether a call takes its GELU factors from a table.
+bool drop_table(int op, int dtype, int64_t rows, int64_t C, bool vec) {
+  return op == kGeluFwd && dtype == TERRA_DTYPE_BF16 && vec && rows * C >= kTableElements;
+}
+
 template <int kOp, int DT>
-void launch_drop(const DropParams& a, const DropPlan& p, bool vec, hipStream_t s) {
+void launch_drop(DropParams a, bool vec, hipStream_t s) {
+  const bool table = drop_table(kOp, DT, a.rows, a.C, vec);
+  const DropPlan p = drop_plan(a.rows, a.C, DT == TERRA_DTYPE_F32, table ? kTableBlocks : (kOp == kGeluBwdSum ? kSumBlocks : 0));
+  a.T = p.T;
+  a.R = p.R;
   const dim3 grid((unsigned)p.blocks, (unsigned)p.strips);
   const int threads = (p.T * p.R + 63) / 64 * 64;
-  if (vec) drop_kernel<kOp, DT, true><<<grid, threads, 0, s>>>(a);
-  else drop_kernel<kOp, DT, false><<<grid, threads, 0, s>>>(a);
+  if constexpr (kOp == kGeluFwd && DT == TERRA_DTYPE_BF16)
+    if (table) return (void)(drop_kernel<kOp, DT, true, true><<<grid, threads, 0, s>>>(a));
+  if (vec) drop_kernel<kOp, DT, true, false><<<grid, threads, 0, s>>>(a);
+  else drop_kernel<kOp, DT, false, false><<<grid, threads, 0, s>>>(a);
 }
 
 template <int kOp>
-void dispatch_drop(int dtype, const DropParams& a, const DropPlan& p, bool vec, hipStream_t s) {
-  if (dtype == TERRA_DTYPE_F32) launch_drop<kOp, TERRA_DTYPE_F32>(a, p, vec, s);
-  else if (dtype == TERRA_DTYPE_BF16) launch_drop<kOp, TERRA_DTYPE_BF16>(a, p, vec, s);
-  else launch_drop<kOp, TERRA_DTYPE_F16>(a, p, vec, s);
+void dispatch_drop(int dtype, const DropParams& a, bool vec, hipStream_t s) {
+  if (dtype == TERRA_DTYPE_F32) launch_drop<kOp, TERRA_DTYPE_F32>(a, vec, s);
+  else if (dtype == TERRA_DTYPE_BF16) launch_drop<kOp, TERRA_DTYPE_BF16>(a, vec, s);
+  else launch_drop<kOp, TERRA_DTYPE_F16>(a, vec, s);
 }
 
 // The checks that the three entry points share; fills all but the pointers of `a`.
@@ -246,10 +344,7 @@ extern "C" int terra_swin_dropout(const void* x, void* y, int dtype, int64_t row
     return fail(TERRA_ERR_SHAPE, "y may be x itself (of packed rows) and must not overlap it otherwise");
   a.in = (const uint8_t*)x;
   a.out = (uint8_t*)y;
-  const DropPlan plan = drop_plan(rows, (int)columns, false);
-  a.T = plan.T;
-  a.R = plan.R;
-  dispatch_drop<kDropout>(dtype, a, plan, vec, (hipStream_t)stream);
+  dispatch_drop<kDropout>(dtype, a, vec, (hipStream_t)stream);
   return drop_launched("terra_swin_dropout");
 }
 
@@ -265,10 +360,7 @@ extern "C" int terra_swin_gelu_dropout(const void* h, void* a_out, int dtype, in
     return fail(TERRA_ERR_SHAPE, "a may be h itself and must not overlap it otherwise");
   a.in = (const uint8_t*)h;
   a.out = (uint8_t*)a_out;
-  const DropPlan plan = drop_plan(rows, (int)columns, false);
-  a.T = plan.T;
-  a.R = plan.R;
-  dispatch_drop<kGeluFwd>(dtype, a, plan, vec, (hipStream_t)stream);
+  dispatch_drop<kGeluFwd>(dtype, a, vec, (hipStream_t)stream);
   return drop_launched("terra_swin_gelu_dropout");
 }
 
@@ -276,7 +368,7 @@ extern "C" int terra_swin_gelu_dropout_workspace(int64_t rows, int64_t columns) 
   clear_error();
   if (rows < 0 || columns <= 0 || rows >= (1ll << 31) || columns >= (1ll << 24))
     return fail(TERRA_ERR_SHAPE, "at most 2^31 - 1 rows of 1 to 2^24 - 1 columns");
-  return rows == 0 ? 0 : (int)(drop_plan(rows, (int)columns, true).blocks * columns);
+  return rows == 0 ? 0 : (int)(drop_plan(rows, (int)columns, true, kSumBlocks).blocks * columns);
 }
 
 extern "C" int terra_swin_gelu_dropout_bwd(const void* da, const void* h, void* dh, int dtype, int64_t rows,
@@ -307,14 +399,11 @@ extern "C" int terra_swin_gelu_dropout_bwd(const void* da, const void* h, void* 
   a.h = (const uint8_t*)h;
   a.out = (uint8_t*)dh;
   a.partial = workspace;
-  const DropPlan plan = drop_plan(rows, (int)columns, column_sums != nullptr);
-  a.T = plan.T;
-  a.R = plan.R;
   if (column_sums == nullptr) {
-    dispatch_drop<kGeluBwd>(dtype, a, plan, vec, s);
+    dispatch_drop<kGeluBwd>(dtype, a, vec, s);
   } else {
-    dispatch_drop<kGeluBwdSum>(dtype, a, plan, vec, s);
-    jobs.job[0] = {workspace, column_sums, columns, (int32_t)plan.blocks, 1};
+    dispatch_drop<kGeluBwdSum>(dtype, a, vec, s);
+    jobs.job[0] = {workspace, column_sums, columns, (int32_t)drop_plan(rows, (int)columns, dtype == TERRA_DTYPE_F32, kSumBlocks).blocks, 1};
     launch_sums(jobs, 1, s);
   }
   return drop_launched("terra_swin_gelu_dropout_bwd");

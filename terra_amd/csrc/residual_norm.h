@@ -93,7 +93,7 @@ struct TailShape {
 // is accessed 16 bytes, four columns, a lane, neighbouring lanes side by
 // side, and the chunk is two such pieces kG lanes apart: eight columns in a row would
 // be two loads of every other 16 bytes, each line fetched, and worse, written,
-// in two halves (524288 x 192, bf16 h and fp32 x, forward: 365 us against FWDMIX).
+// in two halves (524288 x 192, bf16 h and fp32 x, forward: 365 us against 229).
 template <int kG, int kK, int kP>
 struct RowLanes {
   static_assert(kP == 8 || kP == 4, "columns a lane holds side by side");
@@ -225,19 +225,14 @@ struct RowLanes {
     }
   }
 
-  // The draws of chunk k's eight values.  Where a chunk is two pieces, lanes 2i
-  // and 2i + 1 hold the halves of two chunks of the mask: the even lane
-  // draws the first, the odd one the second, and they swap halves.
-  // Without dropout they are never below the threshold.
+  // The draws of chunk k's eight values; without dropout never below the threshold.
   __device__ __forceinline__ ChunkDraws draws(bool drop, uint64_t seed, int k, uint32_t row, uint32_t stream) const {
     if (!drop) return {{~0u, ~0u, ~0u, ~0u}};
     if constexpr (kP == 8) {
       return chunk_draws(seed, (uint32_t)(lane + kG * k), row, stream);
     } else {
-      const bool odd = lane & 1;
-      const ChunkDraws d = chunk_draws(seed, (uint32_t)((lane >> 1) + kG * k + (odd ? kG / 2 : 0)), row, stream);
-      const uint32_t r0 = lane_xor1(odd ? d.w[0] : d.w[2]), r1 = lane_xor1(odd ? d.w[1] : d.w[3]);
-      return {{odd ? r0 : d.w[0], odd ? r1 : d.w[1], odd ? d.w[2] : r0, odd ? d.w[3] : r1}};
+      const uint32_t first = (uint32_t)((lane >> 1) + kG * k);
+      return half_draws(seed, lane & 1, first, first + kG / 2, row, stream);
     }
   }
 };

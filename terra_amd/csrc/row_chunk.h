@@ -1,11 +1,13 @@
-// Rows in chunks of eight columns, shared by the dropout and residual-norm
-// kernels: loads, stores, the dropout mask of a chunk, and sums over the lanes
-// that hold a row.
+// What the dropout and residual-norm kernels share: the eight values a lane
+// holds of a row, the dropout mask, and sums over lanes and over workgroups.
 //
-// A chunk is the unit of the dropout mask (one Philox call gives its eight
-// 16-bit draws) and of memory access (16 bytes in 16-bit types, two times 16
-// in fp32).  kVec: rows of whole, 16-byte aligned chunks; otherwise the eight
-// columns are accessed one by one and those from C on are absent.
+// A chunk is eight columns, the unit of the dropout mask (one Philox call gives
+// its eight 16-bit draws).  A lane holds eight values as two halves of four
+// columns: one chunk in 16-bit types (16 bytes a load); in fp32 two halves apart,
+// neighbouring lanes side by side (16 bytes a load), so that lanes 2i and 2i + 1
+// hold the halves of two chunks and share their draws.  kVec: rows of whole,
+// 16-byte aligned chunks; otherwise columns are accessed one by one and those
+// from C on are absent.
 #pragma once
 
 #include "common.h"
@@ -23,34 +25,6 @@ struct RowChunk {
   static constexpr int kWords = ChunkElt<DT>::kBytes / 2;
   stream_u32x4 q[kWords];
 };
-
-// The chunk at columns [col, col + 8) of the row at `row`, whose addresses are
-// valid whatever `present` says; a chunk that is not present reads the row's
-// first one, and what was read is discarded by unpack (no branch: a load under
-// one gets a wait of its own at the join).
-template <int DT, bool kVec>
-__device__ __forceinline__ RowChunk<DT> load_chunk(const uint8_t* row, int col, int C, bool present) {
-  constexpr int kB = ChunkElt<DT>::kBytes;
-  RowChunk<DT> r;
-  if constexpr (kVec) {
-    const stream_u32x4* p = reinterpret_cast<const stream_u32x4*>(row + (present ? (int64_t)col * kB : 0));
-#pragma unroll
-    for (int i = 0; i < RowChunk<DT>::kWords; ++i) r.q[i] = __builtin_nontemporal_load(p + i);
-  } else {
-#pragma unroll
-    for (int j = 0; j < kChunkCols; ++j) {
-      const int c = present && col + j < C ? col + j : 0;
-      if constexpr (kB == 4) {
-        r.q[j >> 2][j & 3] = reinterpret_cast<const uint32_t*>(row)[c];
-      } else {
-        const uint32_t v = reinterpret_cast<const uint16_t*>(row)[c];
-        if (j & 1) r.q[0][j >> 1] |= v << 16;
-        else r.q[0][j >> 1] = v;
-      }
-    }
-  }
-  return r;
-}
 
 // Value j of a chunk in fp32.
 template <int DT>
@@ -73,31 +47,6 @@ __device__ __forceinline__ uint32_t pack2(float a, float b) {
     return __builtin_bit_cast(uint32_t, v);
   } else {
     return (uint32_t)__half_as_ushort(__float2half_rn(a)) | ((uint32_t)__half_as_ushort(__float2half_rn(b)) << 16);
-  }
-}
-
-// Stores the chunk's values at byte offset `off` (its first column) of the
-// descriptor's range, rounded once to DT; the caller checks that it is present.
-template <int DT, bool kVec>
-__device__ __forceinline__ void store_chunk(const float (&f)[kChunkCols], __amdgpu_buffer_rsrc_t out, uint32_t off,
-                                            int col, int C) {
-  if constexpr (kVec) {
-    if constexpr (DT == TERRA_DTYPE_F32) {
-      stream_store_sc1(stream_u32x4{__float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]),
-                                    __float_as_uint(f[3])}, out, off);
-      stream_store_sc1(stream_u32x4{__float_as_uint(f[4]), __float_as_uint(f[5]), __float_as_uint(f[6]),
-                                    __float_as_uint(f[7])}, out, off + 16);
-    } else {
-      stream_store_sc1(stream_u32x4{pack2<DT>(f[0], f[1]), pack2<DT>(f[2], f[3]), pack2<DT>(f[4], f[5]),
-                                    pack2<DT>(f[6], f[7])}, out, off);
-    }
-  } else {
-#pragma unroll
-    for (int j = 0; j < kChunkCols; ++j) {
-      if (col + j >= C) break;
-      if constexpr (DT == TERRA_DTYPE_F32) stream_store_sc1(__float_as_uint(f[j]), out, off + 4 * j);
-      else stream_store_sc1((uint16_t)pack2<DT>(f[j], 0.f), out, off + 2 * j);
-    }
   }
 }
 
@@ -145,6 +94,18 @@ __device__ __forceinline__ bool kept(const ChunkDraws& d, int j, uint32_t thresh
 // The value of the neighbouring lane l ^ 1 (quad permute [1, 0, 3, 2]).
 __device__ __forceinline__ uint32_t lane_xor1(uint32_t v) {
   return (uint32_t)__builtin_amdgcn_mov_dpp((int)v, 0xb1, 0xf, 0xf, false);
+}
+
+// The draws of a lane that holds two halves: of chunk `first` in its first
+// half and of chunk `second` in the other, the low half of each in an even lane
+// and the high half in an odd one.  The even lane draws the first, the odd one
+// the second, and they swap.  (An odd lane's columns are beyond an even one's: where
+// only the even lane is active, its other half is absent.)
+__device__ __forceinline__ ChunkDraws half_draws(uint64_t seed, bool odd, uint32_t first, uint32_t second, uint32_t row,
+                                                 uint32_t stream) {
+  const ChunkDraws d = chunk_draws(seed, odd ? second : first, row, stream);
+  const uint32_t r0 = lane_xor1(odd ? d.w[0] : d.w[2]), r1 = lane_xor1(odd ? d.w[1] : d.w[3]);
+  return {{odd ? r0 : d.w[0], odd ? r1 : d.w[1], odd ? d.w[2] : r0, odd ? d.w[3] : r1}};
 }
 
 // ---- sums over the lanes of a row ---------------------------------------------
