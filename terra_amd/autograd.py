@@ -712,26 +712,24 @@ class _ResidualNorm(torch.autograd.Function):
     the forward to the backward, which on small inputs is bound by the host."""
 
     @staticmethod
-    def forward(ctx, h, x, post_w, post_b, gate, next_w, next_b, seed, tail, norms):
-        ctx.tail, ctx.norms = tail, norms
-        ctx.save_for_backward(h, x, post_w, post_b, gate, next_w, next_b, seed)
+    def forward(ctx, h, x, post_w, post_b, gate, next_w, next_b, seed, tail):
+        params = (post_w, post_b, gate, next_w, next_b)
+        ctx.tail = tail
+        ctx.save_for_backward(h, x, *params, seed)
         ctx.set_materialize_grads(False)
-        return tail.forward(h, x, tail.params(norms[0], gate, norms[1]), seed)
+        return tail.forward(h, x, params, seed)
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dy, dz=None):
-        h, x, post_w, post_b, gate, next_w, next_b, seed = ctx.saved_tensors
+        h, x, *params, seed = ctx.saved_tensors
         if dy is not None and not dy.is_contiguous():
             dy = dy.contiguous()
         if dz is not None and not dz.is_contiguous():
             dz = dz.contiguous()
-        post, nxt = ctx.norms
-        ps = ctx.tail.params(None if post is None else Norm(post_w, post_b), gate,
-                             None if nxt is None else Norm(next_w, next_b))
-        g = ctx.tail.backward(h, x, dy, dz, ps, seed, ctx.needs_input_grad[2:7])
-        return (g.dh, g.dx, *(t if t is None or t.dtype == q.dtype else t.to(q.dtype)
-                              for t, q in zip(g[2:], (post_w, post_b, gate, next_w, next_b))), None, None, None)
+        g = ctx.tail.backward(h, x, dy, dz, params, seed, ctx.needs_input_grad[2:7])
+        return (g.dh, g.dx, *(t if t is None or t.dtype is q.dtype else t.to(q.dtype) for t, q in zip(g[2:], params)),
+                None, None)
 
 
 def residual_norm(h: torch.Tensor, x: torch.Tensor, post_norm: Optional[Norm] = None,
@@ -745,9 +743,8 @@ def residual_norm(h: torch.Tensor, x: torch.Tensor, post_norm: Optional[Norm] = 
     seed = _seed(h, p, seed)
     if x.dtype != h.dtype and x.dtype != torch.float32:
         x = x.to(torch.promote_types(x.dtype, h.dtype))
-    params = [t for n in (post_norm, next_norm) for t in ((None, None) if n is None else (n.weight, n.bias))]
-    if _needs_grad(h, x, gate, *params):
-        tail = kernels._Tail(h, x, post_norm, gate, next_norm, geom, residual_scale, p, seed, stream)
-        return _ResidualNorm.apply(h, x, params[0], params[1], gate, params[2], params[3], seed, tail,
-                                   (post_norm, next_norm))
-    return kernels.residual_norm(h, x, post_norm, gate, next_norm, geom, residual_scale, p, seed, stream)
+    tail = kernels._Tail(h, x, post_norm, gate, next_norm, geom, residual_scale, p, seed, stream)
+    params = tail.params(post_norm, gate, next_norm)
+    if _needs_grad(h, x, *params):
+        return _ResidualNorm.apply(h, x, *params, seed, tail)
+    return tail.forward(h, x, params, seed)

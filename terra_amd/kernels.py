@@ -1458,6 +1458,12 @@ class ResidualNormGrads(NamedTuple):
     dnext_bias: Optional[torch.Tensor]
 
 
+def _packed_f32(ts):
+    """Contiguous fp32 versions of the tensors, themselves where they are."""
+    return [t if t is None or (t.dtype is torch.float32 and t.is_contiguous())
+            else t.detach().to(torch.float32).contiguous() for t in ts]
+
+
 class _Tail:
     """The checked arguments of a residual_norm call but the tensors: the
     descriptor, and what its outputs look like."""
@@ -1502,35 +1508,36 @@ class _Tail:
             d.gate_rows = gate.shape[0] if gate.dim() == 2 else 1
 
     def params(self, post_norm, gate, next_norm):
-        """post weight, post bias, gate, next weight, next bias as the kernels
-        read them: fp32, contiguous, checked (None where absent)."""
-        ps, C = [], self.C
-        for name, t in (("post_norm's weight", None if post_norm is None else post_norm.weight),
-                        ("post_norm's bias", None if post_norm is None else post_norm.bias), ("gate", gate),
-                        ("next_norm's weight", None if next_norm is None else next_norm.weight),
-                        ("next_norm's bias", None if next_norm is None else next_norm.bias)):
+        """post weight, post bias, gate, next weight, next bias (None where
+        absent), their shapes and devices checked."""
+        pw, pb = (None, None) if post_norm is None else (post_norm.weight, post_norm.bias)
+        nw, nb = (None, None) if next_norm is None else (next_norm.weight, next_norm.bias)
+        for name, t in (("post_norm's weight", pw), ("post_norm's bias", pb), ("gate", gate), ("next_norm's weight", nw),
+                        ("next_norm's bias", nb)):
             if t is not None:
-                if t.shape[-1:] != (C,) or t.dim() != 1 and (name != "gate" or t.dim() != 2):
-                    raise ValueError(f"{name} must have {C} channels, got {list(t.shape)}")
+                if t.shape[-1:] != (self.C,) or t.dim() != 1 and (t is not gate or t.dim() != 2):
+                    raise ValueError(f"{name} must have {self.C} channels, got {list(t.shape)}")
                 if t.device != self.dev:
                     raise ValueError(f"tensors on different devices: {self.dev} and {t.device}")
-                if t.dtype != torch.float32 or not t.is_contiguous():
-                    t = t.detach().to(torch.float32).contiguous()
-            ps.append(t)
-        return ps
+        return pw, pb, gate, nw, nb
 
-    def forward(self, h, x, ps, seed):
-        y = torch.empty(x.shape, dtype=x.dtype, device=self.dev)
-        z = torch.empty(x.shape, dtype=h.dtype, device=self.dev) if self.desc.next_norm else None
+    def forward(self, h, x, params, seed):
+        ps = _packed_f32(params)
+        y = x.new_empty(x.shape)
+        z = h.new_empty(x.shape) if self.desc.next_norm else None
         if self.rows > 0:
             _enqueue("terra_swin_residual_norm", self.dev, h.data_ptr(), x.data_ptr(), y.data_ptr(), _ptr(z),
                      ctypes.byref(self.desc), *map(_ptr, ps), _ptr(seed))
         return y if z is None else (y, z)
 
-    def backward(self, h, x, dy, dz, ps, seed, needs) -> "ResidualNormGrads":
-        dev = self.dev
-        dh = (torch.empty if self.covered else torch.zeros)(h.shape, dtype=h.dtype, device=dev)
-        dx = torch.empty(x.shape, dtype=x.dtype, device=dev)
+    def backward(self, h, x, dy, dz, params, seed, needs) -> "ResidualNormGrads":
+        dev, ps, d = self.dev, _packed_f32(params), self.desc
+        strides = _token_rows(h, "h")[2], _token_rows(x, "x")[2]
+        if strides != (d.h_stride, d.x_stride):  # tensors saved by a hook may come back packed
+            d = type(d).from_buffer_copy(d)
+            d.h_stride, d.x_stride = strides
+        dh = h.new_empty(h.shape) if self.covered else h.new_zeros(h.shape)
+        dx = x.new_empty(x.shape)
         want = [t is not None and need for t, need in zip(ps, needs)]
         grads, work, vectors = [None] * 5, None, sum(want)
         if vectors:
@@ -1539,10 +1546,10 @@ class _Tail:
                 vectors -= 1
             rows = iter(torch.empty((vectors, self.C), dtype=torch.float32, device=dev).unbind(0))
             grads = [g if g is not None or not w else next(rows) for g, w in zip(grads, want)]
-            n = _lib.load().terra_swin_residual_norm_workspace(ctypes.byref(self.desc))
+            n = _lib.load().terra_swin_residual_norm_workspace(ctypes.byref(d))
             work = torch.empty(_size(n, "terra_swin_residual_norm_workspace"), dtype=torch.float32, device=dev)
         _enqueue("terra_swin_residual_norm_bwd", dev, h.data_ptr(), x.data_ptr(), _ptr(dy), _ptr(dz), dh.data_ptr(),
-                 dx.data_ptr(), ctypes.byref(self.desc), *map(_ptr, ps[:4]), _ptr(seed), *map(_ptr, grads), _ptr(work))
+                 dx.data_ptr(), ctypes.byref(d), *map(_ptr, ps[:4]), _ptr(seed), *map(_ptr, grads), _ptr(work))
         return ResidualNormGrads(dh, dx, *grads)
 
 

@@ -366,6 +366,22 @@ def test_autograd_forms(dev):
         dh.float().sum().backward()
 
 
+def test_saved_tensors_that_come_back_packed(dev):
+    """save_on_cpu keeps a copy of a column block, and gives it back packed."""
+    c = Case((9, 64), (BF16, F32), p=0.1, seed=16)
+    t, kw = c.args(dev)
+    wide = torch.zeros(9, 200, dtype=BF16, device=dev)
+    wide[:, 8:72] = t["h"]
+    grads = []
+    for hooks in (False, True):
+        h, x = wide.clone().requires_grad_(), t["x"].clone().requires_grad_()
+        with torch.autograd.graph.save_on_cpu() if hooks else torch.enable_grad():
+            y, z = autograd.residual_norm(h[:, 8:72], x, **kw)
+        grads.append(torch.autograd.grad((y, z), (h, x), (t["dy"], t["dz"])))
+    for a, b in zip(*grads):
+        assert torch.equal(a, b)
+
+
 def test_refusals(dev):
     c = Case((4, 6, 32), (BF16, BF16), gate="sample")
     t, kw = c.args(dev)
