@@ -205,13 +205,9 @@ __global__ __launch_bounds__(kDropThreads) void drop_kernel(const DropParams a) 
                                           __float_as_uint(f[4 * q + 2]), __float_as_uint(f[4 * q + 3])}, out,
                              off + (uint32_t)(c[q] * kB));
       } else {
-#pragma unroll
-        for (int j = 0; j < kChunkCols; ++j) {
-          const int at = c[j >> 2] + (j & 3);
-          if (at >= width) continue;
-          if constexpr (kB == 4) stream_store_sc1(__float_as_uint(f[j]), out, off + (uint32_t)(at * kB));
-          else stream_store_sc1((uint16_t)pack2<DT>(f[j], 0.f), out, off + (uint32_t)(at * kB));
-        }
+        uint8_t* const to = a.out + (int64_t)(base + (uint64_t)tr) * a.row_bytes;
+        store_half<DT>(f, to, strip_col + c[0], a.C);
+        store_half<DT>(f + 4, to, strip_col + c[1], a.C);
       }
     }
   }

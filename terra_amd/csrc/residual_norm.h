@@ -159,9 +159,9 @@ struct RowLanes {
     for (int j = 0; j < kChunkCols; ++j) f[j] = chunk_value<DT>(r, j);
   }
 
-  // Stores chunk k, rounded once, into the row that begins `off` bytes into the descriptor's range.
+  // Stores chunk k, rounded once, into the row at `row`, which begins `off` bytes into the descriptor's range.
   template <int DT, bool kVec>
-  __device__ __forceinline__ void store(const float (&f)[kChunkCols], __amdgpu_buffer_rsrc_t out, uint32_t off, int k) const {
+  __device__ __forceinline__ void store(const float (&f)[kChunkCols], __amdgpu_buffer_rsrc_t out, uint32_t off, uint8_t* row, int k) const {
     constexpr uint32_t kB = ChunkElt<DT>::kBytes;
     if constexpr (kVec && kB == 2 && kP == 8) {
       const int col = base(k, 0);
@@ -181,13 +181,8 @@ struct RowLanes {
                            off + (uint32_t)col * kB);
       }
     } else {
-#pragma unroll
-      for (int j = 0; j < kChunkCols; ++j) {
-        const int col = base(k, j >> 2) + (j & 3);
-        if (col >= C) continue;
-        if constexpr (kB == 4) stream_store_sc1(__float_as_uint(f[j]), out, off + (uint32_t)col * kB);
-        else stream_store_sc1((uint16_t)pack2<DT>(f[j], 0.f), out, off + (uint32_t)col * kB);
-      }
+      store_half<DT>(f, row, base(k, 0), C);
+      store_half<DT>(f + 4, row, base(k, 1), C);
     }
   }
 
@@ -215,13 +210,8 @@ struct RowLanes {
                                       reinterpret_cast<stream_u32x2*>(row + (int64_t)col * kB));
       }
     } else {
-#pragma unroll
-      for (int j = 0; j < kChunkCols; ++j) {
-        const int col = base(k, j >> 2) + (j & 3);
-        if (col >= C) continue;
-        if constexpr (kB == 4) reinterpret_cast<float*>(row)[col] = f[j];
-        else reinterpret_cast<uint16_t*>(row)[col] = (uint16_t)pack2<DT>(f[j], 0.f);
-      }
+      store_half<DT>(f, row, base(k, 0), C);
+      store_half<DT>(f + 4, row, base(k, 1), C);
     }
   }
 

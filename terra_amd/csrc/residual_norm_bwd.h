@@ -202,7 +202,7 @@ __global__ __launch_bounds__(tail_threads(kG), kG == 512 && kK == 1 ? 4 : (kK ==
         float out[kChunkCols], gw[kChunkCols];
 #pragma unroll
         for (int j = 0; j < kChunkCols; ++j) out[j] = a.alpha * dv[k][j];
-        if (live) at.template store<DTX, kVec>(out, dx_out, (uint32_t)(group * C) * kXB, k);
+        if (live) at.template store<DTX, kVec>(out, dx_out, (uint32_t)(group * C) * kXB, a.dx + (int64_t)r * C * kXB, k);
 #pragma unroll
         for (int j = 0; j < kChunkCols; ++j) dv[k][j] = kept(draws[k], j, a.drop.threshold) ? dv[k][j] : 0.f;
         if (live && has)
@@ -240,7 +240,7 @@ __global__ __launch_bounds__(tail_threads(kG), kG == 512 && kK == 1 ? 4 : (kK ==
             buffer_rsrc(a.dh + (int64_t)base * C * kHB, min(end - base, (uint32_t)kGroups) * (uint32_t)(C * kHB));
 #pragma unroll
         for (int k = 0; k < kK; ++k) {
-          if (live) at.template store<DTH, kVec>(dv[k], dh_out, (uint32_t)(group * C) * kHB, k);
+          if (live) at.template store<DTH, kVec>(dv[k], dh_out, (uint32_t)(group * C) * kHB, a.dh + (int64_t)r * C * kHB, k);
         }
       }
     }

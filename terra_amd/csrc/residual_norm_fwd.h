@@ -88,7 +88,7 @@ __global__ __launch_bounds__(tail_threads(kG)) void tail_kernel(const TailArgs a
 #pragma unroll
       for (int j = 0; j < kChunkCols; ++j)
         v[k][j] = fmaf(a.alpha, xv[j], kept(d, j, a.drop.threshold) ? v[k][j] : 0.f);
-      if (live) at.template store<DTX, kVec>(v[k], y_out, (uint32_t)(group * C) * kXB, k);
+      if (live) at.template store<DTX, kVec>(v[k], y_out, (uint32_t)(group * C) * kXB, a.y + (int64_t)r * C * kXB, k);
     }
     if (tail_has<kF>(a, kTailNext)) {
       normalise<kG, kK, kP, kVec>(v, a.flags & kTailNextLayer, a.next_eps, a.inv_c, at, sum);
@@ -100,7 +100,7 @@ __global__ __launch_bounds__(tail_threads(kG)) void tail_kernel(const TailArgs a
         par.get(3, k, at, b);
 #pragma unroll
         for (int j = 0; j < kChunkCols; ++j) v[k][j] = fmaf(v[k][j], w[j], b[j]);
-        if (live) at.template store<DTH, kVec>(v[k], z_out, (uint32_t)(group * C) * kHB, k);
+        if (live) at.template store<DTH, kVec>(v[k], z_out, (uint32_t)(group * C) * kHB, a.z + (int64_t)r * C * kHB, k);
       }
     }
   }
