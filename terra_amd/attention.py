@@ -37,6 +37,14 @@ def make_linear_with_seed(in_dim: int, out_dim: int, bias: bool = True,
     return run_with_seed(init_seed, lambda: torch.nn.Linear(in_dim, out_dim, bias=bias))
 
 
+def probability(p: float, name: str) -> float:
+    """``p`` checked to be a probability."""
+    p = float(p)
+    if not 0.0 <= p <= 1.0:
+        raise ValueError(f"{name} must be in [0, 1] (got {p})")
+    return p
+
+
 def relative_position_index(window_size: Sequence[int]) -> torch.Tensor:
     """Swin relative-position index [Wh*Ww, Wh*Ww] (models/attention.py:205-214):
     idx[i, j] = (hi - hj + Wh - 1) * (2*Ww - 1) + (wi - wj + Ww - 1)."""

@@ -712,9 +712,9 @@ class _ResidualNorm(torch.autograd.Function):
     the forward to the backward, which on small inputs is bound by the host."""
 
     @staticmethod
-    def forward(ctx, h, x, post_w, post_b, gate, next_w, next_b, seed, tail):
+    def forward(ctx, h, x, post_w, post_b, gate, next_w, next_b, seed, tail, link):
         params = (post_w, post_b, gate, next_w, next_b)
-        ctx.tail = tail
+        ctx.tail, ctx.link = tail, link
         ctx.save_for_backward(h, x, *params, seed)
         ctx.set_materialize_grads(False)
         return tail.forward(h, x, params, seed)
@@ -728,23 +728,30 @@ class _ResidualNorm(torch.autograd.Function):
         if dz is not None and not dz.is_contiguous():
             dz = dz.contiguous()
         g = ctx.tail.backward(h, x, dy, dz, params, seed, ctx.needs_input_grad[2:7])
-        return (g.dh, g.dx, *(t if t is None or t.dtype is q.dtype else t.to(q.dtype) for t, q in zip(g[2:], params)),
-                None, None)
+        dx = g.dx
+        if ctx.link is not None:
+            ctx.link.grad, dx = dx, None
+        return (g.dh, dx, *(t if t is None or t.dtype is q.dtype else t.to(q.dtype) for t, q in zip(g[2:], params)),
+                None, None, None)
 
 
 def residual_norm(h: torch.Tensor, x: torch.Tensor, post_norm: Optional[Norm] = None,
                   gate: Optional[torch.Tensor] = None, next_norm: Optional[Norm] = None,
                   geom: Optional[WindowGeometry] = None, residual_scale: float = 1.0, p: float = 0.0,
-                  seed: Optional[torch.Tensor] = None, stream: int = 0):
+                  seed: Optional[torch.Tensor] = None, stream: int = 0, link: Optional[ResidualLink] = None):
     """:func:`kernels.residual_norm` with gradients for h, x, the gate and the
     norms' parameters.  ``seed`` None draws one from torch's generator.  An x of
     a type that the kernel does not take beside h's is promoted first, as
-    ``x + h`` would be."""
+    ``x + h`` would be.  ``link``: the :class:`ResidualLink` of the
+    :func:`partition_ln` that h comes from and whose input x is; x's gradient
+    is then added in that one's backward kernel."""
     seed = _seed(h, p, seed)
     if x.dtype != h.dtype and x.dtype != torch.float32:
-        x = x.to(torch.promote_types(x.dtype, h.dtype))
+        x, link = x.to(torch.promote_types(x.dtype, h.dtype)), None
+    if link is not None:
+        x = x.detach()
     tail = kernels._Tail(h, x, post_norm, gate, next_norm, geom, residual_scale, p, seed, stream)
     params = tail.params(post_norm, gate, next_norm)
     if _needs_grad(h, x, *params):
-        return _ResidualNorm.apply(h, x, *params, seed, tail)
+        return _ResidualNorm.apply(h, x, *params, seed, tail, link)
     return tail.forward(h, x, params, seed)

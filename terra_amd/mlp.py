@@ -19,7 +19,17 @@ backward (residual gradient included) on the HIP LayerNorm kernels over the
 token rows, the GEMMs on the linear and weight-gradient kernels where they
 serve the shapes, else on hipBLASLt.  Other shapes and dtypes run the
 reference's own sequence of torch modules on the device (norm2, fc1, act,
-fc2, residual).  Parameter names (``norm2``, ``fc1``, ``fc2``) and the seeded
+fc2, residual).
+
+Optional and build-defined, for regularised training: ``hidden_dropout``
+(after the GELU, in one launch with it), and the half-block's end, y =
+residual_scale * x + layer_scale * dropout(post_norm(fc2(..))) in one launch
+each way (``kernels.residual_norm``): ``post_norm``, ``layer_scale`` (a gate per
+channel, its initial value), ``residual_scale``, ``dropout``; dropout acts in
+training mode, its mask drawn from torch's seed and never stored.  The
+reference's own ``drop`` stays without effect, as it is there.
+``forward(x, normed=z)`` takes norm2(x) as computed elsewhere
+(``SequentialSwinTransformer.forward(.., next_norm=norm2)``).  Parameter names (``norm2``, ``fc1``, ``fc2``) and the seeded
 initialisation follow the reference so its checkpoints load.
 """
 from __future__ import annotations
@@ -30,7 +40,7 @@ import torch
 import torch.nn.functional as F
 
 from . import autograd, config, kernels
-from .attention import make_linear_with_seed
+from .attention import make_linear_with_seed, probability
 
 
 def _disable_parameters_if_mlp_off(module: torch.nn.Module) -> None:
@@ -42,7 +52,8 @@ def _disable_parameters_if_mlp_off(module: torch.nn.Module) -> None:
 
 class SequentialMlp(torch.nn.Module):
     def __init__(self, in_features, hidden_features=None, out_features=None, act_layer=torch.nn.GELU, drop=0.,
-                 init_seed_base=None):
+                 init_seed_base=None, post_norm: bool = False, layer_scale: Optional[float] = None,
+                 residual_scale: float = 1.0, hidden_dropout: float = 0.0, dropout: float = 0.0):
         super().__init__()
         out_features = out_features or in_features
         hidden_features = hidden_features or in_features
@@ -52,6 +63,12 @@ class SequentialMlp(torch.nn.Module):
         self.fc1 = make_linear_with_seed(in_features, hidden_features, init_seed=seed(1))
         self.act = act_layer()
         self.fc2 = make_linear_with_seed(hidden_features, out_features, init_seed=seed(2))
+        self.post_norm2 = torch.nn.LayerNorm(out_features) if post_norm else None
+        self.layer_scale2 = None if layer_scale is None else torch.nn.Parameter(
+            torch.full((out_features,), float(layer_scale)))
+        self.residual_scale = float(residual_scale)
+        self.hidden_dropout = probability(hidden_dropout, "hidden_dropout")
+        self.dropout = probability(dropout, "dropout")
         _disable_parameters_if_mlp_off(self)
         self.use_fused_mlp = True
 
@@ -188,11 +205,52 @@ class SequentialMlp(torch.nn.Module):
         self._fused_cache = (key, args)
         return args
 
-    def forward(self, x: torch.Tensor, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    def _tail_forward(self, x: torch.Tensor, normed: Optional[torch.Tensor]) -> torch.Tensor:
+        """The MLP with dropout after its activation and kernels.residual_norm
+        at its end (see the module's docstring)."""
+        C = x.shape[-1]
+        rows = x.reshape(-1, C).contiguous()
+        link, p, hidden_p = None, self.dropout if self.training else 0.0, self.hidden_dropout if self.training else 0.0
+        seed = kernels.dropout_seed(x.device) if p > 0.0 or hidden_p > 0.0 else None
+        if normed is not None:
+            xn = normed.reshape(rows.shape)
+        elif not config.use_layernorm:
+            xn = rows
+        elif type(self.norm2) is torch.nn.LayerNorm and tuple(self.norm2.normalized_shape) == (C,) and C <= 1024 \
+                and (C * x.element_size()) % 16 == 0 and rows.shape[0] > 0:
+            n = self.norm2
+            # The gradient that reaches x beside the branch is added in the LayerNorm backward's kernel.
+            link = autograd.ResidualLink() if torch.is_grad_enabled() and x.requires_grad else None
+            xn = autograd.partition_ln(rows.view(1, -1, 1, C), kernels.rows_geometry(rows.shape[0], C), n.weight, n.bias,
+                                       n.eps, out_dtype=autograd.linear_input_dtype(rows), link=link).view(-1, C)
+        else:
+            xn = self.norm2(rows)
+        bias_sums = None
+        gelu = type(self.act) is torch.nn.GELU and self.act.approximate == "none"
+        if gelu and hidden_p > 0.0 and self.fc1.bias is not None and torch.is_grad_enabled():
+            bias_sums = autograd.ColumnSumLink()  # fc1's bias gradient, summed where the GELU's backward writes dh
+        a = autograd.linear(xn, self.fc1.weight, self.fc1.bias, bias_sums=bias_sums)
+        if gelu and hidden_p > 0.0:
+            a = autograd.gelu_dropout(a, hidden_p, seed, stream=1, bias_sums=bias_sums)
+        else:
+            a = self.act(a)
+            if hidden_p > 0.0:
+                a = autograd.dropout(a, hidden_p, seed, stream=1)
+        h = autograd.linear(a, self.fc2.weight, self.fc2.bias)
+        return autograd.residual_norm(h, rows, kernels.Norm.of(self.post_norm2), self.layer_scale2, None, None,
+                                      self.residual_scale, p, seed, link=link if h.requires_grad else None).view(x.shape)
+
+    def forward(self, x: torch.Tensor, out: Optional[torch.Tensor] = None,
+                normed: Optional[torch.Tensor] = None) -> torch.Tensor:
         if not config.use_MLP:
             return x
         if x.device.type != "cuda":
             raise RuntimeError("terra_amd: SequentialMlp runs on device tensors only (got a CPU tensor)")
+        if normed is not None or self.post_norm2 is not None or self.layer_scale2 is not None \
+                or self.residual_scale != 1.0 or (self.training and (self.dropout > 0.0 or self.hidden_dropout > 0.0)):
+            if out is not None:
+                raise ValueError("out is for the forward without normed, post_norm, layer_scale, residual_scale and dropout")
+            return self._tail_forward(x, normed)
         if self._fusable(x):
             return kernels.swin_mlp(x.contiguous(), out=out, **self._fused_args())
         if self._gemm_path(x):

@@ -22,11 +22,20 @@ is evaluated in closed form inside the attention kernel; the dense
 ``attn_mask`` buffer is kept only for state-dict compatibility and equals that
 closed form element for element.
 
-Additions that the reference does not have (both optional, build-defined):
+Additions that the reference does not have (all optional, build-defined):
 ``land_mask`` — a [H, W] boolean grid whose land keys receive the mask value
 -100 in every window (folded into the attention mask); ``geometry`` overrides
 (padding, window-row range, valid-window range) for slabs such as one rank's
-share of a window-parallel grid.
+share of a window-parallel grid; and the half-block's end,
+
+    y = residual_scale * x + layer_scale * dropout(post_norm(branch)),
+
+with the window reverse and the roll in one launch each way
+(``kernels.residual_norm``): ``post_norm`` (a norm over the branch),
+``layer_scale`` (a gate per channel, its initial value), ``residual_scale`` and
+``dropout`` (in training mode; the mask is drawn from torch's seed and never
+stored).  ``forward(x, next_norm=norm)`` also gives ``norm(y)`` from the same
+launch, for an MLP half that takes it (``SequentialMlp.forward(y, normed=z)``).
 """
 from __future__ import annotations
 
@@ -35,7 +44,7 @@ from typing import Optional, Tuple
 import torch
 
 from . import autograd, config, kernels
-from .attention import WindowAttention
+from .attention import WindowAttention, probability
 from .kernels import ShiftMask, WindowGeometry, WindowMask
 from .utils import get_swin_attention_mask, land_window_bits
 
@@ -46,7 +55,9 @@ class SequentialSwinTransformer(torch.nn.Module):
                  use_attn_mask=True, use_relative_position_bias=True, use_flash_attention=False,
                  init_seed_base=None, land_mask: Optional[torch.Tensor] = None,
                  pad: Tuple[int, int, int, int] = (0, 0, 0, 0), win_row_begin: int = 0,
-                 win_rows: Optional[int] = None, valid_windows: Optional[Tuple[int, int]] = None):
+                 win_rows: Optional[int] = None, valid_windows: Optional[Tuple[int, int]] = None,
+                 post_norm: bool = False, layer_scale: Optional[float] = None, residual_scale: float = 1.0,
+                 dropout: float = 0.0):
         super().__init__()
         self.layer_idx = layer_idx
         self.init_seed_base = None if init_seed_base is None else int(init_seed_base) + int(layer_idx) * 100
@@ -81,6 +92,10 @@ class SequentialSwinTransformer(torch.nn.Module):
             self.register_buffer("land_mask", land_mask, persistent=False)
         else:
             self.land_mask = None
+        self.post_norm1 = norm_layer(embedding_dim) if post_norm else None
+        self.layer_scale1 = None if layer_scale is None else torch.nn.Parameter(
+            torch.full((embedding_dim,), float(layer_scale)))
+        self.residual_scale, self.dropout = float(residual_scale), probability(dropout, "dropout")
         self._land_bits_cache = {}
         self._mask_cache = None
         # Run the whole half-block as one kernel where the shapes allow it
@@ -272,11 +287,36 @@ class SequentialSwinTransformer(torch.nn.Module):
         self._fused_cache = (key, args)
         return args
 
-    def forward(self, x: torch.Tensor) -> torch.Tensor:
+    def _tail_forward(self, x: torch.Tensor, next_norm: Optional[torch.nn.Module]):
+        """The staged path with kernels.residual_norm at its end (see the
+        module's docstring): y, or (y, next_norm(y))."""
+        B, L, C = x.shape
+        geom = self.geometry(B)
+        grid = x.contiguous().view(B, *self.input_resolution, C)
+        link = None
+        if config.use_layernorm and self._fusable_norm(grid.dtype):
+            # The gradient that reaches x beside the branch is added in the LayerNorm backward's kernel.
+            link = autograd.ResidualLink() if torch.is_grad_enabled() and x.requires_grad else None
+            n = self.norm1
+            windows = autograd.partition_ln(grid, geom, n.weight, n.bias, n.eps,
+                                            out_dtype=autograd.linear_input_dtype(grid), link=link)
+        else:
+            windows = self.norm1(x).contiguous().view(grid.shape) if config.use_layernorm else grid
+            windows = autograd.partition(windows, geom)
+        h = self.attn(windows, mask=self.window_mask(geom)).contiguous()
+        out = autograd.residual_norm(h, grid, kernels.Norm.of(self.post_norm1), self.layer_scale1,
+                                     kernels.Norm.of(next_norm), geom, self.residual_scale,
+                                     self.dropout if self.training else 0.0, link=link if h.requires_grad else None)
+        return out.view(B, L, C) if next_norm is None else tuple(t.view(B, L, C) for t in out)
+
+    def forward(self, x: torch.Tensor, next_norm: Optional[torch.nn.Module] = None):
         H, W = self.input_resolution
         B, L, C = x.shape
         if L != H * W:
             raise AssertionError("input feature has wrong size")
+        if next_norm is not None or self.post_norm1 is not None or self.layer_scale1 is not None \
+                or self.residual_scale != 1.0 or (self.training and self.dropout > 0.0):
+            return self._tail_forward(x, next_norm)
         shortcut = x
         geom = self.geometry(B)
         grid = x.contiguous().view(B, H, W, C)
