@@ -596,7 +596,7 @@ int terra_swin_gelu_bwd(const void* dout, const void* h, void* dh, int dtype, in
 
 /* y = dropout(x) for x [rows, columns] with row stride x_stride (elements), y
  * packed; f32, bf16 or f16; y may be x itself (packed rows).  The backward is
- * the same call on the output's gradient.  columns < 2^24. */
+ * the same call on the output's gradient.  columns < 2^27. */
 int terra_swin_dropout(const void* x, void* y, int dtype, int64_t rows, int64_t columns, int64_t x_stride,
                        double p, const void* seed, uint32_t stream_id, void* stream);
 

@@ -235,6 +235,9 @@ constexpr int kSumBlocks = 1024, kTableBlocks = 2048;
 // Elements from which the forward's table pays (50176 x 512: 22.8 us, without it 33.9; 8192 x 512 7.2 and 6.9).
 constexpr int64_t kTableElements = 1ll << 22;
 
+// 2^16 strips of 2^11 columns: what the grid's second dimension holds.
+constexpr int64_t kDropMaxColumns = 1ll << 27;
+
 struct DropPlan {
   int32_t T, R, strips;
   int64_t blocks;  // row slabs
@@ -288,8 +291,8 @@ int drop_prepare(int dtype, int64_t rows, int64_t C, int64_t in_stride, double p
   if (dtype != TERRA_DTYPE_F32 && dtype != TERRA_DTYPE_BF16 && dtype != TERRA_DTYPE_F16)
     return fail(TERRA_ERR_DTYPE, "dropout supports f32, bf16 and f16 (got dtype %d)", dtype);
   if (rows < 0 || C <= 0) return fail(TERRA_ERR_SHAPE, "rows must be >= 0 and columns > 0");
-  if (rows >= (1ll << 31) || C >= (1ll << 24))
-    return fail(TERRA_ERR_SHAPE, "%lld rows of %lld columns: at most 2^31 - 1 rows of 2^24 - 1", (long long)rows, (long long)C);
+  if (rows >= (1ll << 31) || C >= kDropMaxColumns)
+    return fail(TERRA_ERR_SHAPE, "%lld rows of %lld columns: at most 2^31 - 1 rows of 2^27 - 1", (long long)rows, (long long)C);
   if (in_stride < C) return fail(TERRA_ERR_SHAPE, "the row stride %lld is below the %lld columns", (long long)in_stride, (long long)C);
   const int st = dropout_args(p, seed, stream, &a->drop);
   if (st != TERRA_OK) return st;
@@ -362,8 +365,8 @@ extern "C" int terra_swin_gelu_dropout(const void* h, void* a_out, int dtype, in
 
 extern "C" int terra_swin_gelu_dropout_workspace(int64_t rows, int64_t columns) {
   clear_error();
-  if (rows < 0 || columns <= 0 || rows >= (1ll << 31) || columns >= (1ll << 24))
-    return fail(TERRA_ERR_SHAPE, "at most 2^31 - 1 rows of 1 to 2^24 - 1 columns");
+  if (rows < 0 || columns <= 0 || rows >= (1ll << 31) || columns >= kDropMaxColumns)
+    return fail(TERRA_ERR_SHAPE, "at most 2^31 - 1 rows of 1 to 2^27 - 1 columns");
   return rows == 0 ? 0 : (int)(drop_plan(rows, (int)columns, true, kSumBlocks).blocks * columns);
 }
 

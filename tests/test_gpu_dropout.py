@@ -114,6 +114,16 @@ def test_dropout_large_rows_and_offsets(dev):
     torch.cuda.empty_cache()
 
 
+def test_one_long_row(dev):
+    """A flat tensor of 2^25 + 3 elements: one row of many strips of columns."""
+    n = (1 << 25) + 3
+    y = kernels.dropout(torch.ones(n, dtype=torch.float16, device=dev), 0.5, _seed(dev), 1)
+    assert torch.equal(y.cpu() != 0, rg.keep_mask(SEED, 1, n, 0.5, 1)[0])
+    h, da = torch.ones(n, device=dev), torch.ones(n, device=dev)
+    dh, sums = kernels.gelu_dropout_backward(da, h, 0.5, _seed(dev), 1, column_sums=True)
+    assert torch.equal(dh, sums) and torch.equal(dh != 0, y != 0)
+
+
 def test_dropout_empty(dev):
     for shape in ((0, 8), (3, 0), (0,)):
         assert kernels.dropout(torch.empty(shape, device=dev), 0.5, _seed(dev)).shape == shape
