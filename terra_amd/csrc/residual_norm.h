@@ -47,8 +47,8 @@ struct WindowMap {
 
 // What a launch has.  The first three are template parameters of the kernels:
 // tested at run time they cost the rows' loops a register copy of every value
-// that either side of a test may hold (a backward of 156672 x 1024 bf16: MOVS
-// instead of SPEC us).
+// that either side of a test may hold, and the backward of three chunks a lane the
+// room for a second wave (524288 x 192 bf16: 276 us, 253 so).
 enum TailFlags : uint32_t {
   kTailPost = 1,       // a post-norm
   kTailNext = 2,       // a next norm (backward: whose gradient is given)

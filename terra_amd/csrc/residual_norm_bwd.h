@@ -17,7 +17,7 @@
 //
 // Sums over rows: a unit is every slabs-th group of rows of one sample (so
 // that workgroups side by side read rows side by side; with a run of rows each,
-// 156672 x 1024 bf16 took RUNS us), workgroups take units in grid strides, and
+// 156672 x 1024 bf16 took 402 us, 363 so), workgroups take units in grid strides, and
 // each lane keeps the sums of its columns in registers; A and B leave them unit by unit, since the gate changes
 // with the sample.  A second launch adds the workgroups' sums
 // (sum_partials_kernel): no atomics, an order that the sizes fix.
@@ -214,7 +214,7 @@ __global__ __launch_bounds__(tail_threads(kG), kG == 512 && kK == 1 ? 4 : (kK ==
         par.get(0, k, at, gw);
 #pragma unroll
         for (int j = 0; j < kChunkCols; ++j) {
-          dv[k][j] *= gw[j];
+          dv[k][j] = kept(draws[k], j, a.drop.threshold) ? dv[k][j] * gw[j] : 0.f;  // 0 whatever the gate is
           s0 += dv[k][j];
           s1 = fmaf(dv[k][j], nv[k][j], s1);
         }

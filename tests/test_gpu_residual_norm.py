@@ -17,6 +17,7 @@ and the parameters' gradients K times the sum over rows of the scales of their
 terms.
 """
 import itertools
+import threading
 
 import pytest
 import torch
@@ -382,6 +383,42 @@ def test_saved_tensors_that_come_back_packed(dev):
         assert torch.equal(a, b)
 
 
+@pytest.mark.parametrize("C,rows", [(1024, (1 << 21) + 37), (8, (1 << 28) + 5)])
+def test_offsets_past_32_bits(dev, C, rows):
+    """Tensors of over 2^32 bytes, and more row groups than one launch has workgroups: the last
+    rows are those of a call of their own."""
+    h = torch.empty(rows, C, dtype=BF16, device=dev).normal_(generator=torch.Generator(dev).manual_seed(1))
+    x = h.roll(1, 0)
+    ln = Norm(1 + 0.1 * torch.randn(C, device=dev), 0.1 * torch.randn(C, device=dev))
+    kw = dict(post_norm=ln, gate=torch.rand(C, device=dev), next_norm=ln)
+    y, z = kernels.residual_norm(h, x, **kw)
+    for at in (slice(rows - 9, rows), slice(rows // 2, rows // 2 + 9)):
+        a, b = kernels.residual_norm(h[at].contiguous(), x[at].contiguous(), **kw)
+        assert torch.equal(y[at], a) and torch.equal(z[at], b)
+    del y
+    g = kernels.residual_norm_backward(h, x, z, x, **kw)
+    for at in (slice(rows - 9, rows), slice(rows // 2, rows // 2 + 9)):
+        part = kernels.residual_norm_backward(*(t[at].contiguous() for t in (h, x, z, x)), **kw)
+        assert torch.equal(g.dh[at], part.dh) and torch.equal(g.dx[at], part.dx)
+    total = x.sum(0, dtype=torch.float64)
+    # each of the at most 2^19 terms a lane adds in a row, and the rest in fp64, by magnitude
+    assert bool(((g.dnext_bias.double() - total).abs() <= 2 ** 18 * E32 * x.abs().sum(0, dtype=torch.float64)).all())
+    del h, x, z, g
+    torch.cuda.empty_cache()
+
+
+def test_infinite_gate_of_dropped_elements(dev):
+    """A dropped element's branch and its gradient are 0 whatever the gate is."""
+    c = Case((16, 40), (F32, F32), None, "layer", "channel", p=0.5, seed=17)
+    t, kw = c.args(dev)
+    keep = rg.keep_mask(SEED, 16, 40, 0.5, c.stream).to(dev)
+    for bad in (float("inf"), float("nan")):
+        kw["gate"] = torch.where(torch.arange(40, device=dev) == 3, bad, t["gate"])
+        y = kernels.residual_norm(t["h"], t["x"], **kw)[0]
+        dh = kernels.residual_norm_backward(t["h"], t["x"], t["dy"], None, **kw).dh
+        assert torch.equal(y[~keep], t["x"][~keep]) and bool((dh[~keep] == 0).all())
+
+
 def test_refusals(dev):
     c = Case((4, 6, 32), (BF16, BF16), gate="sample")
     t, kw = c.args(dev)
@@ -407,6 +444,57 @@ def test_refusals(dev):
         kernels.residual_norm_backward(h, x, t["dy"], t["dz"].float(), **kw)
     with pytest.raises(ValueError, match="without a next_norm"):
         kernels.residual_norm_backward(h, x, t["dy"], t["dz"], **{**kw, "next_norm": None})
+
+
+def test_a_call_like_an_earlier_one(dev):
+    """Calls of the same shapes and options check what they are given anew, and take numbers of any kind."""
+    c = Case((2, 16, 24, 40), (BF16, F32), p=0.25, alpha=0.5, seed=30, geom=WindowGeometry(2, 16, 24, 40, 8, 4, 4))
+    t, kw = c.args(dev)
+    want = kernels.residual_norm(t["h"], t["x"], **kw)
+    listed = WindowGeometry(2, 16, 24, 40, 8, 4, 4, [0, 0, 0, 0])
+    for change in (dict(geom=listed), dict(residual_scale=torch.tensor(0.5), p=torch.tensor(0.25)), dict()):
+        got = kernels.residual_norm(t["h"], t["x"], **{**kw, **change})
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+    for seed in (None, torch.zeros(2, dtype=torch.int64, device=dev), torch.zeros(1, dtype=torch.int64)):
+        with pytest.raises(ValueError, match="seed"):
+            kernels.residual_norm(t["h"], t["x"], **{**kw, "seed": seed})
+    with pytest.raises(ValueError, match="gate"):
+        kernels.residual_norm(t["h"], t["x"], **{**kw, "gate": kw["gate"][:1]})
+    changed = kernels.residual_norm(t["h"], t["x"], **{**kw, "residual_scale": torch.tensor(2.0)})
+    assert not torch.equal(changed[0], want[0])
+
+
+def test_one_tensor_twice(dev):
+    """h and x may be one tensor, whose gradient is the sum of both."""
+    g = torch.Generator(dev).manual_seed(31)
+    v = torch.randn(50, 96, device=dev, generator=g, requires_grad=True)
+    w = torch.randn(96, device=dev, generator=g, requires_grad=True)
+    y = autograd.residual_norm(v, v, Norm(w), w)
+    dy = torch.randn(50, 96, device=dev, generator=g)
+    dv, dw = torch.autograd.grad(y, (v, w), dy)
+    part = kernels.residual_norm_backward(v.detach(), v.detach(), dy, None, Norm(w.detach()), w.detach())
+    assert torch.equal(dv, part.dh + part.dx) and torch.equal(dw, part.dpost_weight + part.dgate)
+
+
+def test_calls_of_two_threads(dev):
+    cs = [Case((3, 130, 96), (BF16, F32), gate="sample", p=0.2, seed=s) for s in (32, 33)]
+    want, bad = [c.run(dev) for c in cs], []
+
+    def calls(c, ref):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for _ in range(50):
+                y, z, g = c.run(dev)
+                torch.cuda.current_stream().synchronize()
+                if not all(torch.equal(a, b) for a, b in zip((y, z, *g), (ref[0], ref[1], *ref[2]))):
+                    bad.append(c)
+
+    torch.cuda.synchronize()
+    threads = [threading.Thread(target=calls, args=a) for a in zip(cs, want)]
+    for th in threads:
+        th.start()
+    for th in threads:
+        th.join()
+    assert not bad
 
 
 def test_other_streams_and_graphs(dev):
