@@ -750,7 +750,7 @@ def residual_norm(h: torch.Tensor, x: torch.Tensor, post_norm: Optional[Norm] = 
         x, link = x.to(torch.promote_types(x.dtype, h.dtype)), None
     if link is not None:
         x = x.detach()
-    tail = kernels._Tail(h, x, post_norm, gate, next_norm, geom, residual_scale, p, seed, stream)
+    tail = kernels._tail(h, x, post_norm, gate, next_norm, geom, residual_scale, p, seed, stream)
     params = tail.params(post_norm, gate, next_norm)
     if _needs_grad(h, x, *params):
         return _ResidualNorm.apply(h, x, *params, seed, tail, link)
