@@ -720,19 +720,24 @@ class _ResidualNorm(torch.autograd.Function):
         return tail.forward(h, x, params, seed)
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, dy, dz=None):
-        h, x, *params, seed = ctx.saved_tensors
-        if dy is not None and not dy.is_contiguous():
-            dy = dy.contiguous()
-        if dz is not None and not dz.is_contiguous():
-            dz = dz.contiguous()
-        g = ctx.tail.backward(h, x, dy, dz, params, seed, ctx.needs_input_grad[2:7])
-        dx = g.dx
-        if ctx.link is not None:
-            ctx.link.grad, dx = dx, None
-        return (g.dh, dx, *(t if t is None or t.dtype is q.dtype else t.to(q.dtype) for t, q in zip(g[2:], params)),
-                None, None, None)
+        # once_differentiable's wrapper is only needed where the gradient's own graph is asked for.
+        f = once_differentiable(_residual_norm_grads) if torch.is_grad_enabled() else _residual_norm_grads
+        return f(ctx, dy, dz)
+
+
+def _residual_norm_grads(ctx, dy, dz):
+    h, x, *params, seed = ctx.saved_tensors
+    if dy is not None and not dy.is_contiguous():
+        dy = dy.contiguous()
+    if dz is not None and not dz.is_contiguous():
+        dz = dz.contiguous()
+    g = ctx.tail.backward(h, x, dy, dz, params, seed, ctx.needs_input_grad[2:7])
+    dx = g.dx
+    if ctx.link is not None:
+        ctx.link.grad, dx = dx, None
+    return (g.dh, dx, *(t if t is None or t.dtype is q.dtype else t.to(q.dtype) for t, q in zip(g[2:], params)),
+            None, None, None)
 
 
 def residual_norm(h: torch.Tensor, x: torch.Tensor, post_norm: Optional[Norm] = None,

@@ -1464,11 +1464,15 @@ def _packed_f32(ts):
             else t.detach().to(torch.float32).contiguous() for t in ts]
 
 
+def _packed_like(t: torch.Tensor) -> torch.Tensor:
+    return torch.empty_like(t) if t.is_contiguous() else t.new_empty(t.shape)
+
+
 class _Tail:
     """The checked arguments of a residual_norm call but the tensors: the
     descriptor, and what its outputs look like."""
 
-    __slots__ = ("dev", "desc", "rows", "C", "covered", "geom")
+    __slots__ = ("dev", "desc", "rows", "C", "covered", "strides", "work")
 
     def __init__(self, h, x, post_norm, gate, next_norm, geom, residual_scale, p, seed, stream):
         self.dev = _require_device(h, x)
@@ -1481,7 +1485,7 @@ class _Tail:
         h_rows, hc, d.h_stride = _token_rows(h, "h")
         if hc != C or C == 0:
             raise ValueError(f"h {tuple(h.shape)} and x {tuple(x.shape)} must have the same channels, at least one")
-        self.covered, self.geom = True, geom
+        self.covered, self.strides, self.work = True, (h.stride(), x.stride()), None
         if geom is None:
             if h.shape != x.shape:
                 raise ValueError(f"h {tuple(h.shape)} must have x's shape {tuple(x.shape)} (or a geometry)")
@@ -1524,7 +1528,7 @@ class _Tail:
 
     def forward(self, h, x, params, seed):
         ps = _packed_f32(params)
-        y = x.new_empty(x.shape)
+        y = _packed_like(x)
         z = h.new_empty(x.shape) if self.desc.next_norm else None
         if self.rows > 0:
             _enqueue("terra_swin_residual_norm", self.dev, h.data_ptr(), x.data_ptr(), y.data_ptr(), _ptr(z),
@@ -1533,22 +1537,18 @@ class _Tail:
 
     def backward(self, h, x, dy, dz, params, seed, needs) -> "ResidualNormGrads":
         dev, ps, d = self.dev, _packed_f32(params), self.desc
-        strides = _token_rows(h, "h")[2], _token_rows(x, "x")[2]
-        if strides != (d.h_stride, d.x_stride):  # tensors saved by a hook may come back packed
+        if (h.stride(), x.stride()) != self.strides:  # tensors saved by a hook may come back packed
             d = type(d).from_buffer_copy(d)
-            d.h_stride, d.x_stride = strides
-        dh = h.new_empty(h.shape) if self.covered else h.new_zeros(h.shape)
-        dx = x.new_empty(x.shape)
-        want = [t is not None and need for t, need in zip(ps, needs)]
-        grads, work, vectors = [None] * 5, None, sum(want)
-        if vectors:
-            if want[2] and ps[2].dim() == 2:
-                grads[2] = torch.empty(ps[2].shape, dtype=torch.float32, device=dev)
-                vectors -= 1
-            rows = iter(torch.empty((vectors, self.C), dtype=torch.float32, device=dev).unbind(0))
-            grads = [g if g is not None or not w else next(rows) for g, w in zip(grads, want)]
-            n = _lib.load().terra_swin_residual_norm_workspace(ctypes.byref(d))
-            work = torch.empty(_size(n, "terra_swin_residual_norm_workspace"), dtype=torch.float32, device=dev)
+            d.h_stride, d.x_stride = _token_rows(h, "h")[2], _token_rows(x, "x")[2]
+        dh = _packed_like(h) if self.covered else h.new_zeros(h.shape)
+        dx = _packed_like(x)
+        grads = [torch.empty_like(t) if need and t is not None else None for t, need in zip(ps, needs)]
+        work = None
+        if any(g is not None for g in grads):
+            if self.work is None:
+                self.work = _size(_lib.load().terra_swin_residual_norm_workspace(ctypes.byref(d)),
+                                  "terra_swin_residual_norm_workspace")
+            work = torch.empty(self.work, dtype=torch.float32, device=dev)
         _enqueue("terra_swin_residual_norm_bwd", dev, h.data_ptr(), x.data_ptr(), _ptr(dy), _ptr(dz), dh.data_ptr(),
                  dx.data_ptr(), ctypes.byref(d), *map(_ptr, ps[:4]), _ptr(seed), *map(_ptr, grads), _ptr(work))
         return ResidualNormGrads(dh, dx, *grads)
@@ -1560,8 +1560,8 @@ _TAILS_MAX = 512
 
 def _tail(h, x, post_norm, gate, next_norm, geom, residual_scale, p, seed, stream) -> _Tail:
     """The :class:`_Tail` of a call, made once for each set of shapes, strides,
-    types and options (a call of one token 15.1 -> 13.1 us).  A _Tail does not
-    change after it is made, so calls of any thread may share it."""
+    types and options (a call of one token 15.1 -> 13.1 us).  What a _Tail holds
+    depends on these alone, so calls of any thread may share it."""
     residual_scale, p, stream = float(residual_scale), float(p), int(stream)
     key = (h.shape, h.stride(), h.dtype, h.device, x.shape, x.stride(), x.dtype, x.device,
            None if post_norm is None else (float(post_norm.eps), bool(post_norm.rms)),
