@@ -45,6 +45,14 @@ def probability(p: float, name: str) -> float:
     return p
 
 
+def plain(module: torch.nn.Module, kind: type) -> bool:
+    """``module`` is a ``kind`` itself whose call no forward hook would see, so
+    that its parameters may be used in its place."""
+    d, hooks = module.__dict__, torch.nn.modules.module
+    return (type(module) is kind and "forward" not in d and not d["_forward_hooks"] and not d["_forward_pre_hooks"]
+            and not hooks._global_forward_hooks and not hooks._global_forward_pre_hooks)
+
+
 def relative_position_index(window_size: Sequence[int]) -> torch.Tensor:
     """Swin relative-position index [Wh*Ww, Wh*Ww] (models/attention.py:205-214):
     idx[i, j] = (hi - hj + Wh - 1) * (2*Ww - 1) + (wi - wj + Ww - 1)."""

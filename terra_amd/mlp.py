@@ -40,7 +40,7 @@ import torch
 import torch.nn.functional as F
 
 from . import autograd, config, kernels
-from .attention import make_linear_with_seed, probability
+from .attention import make_linear_with_seed, plain, probability
 
 
 def _disable_parameters_if_mlp_off(module: torch.nn.Module) -> None:
@@ -225,18 +225,19 @@ class SequentialMlp(torch.nn.Module):
                                        n.eps, out_dtype=autograd.linear_input_dtype(rows), link=link).view(-1, C)
         else:
             xn = self.norm2(rows)
-        bias_sums = None
-        gelu = type(self.act) is torch.nn.GELU and self.act.approximate == "none"
-        if gelu and hidden_p > 0.0 and self.fc1.bias is not None and torch.is_grad_enabled():
+        fc1, fc2, bias_sums = self.fc1, self.fc2, None
+        own = [plain(fc, torch.nn.Linear) for fc in (fc1, fc2)]
+        gelu = plain(self.act, torch.nn.GELU) and self.act.approximate == "none"
+        if own[0] and gelu and hidden_p > 0.0 and fc1.bias is not None and torch.is_grad_enabled():
             bias_sums = autograd.ColumnSumLink()  # fc1's bias gradient, summed where the GELU's backward writes dh
-        a = autograd.linear(xn, self.fc1.weight, self.fc1.bias, bias_sums=bias_sums)
+        a = autograd.linear(xn, fc1.weight, fc1.bias, bias_sums=bias_sums) if own[0] else fc1(xn)
         if gelu and hidden_p > 0.0:
             a = autograd.gelu_dropout(a, hidden_p, seed, stream=1, bias_sums=bias_sums)
         else:
             a = self.act(a)
             if hidden_p > 0.0:
                 a = autograd.dropout(a, hidden_p, seed, stream=1)
-        h = autograd.linear(a, self.fc2.weight, self.fc2.bias)
+        h = autograd.linear(a, fc2.weight, fc2.bias) if own[1] else fc2(a)
         return autograd.residual_norm(h, rows, kernels.Norm.of(self.post_norm2), self.layer_scale2, None, None,
                                       self.residual_scale, p, seed, link=link if h.requires_grad else None).view(x.shape)
 

@@ -230,6 +230,33 @@ def test_empty_batch_and_out(dev):
         mlp(x, out=torch.empty_like(x))
 
 
+def test_layers_of_another_kind_are_called(dev):
+    """A hook on a layer sees and may change its output, and a layer of another class runs its own forward,
+    in the regularised path as in the others."""
+    _, mlp = _blocks(96, 3, 7, 14, 14, dropout=0.0, hidden_dropout=0.25)
+    mlp = mlp.to(dev).train()
+    x = torch.randn(1, 196, 96, device=dev)
+    with torch.no_grad():
+        torch.manual_seed(4)
+        want = mlp(x)
+        for name in ("fc1", "fc2", "act"):
+            seen = []
+            handle = getattr(mlp, name).register_forward_hook(lambda m, i, o: seen.append(o.shape))
+            torch.manual_seed(4)
+            assert (mlp(x) - want).norm() <= 2e-5 * want.norm() and len(seen) == 1
+            handle.remove()
+
+        class Halved(torch.nn.Linear):
+            def forward(self, v):
+                return super().forward(v) / 2
+
+        fc2 = Halved(384, 96).to(dev)
+        fc2.load_state_dict({k: 2 * v for k, v in mlp.fc2.state_dict().items()})
+        mlp.fc2 = fc2
+        torch.manual_seed(4)
+        assert (mlp(x) - want).norm() <= 2e-5 * want.norm()
+
+
 def _captured(step):
     side = torch.cuda.Stream()
     side.wait_stream(torch.cuda.current_stream())
