@@ -213,6 +213,26 @@ def library_path() -> str:
     return LIB_PATH
 
 
+_binding = None
+
+
+def load_binding():
+    """The module of the C++ autograd node (csrc/residual_norm_autograd.cpp), bound once to the library's entry points."""
+    global _binding
+    if _binding is None:
+        lib = load()
+        try:
+            from . import _residual_norm as module
+        except ImportError as e:
+            raise RuntimeError("terra_amd: _residual_norm.so is not built or does not fit this torch; run "
+                               "`python -m terra_amd.build` first (there is no fallback)") from e
+        address = lambda f: ctypes.cast(f, ctypes.c_void_p).value  # noqa: E731
+        module.bind(address(lib.terra_swin_residual_norm), address(lib.terra_swin_residual_norm_bwd),
+                    address(lib.terra_last_error))
+        _binding = module
+    return _binding
+
+
 def load() -> ctypes.CDLL:
     """Open the library once and declare the entry-point signatures."""
     global _lib

@@ -23,7 +23,7 @@ from typing import Optional, Tuple, Union
 import torch
 from torch.autograd.function import once_differentiable
 
-from . import kernels
+from . import _lib, kernels
 from .kernels import Norm, ShiftMask, WindowGeometry, WindowMask
 
 MaskArg = Union[None, torch.Tensor, ShiftMask, WindowMask]
@@ -706,40 +706,6 @@ def gelu_dropout(h: torch.Tensor, p: float, seed: Optional[torch.Tensor] = None,
     return kernels.gelu_dropout(h, p, seed, stream)
 
 
-class _ResidualNorm(torch.autograd.Function):
-    """kernels.residual_norm; the backward keeps h, x and the parameters and
-    recomputes the norms and the mask.  The call's checked arguments go from
-    the forward to the backward, which on small inputs is bound by the host."""
-
-    @staticmethod
-    def forward(ctx, h, x, post_w, post_b, gate, next_w, next_b, seed, tail, link):
-        params = (post_w, post_b, gate, next_w, next_b)
-        ctx.tail, ctx.link = tail, link
-        ctx.save_for_backward(h, x, *params, seed)
-        ctx.set_materialize_grads(False)
-        return tail.forward(h, x, params, seed)
-
-    @staticmethod
-    def backward(ctx, dy, dz=None):
-        # once_differentiable's wrapper is only needed where the gradient's own graph is asked for.
-        f = once_differentiable(_residual_norm_grads) if torch.is_grad_enabled() else _residual_norm_grads
-        return f(ctx, dy, dz)
-
-
-def _residual_norm_grads(ctx, dy, dz):
-    h, x, *params, seed = ctx.saved_tensors
-    if dy is not None and not dy.is_contiguous():
-        dy = dy.contiguous()
-    if dz is not None and not dz.is_contiguous():
-        dz = dz.contiguous()
-    g = ctx.tail.backward(h, x, dy, dz, params, seed, ctx.needs_input_grad[2:7])
-    dx = g.dx
-    if ctx.link is not None:
-        ctx.link.grad, dx = dx, None
-    return (g.dh, dx, *(t if t is None or t.dtype is q.dtype else t.to(q.dtype) for t, q in zip(g[2:], params)),
-            None, None, None)
-
-
 def residual_norm(h: torch.Tensor, x: torch.Tensor, post_norm: Optional[Norm] = None,
                   gate: Optional[torch.Tensor] = None, next_norm: Optional[Norm] = None,
                   geom: Optional[WindowGeometry] = None, residual_scale: float = 1.0, p: float = 0.0,
@@ -749,14 +715,13 @@ def residual_norm(h: torch.Tensor, x: torch.Tensor, post_norm: Optional[Norm] = 
     a type that the kernel does not take beside h's is promoted first, as
     ``x + h`` would be.  ``link``: the :class:`ResidualLink` of the
     :func:`partition_ln` that h comes from and whose input x is; x's gradient
-    is then added in that one's backward kernel."""
+    is then added in that one's backward kernel.  The autograd node is a C++ one
+    (csrc/residual_norm_autograd.cpp) that keeps h, x, the parameters and the
+    seed, and recomputes the norms and the mask."""
     seed = _seed(h, p, seed)
     if x.dtype != h.dtype and x.dtype != torch.float32:
         x, link = x.to(torch.promote_types(x.dtype, h.dtype)), None
     if link is not None:
         x = x.detach()
     tail = kernels._tail(h, x, post_norm, gate, next_norm, geom, residual_scale, p, seed, stream)
-    params = tail.params(post_norm, gate, next_norm)
-    if _needs_grad(h, x, *params):
-        return _ResidualNorm.apply(h, x, *params, seed, tail, link)
-    return tail.forward(h, x, params, seed)
+    return _lib.load_binding().residual_norm(tail.call(), h, x, *tail.params(post_norm, gate, next_norm), seed, link)

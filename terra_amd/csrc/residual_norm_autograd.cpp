@@ -1,0 +1,232 @@
+// The autograd node of the end of a half-block (terra_swin_residual_norm and its
+// backward), as a Python module beside the library.  Training steps of small
+// inputs are bound by the host, and the backward of a node written in Python
+// runs in the autograd engine's thread, which has to wait for the interpreter: a step of
+// 3136 x 96 fp32 took 76 us with the engine in the caller's thread and up to 160 with its own, 50 and
+// 101 with this one (x * 2 and its gradient: 18 and 41).  Allocations and the
+// checks of a call's shapes are torch's and the caller's; the arithmetic is the
+// library's, reached by the addresses that bind() is given.
+#include <torch/csrc/autograd/function.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/autograd/functions/utils.h>
+#include <torch/csrc/autograd/saved_variable.h>
+#include <torch/csrc/autograd/variable.h>
+#include <torch/csrc/utils/pybind.h>
+
+#include <ATen/ATen.h>
+#include <c10/core/DeviceGuard.h>
+#include <c10/hip/HIPStream.h>
+
+#include <cstring>
+#include <optional>
+
+#include "../../include/terra_swin.h"
+
+namespace {
+
+using at::Tensor;
+using torch::autograd::SavedVariable;
+using torch::autograd::variable_list;
+
+decltype(&terra_swin_residual_norm) forward_entry = nullptr;
+decltype(&terra_swin_residual_norm_bwd) backward_entry = nullptr;
+decltype(&terra_last_error) last_error = nullptr;
+
+void check(int status, const char* what) {
+  TORCH_CHECK(status != TERRA_ERR_LAUNCH, what, ": ", last_error());
+  TORCH_CHECK_VALUE(status == TERRA_OK, what, ": ", last_error());
+}
+
+// The parameters of a call, in the order of the entry points.
+enum Param { kPostWeight, kPostBias, kGate, kNextWeight, kNextBias, kParams };
+
+const float* f32(const Tensor& t) { return t.defined() ? static_cast<const float*>(t.const_data_ptr()) : nullptr; }
+const void* ptr(const Tensor& t) { return t.defined() ? t.const_data_ptr() : nullptr; }
+
+// What the checked arguments of a call say about it, but the tensors.
+struct Call {
+  terra_swin_residual_norm_desc desc;
+  bool covered;       // the backward writes all of dh
+  int64_t workspace;  // of the backward, fp32 values
+};
+
+std::shared_ptr<Call> make_call(const std::string& desc, bool covered, int64_t workspace) {
+  auto c = std::make_shared<Call>();
+  TORCH_CHECK(desc.size() == sizeof(c->desc), "descriptor of ", desc.size(), " bytes, expected ", sizeof(c->desc));
+  std::memcpy(&c->desc, desc.data(), sizeof(c->desc));
+  c->covered = covered;
+  c->workspace = workspace;
+  return c;
+}
+
+// The current stream of the tensor's device.
+void* current_stream(const Tensor& t) { return c10::hip::getCurrentHIPStream(t.device().index()).stream(); }
+
+Tensor packed_like(const Tensor& t) { return t.is_contiguous() ? at::empty_like(t) : at::empty(t.sizes(), t.options()); }
+
+Tensor packed_f32(const Tensor& t) {
+  if (!t.defined() || (t.scalar_type() == at::kFloat && t.is_contiguous())) return t;
+  return t.to(at::kFloat).contiguous();
+}
+
+constexpr const char* kOnce = "residual_norm cannot be differentiated twice: its gradient has no gradient";
+
+struct ResidualNormBackward : public torch::autograd::Node {
+  std::shared_ptr<Call> call;
+  SavedVariable h, x, seed, params[kParams];
+  std::vector<int64_t> h_strides, x_strides;
+  bool seeded = false, has[kParams] = {};
+  PyObject* link = nullptr;  // a ResidualLink that takes x's gradient, or null
+
+  ~ResidualNormBackward() override {
+    if (link != nullptr && Py_IsInitialized()) {
+      pybind11::gil_scoped_acquire gil;
+      Py_DECREF(link);
+    }
+  }
+
+  std::string name() const override { return "ResidualNormBackward"; }
+
+  void release_variables() override {
+    std::lock_guard<std::mutex> lock(mutex_);
+    h.reset_data();
+    x.reset_data();
+    seed.reset_data();
+    for (auto& p : params) p.reset_data();
+  }
+
+  variable_list apply(variable_list&& grads) override {
+    std::lock_guard<std::mutex> lock(mutex_);
+    variable_list out;
+    {
+      at::AutoGradMode off(false);
+      out = gradients(grads[0], grads.size() > 1 ? grads[1] : Tensor());
+    }
+    if (!at::GradMode::is_enabled()) return out;
+    // Asked for with create_graph: gradients that refuse to be differentiated.
+    variable_list marked;
+    for (auto& t : out)
+      if (t.defined()) marked.push_back(t.detach().set_requires_grad(true));
+    const auto refuse = std::make_shared<torch::autograd::DelayedError>(kOnce, (int64_t)marked.size());
+    marked = (*refuse)(std::move(marked));
+    size_t i = 0;
+    for (auto& t : out)
+      if (t.defined()) t = marked[i++];
+    return out;
+  }
+
+  variable_list gradients(Tensor dy, Tensor dz) {
+    Tensor hv = h.unpack(), xv = x.unpack(), ps[kParams], own[kParams];
+    for (int i = 0; i < kParams; ++i)
+      if (has[i]) {
+        own[i] = params[i].unpack();
+        ps[i] = packed_f32(own[i]);
+      }
+    const Tensor sv = seeded ? seed.unpack() : Tensor();
+    terra_swin_residual_norm_desc d = call->desc;
+    if (hv.strides() != at::IntArrayRef(h_strides)) {  // tensors saved by a hook may come back with others
+      hv = hv.contiguous();
+      d.h_stride = d.channels;
+    }
+    if (xv.strides() != at::IntArrayRef(x_strides)) {
+      xv = xv.contiguous();
+      d.x_stride = d.channels;
+    }
+    if (dy.defined()) dy = dy.contiguous();
+    if (dz.defined()) dz = dz.contiguous();
+    const c10::DeviceGuard guard(hv.device());
+    Tensor dh = call->covered ? packed_like(hv) : at::zeros(hv.sizes(), hv.options());
+    Tensor dx = packed_like(xv), dps[kParams], work;
+    float* dp[kParams] = {};
+    for (int i = 0, edge = 2; i < kParams; ++i) {
+      if (!has[i]) continue;
+      if (task_should_compute_output(edge++)) {
+        dps[i] = at::empty_like(ps[i]);
+        dp[i] = static_cast<float*>(dps[i].data_ptr());
+        if (!work.defined()) work = at::empty({call->workspace}, ps[i].options());
+      }
+    }
+    check(backward_entry(hv.const_data_ptr(), xv.const_data_ptr(), ptr(dy), ptr(dz), dh.data_ptr(), dx.data_ptr(), &d,
+                         f32(ps[kPostWeight]), f32(ps[kPostBias]), f32(ps[kGate]), f32(ps[kNextWeight]), ptr(sv),
+                         dp[kPostWeight], dp[kPostBias], dp[kGate], dp[kNextWeight], dp[kNextBias],
+                         work.defined() ? static_cast<float*>(work.data_ptr()) : nullptr, current_stream(hv)),
+          "terra_swin_residual_norm_bwd");
+    if (link != nullptr) {
+      pybind11::gil_scoped_acquire gil;
+      pybind11::handle(link).attr("grad") = dx;
+      dx = Tensor();
+    }
+    variable_list out = {dh, dx};
+    for (int i = 0; i < kParams; ++i)
+      if (has[i]) out.push_back(dps[i].defined() ? dps[i].to(own[i].scalar_type()) : Tensor());
+    return out;
+  }
+};
+
+// y, or with a next norm (y, z); `link` None or the ResidualLink of x.
+pybind11::object residual_norm(const std::shared_ptr<Call>& call, const Tensor& h, const Tensor& x,
+                               const std::optional<Tensor>& post_weight, const std::optional<Tensor>& post_bias,
+                               const std::optional<Tensor>& gate, const std::optional<Tensor>& next_weight,
+                               const std::optional<Tensor>& next_bias, const std::optional<Tensor>& seed,
+                               const pybind11::object& link) {
+  const std::optional<Tensor>* given[kParams] = {&post_weight, &post_bias, &gate, &next_weight, &next_bias};
+  Tensor ps[kParams], y, z;
+  const c10::DeviceGuard guard(h.device());
+  {
+    at::AutoGradMode off(false);
+    for (int i = 0; i < kParams; ++i)
+      if (given[i]->has_value()) ps[i] = packed_f32(**given[i]);
+    y = packed_like(x);
+    if (call->desc.next_norm != TERRA_NORM_NONE) z = at::empty(x.sizes(), h.options());
+    if (call->desc.rows > 0)
+      check(forward_entry(h.const_data_ptr(), x.const_data_ptr(), y.data_ptr(), z.defined() ? z.data_ptr() : nullptr,
+                          &call->desc, f32(ps[kPostWeight]), f32(ps[kPostBias]), f32(ps[kGate]), f32(ps[kNextWeight]),
+                          f32(ps[kNextBias]), seed.has_value() ? seed->const_data_ptr() : nullptr, current_stream(h)),
+            "terra_swin_residual_norm");
+  }
+  bool grad = at::GradMode::is_enabled();
+  if (grad) {
+    bool any = h.requires_grad() || x.requires_grad();
+    for (const auto* p : given) any = any || (p->has_value() && (*p)->requires_grad());
+    grad = any;
+  }
+  if (grad) {
+    std::shared_ptr<ResidualNormBackward> node(new ResidualNormBackward(), torch::autograd::deleteNode);
+    torch::autograd::edge_list edges = {torch::autograd::impl::gradient_edge(h), torch::autograd::impl::gradient_edge(x)};
+    for (int i = 0; i < kParams; ++i)
+      if (given[i]->has_value()) {
+        edges.push_back(torch::autograd::impl::gradient_edge(**given[i]));
+        node->has[i] = true;
+        node->params[i] = SavedVariable(**given[i], false);
+      }
+    node->set_next_edges(std::move(edges));
+    node->call = call;
+    node->h = SavedVariable(h, false);
+    node->x = SavedVariable(x, false);
+    node->h_strides = h.strides().vec();
+    node->x_strides = x.strides().vec();
+    if (seed.has_value()) {
+      node->seeded = true;
+      node->seed = SavedVariable(*seed, false);
+    }
+    if (!link.is_none()) node->link = pybind11::object(link).release().ptr();
+    torch::autograd::set_history(y, node);
+    if (z.defined()) torch::autograd::set_history(z, node);
+  }
+  if (!z.defined()) return pybind11::cast(y);
+  return pybind11::make_tuple(y, z);
+}
+
+void bind(uintptr_t forward, uintptr_t backward, uintptr_t error) {
+  forward_entry = reinterpret_cast<decltype(forward_entry)>(forward);
+  backward_entry = reinterpret_cast<decltype(backward_entry)>(backward);
+  last_error = reinterpret_cast<decltype(last_error)>(error);
+}
+
+}  // namespace
+
+PYBIND11_MODULE(_residual_norm, m) {
+  pybind11::class_<Call, std::shared_ptr<Call>>(m, "Call").def(pybind11::init(&make_call));
+  m.def("bind", &bind);
+  m.def("residual_norm", &residual_norm);
+}

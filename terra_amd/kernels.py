@@ -1472,7 +1472,7 @@ class _Tail:
     """The checked arguments of a residual_norm call but the tensors: the
     descriptor, and what its outputs look like."""
 
-    __slots__ = ("dev", "desc", "rows", "C", "covered", "strides", "work")
+    __slots__ = ("dev", "desc", "rows", "C", "covered", "strides", "work", "node_call")
 
     def __init__(self, h, x, post_norm, gate, next_norm, geom, residual_scale, p, seed, stream):
         self.dev = _require_device(h, x)
@@ -1485,7 +1485,7 @@ class _Tail:
         h_rows, hc, d.h_stride = _token_rows(h, "h")
         if hc != C or C == 0:
             raise ValueError(f"h {tuple(h.shape)} and x {tuple(x.shape)} must have the same channels, at least one")
-        self.covered, self.strides, self.work = True, (h.stride(), x.stride()), None
+        self.covered, self.strides, self.work, self.node_call = True, (h.stride(), x.stride()), None, None
         if geom is None:
             if h.shape != x.shape:
                 raise ValueError(f"h {tuple(h.shape)} must have x's shape {tuple(x.shape)} (or a geometry)")
@@ -1526,6 +1526,19 @@ class _Tail:
                     raise ValueError(f"tensors on different devices: {dev} and {t.device}")
         return pw, pb, gate, nw, nb
 
+    def workspace(self) -> int:
+        """fp32 values that the backward's workspace holds."""
+        if self.work is None:
+            self.work = _size(_lib.load().terra_swin_residual_norm_workspace(ctypes.byref(self.desc)),
+                              "terra_swin_residual_norm_workspace")
+        return self.work
+
+    def call(self):
+        """These arguments as the C++ autograd node takes them."""
+        if self.node_call is None:
+            self.node_call = _lib.load_binding().Call(bytes(self.desc), self.covered, self.workspace())
+        return self.node_call
+
     def forward(self, h, x, params, seed):
         ps = _packed_f32(params)
         y = _packed_like(x)
@@ -1545,10 +1558,7 @@ class _Tail:
         grads = [torch.empty_like(t) if need and t is not None else None for t, need in zip(ps, needs)]
         work = None
         if any(g is not None for g in grads):
-            if self.work is None:
-                self.work = _size(_lib.load().terra_swin_residual_norm_workspace(ctypes.byref(d)),
-                                  "terra_swin_residual_norm_workspace")
-            work = torch.empty(self.work, dtype=torch.float32, device=dev)
+            work = torch.empty(self.workspace(), dtype=torch.float32, device=dev)
         _enqueue("terra_swin_residual_norm_bwd", dev, h.data_ptr(), x.data_ptr(), _ptr(dy), _ptr(dz), dh.data_ptr(),
                  dx.data_ptr(), ctypes.byref(d), *map(_ptr, ps[:4]), _ptr(seed), *map(_ptr, grads), _ptr(work))
         return ResidualNormGrads(dh, dx, *grads)

@@ -260,3 +260,12 @@ class TestWrappers:
         for bad in (torch.nn.LayerNorm((2, 8)), torch.nn.Identity(), torch.nn.BatchNorm1d(8)):
             with pytest.raises(TypeError, match="LayerNorm or nn.RMSNorm"):
                 Norm.of(bad)
+
+
+def test_autograd_node_module():
+    """The C++ node's module loads against this torch and takes descriptors of the library's size alone."""
+    module = L.load_binding()
+    d = L.ResidualNormDesc()
+    assert module.Call(bytes(d), True, 0) is not None
+    with pytest.raises(RuntimeError, match="descriptor of"):
+        module.Call(bytes(d)[:-1], True, 0)

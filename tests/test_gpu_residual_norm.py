@@ -367,6 +367,40 @@ def test_autograd_forms(dev):
         dh.float().sum().backward()
 
 
+def test_the_node_keeps_torchs_rules(dev):
+    """A graph that is kept gives its gradients again, one that is freed or whose saved tensors changed refuses;
+    the engine may run in the caller's thread; only the gradients asked for are taken."""
+    c = Case((3, 17, 96), (BF16, F32), gate="sample", p=0.2, seed=34)
+    t, kw = c.args(dev)
+    want = kernels.residual_norm_backward(t["h"], t["x"], t["dy"], t["dz"], **kw)
+    leaves = {k: t[k].clone().requires_grad_() for k in ("h", "x", "pw", "pb", "gate", "nw", "nb")}
+    given = dict(kw, post_norm=Norm(leaves["pw"], leaves["pb"], 1e-5), gate=leaves["gate"],
+                 next_norm=Norm(leaves["nw"], leaves["nb"], 1e-5))
+    call = lambda: autograd.residual_norm(leaves["h"], leaves["x"], **given)  # noqa: E731
+    outs = call()
+    with torch.autograd.set_multithreading_enabled(False):
+        first = torch.autograd.grad(outs, list(leaves.values()), (t["dy"], t["dz"]), retain_graph=True)
+    again = torch.autograd.grad(outs, list(leaves.values()), (t["dy"], t["dz"]))
+    order = (want.dh, want.dx, want.dpost_weight, want.dpost_bias, want.dgate, want.dnext_weight, want.dnext_bias)
+    for a, b, ref in zip(first, again, order):
+        assert torch.equal(a, ref) and torch.equal(b, ref)
+    with pytest.raises(RuntimeError, match="second time"):
+        torch.autograd.grad(outs, leaves["h"], (t["dy"], t["dz"]))
+    for name in ("h", "pw"):
+        outs = call()
+        with torch.no_grad():
+            leaves[name].mul_(1)
+        with pytest.raises(RuntimeError, match="inplace|in-place"):
+            torch.autograd.grad(outs, leaves["x"], (t["dy"], t["dz"]))
+    dnb, = torch.autograd.grad(call(), leaves["nb"], (t["dy"], t["dz"]))
+    assert torch.equal(dnb, want.dnext_bias)
+    leaves["h"].requires_grad_(False)
+    y, z = autograd.residual_norm(leaves["h"], t["x"], **kw)
+    assert not y.requires_grad and not z.requires_grad
+    with torch.no_grad():
+        assert not call()[0].requires_grad
+
+
 def test_saved_tensors_that_come_back_packed(dev):
     """save_on_cpu keeps a copy of a column block, and gives it back packed."""
     c = Case((9, 64), (BF16, F32), p=0.1, seed=16)
