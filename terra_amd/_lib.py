@@ -217,18 +217,18 @@ _binding = None
 
 
 def load_binding():
-    """The module of the C++ autograd node (csrc/residual_norm_autograd.cpp), bound once to the library's entry points."""
+    """The regularised operators' host module (csrc/regularize_binding.cpp), bound once to the library's entry points."""
     global _binding
     if _binding is None:
         lib = load()
         try:
-            from . import _residual_norm as module
+            from . import _regularize as module
         except ImportError as e:
-            raise RuntimeError("terra_amd: _residual_norm.so is not built or does not fit this torch; run "
+            raise RuntimeError("terra_amd: _regularize.so is not built or does not fit this torch; run "
                                "`python -m terra_amd.build` first (there is no fallback)") from e
-        address = lambda f: ctypes.cast(f, ctypes.c_void_p).value  # noqa: E731
-        module.bind(address(lib.terra_swin_residual_norm), address(lib.terra_swin_residual_norm_bwd),
-                    address(lib.terra_last_error))
+        module.bind(*(ctypes.cast(f, ctypes.c_void_p).value for f in (
+            lib.terra_swin_residual_norm, lib.terra_swin_residual_norm_bwd, lib.terra_swin_dropout,
+            lib.terra_swin_gelu_dropout, lib.terra_swin_gelu_dropout_bwd, lib.terra_last_error)))
         _binding = module
     return _binding
 

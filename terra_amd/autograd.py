@@ -716,7 +716,7 @@ def residual_norm(h: torch.Tensor, x: torch.Tensor, post_norm: Optional[Norm] = 
     ``x + h`` would be.  ``link``: the :class:`ResidualLink` of the
     :func:`partition_ln` that h comes from and whose input x is; x's gradient
     is then added in that one's backward kernel.  The autograd node is a C++ one
-    (csrc/residual_norm_autograd.cpp) that keeps h, x, the parameters and the
+    (csrc/regularize_binding.cpp); it keeps h, x, the parameters and the
     seed, and recomputes the norms and the mask."""
     seed = _seed(h, p, seed)
     if x.dtype != h.dtype and x.dtype != torch.float32:

@@ -1,5 +1,5 @@
 """Builds ``terra_amd/libterra_swin.so`` from ``terra_amd/csrc`` with hipcc for gfx950,
-and the Python module of the C++ autograd node beside it.
+and the regularised operators' host module beside it.
 
     python -m terra_amd.build
 
@@ -96,23 +96,22 @@ def build_library(verbose: bool = False, jobs: int = 0, asan_host: bool = False)
 
 
 def build_binding(verbose: bool = False) -> str:
-    """Compile the Python module of the C++ autograd node
-    (``csrc/residual_norm_autograd.cpp``, host code against torch's headers)
-    into ``terra_amd/_residual_norm.so``; returns its path."""
+    """Compile the regularised operators' host module
+    (``csrc/regularize_binding.cpp``, against torch's headers) into ``terra_amd/_regularize.so``; returns its path."""
     import sysconfig
 
     import torch
     from torch.utils import cpp_extension
 
-    path = os.path.join(HERE, "_residual_norm.so")
+    path = os.path.join(HERE, "_regularize.so")
     root = os.path.dirname(torch.__file__)
     cmd = [hipcc(), "-x", "c++", "-O2", "-std=c++17", "-fPIC", "-shared", "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1",
            f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}",
            *(f"-isystem{d}" for d in [*cpp_extension.include_paths(), "/opt/rocm/include",
                                       sysconfig.get_paths()["include"]]),
-           os.path.join(CSRC, "residual_norm_autograd.cpp"), f"-L{os.path.join(root, 'lib')}", "-ltorch_python",
+           os.path.join(CSRC, "regularize_binding.cpp"), f"-L{os.path.join(root, 'lib')}", "-ltorch_python",
            "-ltorch_cpu", "-ltorch", "-lc10", "-lc10_hip"]
-    fd, tmp = tempfile.mkstemp(prefix="_residual_norm.", suffix=".so.tmp", dir=HERE)
+    fd, tmp = tempfile.mkstemp(prefix="_regularize.", suffix=".so.tmp", dir=HERE)
     os.close(fd)
     try:
         _run([*cmd, "-o", tmp], verbose)

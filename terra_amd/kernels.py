@@ -1276,7 +1276,7 @@ def _enqueue(name: str, dev: torch.device, *args) -> None:
     operators are short enough on small inputs for the host to set their pace, so
     the device is switched only where another one is current, and the stream's
     handle is read directly (a torch.cuda.device block and a Stream object
-    cost 7 us a call, of 11 for a small dropout)."""
+    cost 7 us a call)."""
     fn = getattr(_lib.load(), name)
     if dev.index == torch._C._cuda_getDevice():
         st = fn(*args, torch._C._cuda_getCurrentRawStream(dev.index))
@@ -1295,12 +1295,16 @@ def dropout_seed(device: Union[str, torch.device, None] = None,
     return torch.empty(1, dtype=torch.int64, device="cuda" if device is None else device).random_(generator=generator)
 
 
-def _dropout_args(x: torch.Tensor, p: float, seed: Optional[torch.Tensor], stream: int) -> Tuple[float, int]:
-    p, stream = float(p), int(stream)
+def _dropout_range(p: float, stream: int) -> None:
     if not 0.0 <= p <= 1.0:
         raise ValueError(f"the dropout probability must be in [0, 1] (got {p})")
     if not 0 <= stream < 1 << 32:
         raise ValueError(f"stream must be in [0, 2^32) (got {stream})")
+
+
+def _dropout_args(x: torch.Tensor, p: float, seed: Optional[torch.Tensor], stream: int) -> Tuple[float, int]:
+    p, stream = float(p), int(stream)
+    _dropout_range(p, stream)
     if seed is None:
         if p > 0.0:
             raise ValueError("dropout with p > 0 needs a seed (see dropout_seed)")
@@ -1336,13 +1340,31 @@ def _token_rows(t: torch.Tensor, name: str) -> Tuple[int, int, int]:
     return rows, C, stride
 
 
-def _same(out: Optional[torch.Tensor], like: torch.Tensor) -> torch.Tensor:
-    """``out``, checked, or a new packed tensor like ``like``."""
-    if out is None:
-        return torch.empty(like.shape, dtype=like.dtype, device=like.device)
-    if out.shape != like.shape or out.dtype != like.dtype or not out.is_contiguous() or out.device != like.device:
-        raise ValueError(f"out must be a contiguous {like.dtype} tensor of shape {tuple(like.shape)} on {like.device}")
-    return out
+_ROWS = {}  # checked arguments by shape, type and options
+_KEPT_CALLS = 512
+
+
+def _rows_call(x: torch.Tensor, p: float, stream: int, packed: bool):
+    """The arguments of a dropout call (of contiguous rows where ``packed``) as
+    the host module takes them, checked once for each shape, type and options."""
+    p, stream = float(p), int(stream)
+    key = (packed, x.shape, x.stride(), x.dtype, x.device, p, stream)
+    call = _ROWS.get(key)
+    if call is None:
+        _require_device(x)
+        code = _dtype_code(x, _FLOATS)
+        _dropout_range(p, stream)
+        if packed and (x.dim() < 1 or not x.is_contiguous()):
+            raise ValueError("h must be a contiguous [..., features] tensor")
+        rows, C, stride = _token_rows(x, "x")
+        work = 0
+        if rows > 0 and packed:
+            work = _size(_lib.load().terra_swin_gelu_dropout_workspace(rows, C), "terra_swin_gelu_dropout_workspace")
+        call = _lib.load_binding().Rows(code, rows, C, stride, p, stream, work)
+        if len(_ROWS) >= _KEPT_CALLS:
+            _ROWS.clear()
+        _ROWS[key] = call
+    return call
 
 
 def dropout(x: torch.Tensor, p: float, seed: Optional[torch.Tensor], stream: int = 0,
@@ -1355,15 +1377,7 @@ def dropout(x: torch.Tensor, p: float, seed: Optional[torch.Tensor], stream: int
     the backward is the same call on the output's gradient.  ``p`` is rounded
     to a multiple of 2^-16, and the scale is that of the rounded one.
     ``out`` may be ``x``."""
-    dev = _require_device(x)
-    code = _dtype_code(x, _FLOATS)
-    p, stream = _dropout_args(x, p, seed, stream)
-    rows, C, stride = _token_rows(x, "x")
-    out = _same(out, x)
-    if rows == 0:
-        return out
-    _enqueue("terra_swin_dropout", dev, x.data_ptr(), out.data_ptr(), code, rows, C, stride, p, _ptr(seed), stream)
-    return out
+    return _lib.load_binding().dropout(_rows_call(x, p, stream, False), x, seed, out)
 
 
 def gelu_dropout(h: torch.Tensor, p: float, seed: Optional[torch.Tensor], stream: int = 0,
@@ -1371,17 +1385,7 @@ def gelu_dropout(h: torch.Tensor, p: float, seed: Optional[torch.Tensor], stream
     """``dropout(GELU(h))`` (erf form, models/mlp.py:165) of a contiguous ``h``
     [..., features] in one pass, rounded once; the mask as :func:`dropout`'s.
     ``out`` may be ``h``."""
-    dev = _require_device(h)
-    code = _dtype_code(h, _FLOATS)
-    p, stream = _dropout_args(h, p, seed, stream)
-    if h.dim() < 1 or not h.is_contiguous():
-        raise ValueError("h must be a contiguous [..., features] tensor")
-    out = _same(out, h)
-    if h.numel() == 0:
-        return out
-    C = h.shape[-1]
-    _enqueue("terra_swin_gelu_dropout", dev, h.data_ptr(), out.data_ptr(), code, h.numel() // C, C, p, _ptr(seed), stream)
-    return out
+    return _lib.load_binding().gelu_dropout(_rows_call(h, p, stream, True), h, seed, out)
 
 
 def gelu_dropout_backward(dout: torch.Tensor, h: torch.Tensor, p: float, seed: Optional[torch.Tensor], stream: int = 0,
@@ -1392,26 +1396,7 @@ def gelu_dropout_backward(dout: torch.Tensor, h: torch.Tensor, p: float, seed: O
     (fp32 [features], the bias gradient of the Linear that produced ``h``),
     before the rounding and in an order that the sizes fix: ``(dh, sums)``.
     ``out`` may be ``dout`` or ``h``."""
-    dev = _require_device(dout, h)
-    code = _dtype_code(h, _FLOATS)
-    p, stream = _dropout_args(h, p, seed, stream)
-    if dout.shape != h.shape or dout.dtype != h.dtype:
-        raise ValueError(f"dout {tuple(dout.shape)} {dout.dtype} must match h {tuple(h.shape)} {h.dtype}")
-    if h.dim() < 1 or not (dout.is_contiguous() and h.is_contiguous()):
-        raise ValueError("dout and h must be contiguous [..., features] tensors")
-    out = _same(out, h)
-    C = h.shape[-1]
-    if h.numel() == 0:
-        return (out, torch.zeros(C, dtype=torch.float32, device=dev)) if column_sums else out
-    lib, rows = _lib.load(), h.numel() // C
-    sums = work = None
-    if column_sums:
-        sums = torch.empty(C, dtype=torch.float32, device=dev)
-        work = torch.empty(_size(lib.terra_swin_gelu_dropout_workspace(rows, C), "terra_swin_gelu_dropout_workspace"),
-                           dtype=torch.float32, device=dev)
-    _enqueue("terra_swin_gelu_dropout_bwd", dev, dout.data_ptr(), h.data_ptr(), out.data_ptr(), code, rows, C, p, _ptr(seed),
-             stream, _ptr(sums), _ptr(work))
-    return (out, sums) if column_sums else out
+    return _lib.load_binding().gelu_dropout_backward(_rows_call(h, p, stream, True), dout, h, seed, column_sums, out)
 
 
 def _size(n: int, what: str) -> int:
@@ -1565,7 +1550,6 @@ class _Tail:
 
 
 _TAILS = {}  # checked arguments by shapes, types and options
-_TAILS_MAX = 512
 
 
 def _tail(h, x, post_norm, gate, next_norm, geom, residual_scale, p, seed, stream) -> _Tail:
@@ -1583,7 +1567,7 @@ def _tail(h, x, post_norm, gate, next_norm, geom, residual_scale, p, seed, strea
         return _Tail(h, x, post_norm, gate, next_norm, geom, residual_scale, p, seed, stream)
     if t is None:
         t = _Tail(h, x, post_norm, gate, next_norm, geom, residual_scale, p, seed, stream)
-        if len(_TAILS) >= _TAILS_MAX:
+        if len(_TAILS) >= _KEPT_CALLS:
             _TAILS.clear()
         _TAILS[key] = t
     elif seed is not None or p > 0.0:

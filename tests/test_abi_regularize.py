@@ -263,7 +263,7 @@ class TestWrappers:
 
 
 def test_autograd_node_module():
-    """The C++ node's module loads against this torch and takes descriptors of the library's size alone."""
+    """The host module loads against this torch and takes descriptors of the library's size alone."""
     module = L.load_binding()
     d = L.ResidualNormDesc()
     assert module.Call(bytes(d), True, 0) is not None
