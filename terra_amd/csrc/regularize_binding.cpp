@@ -111,6 +111,7 @@ Tensor output(const std::optional<Tensor>& out, const Tensor& like) {
 
 Tensor dropout(const std::shared_ptr<Rows>& c, const Tensor& x, const std::optional<Tensor>& seed,
                const std::optional<Tensor>& out) {
+  const pybind11::gil_scoped_release no_gil;  // a launch may wait for room in the queue
   const at::AutoGradMode off(false);
   const void* s = seed_ptr(seed, x, c->p);
   const c10::DeviceGuard guard(x.device());
@@ -123,6 +124,7 @@ Tensor dropout(const std::shared_ptr<Rows>& c, const Tensor& x, const std::optio
 
 Tensor gelu_dropout(const std::shared_ptr<Rows>& c, const Tensor& h, const std::optional<Tensor>& seed,
                     const std::optional<Tensor>& out) {
+  const pybind11::gil_scoped_release no_gil;
   const at::AutoGradMode off(false);
   const void* s = seed_ptr(seed, h, c->p);
   const c10::DeviceGuard guard(h.device());
@@ -136,23 +138,27 @@ Tensor gelu_dropout(const std::shared_ptr<Rows>& c, const Tensor& h, const std::
 // dh, or with `column_sums` (dh, its sums over the rows).
 pybind11::object gelu_dropout_backward(const std::shared_ptr<Rows>& c, const Tensor& dout, const Tensor& h,
                                        const std::optional<Tensor>& seed, bool column_sums, const std::optional<Tensor>& out) {
-  const at::AutoGradMode off(false);
-  TORCH_CHECK_VALUE(dout.device() == h.device(), "tensors on different devices: ", h.device(), " and ", dout.device());
-  TORCH_CHECK_VALUE(dout.sizes() == h.sizes() && dout.scalar_type() == h.scalar_type() && dout.is_contiguous(),
-                    "dout must be a contiguous ", h.scalar_type(), " tensor of shape ", h.sizes(), " like h");
-  const void* s = seed_ptr(seed, h, c->p);
-  const c10::DeviceGuard guard(h.device());
-  Tensor dh = output(out, h), sums, work;
-  if (column_sums) {
-    const auto f32_there = h.options().dtype(at::kFloat);
-    sums = c->rows > 0 ? at::empty({c->columns}, f32_there) : at::zeros({c->columns}, f32_there);
-    work = at::empty({c->workspace}, f32_there);
+  Tensor dh, sums, work;
+  {
+    const pybind11::gil_scoped_release no_gil;
+    const at::AutoGradMode off(false);
+    TORCH_CHECK_VALUE(dout.device() == h.device(), "tensors on different devices: ", h.device(), " and ", dout.device());
+    TORCH_CHECK_VALUE(dout.sizes() == h.sizes() && dout.scalar_type() == h.scalar_type() && dout.is_contiguous(),
+                      "dout must be a contiguous ", h.scalar_type(), " tensor of shape ", h.sizes(), " like h");
+    const void* s = seed_ptr(seed, h, c->p);
+    const c10::DeviceGuard guard(h.device());
+    dh = output(out, h);
+    if (column_sums) {
+      const auto f32_there = h.options().dtype(at::kFloat);
+      sums = c->rows > 0 ? at::empty({c->columns}, f32_there) : at::zeros({c->columns}, f32_there);
+      work = at::empty({c->workspace}, f32_there);
+    }
+    if (c->rows > 0)
+      check(gelu_backward_entry(dout.const_data_ptr(), h.const_data_ptr(), dh.data_ptr(), c->dtype, c->rows, c->columns, c->p,
+                                s, c->stream, column_sums ? static_cast<float*>(sums.data_ptr()) : nullptr,
+                                column_sums ? static_cast<float*>(work.data_ptr()) : nullptr, current_stream(h)),
+            "terra_swin_gelu_dropout_bwd");
   }
-  if (c->rows > 0)
-    check(gelu_backward_entry(dout.const_data_ptr(), h.const_data_ptr(), dh.data_ptr(), c->dtype, c->rows, c->columns, c->p, s,
-                              c->stream, column_sums ? static_cast<float*>(sums.data_ptr()) : nullptr,
-                              column_sums ? static_cast<float*>(work.data_ptr()) : nullptr, current_stream(h)),
-          "terra_swin_gelu_dropout_bwd");
   if (!column_sums) return pybind11::cast(dh);
   return pybind11::make_tuple(dh, sums);
 }
@@ -261,9 +267,10 @@ pybind11::object residual_norm(const std::shared_ptr<Call>& call, const Tensor& 
                                const pybind11::object& link) {
   const std::optional<Tensor>* given[kParams] = {&post_weight, &post_bias, &gate, &next_weight, &next_bias};
   Tensor ps[kParams], y, z;
-  const c10::DeviceGuard guard(h.device());
   {
-    at::AutoGradMode off(false);
+    const pybind11::gil_scoped_release no_gil;
+    const at::AutoGradMode off(false);
+    const c10::DeviceGuard guard(h.device());
     for (int i = 0; i < kParams; ++i)
       if (given[i]->has_value()) ps[i] = packed_f32(**given[i]);
     y = packed_like(x);
@@ -274,13 +281,14 @@ pybind11::object residual_norm(const std::shared_ptr<Call>& call, const Tensor& 
                           f32(ps[kNextBias]), seed.has_value() ? seed->const_data_ptr() : nullptr, current_stream(h)),
             "terra_swin_residual_norm");
   }
-  bool grad = at::GradMode::is_enabled();
-  if (grad) {
-    bool any = h.requires_grad() || x.requires_grad();
-    for (const auto* p : given) any = any || (p->has_value() && (*p)->requires_grad());
-    grad = any;
-  }
-  if (grad) {
+  bool grad = h.requires_grad() || x.requires_grad(), tangent = h._fw_grad(0).defined() || x._fw_grad(0).defined();
+  for (const auto* p : given)
+    if (p->has_value()) {
+      grad = grad || (*p)->requires_grad();
+      tangent = tangent || (*p)->_fw_grad(0).defined();
+    }
+  TORCH_CHECK_NOT_IMPLEMENTED(!tangent, "residual_norm has no forward-mode derivative");
+  if (grad && at::GradMode::is_enabled()) {
     std::shared_ptr<ResidualNormBackward> node(new ResidualNormBackward(), torch::autograd::deleteNode);
     torch::autograd::edge_list edges = {torch::autograd::impl::gradient_edge(h), torch::autograd::impl::gradient_edge(x)};
     for (int i = 0; i < kParams; ++i)

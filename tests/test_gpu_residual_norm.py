@@ -394,6 +394,10 @@ def test_the_node_keeps_torchs_rules(dev):
             torch.autograd.grad(outs, leaves["x"], (t["dy"], t["dz"]))
     dnb, = torch.autograd.grad(call(), leaves["nb"], (t["dy"], t["dz"]))
     assert torch.equal(dnb, want.dnext_bias)
+    import torch.autograd.forward_ad as fwad
+
+    with fwad.dual_level(), pytest.raises(NotImplementedError, match="forward-mode"):
+        autograd.residual_norm(fwad.make_dual(t["h"], t["h"]), t["x"], **kw)
     leaves["h"].requires_grad_(False)
     y, z = autograd.residual_norm(leaves["h"], t["x"], **kw)
     assert not y.requires_grad and not z.requires_grad
