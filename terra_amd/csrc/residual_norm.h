@@ -58,6 +58,7 @@ enum TailFlags : uint32_t {
   kTailPostLayer = 16, kTailNextLayer = 32,  // the norm is a LayerNorm
   kTailWindows = 64,   // h is in window order
   kTailDy = 128,       // backward: the gradient of y is given
+  kTailPairs = 256,    // rows that are not of whole aligned chunks begin at, and hold, whole aligned pairs of 16-bit columns
 };
 
 struct TailArgs {
@@ -80,7 +81,7 @@ struct TailArgs {
 
 template <int kF>
 __device__ __forceinline__ bool tail_has(const TailArgs& a, uint32_t feature) {
-  return (kF == kTailAtRunTime ? a.flags : (uint32_t)kF) & feature;
+  return ((uint32_t)kF & kTailAtRunTime ? a.flags : (uint32_t)kF) & feature;
 }
 
 // How the lanes hold a row: kG lanes with kK chunks each.
@@ -105,7 +106,8 @@ struct RowLanes {
   __device__ __forceinline__ bool has(int k, int j) const { return base(k, j >> 2) + (kVec ? 0 : (j & 3)) < C; }
 
   // The lane's chunk k of the row at `row`, whose addresses are valid; absent columns read column 0.
-  template <int DT, bool kVec>
+  // kPairs: as kTailPairs.
+  template <int DT, bool kVec, bool kPairs>
   __device__ __forceinline__ RowChunk<DT> load(const uint8_t* row, int k) const {
     constexpr int kB = ChunkElt<DT>::kBytes;
     RowChunk<DT> r;
@@ -125,6 +127,12 @@ struct RowLanes {
     } else if constexpr (kVec) {
       const int col = base(k, 0);
       r.q[0] = __builtin_nontemporal_load(reinterpret_cast<const stream_u32x4*>(row + (col < C ? (int64_t)col * kB : 0)));
+    } else if constexpr (kB == 2 && kPairs) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int at = base(k, i >> 1) + 2 * (i & 1);
+        r.q[0][i] = *reinterpret_cast<const uint32_t*>(row + (at < C ? (int64_t)at * kB : 0));
+      }
     } else {
 #pragma unroll
       for (int j = 0; j < kChunkCols; ++j) {
@@ -231,7 +239,8 @@ struct RowLanes {
 // side by side: what a row costs beside its values (addresses, sums over lanes,
 // row tests) is paid once for all chunks of a lane.  most: three chunks, but two
 // in the backward of an fp32 x, whose registers then hold two waves a SIMD
-// (524288 x 192, bf16 h: 347 us, with three 693).  Eight lanes a row only where
+// (524288 x 192, bf16 h: 347 us, with three 693) or of rows that are not aligned, whose
+// single columns take more (524288 x 190 bf16: 530 us, with three 1091).  Eight lanes a row only where
 // columns stand eight by eight: as 16-byte pieces of fp32 they would read a
 // 16-bit h in runs of 64 bytes.  From 129 chunks on a workgroup holds the row.
 inline TailShape tail_shape(int C, bool pieces, int most) {
@@ -248,7 +257,7 @@ inline TailShape tail_shape(int C, bool pieces, int most) {
   return {64, 2};
 }
 inline bool tail_pieces(int x_dtype) { return x_dtype == TERRA_DTYPE_F32; }
-inline int tail_bwd_most(int x_dtype) { return x_dtype == TERRA_DTYPE_F32 ? 2 : 3; }
+inline int tail_bwd_most(int x_dtype, bool vec) { return x_dtype == TERRA_DTYPE_F32 || !vec ? 2 : 3; }
 constexpr int kTailMaxChannels = 8192;
 
 constexpr int tail_threads(int lanes) { return lanes > 256 ? lanes : 256; }
@@ -351,9 +360,15 @@ struct ColumnParams {
 };
 
 // Calls f<DTH, DTX, lanes, chunks, kVec, features>(...) for the call's shape and
-// features: those of aligned rows each have kernels of their own, other rows one for all.
+// features: those of aligned rows each have kernels of their own, other rows one for all,
+// or two: 16-bit columns read by pairs where they can be (262144 x 382 bf16: forward
+// 256 us, one by one 289, backward 397 and 492; as a run-time choice, 1009 one by one).
 #define TERRA_TAIL_FEATURES(f, g, k, features, vec, ...)                                                      \
-  if (!(vec)) return f<DTH, DTX, g, k, false, kTailAtRunTime>(__VA_ARGS__);                                   \
+  if (!(vec)) {                                                                                               \
+    if constexpr (DTH != TERRA_DTYPE_F32)                                                                     \
+      if ((features) & kTailPairs) return f<DTH, DTX, g, k, false, kTailAtRunTime | kTailPairs>(__VA_ARGS__); \
+    return f<DTH, DTX, g, k, false, kTailAtRunTime>(__VA_ARGS__);                                             \
+  }                                                                                                           \
   switch ((features) & kTailFeatures) {                                                                       \
     case 0: return f<DTH, DTX, g, k, true, 0>(__VA_ARGS__);                                                   \
     case 1: return f<DTH, DTX, g, k, true, 1>(__VA_ARGS__);                                                   \

@@ -27,8 +27,16 @@ int check_spans(std::initializer_list<Span> in, std::initializer_list<Span> out)
   return TERRA_OK;
 }
 
-// Checks the descriptor; fills the sizes of `a`.  h_rows: rows of h.
-int prepare(const terra_swin_residual_norm_desc* d, TailArgs* a, bool* vec, int64_t* h_rows) {
+// How a call's rows are aligned: the bits that any of its addresses and row strides has set.
+struct Alignment {
+  uintptr_t bits = 0;
+  int C = 0;
+  bool vec() const { return C % kChunkCols == 0 && bits % 16 == 0; }
+  bool pairs() const { return C % 2 == 0 && bits % 4 == 0; }
+};
+
+// Checks the descriptor; fills the sizes of `a` and `al`.  h_rows: rows of h.
+int prepare(const terra_swin_residual_norm_desc* d, TailArgs* a, Alignment* al, int64_t* h_rows) {
   if (d == nullptr) return fail(TERRA_ERR_NULL, "desc is NULL");
   const int h = d->h_dtype, x = d->x_dtype;
   const bool half = h == TERRA_DTYPE_BF16 || h == TERRA_DTYPE_F16;
@@ -59,7 +67,8 @@ int prepare(const terra_swin_residual_norm_desc* d, TailArgs* a, bool* vec, int6
   a->per_sample = a->gate_rows > 1 ? (uint32_t)(d->rows / d->gate_rows) : a->rows;
   a->h_row_bytes = d->h_stride * dtype_size(h);
   a->x_row_bytes = d->x_stride * dtype_size(x);
-  *vec = d->channels % kChunkCols == 0 && a->h_row_bytes % 16 == 0 && a->x_row_bytes % 16 == 0;
+  al->C = d->channels;
+  al->bits = (uintptr_t)a->h_row_bytes | (uintptr_t)a->x_row_bytes;
   *h_rows = d->rows;
   if (d->windows && d->rows > 0) {
     a->flags |= kTailWindows;
@@ -94,9 +103,9 @@ int prepare(const terra_swin_residual_norm_desc* d, TailArgs* a, bool* vec, int6
 
 // Workgroups: what fits the 256 compute units at once; slabs of the rows of a
 // sample so that every workgroup has a unit, and rows enough for its groups.
-TailBwdPlan tail_bwd_plan(uint32_t rows, int C, int gate_rows, int x_dtype) {
+TailBwdPlan tail_bwd_plan(uint32_t rows, int C, int gate_rows, int x_dtype, bool vec) {
   TailBwdPlan p;
-  p.shape = tail_shape(C, tail_pieces(x_dtype), tail_bwd_most(x_dtype));
+  p.shape = tail_shape(C, tail_pieces(x_dtype), tail_bwd_most(x_dtype, vec));
   const uint32_t groups = (uint32_t)(tail_threads(p.shape.lanes) / p.shape.lanes);
   const uint32_t most = p.shape.lanes > 256 ? 512u / (uint32_t)p.shape.chunks : (p.shape.chunks > 1 ? 512u : 1024u);
   const uint32_t samples = gate_rows > 1 ? (uint32_t)gate_rows : 1u, per = rows / samples;
@@ -126,10 +135,10 @@ void by_type(const terra_swin_residual_norm_desc* d, F f) {
 }
 
 // Alignment of a tensor's or a parameter's pointer; NULL where it may be left out.
-int check_pointer(const void* p, int elt, const char* name, bool needed, bool* vec) {
+int check_pointer(const void* p, int elt, const char* name, bool needed, Alignment* al) {
   if (p == nullptr) return needed ? fail(TERRA_ERR_NULL, "%s is NULL", name) : TERRA_OK;
   if ((uintptr_t)p % (uintptr_t)elt != 0) return fail(TERRA_ERR_ALIGN, "%s is not aligned to its elements", name);
-  if ((uintptr_t)p % 16 != 0) *vec = false;
+  al->bits |= (uintptr_t)p;
   return TERRA_OK;
 }
 
@@ -158,20 +167,20 @@ extern "C" int terra_swin_residual_norm(const void* h, const void* x, void* y, v
                                         const void* seed, void* stream) {
   clear_error();
   TailArgs a = {};
-  bool vec = false;
+  Alignment al;
   int64_t h_rows = 0;
-  TERRA_TRY(prepare(desc, &a, &vec, &h_rows));
+  TERRA_TRY(prepare(desc, &a, &al, &h_rows));
   TERRA_TRY(dropout_args(desc->p, seed, desc->stream_id, &a.drop));
   if (a.drop.threshold > 0) a.flags |= kTailDrop;
   if (a.rows == 0) return TERRA_OK;
   const int he = dtype_size(desc->h_dtype), xe = dtype_size(desc->x_dtype);
-  TERRA_TRY(check_pointer(h, he, "h", true, &vec));
-  TERRA_TRY(check_pointer(x, xe, "x", true, &vec));
-  TERRA_TRY(check_pointer(y, xe, "y", true, &vec));
-  TERRA_TRY(check_pointer(z, he, "z", (a.flags & kTailNext) != 0, &vec));
-  TERRA_TRY(check_pointer(gate, 4, "gate", a.gate_rows > 0, &vec));
+  TERRA_TRY(check_pointer(h, he, "h", true, &al));
+  TERRA_TRY(check_pointer(x, xe, "x", true, &al));
+  TERRA_TRY(check_pointer(y, xe, "y", true, &al));
+  TERRA_TRY(check_pointer(z, he, "z", (a.flags & kTailNext) != 0, &al));
+  TERRA_TRY(check_pointer(gate, 4, "gate", a.gate_rows > 0, &al));
   for (const float* p : {post_weight, post_bias, next_weight, next_bias})
-    TERRA_TRY(check_pointer(p, 4, "a norm's parameter", false, &vec));
+    TERRA_TRY(check_pointer(p, 4, "a norm's parameter", false, &al));
   const int64_t C = a.C;
   if ((a.flags & kTailNext) == 0) z = nullptr;
   TERRA_TRY(check_spans({{h, span_bytes(h_rows, a.h_row_bytes, C * he), "h"}, {x, span_bytes(a.rows, a.x_row_bytes, C * xe), "x"}},
@@ -184,7 +193,8 @@ extern "C" int terra_swin_residual_norm(const void* h, const void* x, void* y, v
   if ((a.flags & kTailNext) != 0) a.nw = next_weight, a.nb = next_bias;
   a.gate = gate;
   hipStream_t s = (hipStream_t)stream;
-  by_type(desc, [&](auto t) { t.fwd(&a, vec, s); });
+  if (al.pairs()) a.flags |= kTailPairs;
+  by_type(desc, [&](auto t) { t.fwd(&a, al.vec(), s); });
   return launched("terra_swin_residual_norm");
 }
 
@@ -194,12 +204,17 @@ extern "C" int terra_swin_residual_norm(const void* h, const void* x, void* y, v
 extern "C" int terra_swin_residual_norm_workspace(const terra_swin_residual_norm_desc* desc) {
   clear_error();
   TailArgs a = {};
-  bool vec = false;
+  Alignment al;
   int64_t h_rows = 0;
-  TERRA_TRY(prepare(desc, &a, &vec, &h_rows));
+  TERRA_TRY(prepare(desc, &a, &al, &h_rows));
   if (a.rows == 0) return 0;
-  const TailBwdPlan p = tail_bwd_plan(a.rows, a.C, a.gate_rows, desc->x_dtype);
-  return (int)(p.blocks * 4 * a.C + (a.gate_rows > 0 && p.slabs > 1 ? p.units * a.C : 0));
+  int most = 0;
+  for (const bool vec : {false, true}) {  // which, the call's addresses say
+    const TailBwdPlan p = tail_bwd_plan(a.rows, a.C, a.gate_rows, desc->x_dtype, vec);
+    const int n = (int)(p.blocks * 4 * a.C + (a.gate_rows > 0 && p.slabs > 1 ? p.units * a.C : 0));
+    most = n > most ? n : most;
+  }
+  return most;
 }
 
 extern "C" int terra_swin_residual_norm_bwd(const void* h, const void* x, const void* dy, const void* dz, void* dh, void* dx,
@@ -210,13 +225,13 @@ extern "C" int terra_swin_residual_norm_bwd(const void* h, const void* x, const 
                                             float* dnext_weight, float* dnext_bias, float* workspace, void* stream) {
   clear_error();
   TailArgs a = {};
-  bool vec = false;
+  Alignment al;
   int64_t h_rows = 0;
-  TERRA_TRY(prepare(desc, &a, &vec, &h_rows));
+  TERRA_TRY(prepare(desc, &a, &al, &h_rows));
   TERRA_TRY(dropout_args(desc->p, seed, desc->stream_id, &a.drop));
   if (a.drop.threshold > 0) a.flags |= kTailDrop;
   const int he = dtype_size(desc->h_dtype), xe = dtype_size(desc->x_dtype);
-  bool ignored = false;
+  Alignment ignored;
   for (const float* p : {(const float*)dpost_weight, (const float*)dpost_bias, (const float*)dgate,
                          (const float*)dnext_weight, (const float*)dnext_bias, (const float*)workspace})
     TERRA_TRY(check_pointer(p, 4, "a parameter's gradient or the workspace", false, &ignored));
@@ -236,15 +251,15 @@ extern "C" int terra_swin_residual_norm_bwd(const void* h, const void* x, const 
     if (n > 0) launch_sums(jobs, n, s);
     return launched("terra_swin_residual_norm_bwd");
   }
-  TERRA_TRY(check_pointer(h, he, "h", true, &vec));
-  TERRA_TRY(check_pointer(x, xe, "x", true, &vec));
-  TERRA_TRY(check_pointer(dy, xe, "dy", false, &vec));
-  TERRA_TRY(check_pointer(dz, he, "dz", false, &vec));
-  TERRA_TRY(check_pointer(dh, he, "dh", true, &vec));
-  TERRA_TRY(check_pointer(dx, xe, "dx", true, &vec));
-  TERRA_TRY(check_pointer(gate, 4, "gate", a.gate_rows > 0, &vec));
+  TERRA_TRY(check_pointer(h, he, "h", true, &al));
+  TERRA_TRY(check_pointer(x, xe, "x", true, &al));
+  TERRA_TRY(check_pointer(dy, xe, "dy", false, &al));
+  TERRA_TRY(check_pointer(dz, he, "dz", false, &al));
+  TERRA_TRY(check_pointer(dh, he, "dh", true, &al));
+  TERRA_TRY(check_pointer(dx, xe, "dx", true, &al));
+  TERRA_TRY(check_pointer(gate, 4, "gate", a.gate_rows > 0, &al));
   for (const float* p : {post_weight, post_bias, next_weight})
-    TERRA_TRY(check_pointer(p, 4, "a norm's parameter", false, &vec));
+    TERRA_TRY(check_pointer(p, 4, "a norm's parameter", false, &al));
   const bool sums = dpost_weight != nullptr || dpost_bias != nullptr || dnext_weight != nullptr || dnext_bias != nullptr;
   if ((sums || dgate != nullptr) && workspace == nullptr) return fail(TERRA_ERR_NULL, "parameter gradients need a workspace");
   const int64_t C = a.C;
@@ -262,7 +277,8 @@ extern "C" int terra_swin_residual_norm_bwd(const void* h, const void* x, const 
   if (dz == nullptr) a.flags &= ~kTailNext;
   if (dy != nullptr) a.flags |= kTailDy;
   a.gate = gate;
-  const TailBwdPlan p = tail_bwd_plan(a.rows, a.C, a.gate_rows, desc->x_dtype);
+  if (al.pairs()) a.flags |= kTailPairs;
+  const TailBwdPlan p = tail_bwd_plan(a.rows, a.C, a.gate_rows, desc->x_dtype, al.vec());
   a.slabs = p.slabs;
   a.units = p.units;
   a.partial = sums ? workspace : nullptr;
@@ -271,7 +287,7 @@ extern "C" int terra_swin_residual_norm_bwd(const void* h, const void* x, const 
   const bool direct = dgate != nullptr && p.slabs == 1;
   float* units = workspace + (int64_t)p.blocks * 4 * C;
   a.gate_partial = dgate == nullptr ? nullptr : (direct ? dgate : units);
-  by_type(desc, [&](auto t) { t.bwd(&a, p, vec, s); });
+  by_type(desc, [&](auto t) { t.bwd(&a, p, al.vec(), s); });
   float* dst[4] = {dpost_weight, dpost_bias, dnext_weight, dnext_bias};
   for (int i = 0; i < 4; ++i)
     if (dst[i] != nullptr) jobs.job[n++] = {workspace + i * C, dst[i], 4 * C, (int32_t)p.blocks, 1};

@@ -29,7 +29,7 @@ namespace terra {
 namespace {
 
 template <int DTH, int DTX, int kG, int kK, bool kVec, int kF>
-__global__ __launch_bounds__(tail_threads(kG), kG == 512 && kK == 1 ? 4 : (kK == 3 ? 2 : 1)) void tail_bwd_kernel(const TailArgs a) {
+__global__ __launch_bounds__(tail_threads(kG), kG == 512 && kK == 1 ? 4 : (kK == 3 || (kF & kTailPairs) ? 2 : 1)) void tail_bwd_kernel(const TailArgs a) {
   constexpr int kThreads = tail_threads(kG), kGroups = kThreads / kG, kCols = kG * kK * kChunkCols;
   constexpr int kHB = ChunkElt<DTH>::kBytes, kXB = ChunkElt<DTX>::kBytes;
   constexpr int kP = DTX == TERRA_DTYPE_F32 ? 4 : 8;
@@ -41,6 +41,7 @@ __global__ __launch_bounds__(tail_threads(kG), kG == 512 && kK == 1 ? 4 : (kK ==
   const RowLanes<kG, kK, kP> at = {(int)(threadIdx.x % kG), C};
   RowSum<kG> sum(&s_red);
   const bool full = C == kG * kK * kChunkCols;  // every lane has columns
+  constexpr bool kPairs = kF & kTailPairs;
   Params par(&s_par);  // gw, gb, w2
   auto stage = [&](const float* gate) {
     par.fill(at, [&](int c, float (&v)[3]) {
@@ -119,10 +120,10 @@ __global__ __launch_bounds__(tail_threads(kG), kG == 512 && kK == 1 ? 4 : (kK ==
       const uint8_t* dzp = tail_has<kF>(a, kTailNext) ? a.dz + (int64_t)r * C * kHB : hp;
 #pragma unroll
       for (int k = 0; k < kK; ++k) {
-        hq[k] = at.template load<DTH, kVec>(hp, k);
-        xq[k] = at.template load<DTX, kVec>(xp, k);
-        dzq[k] = at.template load<DTH, kVec>(dzp, k);
-        dyq[k] = at.template load<DTX, kVec>(dyp, k);
+        hq[k] = at.template load<DTH, kVec, kPairs>(hp, k);
+        xq[k] = at.template load<DTX, kVec, kPairs>(xp, k);
+        dzq[k] = at.template load<DTH, kVec, kPairs>(dzp, k);
+        dyq[k] = at.template load<DTX, kVec, kPairs>(dyp, k);
       }
       // The forward: nhat in nv, y in yv.
       float nv[kK][kChunkCols], yv[kK][kChunkCols], dv[kK][kChunkCols];
@@ -272,7 +273,8 @@ __global__ __launch_bounds__(tail_threads(kG), kG == 512 && kK == 1 ? 4 : (kK ==
 
 template <int DTH, int DTX, int kG, int kK, bool kVec, int kF>
 void launch_bwd(const TailArgs& a, const TailBwdPlan& p, hipStream_t s) {
-  tail_bwd_kernel<DTH, DTX, kG, kK, kVec, kF><<<p.blocks, tail_threads(kG), 0, s>>>(a);
+  if constexpr (kVec || kK < 3)  // tail_bwd_most
+    tail_bwd_kernel<DTH, DTX, kG, kK, kVec, kF><<<p.blocks, tail_threads(kG), 0, s>>>(a);
 }
 
 template <int DTH, int DTX>

@@ -20,6 +20,7 @@ __global__ __launch_bounds__(tail_threads(kG)) void tail_kernel(const TailArgs a
   const RowLanes<kG, kK, kP> at = {(int)(threadIdx.x % kG), C};
   RowSum<kG> sum(&s_red);
   const bool full = C == kG * kK * kChunkCols;  // every lane has columns
+  constexpr bool kPairs = kF & kTailPairs;
   Params par(&s_par);  // gw, gb (branch_params), nw, nb
   const uint64_t seed = tail_has<kF>(a, kTailDrop) ? *a.drop.seed : 0;
   // A row's chunks of h and x; a row past the end re-reads the last one.
@@ -39,8 +40,8 @@ __global__ __launch_bounds__(tail_threads(kG)) void tail_kernel(const TailArgs a
     const uint8_t* xp = a.x + (int64_t)q.r * a.x_row_bytes;
 #pragma unroll
     for (int k = 0; k < kK; ++k) {
-      q.h[k] = at.template load<DTH, kVec>(hp, k);
-      q.x[k] = at.template load<DTX, kVec>(xp, k);
+      q.h[k] = at.template load<DTH, kVec, kPairs>(hp, k);
+      q.x[k] = at.template load<DTX, kVec, kPairs>(xp, k);
     }
     return q;
   };
