@@ -43,14 +43,20 @@ __global__ __launch_bounds__(tail_threads(kG), kG == 512 && kK == 1 ? 4 : (kK ==
   const bool full = C == kG * kK * kChunkCols;  // every lane has columns
   constexpr bool kPairs = kF & kTailPairs;
   Params par(&s_par);  // gw, gb, w2
+  // Returns whether a gate is infinite or NaN: only then do the rows' loops see
+  // to it that a dropped element's gradient is 0 (with the test in every case,
+  // 262144 x 384 bf16 took 274 us instead of 243).
   auto stage = [&](const float* gate) {
+    int odd = 0;
     par.fill(at, [&](int c, float (&v)[3]) {
       branch_params(a, gate, c, v[0], v[1]);
       v[2] = param_at(a.nw, 1.f, c);
+      odd |= !(fabsf(v[0]) <= 3.4028235e38f);
     });
+    if (!tail_has<kF>(a, kTailDrop)) odd = 0;
+    return __syncthreads_or(odd) != 0;
   };
-  stage(a.gate_rows == 1 ? a.gate : nullptr);
-  if constexpr (Params::kLds) __syncthreads();
+  bool odd_gate = stage(a.gate_rows == 1 ? a.gate : nullptr);
   const uint64_t seed = tail_has<kF>(a, kTailDrop) ? *a.drop.seed : 0;
 
   float acc_a[kK][kChunkCols] = {}, acc_b[kK][kChunkCols] = {}, acc_nw[kK][kChunkCols] = {}, acc_nb[kK][kChunkCols] = {};
@@ -102,8 +108,7 @@ __global__ __launch_bounds__(tail_threads(kG), kG == 512 && kK == 1 ? 4 : (kK ==
     const float* const gate = a.gate_rows > 0 ? a.gate + (int64_t)sample * C : nullptr;
     if (a.gate_rows > 1) {
       if constexpr (Params::kLds) __syncthreads();
-      stage(gate);
-      if constexpr (Params::kLds) __syncthreads();
+      odd_gate = stage(gate);
     }
     for (uint32_t base = sample * a.per_sample + slab * kGroups; base < end; base += a.slabs * kGroups) {
       par.stay();
@@ -214,8 +219,12 @@ __global__ __launch_bounds__(tail_threads(kG), kG == 512 && kK == 1 ? 4 : (kK ==
           }
         par.get(0, k, at, gw);
 #pragma unroll
+        for (int j = 0; j < kChunkCols; ++j) dv[k][j] *= gw[j];
+        if (odd_gate)
+#pragma unroll
+          for (int j = 0; j < kChunkCols; ++j) dv[k][j] = kept(draws[k], j, a.drop.threshold) ? dv[k][j] : 0.f;
+#pragma unroll
         for (int j = 0; j < kChunkCols; ++j) {
-          dv[k][j] = kept(draws[k], j, a.drop.threshold) ? dv[k][j] * gw[j] : 0.f;  // 0 whatever the gate is
           s0 += dv[k][j];
           s1 = fmaf(dv[k][j], nv[k][j], s1);
         }
