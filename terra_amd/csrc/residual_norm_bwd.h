@@ -28,8 +28,18 @@
 namespace terra {
 namespace {
 
+// Waves a SIMD that the registers of a kernel must leave room for: two where it
+// would otherwise take a few more than half of them (131072 x 768, bf16 h and
+// fp32 x: 353 us, with one wave 421); columns read one by one are slower so
+// (262144 x 385 bf16: 599 us against 505).
+template <int DTX, int kG, int kK, bool kVec, int kF>
+constexpr int tail_bwd_waves() {
+  if (kG == 512 && kK == 1) return 4;
+  return kK == 3 || (kF & kTailPairs) != 0 || (kVec && kG == 64 && DTX == TERRA_DTYPE_F32) ? 2 : 1;
+}
+
 template <int DTH, int DTX, int kG, int kK, bool kVec, int kF>
-__global__ __launch_bounds__(tail_threads(kG), kG == 512 && kK == 1 ? 4 : (kK == 3 || (kF & kTailPairs) ? 2 : 1)) void tail_bwd_kernel(const TailArgs a) {
+__global__ __launch_bounds__(tail_threads(kG), (tail_bwd_waves<DTX, kG, kK, kVec, kF>())) void tail_bwd_kernel(const TailArgs a) {
   constexpr int kThreads = tail_threads(kG), kGroups = kThreads / kG, kCols = kG * kK * kChunkCols;
   constexpr int kHB = ChunkElt<DTH>::kBytes, kXB = ChunkElt<DTX>::kBytes;
   constexpr int kP = DTX == TERRA_DTYPE_F32 ? 4 : 8;
