@@ -103,7 +103,8 @@ __device__ __forceinline__ void table_factors(const stream_u32x4& h, const uint8
       f[j] = drop_factor<kOp>(__uint_as_float(j & 1 ? h[j >> 1] & 0xffff0000u : h[j >> 1] << 16), scale);
 }
 
-template <int kOp, int DT, bool kVec, bool kTable>
+// kPairs: rows that are not of whole aligned chunks, but begin at and hold whole aligned pairs of 16-bit columns.
+template <int kOp, int DT, bool kVec, bool kTable, bool kPairs>
 __global__ __launch_bounds__(kDropThreads) void drop_kernel(const DropParams a) {
   constexpr int kB = ChunkElt<DT>::kBytes;
   constexpr bool kBwd = kOp >= kGeluBwd;
@@ -132,6 +133,12 @@ __global__ __launch_bounds__(kDropThreads) void drop_kernel(const DropParams a) 
       for (int q = 0; q < RowChunk<DT>::kWords; ++q)
         r.q[q] = __builtin_nontemporal_load(
             reinterpret_cast<const stream_u32x4*>(row + (present && c[q] < width ? strip + c[q] * kB : 0)));
+    } else if constexpr (kPairs) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int at = c[i >> 1] + 2 * (i & 1);
+        r.q[0][i] = *reinterpret_cast<const uint32_t*>(row + (present && at < width ? strip + (int64_t)at * kB : 0));
+      }
     } else {
 #pragma unroll
       for (int j = 0; j < kChunkCols; ++j) {
@@ -264,30 +271,40 @@ bool drop_table(int op, int dtype, int64_t rows, int64_t C, bool vec) {
   return op == kGeluFwd && dtype == TERRA_DTYPE_BF16 && vec && rows * C >= kTableElements;
 }
 
+// How a call's rows are aligned: the bits that any of its addresses and row strides has set.
+struct DropAlignment {
+  uintptr_t bits = 0;
+  int64_t C = 0;
+  bool vec() const { return C % kChunkCols == 0 && bits % 16 == 0; }
+  bool pairs() const { return C % 2 == 0 && bits % 4 == 0; }
+};
+
 template <int kOp, int DT>
-void launch_drop(DropParams a, bool vec, hipStream_t s) {
-  const bool table = drop_table(kOp, DT, a.rows, a.C, vec);
+void launch_drop(DropParams a, const DropAlignment& al, hipStream_t s) {
+  const bool vec = al.vec(), table = drop_table(kOp, DT, a.rows, a.C, vec);
   const DropPlan p = drop_plan(a.rows, a.C, DT == TERRA_DTYPE_F32, table ? kTableBlocks : (kOp == kGeluBwdSum ? kSumBlocks : 0));
   a.T = p.T;
   a.R = p.R;
   const dim3 grid((unsigned)p.blocks, (unsigned)p.strips);
   const int threads = (p.T * p.R + 63) / 64 * 64;
   if constexpr (kOp == kGeluFwd && DT == TERRA_DTYPE_BF16)
-    if (table) return (void)(drop_kernel<kOp, DT, true, true><<<grid, threads, 0, s>>>(a));
-  if (vec) drop_kernel<kOp, DT, true, false><<<grid, threads, 0, s>>>(a);
-  else drop_kernel<kOp, DT, false, false><<<grid, threads, 0, s>>>(a);
+    if (table) return (void)(drop_kernel<kOp, DT, true, true, false><<<grid, threads, 0, s>>>(a));
+  if (vec) return (void)(drop_kernel<kOp, DT, true, false, false><<<grid, threads, 0, s>>>(a));
+  if constexpr (DT != TERRA_DTYPE_F32)
+    if (al.pairs()) return (void)(drop_kernel<kOp, DT, false, false, true><<<grid, threads, 0, s>>>(a));
+  drop_kernel<kOp, DT, false, false, false><<<grid, threads, 0, s>>>(a);
 }
 
 template <int kOp>
-void dispatch_drop(int dtype, const DropParams& a, bool vec, hipStream_t s) {
-  if (dtype == TERRA_DTYPE_F32) launch_drop<kOp, TERRA_DTYPE_F32>(a, vec, s);
-  else if (dtype == TERRA_DTYPE_BF16) launch_drop<kOp, TERRA_DTYPE_BF16>(a, vec, s);
-  else launch_drop<kOp, TERRA_DTYPE_F16>(a, vec, s);
+void dispatch_drop(int dtype, const DropParams& a, const DropAlignment& al, hipStream_t s) {
+  if (dtype == TERRA_DTYPE_F32) launch_drop<kOp, TERRA_DTYPE_F32>(a, al, s);
+  else if (dtype == TERRA_DTYPE_BF16) launch_drop<kOp, TERRA_DTYPE_BF16>(a, al, s);
+  else launch_drop<kOp, TERRA_DTYPE_F16>(a, al, s);
 }
 
 // The checks that the three entry points share; fills all but the pointers of `a`.
 int drop_prepare(int dtype, int64_t rows, int64_t C, int64_t in_stride, double p, const void* seed, uint32_t stream,
-                 DropParams* a, bool* vec) {
+                 DropParams* a, DropAlignment* al) {
   if (dtype != TERRA_DTYPE_F32 && dtype != TERRA_DTYPE_BF16 && dtype != TERRA_DTYPE_F16)
     return fail(TERRA_ERR_DTYPE, "dropout supports f32, bf16 and f16 (got dtype %d)", dtype);
   if (rows < 0 || C <= 0) return fail(TERRA_ERR_SHAPE, "rows must be >= 0 and columns > 0");
@@ -301,15 +318,16 @@ int drop_prepare(int dtype, int64_t rows, int64_t C, int64_t in_stride, double p
   a->C = (int32_t)C;
   a->row_bytes = C * elt;
   a->in_row_bytes = in_stride * elt;
-  *vec = C % kChunkCols == 0 && a->in_row_bytes % 16 == 0;
+  al->C = C;
+  al->bits = (uintptr_t)a->in_row_bytes;
   return TERRA_OK;
 }
 
-int drop_pointers(int dtype, std::initializer_list<const void*> tensors, bool* vec) {
+int drop_pointers(int dtype, std::initializer_list<const void*> tensors, DropAlignment* al) {
   for (const void* p : tensors) {
     if (p == nullptr) return fail(TERRA_ERR_NULL, "a tensor is NULL");
     if ((uintptr_t)p % (uintptr_t)dtype_size(dtype) != 0) return fail(TERRA_ERR_ALIGN, "a tensor is not aligned to its elements");
-    if ((uintptr_t)p % 16 != 0) *vec = false;
+    al->bits |= (uintptr_t)p;
   }
   return TERRA_OK;
 }
@@ -334,16 +352,16 @@ extern "C" int terra_swin_dropout(const void* x, void* y, int dtype, int64_t row
                                   double p, const void* seed, uint32_t stream_id, void* stream) {
   clear_error();
   DropParams a = {};
-  bool vec = false;
-  int st = drop_prepare(dtype, rows, columns, x_stride, p, seed, stream_id, &a, &vec);
+  DropAlignment al;
+  int st = drop_prepare(dtype, rows, columns, x_stride, p, seed, stream_id, &a, &al);
   if (st != TERRA_OK || rows == 0) return st;
-  if ((st = drop_pointers(dtype, {x, y}, &vec)) != TERRA_OK) return st;
+  if ((st = drop_pointers(dtype, {x, y}, &al)) != TERRA_OK) return st;
   if (!(x == y && x_stride == columns) &&
       meet(x, (rows - 1) * a.in_row_bytes + a.row_bytes, y, rows * a.row_bytes))
     return fail(TERRA_ERR_SHAPE, "y may be x itself (of packed rows) and must not overlap it otherwise");
   a.in = (const uint8_t*)x;
   a.out = (uint8_t*)y;
-  dispatch_drop<kDropout>(dtype, a, vec, (hipStream_t)stream);
+  dispatch_drop<kDropout>(dtype, a, al, (hipStream_t)stream);
   return drop_launched("terra_swin_dropout");
 }
 
@@ -351,15 +369,15 @@ extern "C" int terra_swin_gelu_dropout(const void* h, void* a_out, int dtype, in
                                        const void* seed, uint32_t stream_id, void* stream) {
   clear_error();
   DropParams a = {};
-  bool vec = false;
-  int st = drop_prepare(dtype, rows, columns, columns, p, seed, stream_id, &a, &vec);
+  DropAlignment al;
+  int st = drop_prepare(dtype, rows, columns, columns, p, seed, stream_id, &a, &al);
   if (st != TERRA_OK || rows == 0) return st;
-  if ((st = drop_pointers(dtype, {h, a_out}, &vec)) != TERRA_OK) return st;
+  if ((st = drop_pointers(dtype, {h, a_out}, &al)) != TERRA_OK) return st;
   if (h != a_out && meet(h, rows * a.row_bytes, a_out, rows * a.row_bytes))
     return fail(TERRA_ERR_SHAPE, "a may be h itself and must not overlap it otherwise");
   a.in = (const uint8_t*)h;
   a.out = (uint8_t*)a_out;
-  dispatch_drop<kGeluFwd>(dtype, a, vec, (hipStream_t)stream);
+  dispatch_drop<kGeluFwd>(dtype, a, al, (hipStream_t)stream);
   return drop_launched("terra_swin_gelu_dropout");
 }
 
@@ -375,8 +393,8 @@ extern "C" int terra_swin_gelu_dropout_bwd(const void* da, const void* h, void* 
                                            float* column_sums, float* workspace, void* stream) {
   clear_error();
   DropParams a = {};
-  bool vec = false;
-  int st = drop_prepare(dtype, rows, columns, columns, p, seed, stream_id, &a, &vec);
+  DropAlignment al;
+  int st = drop_prepare(dtype, rows, columns, columns, p, seed, stream_id, &a, &al);
   if (st != TERRA_OK) return st;
   if (((uintptr_t)column_sums & 3u) != 0 || ((uintptr_t)workspace & 3u) != 0)
     return fail(TERRA_ERR_ALIGN, "column_sums and workspace must be 4-byte aligned");
@@ -389,7 +407,7 @@ extern "C" int terra_swin_gelu_dropout_bwd(const void* da, const void* h, void* 
     launch_sums(jobs, 1, s);
     return drop_launched("terra_swin_gelu_dropout_bwd");
   }
-  if ((st = drop_pointers(dtype, {da, h, dh}, &vec)) != TERRA_OK) return st;
+  if ((st = drop_pointers(dtype, {da, h, dh}, &al)) != TERRA_OK) return st;
   if (column_sums != nullptr && workspace == nullptr) return fail(TERRA_ERR_NULL, "column sums need a workspace");
   const int64_t bytes = rows * a.row_bytes;
   if ((da != dh && meet(da, bytes, dh, bytes)) || (h != dh && meet(h, bytes, dh, bytes)))
@@ -399,9 +417,9 @@ extern "C" int terra_swin_gelu_dropout_bwd(const void* da, const void* h, void* 
   a.out = (uint8_t*)dh;
   a.partial = workspace;
   if (column_sums == nullptr) {
-    dispatch_drop<kGeluBwd>(dtype, a, vec, s);
+    dispatch_drop<kGeluBwd>(dtype, a, al, s);
   } else {
-    dispatch_drop<kGeluBwdSum>(dtype, a, vec, s);
+    dispatch_drop<kGeluBwdSum>(dtype, a, al, s);
     jobs.job[0] = {workspace, column_sums, columns, (int32_t)drop_plan(rows, (int)columns, dtype == TERRA_DTYPE_F32, kSumBlocks).blocks, 1};
     launch_sums(jobs, 1, s);
   }
