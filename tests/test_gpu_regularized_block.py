@@ -257,6 +257,45 @@ def test_layers_of_another_kind_are_called(dev):
         assert (mlp(x) - want).norm() <= 2e-5 * want.norm()
 
 
+def test_checkpointing_repeats_the_masks(dev):
+    from torch.utils.checkpoint import checkpoint
+
+    blocks = [b.to(dev).train() for b in _blocks(96, 3, 7, 14, 14)]
+    x = torch.randn(1, 196, 96, device=dev, requires_grad=True)
+    for b in blocks:
+        torch.manual_seed(8)
+        y = b(x)
+        want, = torch.autograd.grad(y.sum(), x)
+        torch.manual_seed(8)
+        again = checkpoint(b, x, use_reentrant=False)
+        got, = torch.autograd.grad(again.sum(), x)
+        # bit for bit but for the LayerNorm gather's sums, which do not reach x's gradient
+        assert torch.equal(again, y) and torch.equal(got, want)
+
+
+def test_frozen_parameters_and_inference(dev):
+    """A gradient for a gate or for the input alone, and calls in inference mode."""
+    blocks = [b.to(dev).train() for b in _blocks(96, 3, 7, 14, 14)]
+    x = torch.randn(1, 196, 96, device=dev)
+    for b, gate in zip(blocks, (blocks[0].layer_scale1, blocks[1].layer_scale2)):
+        torch.manual_seed(9)
+        want = torch.autograd.grad(b(x.requires_grad_()).sum(), (x, gate))
+        x.requires_grad_(False)
+        b.requires_grad_(False)
+        gate.requires_grad_(True)
+        torch.manual_seed(9)
+        assert torch.equal(torch.autograd.grad(b(x).sum(), gate)[0], want[1])
+        gate.requires_grad_(False)
+        torch.manual_seed(9)
+        assert torch.equal(torch.autograd.grad(b(x.requires_grad_()).sum(), x)[0], want[0])
+        torch.manual_seed(9)
+        y = b(x)
+        x.requires_grad_(False)
+        torch.manual_seed(9)
+        with torch.inference_mode():
+            assert (b(x) - y.detach()).norm() <= 2e-5 * y.detach().norm()
+
+
 def _captured(step):
     side = torch.cuda.Stream()
     side.wait_stream(torch.cuda.current_stream())
