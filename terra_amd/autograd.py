@@ -21,6 +21,7 @@ from __future__ import annotations
 from typing import Optional, Tuple, Union
 
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import _lib, kernels
@@ -31,6 +32,11 @@ MaskArg = Union[None, torch.Tensor, ShiftMask, WindowMask]
 
 def _needs_grad(*tensors: Optional[torch.Tensor]) -> bool:
     return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+
+
+def _has_tangent(x: torch.Tensor) -> bool:
+    """x is a dual tensor of forward-mode differentiation."""
+    return forward_ad._current_level >= 0 and forward_ad.unpack_dual(x).tangent is not None
 
 
 class _Partition(torch.autograd.Function):
@@ -650,13 +656,19 @@ def attention_half(x: torch.Tensor, geom: WindowGeometry, norm: torch.nn.LayerNo
 
 
 class _Dropout(torch.autograd.Function):
-    """kernels.dropout; the backward draws the mask again from the seed."""
+    """kernels.dropout; the backward draws the mask again from the seed.  A
+    tangent is dropped as the values are."""
 
     @staticmethod
     def forward(ctx, x, p, seed, stream):
         ctx.p, ctx.stream = p, stream
         ctx.save_for_backward(seed)
+        ctx.save_for_forward(seed)
         return kernels.dropout(x, p, seed, stream)
+
+    @staticmethod
+    def jvp(ctx, dx, *_):
+        return kernels.dropout(dx.contiguous(), ctx.p, ctx.saved_tensors[0], ctx.stream)
 
     @staticmethod
     @once_differentiable
@@ -669,20 +681,29 @@ def _seed(x: torch.Tensor, p: float, seed: Optional[torch.Tensor]) -> Optional[t
 
 
 def dropout(x: torch.Tensor, p: float, seed: Optional[torch.Tensor] = None, stream: int = 0) -> torch.Tensor:
-    """:func:`kernels.dropout` with a gradient.  ``seed`` None draws one from
-    torch's generator on x's device."""
+    """:func:`kernels.dropout` with a gradient and a forward-mode derivative.
+    ``seed`` None draws one from torch's generator on x's device."""
     seed = _seed(x, p, seed)
-    if _needs_grad(x):
+    if _needs_grad(x) or _has_tangent(x):
         return _Dropout.apply(x, p, seed, stream)
     return kernels.dropout(x, p, seed, stream)
 
 
 class _GeluDropout(torch.autograd.Function):
+    """kernels.gelu_dropout.  It acts element by element, so a tangent is
+    multiplied by what a gradient is."""
+
     @staticmethod
     def forward(ctx, h, p, seed, stream, bias_sums):
         ctx.p, ctx.stream, ctx.bias_sums = p, stream, bias_sums
         ctx.save_for_backward(h, seed)
+        ctx.save_for_forward(h, seed)
         return kernels.gelu_dropout(h, p, seed, stream)
+
+    @staticmethod
+    def jvp(ctx, dh, *_):
+        h, seed = ctx.saved_tensors
+        return kernels.gelu_dropout_backward(dh.contiguous(), h, ctx.p, seed, ctx.stream)
 
     @staticmethod
     @once_differentiable
@@ -697,11 +718,11 @@ class _GeluDropout(torch.autograd.Function):
 
 def gelu_dropout(h: torch.Tensor, p: float, seed: Optional[torch.Tensor] = None, stream: int = 0,
                  bias_sums: Optional[ColumnSumLink] = None) -> torch.Tensor:
-    """:func:`kernels.gelu_dropout` with a gradient.  ``seed`` None draws one
-    from torch's generator.  ``bias_sums``: the :class:`ColumnSumLink` of the
+    """:func:`kernels.gelu_dropout` with a gradient and a forward-mode
+    derivative.  ``seed`` None draws one from torch's generator.  ``bias_sums``: the :class:`ColumnSumLink` of the
     :func:`linear` that produced ``h``, whose bias gradient the backward sums."""
     seed, h = _seed(h, p, seed), h.contiguous()
-    if _needs_grad(h):
+    if _needs_grad(h) or _has_tangent(h):
         return _GeluDropout.apply(h, p, seed, stream, bias_sums)
     return kernels.gelu_dropout(h, p, seed, stream)
 

@@ -1,0 +1,62 @@
+"""Derivatives of autograd.dropout and autograd.gelu_dropout beside the first
+backward: forward mode.
+
+Both maps act element by element, so a tangent is multiplied by what a gradient
+is: equal bit for bit to the backward kernel's result on it.
+"""
+import pytest
+import torch
+from torch.autograd import forward_ad
+
+from terra_amd import autograd, kernels
+
+pytestmark = pytest.mark.gpu
+
+TYPES = [torch.float32, torch.bfloat16, torch.float16]
+
+
+def _rand(shape, dt, seed, dev):
+    return torch.randn(*shape, generator=torch.Generator().manual_seed(seed)).to(dt).to(dev)
+
+
+def _seed(dev, value=0x1234567890ABCDE):
+    return torch.tensor([value], dtype=torch.int64, device=dev)
+
+
+@pytest.mark.parametrize("dt", TYPES)
+@pytest.mark.parametrize("needs_grad", [False, True])
+@pytest.mark.parametrize("p", [0.0, 0.3])
+def test_tangents(dev, dt, needs_grad, p):
+    x, t = _rand((37, 100), dt, 1, dev).requires_grad_(needs_grad), _rand((37, 100), dt, 2, dev)
+    seed = _seed(dev) if p else None
+    with forward_ad.dual_level():
+        dual = forward_ad.make_dual(x, t)
+        y = forward_ad.unpack_dual(autograd.dropout(dual, p, seed, 4))
+        assert torch.equal(y.primal, kernels.dropout(x, p, seed, 4))
+        assert torch.equal(y.tangent, kernels.dropout(t, p, seed, 4))
+        a = forward_ad.unpack_dual(autograd.gelu_dropout(dual, p, seed, 4))
+        assert torch.equal(a.primal, kernels.gelu_dropout(x.detach(), p, seed, 4))
+        assert torch.equal(a.tangent, kernels.gelu_dropout_backward(t, x.detach(), p, seed, 4))
+        with torch.no_grad():
+            assert torch.equal(forward_ad.unpack_dual(autograd.dropout(dual, p, seed, 4)).tangent, y.tangent)
+        # one without a tangent stays without
+        assert forward_ad.unpack_dual(autograd.dropout(x, p, seed, 4)).tangent is None
+
+
+def test_tangent_of_strided_rows(dev):
+    """A tangent comes in its primal's strides, or as an expanded one."""
+    x, t = _rand((20, 192), torch.float32, 3, dev)[:, 64:128], _rand((20, 64), torch.float32, 4, dev)
+    with forward_ad.dual_level():
+        y = forward_ad.unpack_dual(autograd.dropout(forward_ad.make_dual(x, t), 0.25, _seed(dev)))
+        assert torch.equal(y.tangent, kernels.dropout(t, 0.25, _seed(dev)))
+        one = torch.ones((), device=dev).expand(20, 64)
+        y = forward_ad.unpack_dual(autograd.dropout(forward_ad.make_dual(x.contiguous(), one), 0.25, _seed(dev)))
+        assert torch.equal(y.tangent, kernels.dropout(torch.ones(20, 64, device=dev), 0.25, _seed(dev)))
+
+
+def test_tangents_of_no_rows(dev):
+    x = torch.empty(0, 8, device=dev)
+    with forward_ad.dual_level():
+        dual = forward_ad.make_dual(x, x.clone())
+        for f in (autograd.dropout, autograd.gelu_dropout):
+            assert forward_ad.unpack_dual(f(dual, 0.3, _seed(dev))).tangent.shape == (0, 8)
