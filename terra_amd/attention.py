@@ -46,11 +46,13 @@ def probability(p: float, name: str) -> float:
 
 
 def plain(module: torch.nn.Module, kind: type) -> bool:
-    """``module`` is a ``kind`` itself whose call no forward hook would see, so
-    that its parameters may be used in its place."""
+    """``module`` is a ``kind`` itself whose call no hook would see, forward or
+    backward, so that its parameters may be used in its place."""
     d, hooks = module.__dict__, torch.nn.modules.module
     return (type(module) is kind and "forward" not in d and not d["_forward_hooks"] and not d["_forward_pre_hooks"]
-            and not hooks._global_forward_hooks and not hooks._global_forward_pre_hooks)
+            and not d["_backward_hooks"] and not d["_backward_pre_hooks"]
+            and not hooks._global_forward_hooks and not hooks._global_forward_pre_hooks
+            and not hooks._global_backward_hooks and not hooks._global_backward_pre_hooks)
 
 
 def relative_position_index(window_size: Sequence[int]) -> torch.Tensor:
