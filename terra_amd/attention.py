@@ -55,6 +55,12 @@ def plain(module: torch.nn.Module, kind: type) -> bool:
             and not hooks._global_backward_hooks and not hooks._global_backward_pre_hooks)
 
 
+def plain_norm(module: torch.nn.Module, channels: int) -> bool:
+    """``module`` is a LayerNorm or RMSNorm over the channels that is :func:`plain`."""
+    return (any(plain(module, kind) for kind in (torch.nn.LayerNorm, torch.nn.RMSNorm))
+            and tuple(module.normalized_shape) == (channels,))
+
+
 def relative_position_index(window_size: Sequence[int]) -> torch.Tensor:
     """Swin relative-position index [Wh*Ww, Wh*Ww] (models/attention.py:205-214):
     idx[i, j] = (hi - hj + Wh - 1) * (2*Ww - 1) + (wi - wj + Ww - 1)."""

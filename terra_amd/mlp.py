@@ -40,7 +40,7 @@ import torch
 import torch.nn.functional as F
 
 from . import autograd, config, kernels
-from .attention import make_linear_with_seed, plain, probability
+from .attention import make_linear_with_seed, plain, plain_norm, probability
 
 
 def _disable_parameters_if_mlp_off(module: torch.nn.Module) -> None:
@@ -207,7 +207,8 @@ class SequentialMlp(torch.nn.Module):
 
     def _tail_forward(self, x: torch.Tensor, normed: Optional[torch.Tensor]) -> torch.Tensor:
         """The MLP with dropout after its activation and kernels.residual_norm
-        at its end (see the module's docstring)."""
+        at its end (see the module's docstring).  A layer of another class than
+        the kernels take, or that hooks watch, is called."""
         C = x.shape[-1]
         rows = x.reshape(-1, C).contiguous()
         link, p, hidden_p = None, self.dropout if self.training else 0.0, self.hidden_dropout if self.training else 0.0
@@ -216,7 +217,7 @@ class SequentialMlp(torch.nn.Module):
             xn = normed.reshape(rows.shape)
         elif not config.use_layernorm:
             xn = rows
-        elif type(self.norm2) is torch.nn.LayerNorm and tuple(self.norm2.normalized_shape) == (C,) and C <= 1024 \
+        elif plain(self.norm2, torch.nn.LayerNorm) and tuple(self.norm2.normalized_shape) == (C,) and C <= 1024 \
                 and (C * x.element_size()) % 16 == 0 and rows.shape[0] > 0:
             n = self.norm2
             # The gradient that reaches x beside the branch is added in the LayerNorm backward's kernel.
@@ -224,7 +225,7 @@ class SequentialMlp(torch.nn.Module):
             xn = autograd.partition_ln(rows.view(1, -1, 1, C), kernels.rows_geometry(rows.shape[0], C), n.weight, n.bias,
                                        n.eps, out_dtype=autograd.linear_input_dtype(rows), link=link).view(-1, C)
         else:
-            xn = self.norm2(rows)
+            xn = self.norm2(x).reshape(rows.shape)
         fc1, fc2, bias_sums = self.fc1, self.fc2, None
         own = [plain(fc, torch.nn.Linear) for fc in (fc1, fc2)]
         gelu = plain(self.act, torch.nn.GELU) and self.act.approximate == "none"
@@ -237,8 +238,10 @@ class SequentialMlp(torch.nn.Module):
             a = self.act(a)
             if hidden_p > 0.0:
                 a = autograd.dropout(a, hidden_p, seed, stream=1)
-        h = autograd.linear(a, fc2.weight, fc2.bias) if own[1] else fc2(a)
-        return autograd.residual_norm(h, rows, kernels.Norm.of(self.post_norm2), self.layer_scale2, None, None,
+        h, post = autograd.linear(a, fc2.weight, fc2.bias) if own[1] else fc2(a), self.post_norm2
+        if post is not None and not plain_norm(post, C):
+            h, post = post(h.reshape(x.shape)).to(h.dtype).reshape(rows.shape), None
+        return autograd.residual_norm(h, rows, kernels.Norm.of(post), self.layer_scale2, None, None,
                                       self.residual_scale, p, seed, link=link if h.requires_grad else None).view(x.shape)
 
     def forward(self, x: torch.Tensor, out: Optional[torch.Tensor] = None,

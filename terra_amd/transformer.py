@@ -31,10 +31,10 @@ share of a window-parallel grid; and the half-block's end,
     y = residual_scale * x + layer_scale * dropout(post_norm(branch)),
 
 with the window reverse and the roll in one launch each way
-(``kernels.residual_norm``): ``post_norm`` (a norm over the branch),
-``layer_scale`` (a gate per channel, its initial value), ``residual_scale`` and
-``dropout`` (in training mode; the mask is drawn from torch's seed and never
-stored).  ``forward(x, next_norm=norm)`` also gives ``norm(y)`` from the same
+(``kernels.residual_norm``): ``post_norm`` (a ``norm_layer`` over the branch's
+tokens, which stand in window order [B_, N, C]), ``layer_scale`` (a gate per
+channel, its initial value), ``residual_scale`` and ``dropout`` (in training
+mode; the mask is drawn from torch's seed and never stored).  ``forward(x, next_norm=norm)`` also gives ``norm(y)`` from the same
 launch, for an MLP half that takes it (``SequentialMlp.forward(y, normed=z)``).
 """
 from __future__ import annotations
@@ -44,7 +44,7 @@ from typing import Optional, Tuple
 import torch
 
 from . import autograd, config, kernels
-from .attention import WindowAttention, probability
+from .attention import WindowAttention, plain, plain_norm, probability
 from .kernels import ShiftMask, WindowGeometry, WindowMask
 from .utils import get_swin_attention_mask, land_window_bits
 
@@ -289,12 +289,13 @@ class SequentialSwinTransformer(torch.nn.Module):
 
     def _tail_forward(self, x: torch.Tensor, next_norm: Optional[torch.nn.Module]):
         """The staged path with kernels.residual_norm at its end (see the
-        module's docstring): y, or (y, next_norm(y))."""
+        module's docstring): y, or (y, next_norm(y)).  A norm that the kernels
+        do not take, or that hooks watch, is called; the types stay as they are."""
         B, L, C = x.shape
         geom = self.geometry(B)
         grid = x.contiguous().view(B, *self.input_resolution, C)
         link = None
-        if config.use_layernorm and self._fusable_norm(grid.dtype):
+        if config.use_layernorm and self._fusable_norm(grid.dtype) and plain(self.norm1, torch.nn.LayerNorm):
             # The gradient that reaches x beside the branch is added in the LayerNorm backward's kernel.
             link = autograd.ResidualLink() if torch.is_grad_enabled() and x.requires_grad else None
             n = self.norm1
@@ -303,11 +304,17 @@ class SequentialSwinTransformer(torch.nn.Module):
         else:
             windows = self.norm1(x).contiguous().view(grid.shape) if config.use_layernorm else grid
             windows = autograd.partition(windows, geom)
-        h = self.attn(windows, mask=self.window_mask(geom)).contiguous()
-        out = autograd.residual_norm(h, grid, kernels.Norm.of(self.post_norm1), self.layer_scale1,
-                                     kernels.Norm.of(next_norm), geom, self.residual_scale,
+        h, post = self.attn(windows, mask=self.window_mask(geom)).contiguous(), self.post_norm1
+        if post is not None and not plain_norm(post, C):
+            h, post = post(h).to(h.dtype).contiguous(), None
+        fused_next = next_norm if next_norm is not None and plain_norm(next_norm, C) else None
+        out = autograd.residual_norm(h, grid, kernels.Norm.of(post), self.layer_scale1,
+                                     kernels.Norm.of(fused_next), geom, self.residual_scale,
                                      self.dropout if self.training else 0.0, link=link if h.requires_grad else None)
-        return out.view(B, L, C) if next_norm is None else tuple(t.view(B, L, C) for t in out)
+        if fused_next is not None:
+            return tuple(t.view(B, L, C) for t in out)
+        y = out.view(B, L, C)
+        return y if next_norm is None else (y, next_norm(y).to(h.dtype))
 
     def forward(self, x: torch.Tensor, next_norm: Optional[torch.nn.Module] = None):
         H, W = self.input_resolution
