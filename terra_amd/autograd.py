@@ -50,24 +50,41 @@ class _Partition(torch.autograd.Function):
         return kernels.swin_reverse(grad.contiguous(), ctx.geom), None
 
 
-class ResidualLink:
+class _Link:
+    """A tensor that one node's backward hands to another's in the same pass.
+    A pass that ends before the second node leaves its tensor behind; a later
+    pass over a retained graph, which may reach the second node alone, does not
+    take it."""
+
+    def __init__(self):
+        self._value: Optional[torch.Tensor] = None
+        self._task = -1
+
+    def _put(self, value: Optional[torch.Tensor]) -> None:
+        self._value, self._task = value, torch._C._current_graph_task_id()
+
+    def take(self) -> Optional[torch.Tensor]:
+        """What this backward pass has put there, once."""
+        value, self._value = self._value, None
+        return value if self._task == torch._C._current_graph_task_id() else None
+
+
+class ResidualLink(_Link):
     """Hands a half-block's output gradient (the residual's gradient) from the
     scatter's backward to the gather's backward, which adds it into dx in the
     same kernel instead of autograd summing the two paths in a separate pass.
     The scatter then takes its residual detached; the gather's backward runs
     after the scatter's, since the gather's output feeds the scatter."""
 
-    def __init__(self):
-        self.grad: Optional[torch.Tensor] = None
+    grad = property(lambda self: self._value, _Link._put)
 
 
-class ColumnSumLink:
+class ColumnSumLink(_Link):
     """Hands the column sums of a Linear's output gradient (its bias gradient)
     from the backward that produces that gradient, which sums it in the same
     kernel, to the Linear's backward, which then skips its own reduction."""
 
-    def __init__(self):
-        self.sums: Optional[torch.Tensor] = None
+    sums = property(lambda self: self._value, _Link._put)
 
 
 class _Reverse(torch.autograd.Function):
@@ -126,9 +143,9 @@ class _PartitionLN(torch.autograd.Function):
             dw = torch.zeros(weight.shape, dtype=torch.float32, device=x.device)
         if bias is not None and ctx.needs_input_grad[2]:
             db = torch.zeros(bias.shape, dtype=torch.float32, device=x.device)
-        dres = None
-        if ctx.link is not None and ctx.link.grad is not None:  # the residual's gradient, added in the kernel
-            dres, ctx.link.grad = ctx.link.grad.to(x.dtype).contiguous(), None
+        dres = None if ctx.link is None else ctx.link.take()  # the residual's gradient, added in the kernel
+        if dres is not None:
+            dres = dres.to(x.dtype).contiguous()
         dx = kernels.swin_partition_ln_backward(grad.contiguous(), x, ctx.geom, weight, ctx.eps, dresidual=dres,
                                                 dweight=dw, dbias=db)
         return (dx, None if dw is None else dw.to(weight.dtype), None if db is None else db.to(bias.dtype), None, None,
@@ -282,9 +299,7 @@ class _Linear(torch.autograd.Function):
             dx = _input_grad(dy2, wc).view(xc.shape).to(xd)
         if ctx.needs_input_grad[1]:
             dw = weight_grad(dy2, xc.reshape(-1, xc.shape[-1])).to(wd)
-        sums = None
-        if ctx.bias_sums is not None:
-            sums, ctx.bias_sums.sums = ctx.bias_sums.sums, None
+        sums = None if ctx.bias_sums is None else ctx.bias_sums.take()
         if bd is not None and ctx.needs_input_grad[2]:
             db = (sums if sums is not None and dy.dtype == dt else dy2.sum(0, dtype=torch.float32)).to(bd)
         return dx, dw, db, None
