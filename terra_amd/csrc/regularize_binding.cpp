@@ -100,12 +100,14 @@ const void* seed_ptr(const std::optional<Tensor>& seed, const Tensor& x, double 
   return seed->const_data_ptr();
 }
 
-// `out`, checked, or a new packed tensor like `like`.
+// `out`, checked and counted as written (a graph that saved its values refuses
+// them then), or a new packed tensor like `like`.
 Tensor output(const std::optional<Tensor>& out, const Tensor& like) {
   if (!out.has_value()) return packed_like(like);
   TORCH_CHECK_VALUE(out->sizes() == like.sizes() && out->scalar_type() == like.scalar_type() && out->is_contiguous() &&
                         out->device() == like.device(),
                     "out must be a contiguous ", like.scalar_type(), " tensor of shape ", like.sizes(), " on ", like.device());
+  if (!out->is_inference()) torch::autograd::impl::bump_version(*out);  // an inference tensor is in no graph
   return *out;
 }
 

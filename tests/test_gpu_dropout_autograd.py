@@ -60,3 +60,29 @@ def test_tangents_of_no_rows(dev):
         dual = forward_ad.make_dual(x, x.clone())
         for f in (autograd.dropout, autograd.gelu_dropout):
             assert forward_ad.unpack_dual(f(dual, 0.3, _seed(dev))).tangent.shape == (0, 8)
+
+
+def test_out_of_a_saved_tensor(dev):
+    """A tensor that a graph has saved and a call then writes into is refused by the backward, as after torch's own
+    in-place operations."""
+    calls = {
+        "dropout": lambda t: kernels.dropout(t, 0.3, _seed(dev), out=t),
+        "gelu_dropout": lambda t: kernels.gelu_dropout(t, 0.3, _seed(dev), out=t),
+        "gelu_dropout_backward": lambda t: kernels.gelu_dropout_backward(t, t.clone(), 0.3, _seed(dev), out=t),
+    }
+    for name, call in calls.items():
+        for shape in ((16, 64), (0, 64)):
+            x = _rand(shape, torch.float32, 5, dev).requires_grad_()
+            v = torch.exp(x)  # saves its result
+            before = v._version
+            call(v.detach())
+            assert v._version == before + 1, name
+            with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+                v.sum().backward()
+        with pytest.raises(ValueError, match="out must be"):  # a refused call leaves the count
+            kernels.dropout(v.detach(), 0.3, _seed(dev), out=v.detach().half())
+        assert v._version == before + 1
+    with torch.inference_mode():
+        t = torch.ones(8, 8, device=dev)
+        assert kernels.dropout(t, 0.3, _seed(dev), out=t) is t
+    assert kernels.dropout(t, 0.3, _seed(dev), out=t) is t
