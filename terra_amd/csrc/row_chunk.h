@@ -229,6 +229,8 @@ constexpr int kSumThreads = 1024;
 constexpr int kSumCols = 16;
 constexpr int kSumParts = kSumThreads / kSumCols;
 
+constexpr int kSumGrid = 1 << 21;  // workgroups a dimension: a grid holds fewer than 2^32 threads in each
+
 // One workgroup for 16 columns of one row of one job: 64 adders take every
 // 64th partial each, in fp64.  (static: each source file that sums has its own
 // copy.)  Few columns a workgroup, so that a vector of some hundred columns
@@ -237,28 +239,30 @@ static __global__ __launch_bounds__(kSumThreads) void sum_partials_kernel(const 
   const SumJob j = jobs.job[blockIdx.y];
   __shared__ double s[kSumParts][kSumCols];
   const int lane = threadIdx.x % kSumCols, part = threadIdx.x / kSumCols;
-  const int c = blockIdx.x * kSumCols + lane;
-  for (int b = blockIdx.z; b < j.batch; b += gridDim.z) {
-    double sum = 0.0;
-    const float* src = j.src + (int64_t)b * j.count * j.src_stride + (c < jobs.C ? c : 0);
-    constexpr int kAhead = 8;
-    for (int i = part; i < j.count; i += kAhead * kSumParts) {
-      float v[kAhead];
+  for (int first = blockIdx.x * kSumCols; first < jobs.C; first += gridDim.x * kSumCols) {
+    const int c = first + lane;
+    for (int b = blockIdx.z; b < j.batch; b += gridDim.z) {
+      double sum = 0.0;
+      const float* src = j.src + (int64_t)b * j.count * j.src_stride + (c < jobs.C ? c : 0);
+      constexpr int kAhead = 8;
+      for (int i = part; i < j.count; i += kAhead * kSumParts) {
+        float v[kAhead];
 #pragma unroll
-      for (int u = 0; u < kAhead; ++u) {
-        const int at = i + u * kSumParts;
-        v[u] = src[(int64_t)(at < j.count ? at : i) * j.src_stride];
+        for (int u = 0; u < kAhead; ++u) {
+          const int at = i + u * kSumParts;
+          v[u] = src[(int64_t)(at < j.count ? at : i) * j.src_stride];
+        }
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u) sum += i + u * kSumParts < j.count ? (double)v[u] : 0.0;
       }
-#pragma unroll
-      for (int u = 0; u < kAhead; ++u) sum += i + u * kSumParts < j.count ? (double)v[u] : 0.0;
-    }
-    s[part][lane] = sum;
-    __syncthreads();
-    for (int half = kSumParts / 2; half > 0; half /= 2) {
-      if (part < half) s[part][lane] = sum += s[part + half][lane];
+      s[part][lane] = sum;
       __syncthreads();
+      for (int half = kSumParts / 2; half > 0; half /= 2) {
+        if (part < half) s[part][lane] = sum += s[part + half][lane];
+        __syncthreads();
+      }
+      if (part == 0 && c < jobs.C) j.dst[(int64_t)b * jobs.C + c] = (float)sum;
     }
-    if (part == 0 && c < jobs.C) j.dst[(int64_t)b * jobs.C + c] = (float)sum;
   }
 }
 
@@ -266,7 +270,8 @@ static __global__ __launch_bounds__(kSumThreads) void sum_partials_kernel(const 
 inline void launch_sums(const SumJobs& jobs, int n, hipStream_t s) {
   int batch = 1;
   for (int i = 0; i < n; ++i) batch = jobs.job[i].batch > batch ? jobs.job[i].batch : batch;
-  const dim3 grid((unsigned)((jobs.C + kSumCols - 1) / kSumCols), (unsigned)n, (unsigned)(batch < 1024 ? batch : 1024));
+  const int groups = (jobs.C + kSumCols - 1) / kSumCols;  // of columns
+  const dim3 grid((unsigned)(groups < kSumGrid ? groups : kSumGrid), (unsigned)n, (unsigned)(batch < 1024 ? batch : 1024));
   sum_partials_kernel<<<grid, kSumThreads, 0, s>>>(jobs);
 }
 

@@ -262,3 +262,30 @@ def test_drawn_seeds_in_a_graph_differ_from_replay_to_replay(dev):
         torch.cuda.synchronize()
         got.append(y.clone())
     assert not torch.equal(got[0], got[1]) and not torch.equal(got[1], got[2])
+
+
+def test_columns_to_the_limit(dev):
+    """A row of more columns than one grid of the column sums' launch has workgroups for (2^25 at a time, 2^26 and a few
+    here), sums of no rows, and a row of the most columns there may be."""
+    n = (1 << 26) + 5
+    da, h = torch.randn(1, n, device=dev, generator=torch.Generator(dev).manual_seed(1)), torch.ones(1, n, device=dev)
+    dh, sums = kernels.gelu_dropout_backward(da, h, 0.0, None, column_sums=True)
+    assert torch.equal(dh[0], sums)  # one row: its own sum
+    slope = 0.5 * (1 + torch.erf(torch.tensor(0.5, dtype=torch.float64).sqrt())) + torch.exp(
+        torch.tensor(-0.5, dtype=torch.float64)) / (2 * torch.pi) ** 0.5
+    assert bool(((sums.double() - da[0].double() * slope).abs() <= 16 * E32 * 2 * da[0].double().abs()).all())
+    del da, h, dh, sums
+    empty = torch.empty(0, n, device=dev)
+    sums = kernels.gelu_dropout_backward(empty, empty, 0.0, None, column_sums=True)[1]
+    assert not bool(sums.any())
+    del sums, empty
+    n = (1 << 27) - 1
+    y = kernels.dropout(torch.ones(1, n, dtype=torch.bfloat16, device=dev), 0.5, _seed(dev), 1)
+    first = (n // 8) - 100  # the last chunks' draws
+    words = rg.philox4x32_10((torch.arange(first, n // 8 + 1).numpy().astype("uint64"), 0, 0, 1),
+                             (SEED & 0xFFFFFFFF, SEED >> 32))
+    draws = torch.stack([torch.from_numpy((w >> (16 * k) & 0xFFFF).astype("int64")) for w in map(lambda w: w.astype("int64"), words)
+                         for k in (0, 1)], -1).view(-1)
+    assert torch.equal(y[0, 8 * first:].cpu() != 0, (draws >= rg.threshold(0.5))[:n - 8 * first])
+    del y
+    torch.cuda.empty_cache()
