@@ -672,7 +672,8 @@ def attention_half(x: torch.Tensor, geom: WindowGeometry, norm: torch.nn.LayerNo
 
 class _Dropout(torch.autograd.Function):
     """kernels.dropout; the backward draws the mask again from the seed.  A
-    tangent is dropped as the values are."""
+    linear map: its gradient and a tangent are dropped as the values are, and
+    the gradient may be differentiated again."""
 
     @staticmethod
     def forward(ctx, x, p, seed, stream):
@@ -686,9 +687,8 @@ class _Dropout(torch.autograd.Function):
         return kernels.dropout(dx.contiguous(), ctx.p, ctx.saved_tensors[0], ctx.stream)
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, dy):
-        return kernels.dropout(dy.contiguous(), ctx.p, ctx.saved_tensors[0], ctx.stream), None, None, None
+        return dropout(dy.contiguous(), ctx.p, ctx.saved_tensors[0], ctx.stream), None, None, None
 
 
 def _seed(x: torch.Tensor, p: float, seed: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
@@ -696,8 +696,8 @@ def _seed(x: torch.Tensor, p: float, seed: Optional[torch.Tensor]) -> Optional[t
 
 
 def dropout(x: torch.Tensor, p: float, seed: Optional[torch.Tensor] = None, stream: int = 0) -> torch.Tensor:
-    """:func:`kernels.dropout` with a gradient and a forward-mode derivative.
-    ``seed`` None draws one from torch's generator on x's device."""
+    """:func:`kernels.dropout` with derivatives of every order, backward and
+    forward mode.  ``seed`` None draws one from torch's generator on x's device."""
     seed = _seed(x, p, seed)
     if _needs_grad(x) or _has_tangent(x):
         return _Dropout.apply(x, p, seed, stream)
@@ -733,8 +733,8 @@ class _GeluDropout(torch.autograd.Function):
 
 def gelu_dropout(h: torch.Tensor, p: float, seed: Optional[torch.Tensor] = None, stream: int = 0,
                  bias_sums: Optional[ColumnSumLink] = None) -> torch.Tensor:
-    """:func:`kernels.gelu_dropout` with a gradient and a forward-mode
-    derivative.  ``seed`` None draws one from torch's generator.  ``bias_sums``: the :class:`ColumnSumLink` of the
+    """:func:`kernels.gelu_dropout` with a gradient (which has none itself) and
+    a forward-mode derivative.  ``seed`` None draws one from torch's generator.  ``bias_sums``: the :class:`ColumnSumLink` of the
     :func:`linear` that produced ``h``, whose bias gradient the backward sums."""
     seed, h = _seed(h, p, seed), h.contiguous()
     if _needs_grad(h) or _has_tangent(h):

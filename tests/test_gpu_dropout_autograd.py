@@ -1,5 +1,5 @@
 """Derivatives of autograd.dropout and autograd.gelu_dropout beside the first
-backward: forward mode.
+backward: forward mode, and second derivatives.
 
 Both maps act element by element, so a tangent is multiplied by what a gradient
 is: equal bit for bit to the backward kernel's result on it.
@@ -60,6 +60,23 @@ def test_tangents_of_no_rows(dev):
         dual = forward_ad.make_dual(x, x.clone())
         for f in (autograd.dropout, autograd.gelu_dropout):
             assert forward_ad.unpack_dual(f(dual, 0.3, _seed(dev))).tangent.shape == (0, 8)
+
+
+@pytest.mark.parametrize("dt", TYPES)
+def test_dropout_twice_differentiated(dev, dt):
+    """Of sum(w y^2) with y = d x (d the mask times the scale): the gradient is 2 w d^2 x, its derivative along v
+    2 w d^2 v.  Products of values rounded to the type one after the other: six roundings of half an eps."""
+    x, v, w = (_rand((37, 100), dt, i, dev) for i in (6, 7, 8))
+    x.requires_grad_()
+    d = kernels.dropout(torch.ones(37, 100, device=dev), 0.3, _seed(dev), 4).double()
+    y = autograd.dropout(x, 0.3, _seed(dev), 4)
+    g, = torch.autograd.grad((w * y * y).sum(), x, create_graph=True)
+    want = 2 * w.double() * d * d
+    tol = 3 * torch.finfo(dt).eps + 4 * torch.finfo(torch.float32).eps
+    near = lambda a, b: bool(((a.detach().double() - b).abs() <= tol * b.abs() + 1e-6).all())  # noqa: E731
+    assert near(g, want * x.detach().double())
+    h, = torch.autograd.grad((g * v).sum(), x)
+    assert near(h, want * v.double())
 
 
 def test_out_of_a_saved_tensor(dev):
