@@ -22,7 +22,6 @@ from typing import Optional, Tuple, Union
 
 import torch
 from torch.autograd import forward_ad
-from torch.autograd.function import once_differentiable
 
 from . import _lib, kernels
 from .kernels import Norm, ShiftMask, WindowGeometry, WindowMask
@@ -704,6 +703,21 @@ def dropout(x: torch.Tensor, p: float, seed: Optional[torch.Tensor] = None, stre
     return kernels.dropout(x, p, seed, stream)
 
 
+class _OnceDifferentiable(torch.autograd.Function):
+    """A gradient g that has no derivative itself, tied to the tensors that it
+    depends on: a pass that goes through it to one of them raises, where a
+    gradient without a graph would be left out of the sum."""
+
+    @staticmethod
+    def forward(ctx, name, g, *sources):
+        ctx.name = name
+        return g.detach()
+
+    @staticmethod
+    def backward(ctx, _):
+        raise RuntimeError(f"{ctx.name} cannot be differentiated twice: its gradient has no gradient")
+
+
 class _GeluDropout(torch.autograd.Function):
     """kernels.gelu_dropout.  It acts element by element, so a tangent is
     multiplied by what a gradient is."""
@@ -721,13 +735,14 @@ class _GeluDropout(torch.autograd.Function):
         return kernels.gelu_dropout_backward(dh.contiguous(), h, ctx.p, seed, ctx.stream)
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, da):
         h, seed = ctx.saved_tensors
         dh = kernels.gelu_dropout_backward(da.contiguous(), h, ctx.p, seed, ctx.stream,
                                            column_sums=ctx.bias_sums is not None)
         if ctx.bias_sums is not None:
             dh, ctx.bias_sums.sums = dh
+        if torch.is_grad_enabled():  # asked for with create_graph
+            dh = _OnceDifferentiable.apply("gelu_dropout", dh, da, h)
         return dh, None, None, None, None
 
 

@@ -195,21 +195,22 @@ struct ResidualNormBackward : public torch::autograd::Node {
 
   variable_list apply(variable_list&& grads) override {
     std::lock_guard<std::mutex> lock(mutex_);
+    const Tensor dy = grads[0], dz = grads.size() > 1 ? grads[1] : Tensor();
     variable_list out;
     {
       at::AutoGradMode off(false);
-      out = gradients(grads[0], grads.size() > 1 ? grads[1] : Tensor());
+      out = gradients(dy, dz);
     }
     if (!at::GradMode::is_enabled()) return out;
-    // Asked for with create_graph: gradients that refuse to be differentiated.
-    variable_list marked;
+    // Asked for with create_graph: gradients that refuse to be differentiated, tied
+    // to all they depend on, since a pass to one of those would leave them out otherwise.
+    torch::autograd::edge_list sources = next_edges();
+    for (const Tensor& t : {dy, dz})
+      if (t.defined()) sources.push_back(torch::autograd::impl::gradient_edge(t));
+    const std::shared_ptr<torch::autograd::Node> refuse(new torch::autograd::Error(kOnce, std::move(sources)),
+                                                        torch::autograd::deleteNode);
     for (auto& t : out)
-      if (t.defined()) marked.push_back(t.detach().set_requires_grad(true));
-    const auto refuse = std::make_shared<torch::autograd::DelayedError>(kOnce, (int64_t)marked.size());
-    marked = (*refuse)(std::move(marked));
-    size_t i = 0;
-    for (auto& t : out)
-      if (t.defined()) t = marked[i++];
+      if (t.defined()) torch::autograd::set_history(t, refuse);
     return out;
   }
 
