@@ -46,9 +46,11 @@ struct DropParams {
 // Phi(-a) = e G(a), where G(a) = erfcx(a / sqrt 2) / 2 falls smoothly from 1/2 like
 // 1 / a: a polynomial of degree 8 in u = 1 / (1 + 0.3 a) without a constant term,
 // fitted to the least largest relative error over 0 <= a <= 14 (1.5e-7; in fp32
-// 4.4e-7 relative for h < 0, 1.7e-7 absolute), so the tail keeps its relative
-// precision.  About 20 instructions, of which exp2 and the reciprocal go to the
-// transcendental unit; erfcf and expf took three times as many.
+// 2.5e-7 absolute for h > 0).  So the tail does not vanish as 1 + erf does, but its
+// relative error grows with the exponent, whose fp32 product is rounded twice: 5.5e-7
+// down to h = -2, 1.6e-6 at -5, 3.8e-6 at -9, 7.7e-6 at -12.9, beyond which it is below
+// the smallest normal number.  About 20 instructions, of which exp2 and the
+// reciprocal go to the transcendental unit; erfcf and expf took three times as many.
 __device__ __forceinline__ void normal_parts(float h, float& cdf, float& e) {
   const float a = fabsf(h);
   const float u = __builtin_amdgcn_rcpf(fmaf(0.3f, a, 1.f));

@@ -289,3 +289,58 @@ def test_columns_to_the_limit(dev):
     assert torch.equal(y[0, 8 * first:].cpu() != 0, (draws >= rg.threshold(0.5))[:n - 8 * first])
     del y
     torch.cuda.empty_cache()
+
+
+def _every_value(rows):
+    """[rows, 256] bf16 rows that go through all 2^16 values again and again: 0, values below 2^-12 and from 16 on,
+    infinities and NaN among them."""
+    at = torch.arange(256 * rows, dtype=torch.int32) * 40503  # odd: neighbouring lanes see values far apart
+    return (at & 0xFFFF).to(torch.int16).view(torch.bfloat16).view(rows, 256)
+
+
+@pytest.mark.parametrize("rows,p", [(1 << 14, 0.0), (1 << 14, 0.3), ((1 << 14) + 19, 0.3)])
+def test_gelu_dropout_of_many_bf16_values(dev, rows, p):
+    """From 2^22 aligned bf16 elements on the factors come from a table: against the oracle, and against the calls of
+    fewer rows, which compute them (two roundings to the type from values 32 eps_32 apart: one step of the type)."""
+    h = _every_value(rows)
+    seed = _seed(dev) if p else None
+    a = kernels.gelu_dropout(h.to(dev), p, seed, 2).cpu()
+    hd, s = h.double(), rg.keep_scale(p)
+    ref = rg.dropout(rg.gelu(hd), p, SEED, 2)
+    fine = torch.isfinite(hd)
+    tol = _half(torch.bfloat16) * ref.abs() + 16 * E32 * hd.abs() * s + _tiny(torch.bfloat16)
+    top = torch.finfo(torch.bfloat16).max
+    near = ((a.double() - ref).abs() <= tol) | ((ref.abs() > top * (1 - _half(torch.bfloat16))) & torch.isinf(a))
+    assert bool(near[fine].all())
+    keep = rg.keep_mask(SEED, rows, 256, p, 2)
+    assert bool((a[~keep] == 0).all())
+    assert bool(torch.isnan(a[keep & torch.isnan(hd)]).all())
+    assert bool((a[keep & (hd == float("inf"))] == float("inf")).all())
+    assert bool(torch.isnan(a[keep & (hd == -float("inf"))]).all())
+    few = kernels.gelu_dropout(h[:4099].to(dev), p, seed, 2).cpu()
+    big = a[:4099]
+    assert torch.equal(torch.isnan(few), torch.isnan(big)) and torch.equal(torch.isinf(few), torch.isinf(big))
+    both = torch.isfinite(few)
+    step = torch.finfo(torch.bfloat16).eps * torch.maximum(few.abs(), big.abs()).float() + 2 * _tiny(torch.bfloat16)
+    wide = 32 * E32 * hd[:4099].abs().nan_to_num() * s  # a dropped NaN is 0 in both
+    assert bool(((few.float() - big.float()).abs() <= step + wide)[both].all())
+    dst = h.to(dev)
+    assert torch.equal(kernels.gelu_dropout(dst, p, seed, 2, out=dst).view(torch.int16).cpu(), a.view(torch.int16))
+
+
+def test_gelu_tail_in_fp32(dev):
+    """The negative tail keeps its relative precision but for the exponent's: exp(-h^2 / 2) is taken from a product
+    rounded twice (half an eps of h^2 / 2 each) with a constant rounded once (another half), 0.75 eps h^2 in all; the
+    polynomial, its seven steps, the reciprocal and exp2 (one ulp each) and the last products add 8 eps.  The
+    slope at h <= -2 takes both terms' errors, at most (1 + h^2) / (h^2 - 1) <= 5 / 3 of it."""
+    h = torch.linspace(-12.5, -0.001, 200_003)
+    a = kernels.gelu_dropout(h.to(dev).view(1, -1), 0.0, None)[0].double().cpu()
+    hd = h.double()
+    ref = rg.gelu(hd)
+    tol = E32 * (8 + 0.75 * hd * hd)
+    assert bool(((a - ref).abs() <= tol * ref.abs()).all())
+    far = h <= -2
+    h, hd, tol = h[far], hd[far], tol[far] * 5 / 3
+    dh = kernels.gelu_dropout_backward(torch.ones(1, len(h), device=dev), h.to(dev).view(1, -1), 0.0, None)[0].double().cpu()
+    slope = 0.5 * torch.erfc(-hd / 2 ** 0.5) + hd * torch.exp(-0.5 * hd * hd) / (2 * torch.pi) ** 0.5
+    assert bool(((dh - slope).abs() <= tol * slope.abs()).all())
