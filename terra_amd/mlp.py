@@ -72,6 +72,14 @@ class SequentialMlp(torch.nn.Module):
         _disable_parameters_if_mlp_off(self)
         self.use_fused_mlp = True
 
+    def __setstate__(self, state):
+        """A module pickled when these options were not there yet has them off."""
+        super().__setstate__(state)
+        for name, off in (("post_norm2", None), ("layer_scale2", None), ("residual_scale", 1.0), ("hidden_dropout", 0.0),
+                          ("dropout", 0.0)):
+            if not hasattr(self, name):
+                setattr(self, name, off)
+
     def _fusable(self, x: torch.Tensor) -> bool:
         """One kernel serves the call: bf16 rows of C in {128, 192, 384, 768}, hidden
         4C, out C, the exact GELU, a plain LayerNorm over C (or none), biased

@@ -103,6 +103,13 @@ class SequentialSwinTransformer(torch.nn.Module):
         # False forces the five-stage path.
         self.use_fused_block = True
 
+    def __setstate__(self, state):
+        """A module pickled when these options were not there yet has them off."""
+        super().__setstate__(state)
+        for name, off in (("post_norm1", None), ("layer_scale1", None), ("residual_scale", 1.0), ("dropout", 0.0)):
+            if not hasattr(self, name):
+                setattr(self, name, off)
+
     def geometry(self, batch: int) -> WindowGeometry:
         H, W = self.input_resolution
         return WindowGeometry(batch, H, W, self.embedding_dim, self.window_size, self.shift_size,
