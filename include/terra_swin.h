@@ -588,10 +588,10 @@ int terra_swin_gelu_bwd(const void* dout, const void* h, void* dh, int dtype, in
  * value is 0) where its draw is below t = round(p * 65536), and the others are
  * scaled by 65536 / (65536 - t).  So the mask depends on the seed, the stream and
  * the element's row and column alone, a backward call with the same ones sees the
- * same mask, and p is rounded to 2^-16.  `seed`: a 64-bit integer in device memory
- * (8-byte aligned; may be NULL where t is 0), read when the kernel runs, so that a
- * replayed graph takes the seed that is there then.  Calls that must not share a
- * mask take other seeds or other stream ids.  0 <= p <= 1; rows < 2^31.
+ * same mask, and p is rounded to a multiple of 2^-16.  `seed`: a 64-bit integer
+ * in device memory (8-byte aligned; may be NULL where t is 0), read when the kernel
+ * runs, so that a replayed graph takes the seed that is there then.  Calls that
+ * must not share a mask take other seeds or other stream ids.  0 <= p <= 1; rows < 2^31.
  */
 
 /* y = dropout(x) for x [rows, columns] with row stride x_stride (elements), y

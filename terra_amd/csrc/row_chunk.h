@@ -88,10 +88,10 @@ __device__ __forceinline__ void store_half(const float* f, uint8_t* row, int col
 // 128-bit counter under a 64-bit key.  Counter = (column >> 3, row, 0, stream),
 // key = the seed; the four result words are the draws of the chunk's eight
 // columns, 16 bits each, low half first.  A draw below `threshold` =
-// round(p 65536) drops its element, so p is kept to 2^-17, and the scale of
-// the kept ones, 65536 / (65536 - threshold), makes the expectation exact.
-// 16 bits a draw rather than 32 halve the generator's work, which is as long
-// as the memory traffic of a 16-bit element otherwise.
+// round(p 65536) drops its element, so p is rounded to a multiple of 2^-16, and
+// the scale of the kept ones, 65536 / (65536 - threshold), makes the expectation
+// exact.  16 bits a draw rather than 32 halve the generator's work, which is as
+// long as the memory traffic of a 16-bit element otherwise.
 struct DropoutArgs {
   const uint64_t* seed;
   uint32_t threshold;  // 0: nothing is dropped (seed not read); 65536: everything
