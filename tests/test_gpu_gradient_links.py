@@ -83,3 +83,19 @@ def test_links_in_a_checkpointed_half(dev, reentrant):
             f(v).square().sum().backward()
             grads.append(v.grad)
         assert torch.equal(*grads)
+
+
+def test_links_with_the_engine_in_the_callers_thread(dev):
+    torch.manual_seed(3)
+    opts = dict(layer_scale=0.3, residual_scale=0.9, dropout=0.2)
+    for half in (SequentialSwinTransformer(1, 16, 16, 96, window_size=8, num_heads=3, **opts),
+                 SequentialMlp(96, 384, hidden_dropout=0.2, **opts)):
+        half.to(dev).train()
+        grads = []
+        for threads in (True, False):
+            torch.manual_seed(8)
+            x = _rand((1, 256, 96), 7, dev).requires_grad_()
+            y = half(x)
+            with torch.autograd.set_multithreading_enabled(threads):
+                grads.append(torch.autograd.grad(y.square().sum(), x)[0])
+        assert torch.equal(*grads)
