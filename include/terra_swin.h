@@ -676,6 +676,130 @@ int terra_swin_residual_norm_bwd(const void* h, const void* x, const void* dy, c
                                  float* dpost_weight, float* dpost_bias, float* dgate,
                                  float* dnext_weight, float* dnext_bias, float* workspace, void* stream);
 
+/* ---- what a training step does beside its products and attention cores --------
+ *
+ * Norms over rows, rotary positions, and the update of the parameters.
+ */
+
+/* Description of a norm over `rows` rows of `channels`: row r of x begins
+ * (r / inner) * outer_stride + (r % inner) * inner_stride elements into x (packed
+ * rows: inner = rows or 1; the heads of a packed q | k | v: inner = heads,
+ * inner_stride = head dim, outer_stride = the token stride).  x, y and the
+ * parameters are f32, bf16 or f16, y of x's dtype unless one of the two is f32.
+ * norm: TERRA_NORM_LAYER or TERRA_NORM_RMS.  rows < 2^31, channels <= 2^24. */
+typedef struct terra_swin_layer_norm_desc {
+  int64_t rows, inner;
+  int64_t outer_stride, inner_stride;
+  int32_t channels;
+  int32_t x_dtype, y_dtype, param_dtype;
+  int32_t norm;
+  float eps;
+} terra_swin_layer_norm_desc;
+
+/* y = norm(x) * weight + bias, in fp32 and rounded once; y packed.  weight and bias [channels] of
+ * param_dtype, or NULL (1, 0).  statistics (fp32 [rows][2], 8-byte aligned: the mean, 0 for
+ * an RMS norm, and the reciprocal root of each row) is written where it is not
+ * NULL; the backward reads it.  Outputs overlap nothing.
+ * Stands where the reference calls nn.LayerNorm
+ *           models/transformer.py:98, 150, models/mlp.py:159 */
+int terra_swin_layer_norm(const void* x, void* y, const terra_swin_layer_norm_desc* desc,
+                          const void* weight, const void* bias, float* statistics, void* stream);
+
+/* Its backward, from the packed gradient of y (y_dtype): dx (packed, x_dtype; NULL: not
+ * taken), and the sums over rows
+ * dweight and dbias (param_dtype, written, not added, in an order that the sizes
+ * and alignments fix), each of which may be NULL.  The sums need a workspace of
+ * terra_swin_layer_norm_workspace fp32 values (a negative result is a status). */
+int terra_swin_layer_norm_workspace(const terra_swin_layer_norm_desc* desc);
+int terra_swin_layer_norm_bwd(const void* dy, const void* x, const float* statistics, void* dx,
+                              const terra_swin_layer_norm_desc* desc, const void* weight,
+                              void* dweight, void* dbias, float* workspace, void* stream);
+
+/* Description of a rotary call over tokens x heads x head_dim: element d of head
+ * h of token t is (t / inner) * outer_stride + (t % inner) * inner_stride + h *
+ * head_stride + d elements into x, and likewise into y.  The first `dim` elements of a head (even)
+ * are rotated, in pairs (2i, 2i + 1) where interleaved, else (i, i + dim / 2); the others
+ * are copied.  Pair i of token t turns by the angle
+ *   position[(t % position_tokens) * axes + i / (dim / 2 / axes)] * turns[i % (dim / 2 / axes)]
+ * of whole turns (the product in 64 bits, brought to one turn there), and its values are
+ * scaled by amplitude; inverse != 0: by the negative angle, which is the backward. */
+typedef struct terra_swin_rotary_desc {
+  int64_t tokens, inner;
+  int64_t position_tokens;
+  int64_t x_outer_stride, x_inner_stride, x_head_stride;
+  int64_t y_outer_stride, y_inner_stride, y_head_stride;
+  int32_t heads, head_dim, dim;
+  int32_t axes;
+  int32_t dtype;           /* f32, bf16 or f16                     */
+  int32_t position_bits;   /* 32 or 64: signed integers            */
+  int32_t interleaved, inverse;
+  float amplitude;
+} terra_swin_rotary_desc;
+
+/* turns: fp64 [dim / 2 / axes].  y may be x itself, with x's strides; it must not
+ * overlap it otherwise. */
+int terra_swin_rotary(const void* x, void* y, const void* positions, const double* turns,
+                      const terra_swin_rotary_desc* desc, void* stream);
+
+/* A tensor of many: `numel` elements (f32, bf16 or f16) that lie side by side. */
+typedef struct terra_swin_tensor {
+  const void* data;
+  int64_t numel;
+  int32_t dtype;
+} terra_swin_tensor;
+
+/* The 2-norm of many gradients as one vector:
+ *   result[0] = norm,  result[1] = min(1, max_norm / (norm + 1e-6)),
+ *   result[2] = 1 where the norm is infinite or NaN, else 0
+ * (fp32; max_norm <= 0: no clipping, result[1] = 1).  Sums are taken in 64 bits, in an order
+ * that the sizes fix.  workspace: terra_swin_gradient_norm_workspace fp64 values (a
+ * negative result is a status). */
+int terra_swin_gradient_norm_workspace(const terra_swin_tensor* grads, int count);
+int terra_swin_gradient_norm(const terra_swin_tensor* grads, int count, double max_norm, float* result,
+                             double* workspace, void* stream);
+
+/* A parameter with its gradient and moments.  scales: NULL for moments in 32
+ * bits (exp_avg and exp_avg_sq fp32); else the moments are e4m3 codes (one byte an element) with
+ * fp32 scales [2][ceil(numel / 256)], one for each 256 elements of exp_avg and then of the
+ * root of exp_avg_sq.  index: the tensor's number in the random numbers' counter. */
+typedef struct terra_swin_adamw_tensor {
+  void* param;
+  const void* grad;
+  void* exp_avg;
+  void* exp_avg_sq;
+  float* scales;
+  int64_t numel;
+  uint32_t index;
+  int32_t param_dtype, grad_dtype;
+} terra_swin_adamw_tensor;
+
+/* A step, for tensors of any mixture of types and moments; the parameters and
+ * gradients are f32, bf16 or f16, of one dtype unless one of the two is f32:
+ *   g = grad * grad_factor (negated where maximize)
+ *   m = beta1 m + (1 - beta1) g,  v = beta2 v + (1 - beta2) g^2
+ *   param = param (1 - lr weight_decay) - lr / (1 - beta1^step) m / (sqrt(v / (1 - beta2^step)) + eps)
+ * step, lr: from device memory where their pointers are not NULL (int64, fp32), so that a replayed graph
+ * takes what is there then.  grad_factor (fp32, NULL: 1).  found_inf (fp32, NULL: 0): where it is not 0
+ * nothing is written.  Moments in 8 bits: m is rounded to the nearest code; of
+ * the two codes a <= sqrt(v) / scale < b the upper one is taken where
+ *   v / scale^2 - a^2 > u (b^2 - a^2),   u = (draw + 1/2) / 65536,
+ * so that the mean of the squares is v; draws as those of dropout with the counter (element >> 3,
+ * index, step, stream_id) and the key seed (8 bytes in device memory); v > 0 has no code of 0.
+ * Stands where the reference's optimizer/ steps AdamW. */
+typedef struct terra_swin_adamw_desc {
+  double lr, beta1, beta2, eps, weight_decay;
+  int64_t step;
+  const void* step_ptr;
+  const float* lr_ptr;
+  const float* grad_factor;
+  const float* found_inf;
+  const void* seed;
+  uint32_t stream_id;
+  int32_t maximize;
+} terra_swin_adamw_desc;
+
+int terra_swin_adamw(const terra_swin_adamw_tensor* tensors, int count, const terra_swin_adamw_desc* desc, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -78,6 +78,13 @@ EXPORTED_SYMBOLS = (
     "terra_swin_residual_norm",
     "terra_swin_residual_norm_workspace",
     "terra_swin_residual_norm_bwd",
+    "terra_swin_layer_norm",
+    "terra_swin_layer_norm_workspace",
+    "terra_swin_layer_norm_bwd",
+    "terra_swin_rotary",
+    "terra_swin_gradient_norm_workspace",
+    "terra_swin_gradient_norm",
+    "terra_swin_adamw",
 )
 
 
@@ -201,6 +208,90 @@ class ResidualNormDesc(ctypes.Structure):
     ]
 
 
+class LayerNormDesc(ctypes.Structure):
+    """Mirror of ``terra_swin_layer_norm_desc``."""
+
+    _fields_ = [
+        ("rows", ctypes.c_int64),
+        ("inner", ctypes.c_int64),
+        ("outer_stride", ctypes.c_int64),
+        ("inner_stride", ctypes.c_int64),
+        ("channels", ctypes.c_int32),
+        ("x_dtype", ctypes.c_int32),
+        ("y_dtype", ctypes.c_int32),
+        ("param_dtype", ctypes.c_int32),
+        ("norm", ctypes.c_int32),
+        ("eps", ctypes.c_float),
+    ]
+
+
+class RotaryDesc(ctypes.Structure):
+    """Mirror of ``terra_swin_rotary_desc``."""
+
+    _fields_ = [
+        ("tokens", ctypes.c_int64),
+        ("inner", ctypes.c_int64),
+        ("position_tokens", ctypes.c_int64),
+        ("x_outer_stride", ctypes.c_int64),
+        ("x_inner_stride", ctypes.c_int64),
+        ("x_head_stride", ctypes.c_int64),
+        ("y_outer_stride", ctypes.c_int64),
+        ("y_inner_stride", ctypes.c_int64),
+        ("y_head_stride", ctypes.c_int64),
+        ("heads", ctypes.c_int32),
+        ("head_dim", ctypes.c_int32),
+        ("dim", ctypes.c_int32),
+        ("axes", ctypes.c_int32),
+        ("dtype", ctypes.c_int32),
+        ("position_bits", ctypes.c_int32),
+        ("interleaved", ctypes.c_int32),
+        ("inverse", ctypes.c_int32),
+        ("amplitude", ctypes.c_float),
+    ]
+
+
+class TensorList(ctypes.Structure):
+    """Mirror of ``terra_swin_tensor``."""
+
+    _fields_ = [("data", ctypes.c_void_p), ("numel", ctypes.c_int64), ("dtype", ctypes.c_int32)]
+
+
+class AdamWTensor(ctypes.Structure):
+    """Mirror of ``terra_swin_adamw_tensor``."""
+
+    _fields_ = [
+        ("param", ctypes.c_void_p),
+        ("grad", ctypes.c_void_p),
+        ("exp_avg", ctypes.c_void_p),
+        ("exp_avg_sq", ctypes.c_void_p),
+        ("scales", ctypes.c_void_p),
+        ("numel", ctypes.c_int64),
+        ("index", ctypes.c_uint32),
+        ("param_dtype", ctypes.c_int32),
+        ("grad_dtype", ctypes.c_int32),
+    ]
+
+
+class AdamWDesc(ctypes.Structure):
+    """Mirror of ``terra_swin_adamw_desc``."""
+
+    _fields_ = [
+        ("lr", ctypes.c_double),
+        ("beta1", ctypes.c_double),
+        ("beta2", ctypes.c_double),
+        ("eps", ctypes.c_double),
+        ("weight_decay", ctypes.c_double),
+        ("step", ctypes.c_int64),
+        ("step_ptr", ctypes.c_void_p),
+        ("lr_ptr", ctypes.c_void_p),
+        ("grad_factor", ctypes.c_void_p),
+        ("found_inf", ctypes.c_void_p),
+        ("seed", ctypes.c_void_p),
+        ("stream_id", ctypes.c_uint32),
+        ("maximize", ctypes.c_int32),
+    ]
+
+
 class TerraError(RuntimeError):
     """A C-ABI call returned a launch-time failure."""
 
@@ -214,6 +305,25 @@ def library_path() -> str:
 
 
 _binding = None
+_training = None
+
+
+def load_training():
+    """The host module of the training step's operators (csrc/training_binding.cpp), bound once to the library's entry points."""
+    global _training
+    if _training is None:
+        lib = load()
+        try:
+            from . import _training as module
+        except ImportError as e:
+            raise RuntimeError("terra_amd: _training.so is not built or does not fit this torch; run "
+                               "`python -m terra_amd.build` first (there is no fallback)") from e
+        module.bind(*(ctypes.cast(f, ctypes.c_void_p).value for f in (
+            lib.terra_swin_layer_norm, lib.terra_swin_layer_norm_bwd, lib.terra_swin_rotary,
+            lib.terra_swin_gradient_norm_workspace, lib.terra_swin_gradient_norm, lib.terra_swin_adamw,
+            lib.terra_last_error)))
+        _training = module
+    return _training
 
 
 def load_binding():
@@ -338,6 +448,20 @@ def load() -> ctypes.CDLL:
         lib.terra_swin_residual_norm_workspace.argtypes = [ctypes.POINTER(ResidualNormDesc)]
         lib.terra_swin_residual_norm_bwd.restype = ctypes.c_int
         lib.terra_swin_residual_norm_bwd.argtypes = [vp] * 6 + [ctypes.POINTER(ResidualNormDesc)] + [vp] * 12
+        lib.terra_swin_layer_norm.restype = ctypes.c_int
+        lib.terra_swin_layer_norm.argtypes = [vp, vp, ctypes.POINTER(LayerNormDesc), vp, vp, vp, vp]
+        lib.terra_swin_layer_norm_workspace.restype = ctypes.c_int
+        lib.terra_swin_layer_norm_workspace.argtypes = [ctypes.POINTER(LayerNormDesc)]
+        lib.terra_swin_layer_norm_bwd.restype = ctypes.c_int
+        lib.terra_swin_layer_norm_bwd.argtypes = [vp] * 4 + [ctypes.POINTER(LayerNormDesc)] + [vp] * 5
+        lib.terra_swin_rotary.restype = ctypes.c_int
+        lib.terra_swin_rotary.argtypes = [vp] * 4 + [ctypes.POINTER(RotaryDesc), vp]
+        lib.terra_swin_gradient_norm_workspace.restype = ctypes.c_int
+        lib.terra_swin_gradient_norm_workspace.argtypes = [ctypes.POINTER(TensorList), ctypes.c_int]
+        lib.terra_swin_gradient_norm.restype = ctypes.c_int
+        lib.terra_swin_gradient_norm.argtypes = [ctypes.POINTER(TensorList), ctypes.c_int, f64, vp, vp, vp]
+        lib.terra_swin_adamw.restype = ctypes.c_int
+        lib.terra_swin_adamw.argtypes = [ctypes.POINTER(AdamWTensor), ctypes.c_int, ctypes.POINTER(AdamWDesc), vp]
         version = lib.terra_abi_version()
         if version != ABI_VERSION:
             raise RuntimeError(f"terra_amd: {LIB_PATH} has ABI version {version}, expected {ABI_VERSION}; rebuild it")

@@ -776,3 +776,54 @@ def residual_norm(h: torch.Tensor, x: torch.Tensor, post_norm: Optional[Norm] = 
         x = x.detach()
     tail = kernels._tail(h, x, post_norm, gate, next_norm, geom, residual_scale, p, seed, stream)
     return _lib.load_binding().residual_norm(tail.call(), h, x, *tail.params(post_norm, gate, next_norm), seed, link)
+
+
+def layer_norm(x: torch.Tensor, norm: Norm, out_dtype: Optional[torch.dtype] = None) -> torch.Tensor:
+    """:func:`kernels.layer_norm` with gradients for x and the norm's parameters.
+    An x whose rows the kernels cannot read in place is copied first.  The autograd
+    node is a C++ one (csrc/training_binding.cpp); it keeps x, the parameters and two fp32 values a row."""
+    try:
+        call = kernels._norm_call(x, norm, out_dtype)
+    except ValueError:
+        if x.is_contiguous():
+            raise
+        x = x.contiguous()
+        call = kernels._norm_call(x, norm, out_dtype)
+    return _lib.load_training().layer_norm(call, x, norm.weight, norm.bias)
+
+
+class _Rotary(torch.autograd.Function):
+    """kernels.rotary.  A linear map: a tangent is turned as the values are, a
+    gradient back, and that may be differentiated again."""
+
+    @staticmethod
+    def forward(ctx, x, rot, positions, inverse):
+        ctx.rot, ctx.inverse = rot, inverse
+        ctx.save_for_backward(positions)
+        ctx.save_for_forward(positions)
+        return kernels.rotary(x, rot, positions, inverse)
+
+    @staticmethod
+    def jvp(ctx, dx, *_):
+        return kernels.rotary(dx.contiguous(), ctx.rot, ctx.saved_tensors[0], ctx.inverse)
+
+    @staticmethod
+    def backward(ctx, dy):
+        return rotary(dy, ctx.rot, ctx.saved_tensors[0], not ctx.inverse), None, None, None
+
+
+def rotary(x: torch.Tensor, rot: kernels.Rotary, positions: torch.Tensor, inverse: bool = False) -> torch.Tensor:
+    """:func:`kernels.rotary` with derivatives of every order, backward and
+    forward mode.  Heads that the kernel cannot read in place are copied first."""
+    if x.dim() >= 2 and x.stride(-1) != 1:
+        x = x.contiguous()
+    positions = positions.contiguous()
+    try:
+        kernels._rotary_call(x, rot, positions, inverse, None)
+    except ValueError:
+        if x.is_contiguous():
+            raise
+        x = x.contiguous()
+    if _needs_grad(x) or _has_tangent(x):
+        return _Rotary.apply(x, rot, positions, inverse)
+    return kernels.rotary(x, rot, positions, inverse)

@@ -1,5 +1,5 @@
 """Builds ``terra_amd/libterra_swin.so`` from ``terra_amd/csrc`` with hipcc for gfx950,
-and the regularised operators' host module beside it.
+and the host modules of the operators that have one beside it.
 
     python -m terra_amd.build
 
@@ -19,7 +19,9 @@ CSRC = os.path.join(HERE, "csrc")
 SOURCES = ("abi.hip", "window_copy.hip", "window_attention.hip", "window_attention_bwd.hip", "swin_block.hip",
            "swin_mlp.hip", "linear.hip", "mlp_backward.hip", "weight_grad.hip", "linear_short.hip", "block_f32.hip",
            "dropout.hip", "residual_norm.hip", "residual_norm_f32_f32.hip", "residual_norm_bf16_bf16.hip",
-           "residual_norm_bf16_f32.hip", "residual_norm_f16_f16.hip", "residual_norm_f16_f32.hip")
+           "residual_norm_bf16_f32.hip", "residual_norm_f16_f16.hip", "residual_norm_f16_f32.hip", "layer_norm.hip", "layer_norm_f32_f32.hip",
+           "layer_norm_f32_bf16.hip", "layer_norm_f32_f16.hip", "layer_norm_bf16_bf16.hip", "layer_norm_bf16_f32.hip",
+           "layer_norm_f16_f16.hip", "layer_norm_f16_f32.hip", "rotary.hip", "optimizer.hip")
 ARCH = "gfx950"
 
 HIPCC_FLAGS = [
@@ -95,23 +97,27 @@ def build_library(verbose: bool = False, jobs: int = 0, asan_host: bool = False)
     return LIB_PATH
 
 
-def build_binding(verbose: bool = False) -> str:
-    """Compile the regularised operators' host module
-    (``csrc/regularize_binding.cpp``, against torch's headers) into ``terra_amd/_regularize.so``; returns its path."""
+# The host modules: name -> source, against torch's headers.
+BINDINGS = {"_regularize": "regularize_binding.cpp", "_training": "training_binding.cpp"}
+
+
+def build_binding(verbose: bool = False, name: str = "_regularize") -> str:
+    """Compile a host module (of the regularised operators, or ``_training`` of
+    the norms, rotary positions and the optimizer's step) into ``terra_amd/<name>.so``; returns its path."""
     import sysconfig
 
     import torch
     from torch.utils import cpp_extension
 
-    path = os.path.join(HERE, "_regularize.so")
+    path = os.path.join(HERE, f"{name}.so")
     root = os.path.dirname(torch.__file__)
     cmd = [hipcc(), "-x", "c++", "-O2", "-std=c++17", "-fPIC", "-shared", "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1",
            f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}",
            *(f"-isystem{d}" for d in [*cpp_extension.include_paths(), "/opt/rocm/include",
                                       sysconfig.get_paths()["include"]]),
-           os.path.join(CSRC, "regularize_binding.cpp"), f"-L{os.path.join(root, 'lib')}", "-ltorch_python",
+           os.path.join(CSRC, BINDINGS[name]), f"-L{os.path.join(root, 'lib')}", "-ltorch_python",
            "-ltorch_cpu", "-ltorch", "-lc10", "-lc10_hip"]
-    fd, tmp = tempfile.mkstemp(prefix="_regularize.", suffix=".so.tmp", dir=HERE)
+    fd, tmp = tempfile.mkstemp(prefix=f"{name}.", suffix=".so.tmp", dir=HERE)
     os.close(fd)
     try:
         _run([*cmd, "-o", tmp], verbose)
@@ -121,6 +127,14 @@ def build_binding(verbose: bool = False) -> str:
     os.chmod(tmp, 0o755)
     os.replace(tmp, path)
     return path
+
+
+def build_bindings(verbose: bool = False) -> list:
+    """Compile every host module, side by side; returns their paths."""
+    from concurrent.futures import ThreadPoolExecutor
+
+    with ThreadPoolExecutor() as pool:
+        return list(pool.map(lambda name: build_binding(verbose, name), BINDINGS))
 
 
 def asan_runtime() -> str:
@@ -140,5 +154,6 @@ if __name__ == "__main__":
     path = build_library(verbose=True, asan_host="--asan-host" in sys.argv)
     print(path)
     if "--asan-host" not in sys.argv:
-        print(build_binding(verbose=True))
+        for path in build_bindings(verbose=True):
+            print(path)
     sys.exit(0)

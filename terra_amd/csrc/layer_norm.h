@@ -1,0 +1,67 @@
+// LayerNorm and RMS norm over rows of C channels, forward and backward:
+//
+//   xh = (x - mean x) r,  r = rsqrt(mean (x - mean x)^2 + eps)     LayerNorm
+//   xh = x r,             r = rsqrt(mean x^2 + eps)                RMS norm
+//   y  = xh w + b
+//   g  = dy w,  dx = r (g - mean g - xh mean(g xh))   (an RMS norm has no mean g)
+//   dw = sum over rows of dy xh,  db = sum over rows of dy
+//
+// All of it in fp32, two-pass statistics, y and dx rounded once; the parameters
+// are read in their own type and their gradients written in it, rounded once
+// from fp64 sums.  Row r of x begins (r / inner) outer + (r % inner) step
+// elements into x, so the heads of a packed q|k|v are rows too; y, dy and dx are packed.
+//
+// Sums over rows: workgroups keep the sums of the rows that they take and write
+// them to a workspace, a second launch adds those up in fp64: no atomics, an
+// order that the sizes and alignments fix.
+#pragma once
+
+#include "residual_norm.h"
+
+namespace terra {
+namespace {
+
+struct NormArgs {
+  const uint8_t *x, *dy;
+  uint8_t *y, *dx;         // dx may be NULL: only sums are asked for
+  const void *w, *b;       // NULL: 1, 0
+  float2* statistics;      // mean and r of each row, or NULL (forward)
+  float* partial;          // backward: [parts][2][C], or NULL: no sums
+  uint32_t rows, parts;
+  FastDiv inner;
+  int64_t outer_bytes, step_bytes;
+  int32_t C, param_dtype;
+  bool layer;
+  float eps, inv_c;
+
+  __device__ __forceinline__ const uint8_t* row(uint32_t r) const {
+    uint32_t q, rest;
+    inner.divmod(r, q, rest);
+    return x + (int64_t)q * outer_bytes + (int64_t)rest * step_bytes;
+  }
+};
+
+// Parameter c in fp32, `none` where the pointer is NULL.
+__device__ __forceinline__ float norm_param(const void* p, int dtype, float none, int c) {
+  if (p == nullptr) return none;
+  if (dtype == TERRA_DTYPE_F32) return reinterpret_cast<const float*>(p)[c];
+  const uint16_t v = reinterpret_cast<const uint16_t*>(p)[c];
+  return dtype == TERRA_DTYPE_BF16 ? bf16_bits_to_f32(v) : __half2float(__ushort_as_half(v));
+}
+
+}  // namespace
+
+// The kernels' launches by the types of x and y, each with a source file of
+// its own; `args` is a NormArgs.
+struct NormPlan {
+  uint32_t parts;  // workgroups of the sums over rows
+  bool held;       // rows are held in registers (else read again)
+  TailShape shape;
+};
+#define TERRA_NORM_TYPES(X) X(f32, f32) X(f32, bf16) X(f32, f16) X(bf16, bf16) X(bf16, f32) X(f16, f16) X(f16, f32)
+#define TERRA_NORM_DECLARE(x, y)                                                        \
+  void norm_fwd_##x##_##y(const void* args, const NormPlan& plan, bool vec, bool pairs, hipStream_t s); \
+  void norm_bwd_##x##_##y(const void* args, const NormPlan& plan, bool vec, bool pairs, hipStream_t s);
+TERRA_NORM_TYPES(TERRA_NORM_DECLARE)
+
+}  // namespace terra

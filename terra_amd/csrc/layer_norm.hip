@@ -1,0 +1,217 @@
+// Entry points of the norms over rows (layer_norm.h).
+#include "layer_norm.h"
+
+#include <initializer_list>
+
+namespace terra {
+namespace {
+
+constexpr int kNormMaxChannels = 1 << 24;
+
+struct NormAlignment {
+  uintptr_t bits = 0;
+  int C = 0;
+  bool vec() const { return C % kChunkCols == 0 && bits % 16 == 0; }
+  bool pairs() const { return C % 2 == 0 && bits % 4 == 0; }
+};
+
+bool is_float(int dtype) { return dtype == TERRA_DTYPE_F32 || dtype == TERRA_DTYPE_BF16 || dtype == TERRA_DTYPE_F16; }
+
+// Checks the descriptor; fills what it says of `a` and `al`.
+int norm_prepare(const terra_swin_layer_norm_desc* d, NormArgs* a, NormAlignment* al) {
+  if (d == nullptr) return fail(TERRA_ERR_NULL, "desc is NULL");
+  const int x = d->x_dtype, y = d->y_dtype;
+  if (!is_float(x) || !is_float(y) || !is_float(d->param_dtype) || (x != y && x != TERRA_DTYPE_F32 && y != TERRA_DTYPE_F32))
+    return fail(TERRA_ERR_DTYPE, "x, y and the parameters are f32, bf16 or f16, y of x's dtype unless one is f32 (got %d, %d, %d)",
+                x, y, d->param_dtype);
+  if (d->rows < 0 || d->channels <= 0) return fail(TERRA_ERR_SHAPE, "rows must be >= 0 and channels > 0");
+  if (d->channels > kNormMaxChannels)
+    return fail(TERRA_ERR_UNSUPPORTED, "rows of up to %d channels (got %d)", kNormMaxChannels, d->channels);
+  if (d->rows >= (1ll << 31)) return fail(TERRA_ERR_SHAPE, "%lld rows: at most 2^31 - 1", (long long)d->rows);
+  if (d->norm != TERRA_NORM_LAYER && d->norm != TERRA_NORM_RMS) return fail(TERRA_ERR_SHAPE, "unknown norm %d", d->norm);
+  if (d->inner <= 0 || d->inner >= (1ll << 31)) return fail(TERRA_ERR_SHAPE, "inner must be in [1, 2^31) (got %lld)", (long long)d->inner);
+  if (d->outer_stride < 0 || d->inner_stride < 0 || d->outer_stride >= (1ll << 40) || d->inner_stride >= (1ll << 40))
+    return fail(TERRA_ERR_SHAPE, "row strides must be in [0, 2^40)");
+  if (!(d->eps >= 0.f)) return fail(TERRA_ERR_SHAPE, "eps must be >= 0 (got %g)", (double)d->eps);
+  const int elt = dtype_size(x);
+  a->rows = (uint32_t)d->rows;
+  a->C = d->channels;
+  a->inner = FastDiv((uint32_t)d->inner);
+  a->outer_bytes = d->outer_stride * elt;
+  a->step_bytes = d->inner_stride * elt;
+  a->param_dtype = d->param_dtype;
+  a->layer = d->norm == TERRA_NORM_LAYER;
+  a->eps = d->eps;
+  a->inv_c = 1.f / (float)d->channels;
+  al->C = a->C;
+  al->bits = (d->rows > d->inner ? (uintptr_t)a->outer_bytes : 0) | (d->inner > 1 ? (uintptr_t)a->step_bytes : 0);
+  return TERRA_OK;
+}
+
+int norm_pointer(const void* p, int dtype, const char* name, bool needed, uintptr_t* bits) {
+  if (p == nullptr) return needed ? fail(TERRA_ERR_NULL, "%s is NULL", name) : TERRA_OK;
+  if ((uintptr_t)p % (uintptr_t)dtype_size(dtype) != 0) return fail(TERRA_ERR_ALIGN, "%s is not aligned to its elements", name);
+  if (bits != nullptr) *bits |= (uintptr_t)p;
+  return TERRA_OK;
+}
+
+// Bytes from the first row of x to the end of its last one.
+int64_t x_span(const terra_swin_layer_norm_desc* d) {
+  if (d->rows == 0) return 0;
+  const int64_t outer = (d->rows - 1) / d->inner, inner = d->rows < d->inner ? d->rows - 1 : d->inner - 1;
+  return (outer * d->outer_stride + inner * d->inner_stride + d->channels) * dtype_size(d->x_dtype);
+}
+
+bool norm_meet(const void* p, int64_t bytes, const void* q, int64_t more) {
+  const uintptr_t a = (uintptr_t)p, b = (uintptr_t)q;
+  return p != nullptr && q != nullptr && bytes > 0 && more > 0 && a < b + (uintptr_t)more && b < a + (uintptr_t)bytes;
+}
+
+NormPlan norm_plan(uint32_t rows, int C) {
+  NormPlan p = {};
+  const uint32_t strips = (uint32_t)((C + 511) / 512), most = strips < 1024 ? 1024 / strips : 1, useful = (rows + 31) / 32;
+  p.parts = useful < most ? useful : most;
+  return p;
+}
+
+// dst[c] = sum over i < parts of partial[i][which][c], in fp64, in the parameters' type.
+struct FinishArgs {
+  const float* partial;
+  void* dst[2];
+  int32_t parts, C, dtype;
+};
+constexpr int kFinishThreads = 1024, kFinishCols = 16, kFinishParts = kFinishThreads / kFinishCols;
+
+__global__ __launch_bounds__(kFinishThreads) void norm_finish_kernel(const FinishArgs a) {
+  __shared__ double s[kFinishParts][kFinishCols];
+  const int which = blockIdx.y, lane = threadIdx.x % kFinishCols, part = threadIdx.x / kFinishCols;
+  const int c = blockIdx.x * kFinishCols + lane;
+  double sum = 0.0;
+  const float* src = a.partial + (int64_t)which * a.C + (c < a.C ? c : 0);
+  constexpr int kAhead = 8;
+  for (int i = part; i < a.parts; i += kAhead * kFinishParts) {
+    float v[kAhead];
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) {
+      const int at = i + u * kFinishParts;
+      v[u] = src[(int64_t)(at < a.parts ? at : i) * 2 * a.C];
+    }
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) sum += i + u * kFinishParts < a.parts ? (double)v[u] : 0.0;
+  }
+  s[part][lane] = sum;
+  __syncthreads();
+  for (int half = kFinishParts / 2; half > 0; half /= 2) {
+    if (part < half) s[part][lane] = sum += s[part + half][lane];
+    __syncthreads();
+  }
+  if (part != 0 || c >= a.C || a.dst[which] == nullptr) return;
+  const float v = (float)sum;
+  if (a.dtype == TERRA_DTYPE_F32) reinterpret_cast<float*>(a.dst[which])[c] = v;
+  else if (a.dtype == TERRA_DTYPE_BF16) reinterpret_cast<uint16_t*>(a.dst[which])[c] = f32_to_bf16_bits(v);
+  else reinterpret_cast<uint16_t*>(a.dst[which])[c] = __half_as_ushort(__float2half_rn(v));
+}
+
+int norm_launched(const char* what) {
+  const hipError_t e = hipGetLastError();
+  return e == hipSuccess ? TERRA_OK : fail(TERRA_ERR_LAUNCH, "%s launch failed: %s", what, hipGetErrorString(e));
+}
+
+#define TERRA_NORM_CASE(x, y) \
+  if (xd == kNorm_##x && yd == kNorm_##y) return backward ? norm_bwd_##x##_##y(&a, p, vec, pairs, s) : norm_fwd_##x##_##y(&a, p, vec, pairs, s);
+constexpr int kNorm_f32 = TERRA_DTYPE_F32, kNorm_bf16 = TERRA_DTYPE_BF16, kNorm_f16 = TERRA_DTYPE_F16;
+void norm_launch(bool backward, int xd, int yd, const NormArgs& a, const NormPlan& p, const NormAlignment& al, hipStream_t s) {
+  const bool vec = al.vec(), pairs = al.pairs();
+  TERRA_NORM_TYPES(TERRA_NORM_CASE)
+}
+
+}  // namespace
+}  // namespace terra
+
+using namespace terra;
+
+#define TERRA_TRY(call)                    \
+  do {                                     \
+    const int st_ = (call);                \
+    if (st_ != TERRA_OK) return st_;       \
+  } while (0)
+
+extern "C" int terra_swin_layer_norm(const void* x, void* y, const terra_swin_layer_norm_desc* desc, const void* weight,
+                                     const void* bias, float* statistics, void* stream) {
+  clear_error();
+  NormArgs a = {};
+  NormAlignment al;
+  TERRA_TRY(norm_prepare(desc, &a, &al));
+  if (a.rows == 0) return TERRA_OK;
+  TERRA_TRY(norm_pointer(x, desc->x_dtype, "x", true, &al.bits));
+  TERRA_TRY(norm_pointer(y, desc->y_dtype, "y", true, &al.bits));
+  TERRA_TRY(norm_pointer(weight, desc->param_dtype, "the weight", false, nullptr));
+  TERRA_TRY(norm_pointer(bias, desc->param_dtype, "the bias", false, nullptr));
+  if (((uintptr_t)statistics & 7u) != 0) return fail(TERRA_ERR_ALIGN, "statistics must be 8-byte aligned");
+  const int64_t out = (int64_t)a.rows * a.C * dtype_size(desc->y_dtype), span = x_span(desc);
+  if (norm_meet(x, span, y, out)) return fail(TERRA_ERR_SHAPE, "y must not overlap x");
+  if (norm_meet(statistics, (int64_t)a.rows * 8, x, span) || norm_meet(statistics, (int64_t)a.rows * 8, y, out))
+    return fail(TERRA_ERR_SHAPE, "statistics must not overlap x or y");
+  a.x = (const uint8_t*)x;
+  a.y = (uint8_t*)y;
+  a.w = weight;
+  a.b = bias;
+  a.statistics = (float2*)statistics;
+  norm_launch(false, desc->x_dtype, desc->y_dtype, a, norm_plan(a.rows, a.C), al, (hipStream_t)stream);
+  return norm_launched("terra_swin_layer_norm");
+}
+
+extern "C" int terra_swin_layer_norm_workspace(const terra_swin_layer_norm_desc* desc) {
+  clear_error();
+  NormArgs a = {};
+  NormAlignment al;
+  TERRA_TRY(norm_prepare(desc, &a, &al));
+  return a.rows == 0 ? 0 : (int)norm_plan(a.rows, a.C).parts * 2 * a.C;
+}
+
+extern "C" int terra_swin_layer_norm_bwd(const void* dy, const void* x, const float* statistics, void* dx,
+                                         const terra_swin_layer_norm_desc* desc, const void* weight, void* dweight,
+                                         void* dbias, float* workspace, void* stream) {
+  clear_error();
+  NormArgs a = {};
+  NormAlignment al;
+  TERRA_TRY(norm_prepare(desc, &a, &al));
+  const int xd = desc->x_dtype, yd = desc->y_dtype;
+  TERRA_TRY(norm_pointer(dweight, desc->param_dtype, "dweight", false, nullptr));
+  TERRA_TRY(norm_pointer(dbias, desc->param_dtype, "dbias", false, nullptr));
+  const bool sums = dweight != nullptr || dbias != nullptr;
+  if (dx == nullptr && !sums) return TERRA_OK;
+  FinishArgs f = {workspace, {dweight, dbias}, 0, a.C, desc->param_dtype};
+  hipStream_t s = (hipStream_t)stream;
+  const dim3 finish((unsigned)((a.C + kFinishCols - 1) / kFinishCols), 2);
+  if (a.rows == 0) {  // the sums of no rows
+    if (!sums) return TERRA_OK;
+    norm_finish_kernel<<<finish, kFinishThreads, 0, s>>>(f);
+    return norm_launched("terra_swin_layer_norm_bwd");
+  }
+  TERRA_TRY(norm_pointer(dy, yd, "dy", true, &al.bits));
+  TERRA_TRY(norm_pointer(x, xd, "x", true, &al.bits));
+  TERRA_TRY(norm_pointer(dx, xd, "dx", false, &al.bits));
+  TERRA_TRY(norm_pointer(weight, desc->param_dtype, "the weight", false, nullptr));
+  if (statistics == nullptr) return fail(TERRA_ERR_NULL, "statistics are NULL");
+  if (((uintptr_t)statistics & 7u) != 0) return fail(TERRA_ERR_ALIGN, "statistics must be 8-byte aligned");
+  if (sums && workspace == nullptr) return fail(TERRA_ERR_NULL, "parameter gradients need a workspace");
+  if (((uintptr_t)workspace & 3u) != 0) return fail(TERRA_ERR_ALIGN, "the workspace must be 4-byte aligned");
+  const int64_t n = (int64_t)a.rows * a.C, in = n * dtype_size(yd), out = n * dtype_size(xd);
+  if (norm_meet(dx, out, x, x_span(desc)) || norm_meet(dx, out, statistics, (int64_t)a.rows * 8) || norm_meet(dx, out, dy, in))
+    return fail(TERRA_ERR_SHAPE, "dx must not overlap x, dy or the statistics");
+  a.x = (const uint8_t*)x;
+  a.dy = (const uint8_t*)dy;
+  a.dx = (uint8_t*)dx;
+  a.w = weight;
+  a.statistics = (float2*)const_cast<float*>(statistics);
+  const NormPlan p = norm_plan(a.rows, a.C);
+  a.parts = p.parts;
+  a.partial = sums ? workspace : nullptr;
+  norm_launch(true, xd, yd, a, p, al, s);
+  if (sums) {
+    f.parts = (int32_t)p.parts;
+    norm_finish_kernel<<<finish, kFinishThreads, 0, s>>>(f);
+  }
+  return norm_launched("terra_swin_layer_norm_bwd");
+}

@@ -8,6 +8,7 @@ without ``libterra_swin.so``, raises.
 from __future__ import annotations
 
 import ctypes
+import math
 import weakref
 from collections import OrderedDict
 from dataclasses import dataclass
@@ -1408,7 +1409,7 @@ def _size(n: int, what: str) -> int:
 
 @dataclass(frozen=True, eq=False)
 class Norm:
-    """A norm over the channels for :func:`residual_norm`: LayerNorm, or with
+    """A norm over the channels for :func:`residual_norm` and :func:`layer_norm`: LayerNorm, or with
     ``rms`` the RMS norm ``v / sqrt(mean(v^2) + eps)``; affine [C] weight and
     bias, either None (1, 0)."""
 
@@ -1619,3 +1620,334 @@ def residual_norm_backward(h: torch.Tensor, x: torch.Tensor, dy: Optional[torch.
     if dz is not None and next_norm is None:
         raise ValueError("dz without a next_norm")
     return t.backward(h, x, dy, dz, t.params(post_norm, gate, next_norm), seed, needs)
+
+
+# ---- what a training step does beside its products and attention cores ---------
+
+
+def _two_level_rows(t: torch.Tensor, dims: int, name: str) -> Tuple[int, int, int, int]:
+    """(rows, inner, outer stride, inner stride) of t's dimensions but the last
+    ``dims``, as rows of which ``inner`` follow each other at one stride, and those groups
+    at another.  Raises ValueError where two strides do not say it."""
+    shape, strides = t.shape[:t.dim() - dims], t.stride()[:t.dim() - dims]
+    levels = []  # [size, stride], the innermost first
+    for n, s in zip(reversed(shape), reversed(strides)):
+        if n == 1:
+            continue
+        if levels and s == levels[-1][0] * levels[-1][1]:
+            levels[-1][0] *= n
+        else:
+            levels.append([n, s])
+    if len(levels) > 2:
+        raise ValueError(f"{name}'s rows must have at most two strides (shape {tuple(t.shape)}, strides {t.stride()})")
+    packed = 1
+    for n in t.shape[t.dim() - dims:]:
+        packed *= n
+    inner, inner_stride = levels[0] if levels else (1, packed)
+    outer, outer_stride = levels[1] if len(levels) > 1 else (1, inner * inner_stride)
+    return inner * outer, inner, outer_stride, inner_stride
+
+
+_NORMS = {}  # checked arguments by shapes, types and options
+
+
+def _norm_call(x: torch.Tensor, norm: Norm, out_dtype: Optional[torch.dtype]):
+    """The arguments of a layer_norm call as the host module takes them, made once
+    for each set of shapes, strides, types and options."""
+    w, b = norm.weight, norm.bias
+    key = (x.shape, x.stride(), x.dtype, x.device, norm.eps, norm.rms, out_dtype,
+           None if w is None else (w.shape, w.dtype, w.device), None if b is None else (b.shape, b.dtype, b.device))
+    call = _NORMS.get(key)
+    if call is not None:
+        return call
+    dev = _require_device(x, *(t for t in (w, b) if t is not None))
+    if x.dim() < 1 or x.shape[-1] < 1:
+        raise ValueError(f"x must be [..., C] with C >= 1, got {tuple(x.shape)}")
+    C = x.shape[-1]
+    d = _lib.LayerNormDesc()
+    d.x_dtype = _dtype_code(x, _FLOATS)
+    out_dtype = x.dtype if out_dtype is None else out_dtype
+    if out_dtype not in _FLOATS or (out_dtype != x.dtype and torch.float32 not in (out_dtype, x.dtype)):
+        raise TypeError(f"out_dtype {out_dtype} is not available for {x.dtype} x (x's own, float32, or of float32 x any)")
+    d.y_dtype = _DTYPES[out_dtype]
+    for name, t in (("weight", w), ("bias", b)):
+        if t is not None:
+            _dtype_code(t, _FLOATS)
+            if tuple(t.shape) != (C,):
+                raise ValueError(f"the norm's {name} must have {C} channels, got {list(t.shape)}")
+    types = {t.dtype for t in (w, b) if t is not None}
+    d.param_dtype = _DTYPES[types.pop()] if len(types) == 1 else _lib.DTYPE_F32  # of two types: both as fp32
+    if C > 1 and x.stride(-1) != 1:
+        raise ValueError(f"x must have unit channel stride (strides {x.stride()})")
+    if x.numel() == 0:
+        d.rows, d.inner, d.outer_stride, d.inner_stride = 0, 1, C, C
+    else:
+        d.rows, d.inner, d.outer_stride, d.inner_stride = _two_level_rows(x, 1, "x")
+    d.channels, d.eps, d.norm = C, float(norm.eps), _lib.NORM_RMS if norm.rms else _lib.NORM_LAYER
+    work = _size(_lib.load().terra_swin_layer_norm_workspace(ctypes.byref(d)), "terra_swin_layer_norm_workspace")
+    call = _lib.load_training().NormCall(bytes(d), work)
+    if len(_NORMS) >= _KEPT_CALLS:
+        _NORMS.clear()
+    _NORMS[key] = call
+    return call
+
+
+def layer_norm(x: torch.Tensor, norm: Norm, out_dtype: Optional[torch.dtype] = None, statistics: bool = False,
+               out: Optional[torch.Tensor] = None):
+    """``norm`` (a LayerNorm or RMS norm, see :class:`Norm`) over the last
+    dimension of ``x`` [..., C], in fp32 and rounded once to ``out_dtype`` (x's by default; fp32,
+    or of an fp32 x bf16 or fp16, as autocast's next product takes it).  Any C up to
+    2^24; the rows need unit channel stride and at most two strides above it (so
+    the heads of a packed q | k | v are rows); the parameters are read in their
+    own dtype.  Returns y, packed, or with ``statistics`` (y, the fp32 [rows, 2] means and
+    reciprocal roots that :func:`layer_norm_backward` reads)."""
+    call = _norm_call(x, norm, out_dtype)
+    return _lib.load_training().layer_norm_forward(call, x, norm.weight, norm.bias, statistics, out)
+
+
+class LayerNormGrads(NamedTuple):
+    """What :func:`layer_norm_backward` gives; None where there is none."""
+
+    dx: Optional[torch.Tensor]
+    dweight: Optional[torch.Tensor]
+    dbias: Optional[torch.Tensor]
+
+
+def layer_norm_backward(dy: torch.Tensor, x: torch.Tensor, norm: Norm, statistics: torch.Tensor,
+                        needs: Sequence[bool] = (True, True, True)) -> LayerNormGrads:
+    """Gradients of :func:`layer_norm` for the contiguous gradient ``dy`` of y:
+    of x (packed) and of the parameters, in their dtypes; the sums over rows are taken in an order
+    that the sizes and alignments fix.  ``needs``: which of the three are taken (where the parameter is there)."""
+    call = _norm_call(x, norm, dy.dtype)
+    _require_device(x, dy, statistics)
+    return LayerNormGrads(*_lib.load_training().layer_norm_backward(call, dy, x, norm.weight, norm.bias, statistics,
+                                                                    *map(bool, needs)))
+
+
+class Rotary:
+    """Rotary positions of a head's first ``dim`` elements for :func:`rotary`: pair
+    i turns by the angle position * rate[i], rate[i] = base^(-2i / dim).
+
+    ``axes``: a token has that many positions (a window's row and column, say); the
+    pairs are dealt to them in equal runs, each with rates over its own pairs.
+    ``interleaved``: the pairs are (2i, 2i + 1), else (i, i + dim / 2).
+
+    ``scaling`` for contexts longer than those trained on, by ``factor``:
+      "linear"  every rate is divided by it;
+      "ntk"     the base grows by factor^(dim / (dim - 2)), so that the slowest pair is slowed
+                by it and the fastest not at all;
+      "yarn"    by parts (Peng, Quesnelle, Fan, Shippole, "YaRN", 2023): with r the turns that a pair makes within
+                ``original_length``, rates of r > ``beta_fast`` stay, those of r < ``beta_slow`` are
+                divided, between them a mixture, and the values are scaled by ``amplitude`` = 0.1 ln(factor) + 1.
+    ``amplitude`` overrides the scale of the rotated values."""
+
+    def __init__(self, dim: int, base: float = 10000.0, axes: int = 1, interleaved: bool = False,
+                 scaling: Optional[str] = None, factor: float = 1.0, original_length: Optional[int] = None,
+                 beta_fast: float = 32.0, beta_slow: float = 1.0, amplitude: Optional[float] = None,
+                 device: Union[str, torch.device, None] = None):
+        dim, axes, base, factor = int(dim), int(axes), float(base), float(factor)
+        if dim < 2 or dim % 2 or axes < 1 or (dim // 2) % axes:
+            raise ValueError(f"dim must be even, its pairs a whole number for each of the axes (got {dim} and {axes})")
+        if not base > 0.0 or not factor > 0.0:
+            raise ValueError(f"base and factor must be positive (got {base} and {factor})")
+        self.dim, self.axes, self.interleaved = dim, axes, bool(interleaved)
+        pairs = dim // 2 // axes
+        scale = 1.0
+        if scaling == "ntk":
+            base *= factor ** (pairs / (pairs - 1)) if pairs > 1 else 1.0
+        rates = base ** (-torch.arange(pairs, dtype=torch.float64) / pairs)
+        if scaling == "linear":
+            rates = rates / factor
+        elif scaling == "yarn":
+            if original_length is None or original_length < 1 or not beta_fast > beta_slow:
+                raise ValueError("yarn needs original_length >= 1 and beta_fast > beta_slow")
+            turns = original_length * rates / (2 * math.pi)
+            keep = ((turns - beta_slow) / (beta_fast - beta_slow)).clamp(0.0, 1.0)
+            rates = rates * keep + rates / factor * (1.0 - keep)
+            scale = 0.1 * math.log(factor) + 1.0 if factor > 1.0 else 1.0
+        elif scaling not in (None, "none", "ntk"):
+            raise ValueError(f"scaling must be None, 'linear', 'ntk' or 'yarn' (got {scaling!r})")
+        self.amplitude = scale if amplitude is None else float(amplitude)
+        self.rates = rates
+        self._turns = {}
+        if device is not None:
+            self.turns(torch.device(device))
+
+    def turns(self, device: torch.device) -> torch.Tensor:
+        """The rates in whole turns a position (fp64) on ``device``, kept there."""
+        t = self._turns.get(device)
+        if t is None:
+            t = (self.rates / (2 * math.pi)).to(device)
+            self._turns[t.device] = t  # with its index, as the devices of tensors have it
+        return t
+
+    def __getstate__(self):
+        return dict(self.__dict__, _turns={})
+
+    def __deepcopy__(self, memo):
+        other = type(self).__new__(type(self))
+        other.__dict__.update(self.__getstate__())
+        return other
+
+
+_ROTARY = {}  # checked arguments by shapes, types and options
+
+
+def _rotary_call(x: torch.Tensor, rotary: Rotary, positions: torch.Tensor, inverse: bool, out: Optional[torch.Tensor]):
+    key = (x.shape, x.stride(), x.dtype, x.device, rotary.dim, rotary.axes, rotary.interleaved, rotary.amplitude, inverse,
+           positions.shape, positions.dtype, positions.device, positions.is_contiguous(),
+           None if out is None else (out.shape, out.stride(), out.dtype, out.device))
+    call = _ROTARY.get(key)
+    if call is not None:
+        return call
+    dev = _require_device(x, positions)
+    if x.dim() < 2:
+        raise ValueError(f"x must be [..., heads, head_dim], got {tuple(x.shape)}")
+    d = _lib.RotaryDesc()
+    d.dtype = _dtype_code(x, _FLOATS)
+    lead, (heads, head_dim) = tuple(x.shape[:-2]), x.shape[-2:]
+    if rotary.dim > head_dim:
+        raise ValueError(f"heads of {head_dim} cannot have {rotary.dim} rotated elements")
+    if positions.dtype not in (torch.int32, torch.int64) or not positions.is_contiguous():
+        raise ValueError(f"positions must be a contiguous int32 or int64 tensor (got {positions.dtype}, strides {positions.stride()})")
+    at = tuple(positions.shape)
+    if rotary.axes > 1:
+        if not at or at[-1] != rotary.axes:
+            raise ValueError(f"positions must have {rotary.axes} values for each token, got {at}")
+        at = at[:-1]
+    if len(at) > len(lead) or at != lead[len(lead) - len(at):]:
+        raise ValueError(f"positions of the tokens {at} must be those of x's last dimensions before its heads, {lead}")
+    if head_dim > 1 and x.stride(-1) != 1:
+        raise ValueError(f"x must have unit stride within a head (strides {x.stride()})")
+    d.heads, d.head_dim, d.dim, d.axes = heads, head_dim, rotary.dim, rotary.axes
+    d.position_bits = 32 if positions.dtype == torch.int32 else 64
+    d.interleaved, d.inverse, d.amplitude = rotary.interleaved, inverse, rotary.amplitude
+    if out is not None and (out.shape != x.shape or out.dtype != x.dtype or out.device != dev
+                            or (head_dim > 1 and out.stride(-1) != 1)):
+        raise ValueError(f"out must be a {x.dtype} tensor of shape {tuple(x.shape)} on {dev} with unit stride within a head")
+    if x.numel() == 0:
+        d.tokens, d.inner, d.position_tokens, d.heads = 0, 1, 1, max(heads, 1)
+    else:
+        tokens, inner, d.x_outer_stride, d.x_inner_stride = _two_level_rows(x, 2, "x")
+        d.tokens, d.inner, d.x_head_stride = tokens, inner, x.stride(-2)
+        if out is None:
+            d.y_head_stride, d.y_inner_stride = head_dim, heads * head_dim
+            d.y_outer_stride = inner * heads * head_dim
+        else:
+            _, y_inner, y_outer_stride, y_inner_stride = _two_level_rows(out, 2, "out")
+            if y_inner != inner:
+                # One of the two has its rows at one stride: its groups of the other's size are as far apart.
+                if inner == tokens:
+                    d.inner, d.x_outer_stride = y_inner, y_inner * d.x_inner_stride
+                elif y_inner == tokens:
+                    y_outer_stride = inner * y_inner_stride
+                else:
+                    raise ValueError(f"out's rows (strides {out.stride()}) are grouped otherwise than x's ({x.stride()})")
+            d.y_outer_stride, d.y_inner_stride, d.y_head_stride = y_outer_stride, y_inner_stride, out.stride(-2)
+        d.position_tokens = math.prod(at)
+    call = _lib.load_training().RotaryCall(bytes(d))
+    if len(_ROTARY) >= _KEPT_CALLS:
+        _ROTARY.clear()
+    _ROTARY[key] = call
+    return call
+
+
+def rotary(x: torch.Tensor, rotary: Rotary, positions: torch.Tensor, inverse: bool = False,
+           out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Rotary positions of the heads ``x`` [..., heads, head_dim] (fp32, bf16 or fp16;
+    query and key heads that lie side by side are one call): the first ``rotary.dim`` elements
+    of each head turned, the others as they are.  ``positions``: int32 or int64, one (or ``rotary.axes``, in a
+    last dimension) for each token of x's last dimensions before the heads, shared over those
+    before them: [N] or [B, N] for x [B, N, heads, head_dim].  Angles are taken in 64 bits, the
+    rotation in fp32, rounded once.  ``inverse``: by the negative angles, which is the backward.
+    The tokens may have two strides, the heads another.  ``out`` may be ``x``, whose unrotated elements are then not touched."""
+    call = _rotary_call(x, rotary, positions, bool(inverse), out)
+    return _lib.load_training().rotary(call, x, positions, rotary.turns(x.device), out)
+
+
+class GradientNorm(NamedTuple):
+    """What :func:`gradient_norm` gives, fp32 scalars on the device."""
+
+    norm: torch.Tensor
+    factor: torch.Tensor     # min(1, max_norm / (norm + 1e-6)), 1 without a max_norm
+    nonfinite: torch.Tensor  # 1 where the norm is infinite or NaN, else 0
+
+
+def gradient_norm(grads: Sequence[torch.Tensor], max_norm: Optional[float] = None) -> GradientNorm:
+    """The 2-norm of all ``grads`` (dense, fp32, bf16 or fp16 in any mixture, on one device) as one
+    vector, summed in 64 bits in an order that the sizes fix, and the factor that
+    clips it to ``max_norm``.  Nothing waits for the device and no gradient is
+    changed: :func:`adamw_step` takes the factor (and ``nonfinite``, to leave a step out)."""
+    if max_norm is not None and not max_norm > 0.0:
+        raise ValueError(f"max_norm must be positive (got {max_norm})")
+    r = _lib.load_training().gradient_norm(list(grads), 0.0 if max_norm is None else float(max_norm))
+    return GradientNorm(*r.unbind())
+
+
+class Moments(NamedTuple):
+    """The moments of a parameter for :func:`adamw_step`: fp32 tensors of its shape
+    and strides; or, with ``scales``, in 8 bits: float8_e4m3fn codes of exp_avg and of the root of
+    exp_avg_sq, and fp32 scales [2, ceil(numel / 256)], one for each 256 elements as they lie in memory."""
+
+    exp_avg: torch.Tensor
+    exp_avg_sq: torch.Tensor
+    scales: Optional[torch.Tensor] = None
+
+    def values(self) -> Tuple[torch.Tensor, torch.Tensor]:
+        """exp_avg and exp_avg_sq in fp32 (as they are, or from their codes)."""
+        if self.scales is None:
+            return self.exp_avg, self.exp_avg_sq
+        n = self.exp_avg.numel()
+        per = self.scales.repeat_interleave(256, 1)[:, :n]
+        out = []
+        for codes, scale in zip((self.exp_avg, self.exp_avg_sq), per):
+            v = torch.empty_like(codes, dtype=torch.float32)
+            flat = torch.as_strided(codes, (n,), (1,)).float() * scale  # in the order of memory
+            torch.as_strided(v, (n,), (1,)).copy_(flat)
+            out.append(v)
+        return out[0], out[1].square_()
+
+
+def moments(param: torch.Tensor, bits: int = 32) -> Moments:
+    """Moments of ``param`` before the first step (zeros), in 32 bits or in 8."""
+    if bits not in (8, 32):
+        raise ValueError(f"moments are held in 32 bits or in 8 (got {bits})")
+    dtype = torch.float32 if bits == 32 else torch.float8_e4m3fn
+    first, second = (torch.zeros_like(param, dtype=dtype, memory_format=torch.preserve_format) for _ in range(2))
+    if bits == 32:
+        return Moments(first, second)
+    return Moments(first, second, torch.zeros(2, -(-param.numel() // 256), device=param.device))
+
+
+def adamw_step(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], moments: Sequence[Moments],
+               step: Union[int, torch.Tensor], lr: Union[float, torch.Tensor] = 1e-3,
+               betas: Tuple[float, float] = (0.9, 0.999), eps: float = 1e-8, weight_decay: float = 1e-2,
+               maximize: bool = False, grad_factor: Optional[torch.Tensor] = None,
+               found_inf: Optional[torch.Tensor] = None, seed: Optional[torch.Tensor] = None, stream: int = 0) -> None:
+    """An AdamW step (decoupled weight decay) over many tensors in a few launches, in place:
+
+        g = grad * grad_factor
+        m = beta1 m + (1 - beta1) g,   v = beta2 v + (1 - beta2) g^2
+        param = param (1 - lr weight_decay) - lr / (1 - beta1^step) m / (sqrt(v / (1 - beta2^step)) + eps)
+
+    params: fp32, bf16 or fp16, dense; grads of the same dtype or fp32 (for fp32 params any of the
+    three).  ``step`` counts from 1.  ``step`` (int64) and ``lr`` (fp32) may be one-element tensors on the device, which a
+    captured graph's replays read anew.  ``grad_factor``, ``found_inf``: fp32 scalars on the device, such as
+    :func:`gradient_norm` gives: the gradients' factor, and where ``found_inf`` is not 0 nothing changes.
+
+    Moments in 8 bits (see :class:`Moments`): the first is rounded to the nearest code; the second up or down at random, with the
+    mean that it has (0.999 v lies far nearer to v's own code than to the next: rounded to nearest it would never move),
+    from ``seed`` (see :func:`dropout_seed`), ``stream``, the step, the tensor's place in
+    the list and the element.  A block of 256 with an infinity or a NaN is NaN as a whole from then on.
+
+    No two of the tensors may overlap, nor a gradient one that is written."""
+    beta1, beta2 = betas
+    if len(moments) != len(params):
+        raise ValueError(f"as many moments as parameters (got {len(moments)} and {len(params)})")
+    if not 0 <= stream < 1 << 32:
+        raise ValueError(f"stream must be in [0, 2^32) (got {stream})")
+    step_at, lr_at = (t if isinstance(t, torch.Tensor) else None for t in (step, lr))
+    _lib.load_training().adamw_step(
+        list(params), list(grads), [m[0] for m in moments], [m[1] for m in moments], [m[2] for m in moments],
+        0.0 if lr_at is not None else float(lr), float(beta1), float(beta2), float(eps), float(weight_decay),
+        0 if step_at is not None else int(step), step_at, lr_at, grad_factor, found_inf, seed, stream, bool(maximize))
