@@ -49,6 +49,36 @@ __device__ __forceinline__ float norm_param(const void* p, int dtype, float none
   return dtype == TERRA_DTYPE_BF16 ? bf16_bits_to_f32(v) : __half2float(__ushort_as_half(v));
 }
 
+// The statistics of a row held as kK chunks a lane: v becomes xh (zero in
+// absent columns), r is returned.
+template <int kG, int kK, int kP, bool kVec>
+__device__ __forceinline__ float norm_row(float (&v)[kK][kChunkCols], bool layer, float eps, float inv_c,
+                                          const RowLanes<kG, kK, kP>& at, RowSum<kG>& sum, float& mean) {
+  mean = 0.f;
+  if (layer) {
+    float s = 0.f;
+#pragma unroll
+    for (int k = 0; k < kK; ++k)
+#pragma unroll
+      for (int j = 0; j < kChunkCols; ++j) s += v[k][j];
+    mean = sum.one(s) * inv_c;
+  }
+  float q = 0.f;
+#pragma unroll
+  for (int k = 0; k < kK; ++k)
+#pragma unroll
+    for (int j = 0; j < kChunkCols; ++j) {
+      v[k][j] -= at.template has<kVec>(k, j) ? mean : 0.f;  // kVec: one select for four
+      q = fmaf(v[k][j], v[k][j], q);
+    }
+  const float r = rsqrtf(sum.one(q) * inv_c + eps);
+#pragma unroll
+  for (int k = 0; k < kK; ++k)
+#pragma unroll
+    for (int j = 0; j < kChunkCols; ++j) v[k][j] *= r;
+  return r;
+}
+
 }  // namespace
 
 // The kernels' launches by the types of x and y, each with a source file of

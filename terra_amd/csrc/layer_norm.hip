@@ -67,12 +67,32 @@ bool norm_meet(const void* p, int64_t bytes, const void* q, int64_t more) {
   return p != nullptr && q != nullptr && bytes > 0 && more > 0 && a < b + (uintptr_t)more && b < a + (uintptr_t)bytes;
 }
 
-NormPlan norm_plan(uint32_t rows, int C) {
+constexpr int kNormHeld = 8192;  // channels of rows that are held in registers
+
+// How many lanes and chunks hold a row, as tail_shape; eight lanes also where a row has at most
+// eight chunks (the heads of a packed q | k | v).
+TailShape norm_shape(int C, bool pieces, int most) {
+  if (C <= 8 * kChunkCols) return {8, 1};
+  return tail_shape(C, pieces, most);
+}
+
+// Workgroups of the sums over rows: what fits the 256 compute units at once, or as many as have rows.
+NormPlan norm_plan(uint32_t rows, int C, bool pieces, bool vec, bool backward) {
   NormPlan p = {};
+  p.held = C <= kNormHeld;
+  if (p.held) {
+    p.shape = norm_shape(C, pieces, backward && (pieces || !vec) ? 2 : 3);
+    const uint32_t groups = (uint32_t)(tail_threads(p.shape.lanes) / p.shape.lanes), useful = (rows + groups - 1) / groups;
+    const uint32_t most = p.shape.lanes > 256 ? 1024u / (uint32_t)p.shape.chunks : 1024u;
+    p.parts = useful < most ? useful : most;
+    return p;
+  }
   const uint32_t strips = (uint32_t)((C + 511) / 512), most = strips < 1024 ? 1024 / strips : 1, useful = (rows + 31) / 32;
   p.parts = useful < most ? useful : most;
   return p;
 }
+
+bool norm_by_pieces(const terra_swin_layer_norm_desc* d) { return d->x_dtype == TERRA_DTYPE_F32 || d->y_dtype == TERRA_DTYPE_F32; }
 
 // dst[c] = sum over i < parts of partial[i][which][c], in fp64, in the parameters' type.
 struct FinishArgs {
@@ -157,7 +177,8 @@ extern "C" int terra_swin_layer_norm(const void* x, void* y, const terra_swin_la
   a.w = weight;
   a.b = bias;
   a.statistics = (float2*)statistics;
-  norm_launch(false, desc->x_dtype, desc->y_dtype, a, norm_plan(a.rows, a.C), al, (hipStream_t)stream);
+  norm_launch(false, desc->x_dtype, desc->y_dtype, a,
+              norm_plan(a.rows, a.C, norm_by_pieces(desc), al.vec(), false), al, (hipStream_t)stream);
   return norm_launched("terra_swin_layer_norm");
 }
 
@@ -166,7 +187,13 @@ extern "C" int terra_swin_layer_norm_workspace(const terra_swin_layer_norm_desc*
   NormArgs a = {};
   NormAlignment al;
   TERRA_TRY(norm_prepare(desc, &a, &al));
-  return a.rows == 0 ? 0 : (int)norm_plan(a.rows, a.C).parts * 2 * a.C;
+  if (a.rows == 0) return 0;
+  int most = 0;
+  for (const bool vec : {false, true}) {  // which, the call's addresses say
+    const int n = (int)norm_plan(a.rows, a.C, norm_by_pieces(desc), vec, true).parts * 2 * a.C;
+    most = n > most ? n : most;
+  }
+  return most;
 }
 
 extern "C" int terra_swin_layer_norm_bwd(const void* dy, const void* x, const float* statistics, void* dx,
@@ -205,7 +232,7 @@ extern "C" int terra_swin_layer_norm_bwd(const void* dy, const void* x, const fl
   a.dx = (uint8_t*)dx;
   a.w = weight;
   a.statistics = (float2*)const_cast<float*>(statistics);
-  const NormPlan p = norm_plan(a.rows, a.C);
+  const NormPlan p = norm_plan(a.rows, a.C, norm_by_pieces(desc), al.vec(), true);
   a.parts = p.parts;
   a.partial = sums ? workspace : nullptr;
   norm_launch(true, xd, yd, a, p, al, s);

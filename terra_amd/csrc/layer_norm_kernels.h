@@ -6,12 +6,165 @@
 namespace terra {
 namespace {
 
+template <int DTX, int DTY>
+constexpr int norm_pieces() { return DTX == TERRA_DTYPE_F32 || DTY == TERRA_DTYPE_F32 ? 4 : 8; }
+
+// ---- rows held in registers ------------------------------------------------------
+
+// The next rows are fetched before the ones at hand are worked on.
+template <int DTX, int DTY, int kG, int kK, bool kVec, bool kPairs>
+__global__ __launch_bounds__(tail_threads(kG)) void norm_kernel(const NormArgs a) {
+  constexpr int kGroups = tail_threads(kG) / kG, kYB = ChunkElt<DTY>::kBytes, kP = norm_pieces<DTX, DTY>();
+  using Params = ColumnParams<2, kG, kK, kP>;
+  __shared__ typename RowSum<kG>::Shared s_red;
+  __shared__ typename Params::Shared s_par;
+  const int group = threadIdx.x / kG, C = a.C;
+  const RowLanes<kG, kK, kP> at = {(int)(threadIdx.x % kG), C};
+  RowSum<kG> sum(&s_red);
+  const bool full = C == kG * kK * kChunkCols;  // every lane has columns
+  Params par(&s_par);
+  struct Row { RowChunk<DTX> x[kK]; };
+  auto fetch = [&](uint32_t base) {  // a row past the end re-reads the last one
+    Row q;
+    const uint32_t row = base + group;
+    const uint8_t* xp = a.row(row < a.rows ? row : a.rows - 1);
+#pragma unroll
+    for (int k = 0; k < kK; ++k) q.x[k] = at.template load<DTX, kVec, kPairs>(xp, k);
+    return q;
+  };
+  const uint32_t step = gridDim.x * kGroups;
+  uint32_t base = blockIdx.x * kGroups;
+  Row ahead = fetch(base);
+  par.fill(at, [&](int c, float (&v)[2]) {
+    v[0] = norm_param(a.w, a.param_dtype, 1.f, c);
+    v[1] = norm_param(a.b, a.param_dtype, 0.f, c);
+  });
+  if constexpr (Params::kLds) RowSum<kG>::lds_sync();
+  for (; base < a.rows; base += step) {
+    par.stay();
+    const Row q = ahead;
+    if (base + step < a.rows) ahead = fetch(base + step);
+    const uint32_t r = base + group;
+    const bool live = r < a.rows;
+    float v[kK][kChunkCols], mean;
+#pragma unroll
+    for (int k = 0; k < kK; ++k) at.template values<DTX, kVec>(q.x[k], k, true, full, v[k]);
+    const float rs = norm_row<kG, kK, kP, kVec>(v, a.layer, a.eps, a.inv_c, at, sum, mean);
+    if (a.statistics != nullptr && live && at.lane == 0) a.statistics[r] = make_float2(mean, rs);
+    const __amdgpu_buffer_rsrc_t out =
+        buffer_rsrc(a.y + (int64_t)base * C * kYB, min(a.rows - base, (uint32_t)kGroups) * (uint32_t)(C * kYB));
+#pragma unroll
+    for (int k = 0; k < kK; ++k) {
+      float w[kChunkCols], b[kChunkCols];
+      par.get(0, k, at, w);
+      par.get(1, k, at, b);
+#pragma unroll
+      for (int j = 0; j < kChunkCols; ++j) v[k][j] = fmaf(v[k][j], w[j], b[j]);
+      if (live) at.template store<DTY, kVec>(v[k], out, (uint32_t)(group * C) * kYB, a.y + (int64_t)r * C * kYB, k);
+    }
+  }
+}
+
+// Each lane keeps the sums of its columns over the rows that it takes.
+template <int DTX, int DTY, int kG, int kK, bool kVec, bool kPairs>
+__global__ __launch_bounds__(tail_threads(kG)) void norm_bwd_kernel(const NormArgs a) {
+  constexpr int kThreads = tail_threads(kG), kGroups = kThreads / kG, kCols = kG * kK * kChunkCols;
+  constexpr int kXB = ChunkElt<DTX>::kBytes, kYB = ChunkElt<DTY>::kBytes, kP = norm_pieces<DTX, DTY>();
+  using Params = ColumnParams<1, kG, kK, kP>;
+  __shared__ typename RowSum<kG>::Shared s_red;
+  __shared__ typename Params::Shared s_par;
+  __shared__ __attribute__((aligned(16))) float s_acc[kGroups > 1 ? kGroups * kCols : 1];
+  const int group = threadIdx.x / kG, C = a.C;
+  const RowLanes<kG, kK, kP> at = {(int)(threadIdx.x % kG), C};
+  RowSum<kG> sum(&s_red);
+  const bool full = C == kG * kK * kChunkCols;
+  Params par(&s_par);
+  par.fill(at, [&](int c, float (&v)[1]) { v[0] = norm_param(a.w, a.param_dtype, 1.f, c); });
+  if constexpr (Params::kLds) RowSum<kG>::lds_sync();
+  float acc_w[kK][kChunkCols] = {}, acc_b[kK][kChunkCols] = {};
+  for (uint32_t base = blockIdx.x * kGroups; base < a.rows; base += gridDim.x * kGroups) {
+    par.stay();
+    const uint32_t row = base + group;
+    const bool live = row < a.rows;
+    const uint32_t r = live ? row : a.rows - 1;  // a row past the end re-reads the last one
+    RowChunk<DTX> xq[kK];
+    RowChunk<DTY> dq[kK];
+    const uint8_t *xp = a.row(r), *dp = a.dy + (int64_t)r * C * kYB;
+    const float2 st = a.statistics[r];
+#pragma unroll
+    for (int k = 0; k < kK; ++k) {
+      xq[k] = at.template load<DTX, kVec, kPairs>(xp, k);
+      dq[k] = at.template load<DTY, kVec, kPairs>(dp, k);
+    }
+    float v[kK][kChunkCols], g[kK][kChunkCols], s0 = 0.f, s1 = 0.f;
+#pragma unroll
+    for (int k = 0; k < kK; ++k) {
+      float w[kChunkCols];
+      par.get(0, k, at, w);
+      at.template values<DTX, kVec>(xq[k], k, true, true, v[k]);  // absent columns have no gradient
+      at.template values<DTY, kVec>(dq[k], k, true, full, g[k]);
+#pragma unroll
+      for (int j = 0; j < kChunkCols; ++j) v[k][j] = (v[k][j] - st.x) * st.y;
+      if (live)
+#pragma unroll
+        for (int j = 0; j < kChunkCols; ++j) {
+          acc_w[k][j] = fmaf(g[k][j], v[k][j], acc_w[k][j]);
+          acc_b[k][j] += g[k][j];
+        }
+#pragma unroll
+      for (int j = 0; j < kChunkCols; ++j) {
+        g[k][j] *= w[j];
+        s0 += g[k][j];
+        s1 = fmaf(g[k][j], v[k][j], s1);
+      }
+    }
+    if (a.dx == nullptr) continue;
+    sum.two(s0, s1);
+    s0 = a.layer ? s0 * a.inv_c : 0.f;
+    s1 *= a.inv_c;
+    const __amdgpu_buffer_rsrc_t out =
+        buffer_rsrc(a.dx + (int64_t)base * C * kXB, min(a.rows - base, (uint32_t)kGroups) * (uint32_t)(C * kXB));
+#pragma unroll
+    for (int k = 0; k < kK; ++k) {
+#pragma unroll
+      for (int j = 0; j < kChunkCols; ++j) g[k][j] = st.y * fmaf(-s1, v[k][j], g[k][j] - s0);
+      if (live) at.template store<DTX, kVec>(g[k], out, (uint32_t)(group * C) * kXB, a.dx + (int64_t)r * C * kXB, k);
+    }
+  }
+  if (a.partial == nullptr) return;
+  float* const mine = a.partial + (int64_t)blockIdx.x * 2 * C;
+#pragma unroll
+  for (int which = 0; which < 2; ++which) {
+    float (&acc)[kK][kChunkCols] = which == 0 ? acc_w : acc_b;
+    if constexpr (kGroups > 1) {
+#pragma unroll
+      for (int k = 0; k < kK; ++k) {
+        *reinterpret_cast<float4*>(&s_acc[group * kCols + at.base(k, 0)]) = make_float4(acc[k][0], acc[k][1], acc[k][2], acc[k][3]);
+        *reinterpret_cast<float4*>(&s_acc[group * kCols + at.base(k, 1)]) = make_float4(acc[k][4], acc[k][5], acc[k][6], acc[k][7]);
+      }
+      __syncthreads();
+      for (int c = threadIdx.x; c < C; c += kThreads) {
+        float t = 0.f;
+#pragma unroll
+        for (int i = 0; i < kGroups; ++i) t += s_acc[i * kCols + c];
+        mine[which * C + c] = t;
+      }
+      __syncthreads();
+    } else {
+#pragma unroll
+      for (int k = 0; k < kK; ++k)
+#pragma unroll
+        for (int j = 0; j < kChunkCols; ++j) {
+          const int c = at.base(k, j >> 2) + (j & 3);
+          if (c < C) mine[which * C + c] = acc[k][j];
+        }
+    }
+  }
+}
+
 // ---- rows of any width, read again for each pass --------------------------------
 // A workgroup a row; what a pass reads again comes from L2.
 constexpr int kWideLanes = 512;
-
-template <int DTX, int DTY>
-constexpr int norm_pieces() { return DTX == TERRA_DTYPE_F32 || DTY == TERRA_DTYPE_F32 ? 4 : 8; }
 
 template <int DTX, int DTY, bool kVec>
 __global__ __launch_bounds__(kWideLanes) void norm_wide_kernel(const NormArgs a) {
@@ -134,15 +287,66 @@ __global__ __launch_bounds__(kSumLanes* kSumRows) void norm_columns_kernel(const
   }
 }
 
+// Row groups of a workgroup of the forward: few, so that workgroups that load and
+// such that compute are side by side, but enough for the parameters, 8 C bytes a workgroup,
+// to be a small part of what it reads.
+template <int DTX, int DTY, int kG, int kK, bool kVec, bool kPairs>
+void launch_norm(const NormArgs& a, hipStream_t s) {
+  constexpr uint32_t kGroups = tail_threads(kG) / kG, kTurns = kG > 64 ? 8 : (kG > 16 ? kG / 16 : 2);
+  const uint32_t need = (a.rows + kGroups - 1) / kGroups, blocks = (need + kTurns - 1) / kTurns;
+  constexpr uint32_t kMost = 1u << 22;  // a grid holds fewer than 2^32 threads
+  norm_kernel<DTX, DTY, kG, kK, kVec, kPairs><<<blocks < kMost ? blocks : kMost, tail_threads(kG), 0, s>>>(a);
+}
+
+template <int DTX, int DTY, int kG, int kK, bool kVec, bool kPairs>
+void launch_norm_bwd(const NormArgs& a, hipStream_t s) {
+  norm_bwd_kernel<DTX, DTY, kG, kK, kVec, kPairs><<<a.parts, tail_threads(kG), 0, s>>>(a);
+}
+
+#define TERRA_NORM_ROWS(f, g, k, ...)                                                        \
+  {                                                                                          \
+    if (vec) return f<DTX, DTY, g, k, true, false>(__VA_ARGS__);                             \
+    if constexpr (DTX != TERRA_DTYPE_F32 && DTY != TERRA_DTYPE_F32)                          \
+      if (pairs) return f<DTX, DTY, g, k, false, true>(__VA_ARGS__);                         \
+    return f<DTX, DTY, g, k, false, false>(__VA_ARGS__);                                     \
+  }
+// Calls f<DTX, DTY, lanes, chunks, kVec, kPairs>(...) for the shape of the call.
+#define TERRA_NORM_SHAPES(f, shape, ...)                                                     \
+  switch ((shape).lanes * 10 + (shape).chunks) {                                             \
+    case 81: TERRA_NORM_ROWS(f, 8, 1, __VA_ARGS__)                                           \
+    case 83: if constexpr (norm_pieces<DTX, DTY>() == 8) TERRA_NORM_ROWS(f, 8, 3, __VA_ARGS__) \
+    case 161: TERRA_NORM_ROWS(f, 16, 1, __VA_ARGS__)                                         \
+    case 162: TERRA_NORM_ROWS(f, 16, 2, __VA_ARGS__)                                         \
+    case 163: TERRA_NORM_ROWS(f, 16, 3, __VA_ARGS__)                                         \
+    case 322: TERRA_NORM_ROWS(f, 32, 2, __VA_ARGS__)                                         \
+    case 323: TERRA_NORM_ROWS(f, 32, 3, __VA_ARGS__)                                         \
+    case 642: TERRA_NORM_ROWS(f, 64, 2, __VA_ARGS__)                                         \
+    case 2561: TERRA_NORM_ROWS(f, 256, 1, __VA_ARGS__)                                       \
+    case 5121: TERRA_NORM_ROWS(f, 512, 1, __VA_ARGS__)                                       \
+    default: TERRA_NORM_ROWS(f, 512, 2, __VA_ARGS__)                                         \
+  }
+
 template <int DTX, int DTY>
-void norm_fwd(const NormArgs& a, const NormPlan&, bool vec, bool, hipStream_t s) {
+void held_fwd(const NormArgs& a, const NormPlan& p, bool vec, bool pairs, hipStream_t s) {
+  TERRA_NORM_SHAPES(launch_norm, p.shape, a, s)
+}
+
+template <int DTX, int DTY>
+void held_bwd(const NormArgs& a, const NormPlan& p, bool vec, bool pairs, hipStream_t s) {
+  TERRA_NORM_SHAPES(launch_norm_bwd, p.shape, a, s)
+}
+
+template <int DTX, int DTY>
+void norm_fwd(const NormArgs& a, const NormPlan& p, bool vec, bool pairs, hipStream_t s) {
+  if (p.held) return held_fwd<DTX, DTY>(a, p, vec, pairs, s);
   const uint32_t blocks = a.rows < (1u << 22) ? a.rows : 1u << 22;  // a grid holds fewer than 2^32 threads
   if (vec) norm_wide_kernel<DTX, DTY, true><<<blocks, kWideLanes, 0, s>>>(a);
   else norm_wide_kernel<DTX, DTY, false><<<blocks, kWideLanes, 0, s>>>(a);
 }
 
 template <int DTX, int DTY>
-void norm_bwd(const NormArgs& a, const NormPlan&, bool vec, bool, hipStream_t s) {
+void norm_bwd(const NormArgs& a, const NormPlan& p, bool vec, bool pairs, hipStream_t s) {
+  if (p.held) return held_bwd<DTX, DTY>(a, p, vec, pairs, s);
   const uint32_t blocks = a.rows < (1u << 22) ? a.rows : 1u << 22;
   if (a.dx != nullptr) {
     if (vec) norm_wide_bwd_kernel<DTX, DTY, true><<<blocks, kWideLanes, 0, s>>>(a);
