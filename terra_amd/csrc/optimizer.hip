@@ -15,7 +15,7 @@
 namespace terra {
 namespace {
 
-constexpr int kListed = 64;  // tensors of a launch: 48 bytes each, of 4 KB of arguments
+constexpr int kListed = 64;  // tensors of a launch: 56 bytes each, of 4 KB of arguments
 
 // Of the tensors whose chunks begin at start[0] <= start[1] <= ..., the one that holds `chunk`.
 __device__ __forceinline__ int tensor_of(const uint32_t* start, int count, uint32_t chunk) {
@@ -80,14 +80,17 @@ __device__ __forceinline__ void put_four(uint8_t* p, int64_t i, int n, const flo
 constexpr int kNormThreads = 256;
 constexpr int64_t kNormChunk = 16384;  // elements of a workgroup
 
+constexpr int kGradListed = 160;  // gradients of a launch: 21 bytes each
+
 struct GradList {
-  const uint8_t* data[kListed];
-  int64_t numel[kListed];
-  uint32_t start[kListed];
-  int32_t dtype[kListed];
+  const uint8_t* data[kGradListed];
+  int64_t numel[kGradListed];
+  uint32_t start[kGradListed];
+  uint8_t dtype[kGradListed];
   double* partials;
   int32_t count;
 };
+static_assert(sizeof(GradList) <= 4096, "arguments of a launch");
 
 __device__ __forceinline__ double wave_sum(double v) {
 #pragma unroll
@@ -95,26 +98,50 @@ __device__ __forceinline__ double wave_sum(double v) {
   return v;
 }
 
-// The thread's sum of squares of elements begin .. end - 1.
+// The thread's sum of squares of elements begin .. end - 1 (begin a multiple of kNormChunk).  Loads of
+// 16 bytes, kNormAhead of them before the first is used.
+constexpr int kNormAhead = 8;
+
 template <int DT>
 __device__ __forceinline__ double squares(const uint8_t* g, int64_t begin, int64_t end) {
-  double sum = 0.0;
-  const bool vec = (uintptr_t)g % (4 * ChunkElt<DT>::kBytes) == 0;
-  int64_t i = begin + threadIdx.x * 4;
-  if (vec)
-    for (; i + 4 <= end; i += kNormThreads * 4) {
-      float f[4];
-      four_values<DT, true>(g, i, 4, f);
+  constexpr int kB = ChunkElt<DT>::kBytes, kN = 16 / kB;
+  double sum[2] = {0.0, 0.0};
+  int64_t i = begin + threadIdx.x * kN;
+  if ((uintptr_t)g % 16 == 0) {
+    for (; i + (kNormAhead - 1) * kNormThreads * kN + kN <= end; i += kNormAhead * kNormThreads * kN) {
+      stream_u32x4 v[kNormAhead];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) sum = fma((double)f[j], (double)f[j], sum);
+      for (int u = 0; u < kNormAhead; ++u)
+        v[u] = __builtin_nontemporal_load(reinterpret_cast<const stream_u32x4*>(g + (i + u * kNormThreads * kN) * kB));
+#pragma unroll
+      for (int u = 0; u < kNormAhead; ++u) {
+        RowChunk<DT> r;
+        r.q[0] = v[u];
+#pragma unroll
+        for (int j = 0; j < kN; ++j) {
+          const double f = (double)chunk_value<DT>(r, j);
+          sum[j & 1] = fma(f, f, sum[j & 1]);
+        }
+      }
     }
-  for (; i < end; i += kNormThreads * 4) {
-    float f[4];
-    four_values<DT, false>(g, i, (int)(end - i < 4 ? end - i : 4), f);
+    for (; i + kN <= end; i += kNormThreads * kN) {
+      RowChunk<DT> r;
+      r.q[0] = *reinterpret_cast<const stream_u32x4*>(g + i * kB);
 #pragma unroll
-    for (int j = 0; j < 4; ++j) sum = fma((double)f[j], (double)f[j], sum);
+      for (int j = 0; j < kN; ++j) {
+        const double f = (double)chunk_value<DT>(r, j);
+        sum[j & 1] = fma(f, f, sum[j & 1]);
+      }
+    }
   }
-  return sum;
+  for (; i < end; i += kNormThreads * kN)
+#pragma unroll
+    for (int j = 0; j < kN; ++j)
+      if (i + j < end) {
+        const double f = (double)one_value<DT>(g, i + j);
+        sum[j & 1] = fma(f, f, sum[j & 1]);
+      }
+  return sum[0] + sum[1];
 }
 
 __global__ __launch_bounds__(kNormThreads) void gradient_norm_kernel(const GradList a) {
@@ -252,35 +279,44 @@ __global__ __launch_bounds__(kAdamThreads) void adamw_kernel(const AdamList a) {
 }
 
 // ---- moments in 8 bits ----------------------------------------------------------
-// In 64 bits up to the codes: a value next to the border of two codes goes to
-// the one that the formula says.
+// The moments in 64 bits: the first one's terms may cancel, the second's squares
+// leave the range of 32 (gradients below 10^-19).  From there on in 32 bits.
 
-__device__ __forceinline__ uint32_t fp8_code(float v) { return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(v, 0.f, 0, false) & 0xffu; }
-__device__ __forceinline__ float fp8_value(uint32_t code) { return __builtin_amdgcn_cvt_f32_fp8((int)code, 0); }
-
-// y (at most 448 and a little in size) to the nearest code of e4m3. Rounded to 32
-// bits towards odd first, so that the second rounding sees on which side of a border it is.
-__device__ __forceinline__ uint32_t nearest_code(double y) {
-  if (y != y) return 0x7fu;
-  float f = (float)y;
-  const double back = (double)f;
-  uint32_t b = __float_as_uint(f);
-  if (back != y && (b & 1u) == 0) b += (fabs(back) > fabs(y)) ? ~0u : 1u;  // to the odd neighbour on y's side
-  f = __uint_as_float(b);
-  f = fminf(fmaxf(f, -448.f), 448.f);
-  return fp8_code(f);
+// The largest of a 32-bit number over the wave's lanes (every lane ends with it).
+__device__ __forceinline__ uint32_t wave_largest(uint32_t v) {
+  v = max(v, (uint32_t)__builtin_amdgcn_mov_dpp((int)v, 0xb1, 0xf, 0xf, false));   // lane ^ 1
+  v = max(v, (uint32_t)__builtin_amdgcn_mov_dpp((int)v, 0x4e, 0xf, 0xf, false));   // lane ^ 2
+  v = max(v, (uint32_t)__builtin_amdgcn_mov_dpp((int)v, 0x141, 0xf, 0xf, false));  // the other quad of eight
+  v = max(v, (uint32_t)__builtin_amdgcn_mov_dpp((int)v, 0x128, 0xf, 0xf, false));  // the other eight of a row
+  auto p = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+  v = max(p[0], p[1]);
+  p = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+  return max(p[0], p[1]);
 }
 
-// w = v / scale^2: one of the codes next to its root, see terra_swin_adamw.
-__device__ __forceinline__ uint32_t root_code(double w, uint32_t draw) {
-  if (!(w > 0.0)) return 0u;
-  const float r = fminf(sqrtf((float)w), 448.f);
-  const int exponent = max((int)(__float_as_uint(r) >> 23) - 127, -6);
-  const float grid = __uint_as_float((uint32_t)(exponent - 3 + 127) << 23);
-  const float low = floorf(r / grid) * grid, high = low + grid;
-  const double span = (double)high * high - (double)low * low;
-  const bool up = w - (double)low * low > ((double)draw + 0.5) * (1.0 / 65536.0) * span && low < 448.f;
-  return fp8_code(fmaxf(up ? high : low, 0.001953125f));
+// Four e4m3 codes of values of at most 448 in size.
+__device__ __forceinline__ uint32_t fp8_codes(const float (&f)[4]) {
+  const int lo = __builtin_amdgcn_cvt_pk_fp8_f32(f[0], f[1], 0, false);
+  return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(f[2], f[3], lo, true);
+}
+template <int kJ>
+__device__ __forceinline__ float fp8_value(uint32_t codes) { return __builtin_amdgcn_cvt_f32_fp8((int)codes, kJ); }
+
+constexpr float kLargestCode = 448.f, kSmallestCode = 0.001953125f, kSmallestNormal = 0.015625f;
+
+// A value on one of the two codes next to r > 0 (at most 448 and a rounding): of low <= r < high the
+// upper one where r^2 - low^2 > u (high^2 - low^2).  Squares of codes are exact.
+__device__ __forceinline__ float root_code(float r, uint32_t draw) {
+  r = fminf(r, kLargestCode);
+  const uint32_t bits = __float_as_uint(r);
+  const float fine = floorf(r * 512.f);
+  const bool normal = r >= kSmallestNormal;
+  const float low = normal ? __uint_as_float(bits & 0xfff00000u) : fine * kSmallestCode;
+  const float high = normal ? __uint_as_float((bits & 0xfff00000u) + 0x100000u) : (fine + 1.f) * kSmallestCode;
+  const float l2 = low * low, span = fmaf(high, high, -l2);
+  const float u = fmaf((float)draw, 1.f / 65536.f, 0.5f / 65536.f);
+  const float v = fmaf(r, r, -l2) > u * span ? high : low;
+  return fminf(fmaxf(v, kSmallestCode), kLargestCode);
 }
 
 __device__ __forceinline__ ChunkDraws adam_draws(uint64_t seed, uint32_t chunk, uint32_t tensor, uint32_t step, uint32_t stream) {
@@ -299,7 +335,56 @@ __device__ __forceinline__ ChunkDraws adam_draws(uint64_t seed, uint32_t chunk, 
   return {{c0, c1, c2, c3}};
 }
 
-// A wave takes blocks of 256 elements, four a lane.
+// The value of lane `from` (the same in all lanes) of a 64-bit number.
+__device__ __forceinline__ double lane_value(double v, int from) {
+  const uint64_t b = (uint64_t)__double_as_longlong(v);
+  const uint32_t lo = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)b, from), hi = (uint32_t)__builtin_amdgcn_readlane((int)(b >> 32), from);
+  return __longlong_as_double((long long)(((uint64_t)hi << 32) | lo));
+}
+
+// Four elements of a lane.
+struct AdamFour {
+  float p[4], g[4];
+  uint32_t first, second;  // codes
+
+  template <int DTP, int DTG>
+  __device__ __forceinline__ void load(const AdamEntry& e, int64_t i, int n, bool whole) {
+    if (whole) {
+      four_values<DTP, true>(e.param, i, 4, p);
+      four_values<DTG, true>(e.grad, i, 4, g);
+      first = __builtin_nontemporal_load(reinterpret_cast<const uint32_t*>(e.first + i));
+      second = __builtin_nontemporal_load(reinterpret_cast<const uint32_t*>(e.second + i));
+    } else {
+      four_values<DTP, false>(e.param, i, n, p);
+      four_values<DTG, false>(e.grad, i, n, g);
+      first = second = 0;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        first |= j < n ? (uint32_t)e.first[i + j] << (8 * j) : 0u;
+        second |= j < n ? (uint32_t)e.second[i + j] << (8 * j) : 0u;
+      }
+    }
+  }
+  template <int DTP>
+  __device__ __forceinline__ void store(const AdamEntry& e, int64_t i, int n, bool whole) const {
+    if (whole) {
+      put_four<DTP, true>(e.param, i, 4, p);
+      __builtin_nontemporal_store(first, reinterpret_cast<uint32_t*>(e.first + i));
+      __builtin_nontemporal_store(second, reinterpret_cast<uint32_t*>(e.second + i));
+    } else {
+      put_four<DTP, false>(e.param, i, n, p);
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (j < n) {
+          e.first[i + j] = (uint8_t)(first >> (8 * j));
+          e.second[i + j] = (uint8_t)(second >> (8 * j));
+        }
+    }
+  }
+};
+
+// A wave takes two blocks of 256 elements at a time, four of each a lane: neighbouring lanes
+// then hold the halves of two chunks of eight and share their draws, as in half_draws.
 template <int DTP, int DTG>
 __global__ __launch_bounds__(kAdamThreads) void adamw_8bit_kernel(const AdamList a) {
   if (a.found_inf != nullptr && *a.found_inf != 0.f) return;
@@ -307,86 +392,85 @@ __global__ __launch_bounds__(kAdamThreads) void adamw_8bit_kernel(const AdamList
   const AdamEntry e = a.tensor[t];
   const AdamStep st(a);
   const uint64_t seed = *a.seed;
-  const double factor = (double)st.factor, b1 = a.beta1, c1 = 1.0 - a.beta1, b2 = a.beta2, c2 = 1.0 - a.beta2;
+  const double c1 = (1.0 - a.beta1) * (double)st.factor, c2 = (1.0 - a.beta2) * (double)st.factor * (double)st.factor;
+  const float root = sqrtf(st.root);
   const int64_t blocks = (e.numel + kScaled - 1) / kScaled;
   const int64_t begin = (int64_t)(blockIdx.x - a.start[t]) * (kAdamChunk / kScaled);
   const int64_t end = begin + kAdamChunk / kScaled < blocks ? begin + kAdamChunk / kScaled : blocks;
   const int lane = threadIdx.x & 63;
   const bool vec = (uintptr_t)e.param % (4 * ChunkElt<DTP>::kBytes) == 0 && (uintptr_t)e.grad % (4 * ChunkElt<DTG>::kBytes) == 0 &&
                    ((uintptr_t)e.first | (uintptr_t)e.second) % 4 == 0;
-  for (int64_t b = begin + (threadIdx.x >> 6); b < end; b += kAdamThreads / 64) {
-    const int64_t i = b * kScaled + lane * 4, left = e.numel - i;
-    const int n = left >= 4 ? 4 : left > 0 ? (int)left : 0;
-    const bool whole = vec && n == 4;
-    float p[4], g[4];
-    uint32_t mc = 0, rc = 0;
-    if (whole) {
-      four_values<DTP, true>(e.param, i, 4, p);
-      four_values<DTG, true>(e.grad, i, 4, g);
-      mc = *reinterpret_cast<const uint32_t*>(e.first + i);
-      rc = *reinterpret_cast<const uint32_t*>(e.second + i);
-    } else {
-      four_values<DTP, false>(e.param, i, n, p);
-      four_values<DTG, false>(e.grad, i, n, g);
+  for (int64_t b = begin + 2 * (threadIdx.x >> 6); b < end; b += 2 * (kAdamThreads / 64)) {
+    AdamFour q[2];
+    int n[2];
+    double scale_m[2], scale_r[2];
+    const bool whole = vec && (b + 2) * kScaled <= e.numel;
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      const int64_t i = (b + k) * kScaled + lane * 4, left = e.numel - i;
+      n[k] = left >= 4 ? 4 : left > 0 ? (int)left : 0;
+      q[k].template load<DTP, DTG>(e, i, n[k], whole);
+      const bool there = b + k < end;
+      scale_m[k] = there ? (double)e.scales[b + k] : 0.0;
+      scale_r[k] = there ? (double)e.scales[blocks + b + k] : 0.0;
+    }
+    double m[2][4];
+    float r[2][4];
+    uint32_t big_m[2], big_r[2];
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      const float fm[4] = {fp8_value<0>(q[k].first), fp8_value<1>(q[k].first), fp8_value<2>(q[k].first), fp8_value<3>(q[k].first)};
+      const float fr[4] = {fp8_value<0>(q[k].second), fp8_value<1>(q[k].second), fp8_value<2>(q[k].second), fp8_value<3>(q[k].second)};
+      const double dm = a.beta1 * scale_m[k], dv = a.beta2 * scale_r[k] * scale_r[k];
+      double v[4];
+      bool far = false;
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        mc |= j < n ? (uint32_t)e.first[i + j] << (8 * j) : 0u;
-        rc |= j < n ? (uint32_t)e.second[i + j] << (8 * j) : 0u;
+        const double g = (double)q[k].g[j];
+        m[k][j] = fma((double)fm[j], dm, c1 * g);
+        v[j] = fma((double)(fr[j] * fr[j]), dv, c2 * g * g);
+        far |= v[j] != 0.0 && !(v[j] >= 0x1p-100 && v[j] <= 0x1p+120);
+        r[k][j] = __builtin_amdgcn_sqrtf((float)v[j]);
       }
-    }
-    const double sm = (double)e.scales[b], sr = (double)e.scales[blocks + b];
-    double m[4], v[4];
+      if (__builtin_amdgcn_ballot_w64(far) != 0)
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const double d = (double)g[j] * factor;
-      const double r = (double)fp8_value((rc >> (8 * j)) & 0xffu) * sr;
-      m[j] = b1 * ((double)fp8_value((mc >> (8 * j)) & 0xffu) * sm) + c1 * d;
-      v[j] = b2 * (r * r) + c2 * (d * d);
-      p[j] = st.updated(p[j], (float)m[j], (float)v[j]);
-    }
-    // The scales: 32-bit roundings of the largest values, which are taken in 64.  With an infinity or a NaN
-    // the scale is infinite, and all of the block NaN when it is read again.
-    double big_m = 0.0, big_v = 0.0;
+        for (int j = 0; j < 4; ++j) r[k][j] = (float)sqrt(v[j]);
+      big_m[k] = big_r[k] = 0;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      big_m = fmax(big_m, fabs(m[j]));
-      big_v = fmax(big_v, v[j]);
-      if (!(fabs(m[j]) <= 1.7976931348623157e308)) big_m = __builtin_inf();
-      if (!(v[j] <= 1.7976931348623157e308)) big_v = __builtin_inf();
+      for (int j = 0; j < 4; ++j) {
+        const float m32 = (float)m[k][j];
+        q[k].p[j] = q[k].p[j] * st.keep - st.rate * (m32 / fmaf(r[k][j], root, st.eps));
+        big_m[k] = max(big_m[k], __float_as_uint(m32) & 0x7fffffffu);  // NaN above infinity above the others
+        big_r[k] = max(big_r[k], __float_as_uint(r[k][j]) & 0x7fffffffu);
+      }
+      big_m[k] = wave_largest(big_m[k]);
+      big_r[k] = wave_largest(big_r[k]);
     }
+    // The scales, and their reciprocals: each of the four in the lanes of its number.  With an infinity or a NaN the scale is
+    // infinite, and all of the block NaN when it is read again.
+    const uint32_t big = lane & 2 ? (lane & 1 ? big_r[1] : big_m[1]) : (lane & 1 ? big_r[0] : big_m[0]);
+    const float scale = big >= 0x7f800000u ? __builtin_inff() : __uint_as_float(big) / kLargestCode;
+    const double inverse = scale > 0.f ? 1.0 / (double)scale : 0.0;
+    // The even lane's draws are of the first block's chunk, the odd one's of the second's.
+    const uint32_t pair = (uint32_t)(b * (kScaled / 8)) + (uint32_t)(lane >> 1);
+    const ChunkDraws d = adam_draws(seed, pair + (lane & 1) * (kScaled / 8), a.index[t], st.step, a.stream);
+    const uint32_t other0 = lane_xor1(lane & 1 ? d.w[0] : d.w[2]), other1 = lane_xor1(lane & 1 ? d.w[1] : d.w[3]);
+    const uint32_t w[2][2] = {{lane & 1 ? other0 : d.w[0], lane & 1 ? other1 : d.w[1]}, {lane & 1 ? d.w[2] : other0, lane & 1 ? d.w[3] : other1}};
 #pragma unroll
-    for (int d = 32; d > 0; d /= 2) {
-      big_m = fmax(big_m, __shfl_xor(big_m, d));
-      big_v = fmax(big_v, __shfl_xor(big_v, d));
-    }
-    const float new_m = (float)(big_m / 448.0), new_r = (float)(sqrt(big_v) / 448.0);
-    const double inv_m = new_m > 0.f ? 1.0 / (double)new_m : 0.0, inv_r = new_r > 0.f ? 1.0 / (double)new_r : 0.0;
-    const uint32_t chunk = (uint32_t)(i >> 3);
-    const ChunkDraws dr = adam_draws(seed, chunk, a.index[t], st.step, a.stream);
-    uint32_t out_m = 0, out_r = 0;
+    for (int k = 0; k < 2; ++k) {
+      const double inv_m = lane_value(inverse, 2 * k), inv_r = lane_value(inverse, 2 * k + 1);
+      float y[4], z[4];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const uint32_t w = lane & 1 ? dr.w[2 + (j >> 1)] : dr.w[j >> 1];
-      out_m |= nearest_code(m[j] * inv_m) << (8 * j);
-      out_r |= root_code(v[j] * inv_r * inv_r, j & 1 ? w >> 16 : w & 0xffffu) << (8 * j);
+      for (int j = 0; j < 4; ++j) {
+        y[j] = __builtin_amdgcn_fmed3f((float)(m[k][j] * inv_m), -kLargestCode, kLargestCode);
+        const float part = (float)((double)r[k][j] * inv_r);
+        z[j] = part > 0.f ? root_code(part, j & 1 ? w[k][j >> 1] >> 16 : w[k][j >> 1] & 0xffffu) : 0.f;
+      }
+      q[k].first = fp8_codes(y);
+      q[k].second = fp8_codes(z);
+      q[k].template store<DTP>(e, (b + k) * kScaled + lane * 4, n[k], whole);
     }
-    if (whole) {
-      put_four<DTP, true>(e.param, i, 4, p);
-      *reinterpret_cast<uint32_t*>(e.first + i) = out_m;
-      *reinterpret_cast<uint32_t*>(e.second + i) = out_r;
-    } else {
-      put_four<DTP, false>(e.param, i, n, p);
-#pragma unroll
-      for (int j = 0; j < 4; ++j)
-        if (j < n) {
-          e.first[i + j] = (uint8_t)(out_m >> (8 * j));
-          e.second[i + j] = (uint8_t)(out_r >> (8 * j));
-        }
-    }
-    if (lane == 0) {
-      e.scales[b] = new_m;
-      e.scales[blocks + b] = new_r;
-    }
+    if (lane < 4 && b + (lane >> 1) < end) e.scales[(lane & 1 ? blocks : 0) + b + (lane >> 1)] = scale;
   }
 }
 
@@ -580,10 +664,10 @@ extern "C" int terra_swin_gradient_norm(const terra_swin_tensor* grads, int coun
   for (int i = 0; i < count; ++i) {
     if (grads[i].numel == 0) continue;
     const uint32_t more = (uint32_t)((grads[i].numel + kNormChunk - 1) / kNormChunk);
-    if (a.count == kListed || chunks + more > kMostChunks) launch();
+    if (a.count == kGradListed || chunks + more > kMostChunks) launch();
     a.data[a.count] = (const uint8_t*)grads[i].data;
     a.numel[a.count] = grads[i].numel;
-    a.dtype[a.count] = grads[i].dtype;
+    a.dtype[a.count] = (uint8_t)grads[i].dtype;
     a.start[a.count++] = chunks;
     chunks += more;
   }

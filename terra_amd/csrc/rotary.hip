@@ -56,7 +56,7 @@ struct RotaryRun {
   __device__ __forceinline__ void load(const uint8_t* p) {
     if constexpr (kAligned) {
       typedef Elt vec __attribute__((ext_vector_type(kN)));
-      const vec t = *reinterpret_cast<const vec*>(p);
+      const vec t = __builtin_nontemporal_load(reinterpret_cast<const vec*>(p));
 #pragma unroll
       for (int i = 0; i < kN; ++i) v[i] = t[i];
     } else {
@@ -70,7 +70,7 @@ struct RotaryRun {
       vec t;
 #pragma unroll
       for (int i = 0; i < kN; ++i) t[i] = v[i];
-      *reinterpret_cast<vec*>(p) = t;
+      __builtin_nontemporal_store(t, reinterpret_cast<vec*>(p));
     } else {
 #pragma unroll
       for (int i = 0; i < kN; ++i) reinterpret_cast<Elt*>(p)[i] = v[i];
@@ -84,6 +84,7 @@ constexpr int kRotaryThreads = 256;
 template <int DT, int kP, bool kInterleaved, bool kAligned>
 __global__ __launch_bounds__(kRotaryThreads) void rotary_kernel(const RotaryArgs a) {
   constexpr int kB = ChunkElt<DT>::kBytes, kRun = kInterleaved ? 2 * kP : kP, kCopy = kAligned ? kRun : 1;
+  constexpr int kAhead = 4;
   typedef RotaryRun<DT, kRun, kAligned> Run;
   const int first = blockIdx.y * a.per_thread, last = min(first + a.per_thread, a.heads);
   uint32_t local, lane;
@@ -97,10 +98,13 @@ __global__ __launch_bounds__(kRotaryThreads) void rotary_kernel(const RotaryArgs
     uint8_t* y = a.y + (int64_t)outer * a.y_outer + (int64_t)inner * a.y_inner + (int64_t)first * a.y_head;
     if (at >= a.turned) {
       const int64_t off = ((int64_t)2 * a.half + (int64_t)(at - a.turned) * kCopy) * kB;
-      for (int h = first; h < last; ++h, x += a.x_head, y += a.y_head) {
-        RotaryRun<DT, kCopy, kAligned> r;
-        r.load(x + off);
-        r.store(y + off);
+      for (int h = first; h < last; h += kAhead, x += kAhead * a.x_head, y += kAhead * a.y_head) {
+        RotaryRun<DT, kCopy, kAligned> r[kAhead];
+#pragma unroll
+        for (int k = 0; k < kAhead; ++k) r[k].load(x + (h + k < last ? k : 0) * a.x_head + off);
+#pragma unroll
+        for (int k = 0; k < kAhead; ++k)
+          if (h + k < last) r[k].store(y + k * a.y_head + off);
       }
       continue;
     }
@@ -121,29 +125,29 @@ __global__ __launch_bounds__(kRotaryThreads) void rotary_kernel(const RotaryArgs
       s[i] = a.amplitude * a.sign * sn;
     }
     const int64_t lo = (int64_t)at * kRun * kB, hi = lo + (int64_t)a.half * kB;
-    for (int h = first; h < last; ++h, x += a.x_head, y += a.y_head) {
-      if constexpr (kInterleaved) {
-        Run r;
-        r.load(x + lo);
+    // Heads kAhead at a time, all read before the first is written.
+    for (int h = first; h < last; h += kAhead, x += kAhead * a.x_head, y += kAhead * a.y_head) {
+      Run p[kAhead], q[kInterleaved ? 1 : kAhead];
+#pragma unroll
+      for (int k = 0; k < kAhead; ++k) {
+        const uint8_t* xh = x + (h + k < last ? k : 0) * a.x_head;
+        p[k].load(xh + lo);
+        if constexpr (!kInterleaved) q[k].load(xh + hi);
+      }
+#pragma unroll
+      for (int k = 0; k < kAhead; ++k) {
+        if (h + k >= last) break;
+        uint8_t* yh = y + k * a.y_head;
 #pragma unroll
         for (int i = 0; i < kP; ++i) {
-          const float u = rotary_value<DT>(r.v[2 * i]), v = rotary_value<DT>(r.v[2 * i + 1]);
-          r.v[2 * i] = rotary_round<DT>(u * c[i] - v * s[i]);
-          r.v[2 * i + 1] = rotary_round<DT>(u * s[i] + v * c[i]);
+          auto& eu = kInterleaved ? p[k].v[kInterleaved ? 2 * i : 0] : p[k].v[i];
+          auto& ev = kInterleaved ? p[k].v[kInterleaved ? 2 * i + 1 : 0] : q[kInterleaved ? 0 : k].v[i];
+          const float u = rotary_value<DT>(eu), v = rotary_value<DT>(ev);
+          eu = rotary_round<DT>(u * c[i] - v * s[i]);
+          ev = rotary_round<DT>(u * s[i] + v * c[i]);
         }
-        r.store(y + lo);
-      } else {
-        Run p, q;
-        p.load(x + lo);
-        q.load(x + hi);
-#pragma unroll
-        for (int i = 0; i < kP; ++i) {
-          const float u = rotary_value<DT>(p.v[i]), v = rotary_value<DT>(q.v[i]);
-          p.v[i] = rotary_round<DT>(u * c[i] - v * s[i]);
-          q.v[i] = rotary_round<DT>(u * s[i] + v * c[i]);
-        }
-        p.store(y + lo);
-        q.store(y + hi);
+        p[k].store(yh + lo);
+        if constexpr (!kInterleaved) q[k].store(yh + hi);
       }
     }
   }

@@ -6,9 +6,11 @@ Moments in 32 bits: g times the factor, the two products and their sum, and the
 betas as fp32 numbers, 4 u of the terms' magnitudes, 6 u for the second moment's square.  The
 parameter: 3 u of itself (its factor's rounding, the product, the difference), of what is taken off 12 u (root, quotient,
 rate, and half of the second moment's 6 u) and the first moment's error in it, and half a step of its type.
-In 8 bits everything up to the codes is computed in 64, so scales are off by one rounding, 2 u
-(the 64-bit value may lie on either side of a border of 32-bit ones), and codes are the oracle's
-except where the oracle's value is within 1e-9 of the border of two codes, or of the draw's threshold.
+In 8 bits the moments are computed in 64 and then rounded to 32: the first one's scale is off by that and a
+division, 2 u; the root by half the rounding of its square and an ulp (2 u), with the division 4 u.  Codes are
+the oracle's except where the oracle's value is within a rounding to 32 bits (2 u) of the border of two
+codes; or within 40 u of its draw's threshold: the root over its scale is off by 4 u, its square by 8 u of high^2, which is
+at most 4.8 times high^2 - low^2 (low / high <= 8 / 9).
 """
 import pytest
 import torch
@@ -250,15 +252,15 @@ def check_step_8bit(p_after, m_after, before, m_before, g, step, seed, index, fa
     top = torch.zeros(2, blocks, dtype=torch.float64).scatter_reduce_(1, block.expand(2, n), torch.stack((m.abs(), v)), "amax")
     top[1] = top[1].sqrt()
     scales = m_after.scales.double()
-    assert bool(((scales - top / 448).abs() <= 2 * U * top / 448 + 1e-44).all())
+    assert bool(((scales - top / 448).abs() <= torch.tensor([[2.0], [4.0]]).double() * U * top / 448 + 1e-44).all())
     inv = torch.where(scales > 0, 1 / scales, torch.zeros_like(scales))
     code, near = tr.nearest_code((m * inv[0][block]).clamp(-448, 448))
     same = code == _codes(m_after.exp_avg)
     zero = (code % 128 == 0) & (_codes(m_after.exp_avg) % 128 == 0)  # of either sign
-    assert bool((same | zero | (near < 1e-9)).all())
+    assert bool((same | zero | (near < 2 * U)).all())
     code, near = tr.root_code(v * inv[1][block].square(), tr.draws(seed, n, index, step, stream))
     same = code == _codes(m_after.exp_avg_sq)
-    assert bool((same | (near < 1e-9)).all())
+    assert bool((same | (near < 40 * U)).all())
     assert int((~same).sum()) <= n // 1000
 
 
