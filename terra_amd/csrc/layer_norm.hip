@@ -69,21 +69,30 @@ bool norm_meet(const void* p, int64_t bytes, const void* q, int64_t more) {
 
 constexpr int kNormHeld = 8192;  // channels of rows that are held in registers
 
-// How many lanes and chunks hold a row, as tail_shape; eight lanes also where a row has at most
-// eight chunks (the heads of a packed q | k | v).
-TailShape norm_shape(int C, bool pieces, int most) {
-  if (C <= 8 * kChunkCols) return {8, 1};
-  return tail_shape(C, pieces, most);
+// How many lanes and chunks hold a row.  Waves rather than workgroups as far as the registers
+// go: what its lanes add up needs no barrier (39168 x 4096 bf16, forward: 118 us, as 512 lanes
+// of one chunk 135; 78336 x 2048: 108 and 143).  The backward, with two sums for each column
+// and two rows, goes so far as four chunks (78336 x 2048: 156 us, as 256 lanes 167; 39168 x 4096 as
+// 256 lanes of two 161, as waves of eight 175); rows that are not aligned or that have fp32 in them as far as two
+// where a few lanes hold them.  Eight lanes where a row has at most eight chunks: the heads of a packed q | k | v.
+TailShape norm_shape(int C, bool pieces, bool vec, bool backward) {
+  const int n = (C + kChunkCols - 1) / kChunkCols;
+  if (n <= 8) return {8, 1};
+  if (n > 512) return {512, 2};
+  if (n > 256) return backward ? TailShape{256, 2} : TailShape{64, 8};
+  if (n > 128) return {64, 4};
+  return tail_shape(C, pieces, backward && (pieces || !vec) ? 2 : 3);
 }
 
-// Workgroups of the sums over rows: what fits the 256 compute units at once, or as many as have rows.
+// Workgroups of the sums over rows, at most what fits the 256 compute units at once (524288 x 192
+// bf16: 512 workgroups 84 us, 1024 93; with four chunks a lane one wave a SIMD does).
 NormPlan norm_plan(uint32_t rows, int C, bool pieces, bool vec, bool backward) {
   NormPlan p = {};
   p.held = C <= kNormHeld;
   if (p.held) {
-    p.shape = norm_shape(C, pieces, backward && (pieces || !vec) ? 2 : 3);
+    p.shape = norm_shape(C, pieces, vec, backward);
     const uint32_t groups = (uint32_t)(tail_threads(p.shape.lanes) / p.shape.lanes), useful = (rows + groups - 1) / groups;
-    const uint32_t most = p.shape.lanes > 256 ? 1024u / (uint32_t)p.shape.chunks : 1024u;
+    const uint32_t most = p.shape.chunks >= 4 ? 256u : p.shape.lanes <= 16 && p.shape.chunks == 1 ? 1024u : 512u;
     p.parts = useful < most ? useful : most;
     return p;
   }

@@ -292,7 +292,7 @@ __global__ __launch_bounds__(kSumLanes* kSumRows) void norm_columns_kernel(const
 // to be a small part of what it reads.
 template <int DTX, int DTY, int kG, int kK, bool kVec, bool kPairs>
 void launch_norm(const NormArgs& a, hipStream_t s) {
-  constexpr uint32_t kGroups = tail_threads(kG) / kG, kTurns = kG > 64 ? 8 : (kG > 16 ? kG / 16 : 2);
+  constexpr uint32_t kGroups = tail_threads(kG) / kG, kTurns = kG > 64 ? 16 : (kG > 16 ? 4 : 2);
   const uint32_t need = (a.rows + kGroups - 1) / kGroups, blocks = (need + kTurns - 1) / kTurns;
   constexpr uint32_t kMost = 1u << 22;  // a grid holds fewer than 2^32 threads
   norm_kernel<DTX, DTY, kG, kK, kVec, kPairs><<<blocks < kMost ? blocks : kMost, tail_threads(kG), 0, s>>>(a);
@@ -310,8 +310,8 @@ void launch_norm_bwd(const NormArgs& a, hipStream_t s) {
       if (pairs) return f<DTX, DTY, g, k, false, true>(__VA_ARGS__);                         \
     return f<DTX, DTY, g, k, false, false>(__VA_ARGS__);                                     \
   }
-// Calls f<DTX, DTY, lanes, chunks, kVec, kPairs>(...) for the shape of the call.
-#define TERRA_NORM_SHAPES(f, shape, ...)                                                     \
+// Calls f<DTX, DTY, lanes, chunks, kVec, kPairs>(...) for the shape of the call; wide: that of 2049 to 4096 channels.
+#define TERRA_NORM_SHAPES(f, shape, wide, ...)                                                   \
   switch ((shape).lanes * 10 + (shape).chunks) {                                             \
     case 81: TERRA_NORM_ROWS(f, 8, 1, __VA_ARGS__)                                           \
     case 83: if constexpr (norm_pieces<DTX, DTY>() == 8) TERRA_NORM_ROWS(f, 8, 3, __VA_ARGS__) \
@@ -321,19 +321,19 @@ void launch_norm_bwd(const NormArgs& a, hipStream_t s) {
     case 322: TERRA_NORM_ROWS(f, 32, 2, __VA_ARGS__)                                         \
     case 323: TERRA_NORM_ROWS(f, 32, 3, __VA_ARGS__)                                         \
     case 642: TERRA_NORM_ROWS(f, 64, 2, __VA_ARGS__)                                         \
-    case 2561: TERRA_NORM_ROWS(f, 256, 1, __VA_ARGS__)                                       \
-    case 5121: TERRA_NORM_ROWS(f, 512, 1, __VA_ARGS__)                                       \
+    case 644: TERRA_NORM_ROWS(f, 64, 4, __VA_ARGS__)                                         \
+    case wide: TERRA_NORM_ROWS(f, wide / 10, wide % 10, __VA_ARGS__)                         \
     default: TERRA_NORM_ROWS(f, 512, 2, __VA_ARGS__)                                         \
   }
 
 template <int DTX, int DTY>
 void held_fwd(const NormArgs& a, const NormPlan& p, bool vec, bool pairs, hipStream_t s) {
-  TERRA_NORM_SHAPES(launch_norm, p.shape, a, s)
+  TERRA_NORM_SHAPES(launch_norm, p.shape, 648, a, s)
 }
 
 template <int DTX, int DTY>
 void held_bwd(const NormArgs& a, const NormPlan& p, bool vec, bool pairs, hipStream_t s) {
-  TERRA_NORM_SHAPES(launch_norm_bwd, p.shape, a, s)
+  TERRA_NORM_SHAPES(launch_norm_bwd, p.shape, 2562, a, s)
 }
 
 template <int DTX, int DTY>

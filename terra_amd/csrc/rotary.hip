@@ -23,141 +23,195 @@ struct RotaryArgs {
   const void* positions;
   const double* turns;
   int64_t x_outer, x_inner, x_head, y_outer, y_inner, y_head;  // bytes
-  FastDiv inner, position_tokens, lanes;  // lanes: threads of a token
+  FastDiv inner, position_tokens, lanes, per_axis;  // lanes: threads of a token
   uint32_t tokens, per_block;             // tokens of a workgroup
+  uint32_t y_span;                        // bytes from a workgroup's first token of y to its end, 0: not at one stride
   int32_t turned, items;                  // items of a token that are rotated, and all
   int32_t heads, per_thread;              // heads, of which a thread takes this many
-  int32_t half;                           // dim / 2
-  int32_t axes, per_axis;
+  int32_t half, rest;                     // dim / 2, elements that are copied
+  int32_t axes;
   int32_t wide_positions;                 // 64-bit positions
   float amplitude, sign;
 };
 
-template <int DT> struct RotaryElt { typedef uint16_t type; };
-template <> struct RotaryElt<TERRA_DTYPE_F32> { typedef uint32_t type; };
-
-template <int DT>
-__device__ __forceinline__ float rotary_value(typename RotaryElt<DT>::type v) {
-  if constexpr (DT == TERRA_DTYPE_F32) return __uint_as_float(v);
-  else if constexpr (DT == TERRA_DTYPE_BF16) return bf16_bits_to_f32(v);
-  else return __half2float(__ushort_as_half(v));
-}
-template <int DT>
-__device__ __forceinline__ typename RotaryElt<DT>::type rotary_round(float v) {
-  if constexpr (DT == TERRA_DTYPE_F32) return __float_as_uint(v);
-  else return (uint16_t)pack2<DT>(v, 0.f);
-}
-
-// kN elements that lie side by side, read or written as one access where aligned (kN elements of alignment).
+// kN elements that lie side by side, one access where aligned (to all of them).
 template <int DT, int kN, bool kAligned>
 struct RotaryRun {
-  typedef typename RotaryElt<DT>::type Elt;
-  Elt v[kN];
+  static constexpr int kB = ChunkElt<DT>::kBytes, kWords = (kN * kB + 3) / 4;
+  typedef uint32_t Vec __attribute__((ext_vector_type(kWords)));
+  uint32_t w[kWords];
+
   __device__ __forceinline__ void load(const uint8_t* p) {
     if constexpr (kAligned) {
-      typedef Elt vec __attribute__((ext_vector_type(kN)));
-      const vec t = __builtin_nontemporal_load(reinterpret_cast<const vec*>(p));
+      if constexpr (kWords == 1) {
+        w[0] = __builtin_nontemporal_load(reinterpret_cast<const uint32_t*>(p));
+      } else {
+        const Vec v = __builtin_nontemporal_load(reinterpret_cast<const Vec*>(p));
 #pragma unroll
-      for (int i = 0; i < kN; ++i) v[i] = t[i];
+        for (int i = 0; i < kWords; ++i) w[i] = v[i];
+      }
+    } else if constexpr (kB == 4) {
+#pragma unroll
+      for (int i = 0; i < kWords; ++i) w[i] = reinterpret_cast<const uint32_t*>(p)[i];
     } else {
+      const uint16_t* h = reinterpret_cast<const uint16_t*>(p);
 #pragma unroll
-      for (int i = 0; i < kN; ++i) v[i] = reinterpret_cast<const Elt*>(p)[i];
+      for (int i = 0; i < kWords; ++i) w[i] = (uint32_t)h[2 * i] | (2 * i + 1 < kN ? (uint32_t)h[2 * i + 1] << 16 : 0u);
     }
   }
   __device__ __forceinline__ void store(uint8_t* p) const {
     if constexpr (kAligned) {
-      typedef Elt vec __attribute__((ext_vector_type(kN)));
-      vec t;
+      if constexpr (kWords == 1) {
+        __builtin_nontemporal_store(w[0], reinterpret_cast<uint32_t*>(p));
+      } else {
+        Vec v;
 #pragma unroll
-      for (int i = 0; i < kN; ++i) t[i] = v[i];
-      __builtin_nontemporal_store(t, reinterpret_cast<vec*>(p));
+        for (int i = 0; i < kWords; ++i) v[i] = w[i];
+        __builtin_nontemporal_store(v, reinterpret_cast<Vec*>(p));
+      }
+    } else if constexpr (kB == 4) {
+#pragma unroll
+      for (int i = 0; i < kWords; ++i) reinterpret_cast<uint32_t*>(p)[i] = w[i];
     } else {
 #pragma unroll
-      for (int i = 0; i < kN; ++i) reinterpret_cast<Elt*>(p)[i] = v[i];
+      for (int i = 0; i < kN; ++i) reinterpret_cast<uint16_t*>(p)[i] = (uint16_t)(w[i >> 1] >> (16 * (i & 1)));
+    }
+  }
+  // The same at byte `off` of a descriptor's range.
+  __device__ __forceinline__ void store(__amdgpu_buffer_rsrc_t out, uint32_t off) const {
+    if constexpr (kWords == 4) stream_store_sc1(stream_u32x4{w[0], w[1], w[2], w[3]}, out, off);
+    else if constexpr (kWords == 2) stream_store_sc1(stream_u32x2{w[0], w[1]}, out, off);
+    else stream_store_sc1(w[0], out, off);
+  }
+  __device__ __forceinline__ float value(int i) const {
+    if constexpr (DT == TERRA_DTYPE_F32) return __uint_as_float(w[i]);
+    const uint32_t v = w[i >> 1];
+    if constexpr (DT == TERRA_DTYPE_BF16) return __uint_as_float(i & 1 ? v & 0xffff0000u : v << 16);
+    return __half2float(__ushort_as_half((uint16_t)(i & 1 ? v >> 16 : v & 0xffffu)));
+  }
+  // The run becomes f, rounded once, where `turned` (else it stays).
+  __device__ __forceinline__ void turn(const float (&f)[kN], bool turned) {
+#pragma unroll
+    for (int i = 0; i < kWords; ++i) {
+      uint32_t v;
+      if constexpr (DT == TERRA_DTYPE_F32) v = __float_as_uint(f[i]);
+      else v = pack2<DT>(f[2 * i], 2 * i + 1 < kN ? f[2 * i + 1] : 0.f);
+      w[i] = turned ? v : w[i];
     }
   }
 };
 
 constexpr int kRotaryThreads = 256;
 
-// An item is kP pairs, or, behind them, a run of elements that are copied.
+// An item is kP pairs: of interleaved ones a run of 2 kP elements, else two runs
+// of kP.  Behind the rotated items come those that are copied, 2 kP elements each, which go
+// through the same loop: a line that holds some of both is read and written at once.
 template <int DT, int kP, bool kInterleaved, bool kAligned>
 __global__ __launch_bounds__(kRotaryThreads) void rotary_kernel(const RotaryArgs a) {
-  constexpr int kB = ChunkElt<DT>::kBytes, kRun = kInterleaved ? 2 * kP : kP, kCopy = kAligned ? kRun : 1;
-  constexpr int kAhead = 4;
+  constexpr int kB = ChunkElt<DT>::kBytes, kRun = kInterleaved ? 2 * kP : kP, kRuns = kInterleaved ? 1 : 2;
+  constexpr int kAhead = kInterleaved ? 4 : 2;  // heads a thread reads at a time
   typedef RotaryRun<DT, kRun, kAligned> Run;
   const int first = blockIdx.y * a.per_thread, last = min(first + a.per_thread, a.heads);
   uint32_t local, lane;
   a.lanes.divmod(threadIdx.x, local, lane);
   if (local >= a.per_block) return;
-  for (uint32_t token = blockIdx.x * a.per_block + local; token < a.tokens; token += gridDim.x * a.per_block)
-  for (int at = (int)lane; at < a.items; at += (int)a.lanes.d) {
-    uint32_t outer, inner;
+  for (uint32_t start = blockIdx.x * a.per_block; start < a.tokens; start += gridDim.x * a.per_block) {
+    const uint32_t token = start + local;
+    if (token >= a.tokens) break;
+    uint32_t outer, inner, begin_outer, begin_inner;
     a.inner.divmod(token, outer, inner);
-    const uint8_t* x = a.x + (int64_t)outer * a.x_outer + (int64_t)inner * a.x_inner + (int64_t)first * a.x_head;
-    uint8_t* y = a.y + (int64_t)outer * a.y_outer + (int64_t)inner * a.y_inner + (int64_t)first * a.y_head;
-    if (at >= a.turned) {
-      const int64_t off = ((int64_t)2 * a.half + (int64_t)(at - a.turned) * kCopy) * kB;
-      for (int h = first; h < last; h += kAhead, x += kAhead * a.x_head, y += kAhead * a.y_head) {
-        RotaryRun<DT, kCopy, kAligned> r[kAhead];
+    a.inner.divmod(start, begin_outer, begin_inner);
+    const uint8_t* x = a.x + (int64_t)outer * a.x_outer + (int64_t)inner * a.x_inner;
+    uint8_t* y = a.y + (int64_t)outer * a.y_outer + (int64_t)inner * a.y_inner;
+    const __amdgpu_buffer_rsrc_t out = buffer_rsrc(
+        a.y + (int64_t)begin_outer * a.y_outer + (int64_t)begin_inner * a.y_inner,
+        a.y_span - (uint32_t)(start + a.per_block > a.tokens ? (start + a.per_block - a.tokens) * (uint64_t)a.y_inner : 0));
+    for (int at = (int)lane; at < a.items; at += (int)a.lanes.d) {
+      const bool turned = at < a.turned;
+      // Where the item's runs begin in a head; a copied one's second may be past its end (kP = 1).
+      const int copied = 2 * a.half + (at - a.turned) * 2 * kP;
+      const int lo = (turned ? at * kRun : copied) * kB, hi = (turned ? at * kRun + a.half : copied + kP) * kB;
+      const bool both = kAligned || kInterleaved || turned || copied + kP < 2 * a.half + a.rest;
+      const bool whole = kAligned || !kInterleaved || turned || copied + 2 * kP <= 2 * a.half + a.rest;
+      struct Heads {
+        Run r[kAhead][kRuns];
+      };
+      auto fetch = [&](int h) {
+        Heads f;
 #pragma unroll
-        for (int k = 0; k < kAhead; ++k) r[k].load(x + (h + k < last ? k : 0) * a.x_head + off);
-#pragma unroll
-        for (int k = 0; k < kAhead; ++k)
-          if (h + k < last) r[k].store(y + k * a.y_head + off);
-      }
-      continue;
-    }
-    float c[kP], s[kP];
-    uint32_t skip, row;
-    a.position_tokens.divmod(token, skip, row);
-#pragma unroll
-    for (int i = 0; i < kP; ++i) {
-      const int pair = at * kP + i, axis = pair / a.per_axis;
-      const int64_t p = (int64_t)row * a.axes + axis;
-      const int64_t position = a.wide_positions ? reinterpret_cast<const int64_t*>(a.positions)[p]
-                                                : (int64_t)reinterpret_cast<const int32_t*>(a.positions)[p];
-      const double t = (double)position * a.turns[pair - axis * a.per_axis];
-      const float part = (float)(t - rint(t));
-      float sn, cs;
-      sincospif(2.f * part, &sn, &cs);
-      c[i] = a.amplitude * cs;
-      s[i] = a.amplitude * a.sign * sn;
-    }
-    const int64_t lo = (int64_t)at * kRun * kB, hi = lo + (int64_t)a.half * kB;
-    // Heads kAhead at a time, all read before the first is written.
-    for (int h = first; h < last; h += kAhead, x += kAhead * a.x_head, y += kAhead * a.y_head) {
-      Run p[kAhead], q[kInterleaved ? 1 : kAhead];
-#pragma unroll
-      for (int k = 0; k < kAhead; ++k) {
-        const uint8_t* xh = x + (h + k < last ? k : 0) * a.x_head;
-        p[k].load(xh + lo);
-        if constexpr (!kInterleaved) q[k].load(xh + hi);
-      }
-#pragma unroll
-      for (int k = 0; k < kAhead; ++k) {
-        if (h + k >= last) break;
-        uint8_t* yh = y + k * a.y_head;
-#pragma unroll
-        for (int i = 0; i < kP; ++i) {
-          auto& eu = kInterleaved ? p[k].v[kInterleaved ? 2 * i : 0] : p[k].v[i];
-          auto& ev = kInterleaved ? p[k].v[kInterleaved ? 2 * i + 1 : 0] : q[kInterleaved ? 0 : k].v[i];
-          const float u = rotary_value<DT>(eu), v = rotary_value<DT>(ev);
-          eu = rotary_round<DT>(u * c[i] - v * s[i]);
-          ev = rotary_round<DT>(u * s[i] + v * c[i]);
+        for (int k = 0; k < kAhead; ++k) {
+          const uint8_t* xh = x + (int64_t)min(h + k, last - 1) * a.x_head;
+          if (whole) {
+            f.r[k][0].load(xh + lo);
+          } else {  // the last element of an odd rest
+            RotaryRun<DT, 1, false> one;
+            one.load(xh + lo);
+            f.r[k][0].w[0] = one.w[0];
+          }
+          if constexpr (kRuns == 2) f.r[k][1].load(xh + (both ? hi : lo));
         }
-        p[k].store(yh + lo);
-        if constexpr (!kInterleaved) q[k].store(yh + hi);
+        return f;
+      };
+      Heads ahead = fetch(first);
+      float c[kP], s[kP];
+      uint32_t skip, row;
+      a.position_tokens.divmod(token, skip, row);
+#pragma unroll
+      for (int i = 0; i < kP; ++i) {
+        uint32_t axis = 0, pair = (uint32_t)((turned ? at : 0) * kP + i);
+        if (a.axes > 1) a.per_axis.divmod(pair, axis, pair);
+        const int64_t p = (int64_t)row * a.axes + axis;
+        const int64_t position = a.wide_positions ? reinterpret_cast<const int64_t*>(a.positions)[p]
+                                                  : (int64_t)reinterpret_cast<const int32_t*>(a.positions)[p];
+        const double t = (double)position * a.turns[pair];
+        const float part = (float)(t - rint(t));
+        float sn, cs;
+        sincospif(2.f * part, &sn, &cs);
+        c[i] = a.amplitude * cs;
+        s[i] = a.amplitude * a.sign * sn;
+      }
+      for (int h = first; h < last; h += kAhead) {
+        Heads f = ahead;
+        if (h + kAhead < last) ahead = fetch(h + kAhead);
+#pragma unroll
+        for (int k = 0; k < kAhead; ++k) {
+          if (h + k >= last) break;
+          float u[kRuns][kRun];
+#pragma unroll
+          for (int i = 0; i < kP; ++i) {
+            const float p = f.r[k][0].value(kInterleaved ? 2 * i : i), q = f.r[k][kRuns - 1].value(kInterleaved ? 2 * i + 1 : i);
+            u[0][kInterleaved ? 2 * i : i] = p * c[i] - q * s[i];
+            u[kRuns - 1][kInterleaved ? 2 * i + 1 : i] = p * s[i] + q * c[i];
+          }
+#pragma unroll
+          for (int i = 0; i < kRuns; ++i) f.r[k][i].turn(u[i], turned);
+          const int64_t head = (int64_t)(h + k) * a.y_head;
+          if (kAligned && a.y_span != 0) {
+            const uint32_t off = (uint32_t)(local * (uint64_t)a.y_inner + head);
+            f.r[k][0].store(out, off + lo);
+            if constexpr (kRuns == 2) f.r[k][1].store(out, off + hi);
+          } else {
+            if (whole) {
+              f.r[k][0].store(y + head + lo);
+            } else {
+              RotaryRun<DT, 1, false> one;
+              one.w[0] = f.r[k][0].w[0];
+              one.store(y + head + lo);
+            }
+            if constexpr (kRuns == 2)
+              if (both) f.r[k][1].store(y + head + hi);
+          }
+        }
       }
     }
   }
 }
 
 template <int DT, int kP, bool kInterleaved, bool kAligned>
-void launch_rotary(RotaryArgs a, int rest, hipStream_t s) {
-  constexpr int kCopy = !kAligned ? 1 : kInterleaved ? 2 * kP : kP;
+void launch_rotary(RotaryArgs a, hipStream_t s) {
+  constexpr int kB = ChunkElt<DT>::kBytes;
   a.turned = a.half / kP;
-  a.items = a.turned + rest / kCopy;
+  a.items = a.turned + (a.rest + 2 * kP - 1) / (2 * kP);
   const int lanes = a.items < kRotaryThreads ? a.items : kRotaryThreads;
   a.lanes = FastDiv((uint32_t)lanes);
   a.per_block = (uint32_t)(kRotaryThreads / lanes);
@@ -166,31 +220,35 @@ void launch_rotary(RotaryArgs a, int rest, hipStream_t s) {
   int64_t groups = (want + threads - 1) / threads;
   groups = groups > a.heads ? a.heads : groups;
   a.per_thread = (int32_t)((a.heads + groups - 1) / groups);
+  // Tokens of y at one stride, a workgroup's within the range of 32-bit offsets: stores through a descriptor.
+  const int64_t span = (a.per_block - 1) * a.y_inner + (a.heads - 1) * a.y_head + (int64_t)(2 * a.half + a.rest) * kB;
+  const bool flat = a.tokens <= a.inner.d || a.y_outer == (int64_t)a.inner.d * a.y_inner;
+  a.y_span = kAligned && flat && span < (1ll << 31) ? (uint32_t)span : 0;
   const uint32_t need = (a.tokens + a.per_block - 1) / a.per_block, most = 1u << 22;
   const dim3 grid(need < most ? need : most, (unsigned)((a.heads + a.per_thread - 1) / a.per_thread));
   rotary_kernel<DT, kP, kInterleaved, kAligned><<<grid, kRotaryThreads, 0, s>>>(a);
 }
 
 template <int DT, bool kInterleaved>
-void dispatch_rotary(const RotaryArgs& a, uintptr_t bits, int rest, hipStream_t s) {
+void dispatch_rotary(const RotaryArgs& a, uintptr_t bits, hipStream_t s) {
   constexpr int kB = ChunkElt<DT>::kBytes;
-  // The widest run, up to 16 bytes, that divides the rotated part and the rest and is aligned everywhere.
+  // The widest run, of 16 bytes down to 4, that divides the rotated part and the rest and is aligned everywhere.
   auto fits = [&](int p) {
     const int run = kInterleaved ? 2 * p : p;
-    return a.half % p == 0 && rest % run == 0 && bits % (uintptr_t)(run * kB) == 0 && (kInterleaved || a.half * kB % (run * kB) == 0);
+    return a.half % p == 0 && a.rest % (2 * p) == 0 && bits % (uintptr_t)(run * kB) == 0;
   };
   if constexpr (kB == 2 && !kInterleaved)
-    if (fits(8)) return launch_rotary<DT, 8, kInterleaved, true>(a, rest, s);
+    if (fits(8)) return launch_rotary<DT, 8, kInterleaved, true>(a, s);
   if constexpr (kB == 2 || !kInterleaved)
-    if (fits(4)) return launch_rotary<DT, 4, kInterleaved, true>(a, rest, s);
-  if (fits(2)) return launch_rotary<DT, 2, kInterleaved, true>(a, rest, s);
-  launch_rotary<DT, 1, kInterleaved, false>(a, rest, s);
+    if (fits(4)) return launch_rotary<DT, 4, kInterleaved, true>(a, s);
+  if (fits(2)) return launch_rotary<DT, 2, kInterleaved, true>(a, s);
+  launch_rotary<DT, 1, kInterleaved, false>(a, s);
 }
 
 template <int DT>
-void rotary_by_layout(const RotaryArgs& a, bool interleaved, uintptr_t bits, int rest, hipStream_t s) {
-  if (interleaved) dispatch_rotary<DT, true>(a, bits, rest, s);
-  else dispatch_rotary<DT, false>(a, bits, rest, s);
+void rotary_by_layout(const RotaryArgs& a, bool interleaved, uintptr_t bits, hipStream_t s) {
+  if (interleaved) dispatch_rotary<DT, true>(a, bits, s);
+  else dispatch_rotary<DT, false>(a, bits, s);
 }
 
 // Elements from the first of a tensor to the end of its last.
@@ -254,7 +312,7 @@ extern "C" int terra_swin_rotary(const void* x, void* y, const void* positions, 
   a.heads = d->heads;
   a.half = d->dim / 2;
   a.axes = d->axes;
-  a.per_axis = a.half / d->axes;
+  a.per_axis = FastDiv((uint32_t)(a.half / d->axes));
   a.wide_positions = d->position_bits == 64;
   a.amplitude = d->amplitude;
   a.sign = d->inverse != 0 ? -1.f : 1.f;
@@ -262,11 +320,11 @@ extern "C" int terra_swin_rotary(const void* x, void* y, const void* positions, 
   if (outer_tokens > 0) bits |= (uintptr_t)(a.x_outer | a.y_outer);
   if (inner_tokens > 1) bits |= (uintptr_t)(a.x_inner | a.y_inner);
   if (d->heads > 1) bits |= (uintptr_t)(a.x_head | a.y_head);
-  const int rest = same ? 0 : d->head_dim - d->dim;
+  a.rest = same ? 0 : d->head_dim - d->dim;
   hipStream_t s = (hipStream_t)stream;
-  if (d->dtype == TERRA_DTYPE_F32) rotary_by_layout<TERRA_DTYPE_F32>(a, d->interleaved != 0, bits, rest, s);
-  else if (d->dtype == TERRA_DTYPE_BF16) rotary_by_layout<TERRA_DTYPE_BF16>(a, d->interleaved != 0, bits, rest, s);
-  else rotary_by_layout<TERRA_DTYPE_F16>(a, d->interleaved != 0, bits, rest, s);
+  if (d->dtype == TERRA_DTYPE_F32) rotary_by_layout<TERRA_DTYPE_F32>(a, d->interleaved != 0, bits, s);
+  else if (d->dtype == TERRA_DTYPE_BF16) rotary_by_layout<TERRA_DTYPE_BF16>(a, d->interleaved != 0, bits, s);
+  else rotary_by_layout<TERRA_DTYPE_F16>(a, d->interleaved != 0, bits, s);
   const hipError_t e = hipGetLastError();
   return e == hipSuccess ? TERRA_OK : fail(TERRA_ERR_LAUNCH, "terra_swin_rotary launch failed: %s", hipGetErrorString(e));
 }
