@@ -220,7 +220,7 @@ __device__ __forceinline__ double power(double beta, int64_t n) {
 
 // What a step multiplies by, the same for all elements.
 struct AdamStep {
-  float keep, rate, root, eps;  // 1 - lr decay, lr / (1 - beta1^t), 1 / (1 - beta2^t), eps
+  float keep, rate, root, eps;  // 1 - lr decay, lr / (1 - beta1^t), 1 / sqrt(1 - beta2^t), eps
   float factor;                 // of the gradients
   uint32_t step;
 
@@ -229,36 +229,45 @@ struct AdamStep {
     const double lr = a.lr_ptr != nullptr ? (double)*a.lr_ptr : a.lr;
     keep = (float)(1.0 - lr * a.decay);
     rate = (float)(lr / (1.0 - power(a.beta1, t)));
-    root = (float)(1.0 / (1.0 - power(a.beta2, t)));
+    root = (float)(1.0 / sqrt(1.0 - power(a.beta2, t)));
     eps = (float)a.eps;
     factor = a.grad_factor != nullptr ? *a.grad_factor : 1.f;
     if (a.maximize) factor = -factor;
     step = (uint32_t)t;
   }
-  __device__ __forceinline__ float updated(float p, float m, float v) const {
-    return p * keep - rate * (m / (sqrtf(v * root) + eps));
+  __device__ __forceinline__ float updated(float p, float m, float r) const {  // r: the second moment's root
+    return fmaf(-rate * m, __builtin_amdgcn_rcpf(fmaf(r, root, eps)), p * keep);
   }
 };
 
+// Four elements of a lane.
 template <int DTP, int DTG, bool kVec>
-__device__ __forceinline__ void adam_elements(const AdamEntry& e, const AdamStep& st, float b1, float c1, float b2, float c2,
-                                              int64_t i, int n) {
+struct AdamElements {
   float p[4], g[4], m[4], v[4];
-  four_values<DTP, kVec>(e.param, i, n, p);
-  four_values<DTG, kVec>(e.grad, i, n, g);
-  four_values<TERRA_DTYPE_F32, kVec>(e.first, i, n, m);
-  four_values<TERRA_DTYPE_F32, kVec>(e.second, i, n, v);
-#pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    const float d = g[j] * st.factor;
-    m[j] = fmaf(c1, d, b1 * m[j]);
-    v[j] = fmaf(c2 * d, d, b2 * v[j]);
-    p[j] = st.updated(p[j], m[j], v[j]);
+
+  __device__ __forceinline__ void load(const AdamEntry& e, int64_t i, int n) {
+    four_values<DTP, kVec>(e.param, i, n, p);
+    four_values<DTG, kVec>(e.grad, i, n, g);
+    four_values<TERRA_DTYPE_F32, kVec>(e.first, i, n, m);
+    four_values<TERRA_DTYPE_F32, kVec>(e.second, i, n, v);
   }
-  put_four<DTP, kVec>(e.param, i, n, p);
-  put_four<TERRA_DTYPE_F32, kVec>(e.first, i, n, m);
-  put_four<TERRA_DTYPE_F32, kVec>(e.second, i, n, v);
-}
+  __device__ __forceinline__ void step(const AdamStep& st, float b1, float c1, float b2, float c2) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const float d = g[j] * st.factor;
+      m[j] = fmaf(c1, d, b1 * m[j]);
+      v[j] = fmaf(c2 * d, d, b2 * v[j]);
+      p[j] = st.updated(p[j], m[j], sqrtf(v[j]));
+    }
+  }
+  __device__ __forceinline__ void store(const AdamEntry& e, int64_t i, int n) const {
+    put_four<DTP, kVec>(e.param, i, n, p);
+    put_four<TERRA_DTYPE_F32, kVec>(e.first, i, n, m);
+    put_four<TERRA_DTYPE_F32, kVec>(e.second, i, n, v);
+  }
+};
+
+constexpr int kAdamAhead = 2;  // groups of four that a thread reads before it writes the first
 
 template <int DTP, int DTG>
 __global__ __launch_bounds__(kAdamThreads) void adamw_kernel(const AdamList a) {
@@ -271,11 +280,26 @@ __global__ __launch_bounds__(kAdamThreads) void adamw_kernel(const AdamList a) {
   const int64_t end = begin + kAdamChunk < e.numel ? begin + kAdamChunk : e.numel;
   const bool vec = (uintptr_t)e.param % (4 * ChunkElt<DTP>::kBytes) == 0 && (uintptr_t)e.grad % (4 * ChunkElt<DTG>::kBytes) == 0 &&
                    ((uintptr_t)e.first | (uintptr_t)e.second) % 16 == 0;
+  constexpr int kStride = kAdamThreads * 4;
   int64_t i = begin + threadIdx.x * 4;
   if (vec)
-    for (; i + 4 <= end; i += kAdamThreads * 4) adam_elements<DTP, DTG, true>(e, st, b1, c1, b2, c2, i, 4);
-  for (; i < end; i += kAdamThreads * 4)
-    adam_elements<DTP, DTG, false>(e, st, b1, c1, b2, c2, i, (int)(end - i < 4 ? end - i : 4));
+    for (; i + (kAdamAhead - 1) * kStride + 4 <= end; i += kAdamAhead * kStride) {
+      AdamElements<DTP, DTG, true> q[kAdamAhead];
+#pragma unroll
+      for (int u = 0; u < kAdamAhead; ++u) q[u].load(e, i + u * kStride, 4);
+#pragma unroll
+      for (int u = 0; u < kAdamAhead; ++u) {
+        q[u].step(st, b1, c1, b2, c2);
+        q[u].store(e, i + u * kStride, 4);
+      }
+    }
+  for (; i < end; i += kStride) {
+    const int n = (int)(end - i < 4 ? end - i : 4);
+    AdamElements<DTP, DTG, false> q;
+    q.load(e, i, n);
+    q.step(st, b1, c1, b2, c2);
+    q.store(e, i, n);
+  }
 }
 
 // ---- moments in 8 bits ----------------------------------------------------------
@@ -302,21 +326,21 @@ __device__ __forceinline__ uint32_t fp8_codes(const float (&f)[4]) {
 template <int kJ>
 __device__ __forceinline__ float fp8_value(uint32_t codes) { return __builtin_amdgcn_cvt_f32_fp8((int)codes, kJ); }
 
-constexpr float kLargestCode = 448.f, kSmallestCode = 0.001953125f, kSmallestNormal = 0.015625f;
+constexpr float kLargestCode = 448.f, kSmallestCode = 0.001953125f;
 
-// A value on one of the two codes next to r > 0 (at most 448 and a rounding): of low <= r < high the
-// upper one where r^2 - low^2 > u (high^2 - low^2).  Squares of codes are exact.
+// A value on one of the two codes next to r >= 0 (at most 448 and a rounding): of low <= r < high the
+// upper one where r^2 - low^2 > u (high^2 - low^2).  Squares of codes are exact.  Without branches: a code's
+// step is 2^-3 of the power of two below r, from 2^-6 down 2^-9.
 __device__ __forceinline__ float root_code(float r, uint32_t draw) {
-  r = fminf(r, kLargestCode);
-  const uint32_t bits = __float_as_uint(r);
-  const float fine = floorf(r * 512.f);
-  const bool normal = r >= kSmallestNormal;
-  const float low = normal ? __uint_as_float(bits & 0xfff00000u) : fine * kSmallestCode;
-  const float high = normal ? __uint_as_float((bits & 0xfff00000u) + 0x100000u) : (fine + 1.f) * kSmallestCode;
+  const float c = fminf(r, kLargestCode);
+  const uint32_t power = max(__float_as_uint(c), 0x3c800000u) & 0x7f800000u;  // of two, at least 2^-6
+  const float step = __uint_as_float(power - (3u << 23)), per_step = __uint_as_float((257u << 23) - power);
+  const float low = floorf(c * per_step) * step, high = low + step;
   const float l2 = low * low, span = fmaf(high, high, -l2);
   const float u = fmaf((float)draw, 1.f / 65536.f, 0.5f / 65536.f);
-  const float v = fmaf(r, r, -l2) > u * span ? high : low;
-  return fminf(fmaxf(v, kSmallestCode), kLargestCode);
+  const float v = fmaf(c, c, -l2) > u * span ? high : low;
+  const float held = __builtin_amdgcn_fmed3f(v, kSmallestCode, kLargestCode);
+  return r > 0.f ? held : 0.f;
 }
 
 __device__ __forceinline__ ChunkDraws adam_draws(uint64_t seed, uint32_t chunk, uint32_t tensor, uint32_t step, uint32_t stream) {
@@ -393,7 +417,6 @@ __global__ __launch_bounds__(kAdamThreads) void adamw_8bit_kernel(const AdamList
   const AdamStep st(a);
   const uint64_t seed = *a.seed;
   const double c1 = (1.0 - a.beta1) * (double)st.factor, c2 = (1.0 - a.beta2) * (double)st.factor * (double)st.factor;
-  const float root = sqrtf(st.root);
   const int64_t blocks = (e.numel + kScaled - 1) / kScaled;
   const int64_t begin = (int64_t)(blockIdx.x - a.start[t]) * (kAdamChunk / kScaled);
   const int64_t end = begin + kAdamChunk / kScaled < blocks ? begin + kAdamChunk / kScaled : blocks;
@@ -423,23 +446,24 @@ __global__ __launch_bounds__(kAdamThreads) void adamw_8bit_kernel(const AdamList
       const float fr[4] = {fp8_value<0>(q[k].second), fp8_value<1>(q[k].second), fp8_value<2>(q[k].second), fp8_value<3>(q[k].second)};
       const double dm = a.beta1 * scale_m[k], dv = a.beta2 * scale_r[k] * scale_r[k];
       double v[4];
-      bool far = false;
+      uint32_t away = 0;
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         const double g = (double)q[k].g[j];
         m[k][j] = fma((double)fm[j], dm, c1 * g);
         v[j] = fma((double)(fr[j] * fr[j]), dv, c2 * g * g);
-        far |= v[j] != 0.0 && !(v[j] >= 0x1p-100 && v[j] <= 0x1p+120);
+        // How far the exponent is above 2^-100 (below it, and for 0, a large number).
+        away = max(away, (uint32_t)((uint64_t)__double_as_longlong(v[j]) >> 32) - ((1023u - 100u) << 20));
         r[k][j] = __builtin_amdgcn_sqrtf((float)v[j]);
       }
-      if (__builtin_amdgcn_ballot_w64(far) != 0)
+      if (__builtin_amdgcn_ballot_w64(away > (220u << 20)) != 0)  // not all in 2^-100 .. 2^120
 #pragma unroll
         for (int j = 0; j < 4; ++j) r[k][j] = (float)sqrt(v[j]);
       big_m[k] = big_r[k] = 0;
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         const float m32 = (float)m[k][j];
-        q[k].p[j] = q[k].p[j] * st.keep - st.rate * (m32 / fmaf(r[k][j], root, st.eps));
+        q[k].p[j] = st.updated(q[k].p[j], m32, r[k][j]);
         big_m[k] = max(big_m[k], __float_as_uint(m32) & 0x7fffffffu);  // NaN above infinity above the others
         big_r[k] = max(big_r[k], __float_as_uint(r[k][j]) & 0x7fffffffu);
       }
@@ -464,7 +488,7 @@ __global__ __launch_bounds__(kAdamThreads) void adamw_8bit_kernel(const AdamList
       for (int j = 0; j < 4; ++j) {
         y[j] = __builtin_amdgcn_fmed3f((float)(m[k][j] * inv_m), -kLargestCode, kLargestCode);
         const float part = (float)((double)r[k][j] * inv_r);
-        z[j] = part > 0.f ? root_code(part, j & 1 ? w[k][j >> 1] >> 16 : w[k][j >> 1] & 0xffffu) : 0.f;
+        z[j] = root_code(part, j & 1 ? w[k][j >> 1] >> 16 : w[k][j >> 1] & 0xffffu);
       }
       q[k].first = fp8_codes(y);
       q[k].second = fp8_codes(z);

@@ -9,7 +9,9 @@
 // The rotation is in fp32, rounded once.
 //
 // A thread has kP pairs of a token and goes through heads with them, so an angle's sine
-// and cosine serve all of those.
+// and cosine serve all of those; its reads are four heads ahead of what it turns.  Bound by memory where
+// a token has several heads: 156672 tokens of 16 heads of 128 bf16 228 us, of two heads at a time 240 (a large
+// copy moves the same bytes in 250); by the sines and cosines where it has one (200000 of 128: 29 us, 3.6 TB/s).
 #include "row_chunk.h"
 
 #include <initializer_list>
@@ -25,7 +27,6 @@ struct RotaryArgs {
   int64_t x_outer, x_inner, x_head, y_outer, y_inner, y_head;  // bytes
   FastDiv inner, position_tokens, lanes, per_axis;  // lanes: threads of a token
   uint32_t tokens, per_block;             // tokens of a workgroup
-  uint32_t y_span;                        // bytes from a workgroup's first token of y to its end, 0: not at one stride
   int32_t turned, items;                  // items of a token that are rotated, and all
   int32_t heads, per_thread;              // heads, of which a thread takes this many
   int32_t half, rest;                     // dim / 2, elements that are copied
@@ -77,12 +78,6 @@ struct RotaryRun {
       for (int i = 0; i < kN; ++i) reinterpret_cast<uint16_t*>(p)[i] = (uint16_t)(w[i >> 1] >> (16 * (i & 1)));
     }
   }
-  // The same at byte `off` of a descriptor's range.
-  __device__ __forceinline__ void store(__amdgpu_buffer_rsrc_t out, uint32_t off) const {
-    if constexpr (kWords == 4) stream_store_sc1(stream_u32x4{w[0], w[1], w[2], w[3]}, out, off);
-    else if constexpr (kWords == 2) stream_store_sc1(stream_u32x2{w[0], w[1]}, out, off);
-    else stream_store_sc1(w[0], out, off);
-  }
   __device__ __forceinline__ float value(int i) const {
     if constexpr (DT == TERRA_DTYPE_F32) return __uint_as_float(w[i]);
     const uint32_t v = w[i >> 1];
@@ -105,11 +100,11 @@ constexpr int kRotaryThreads = 256;
 
 // An item is kP pairs: of interleaved ones a run of 2 kP elements, else two runs
 // of kP.  Behind the rotated items come those that are copied, 2 kP elements each, which go
-// through the same loop: a line that holds some of both is read and written at once.
-template <int DT, int kP, bool kInterleaved, bool kAligned>
+// through the same loop: a line that holds some of both is read and written at once.  kAhead: heads that a
+// thread reads at a time.
+template <int DT, int kP, bool kInterleaved, bool kAligned, int kAhead>
 __global__ __launch_bounds__(kRotaryThreads) void rotary_kernel(const RotaryArgs a) {
   constexpr int kB = ChunkElt<DT>::kBytes, kRun = kInterleaved ? 2 * kP : kP, kRuns = kInterleaved ? 1 : 2;
-  constexpr int kAhead = kInterleaved ? 4 : 2;  // heads a thread reads at a time
   typedef RotaryRun<DT, kRun, kAligned> Run;
   const int first = blockIdx.y * a.per_thread, last = min(first + a.per_thread, a.heads);
   uint32_t local, lane;
@@ -118,14 +113,10 @@ __global__ __launch_bounds__(kRotaryThreads) void rotary_kernel(const RotaryArgs
   for (uint32_t start = blockIdx.x * a.per_block; start < a.tokens; start += gridDim.x * a.per_block) {
     const uint32_t token = start + local;
     if (token >= a.tokens) break;
-    uint32_t outer, inner, begin_outer, begin_inner;
+    uint32_t outer, inner;
     a.inner.divmod(token, outer, inner);
-    a.inner.divmod(start, begin_outer, begin_inner);
     const uint8_t* x = a.x + (int64_t)outer * a.x_outer + (int64_t)inner * a.x_inner;
     uint8_t* y = a.y + (int64_t)outer * a.y_outer + (int64_t)inner * a.y_inner;
-    const __amdgpu_buffer_rsrc_t out = buffer_rsrc(
-        a.y + (int64_t)begin_outer * a.y_outer + (int64_t)begin_inner * a.y_inner,
-        a.y_span - (uint32_t)(start + a.per_block > a.tokens ? (start + a.per_block - a.tokens) * (uint64_t)a.y_inner : 0));
     for (int at = (int)lane; at < a.items; at += (int)a.lanes.d) {
       const bool turned = at < a.turned;
       // Where the item's runs begin in a head; a copied one's second may be past its end (kP = 1).
@@ -140,7 +131,8 @@ __global__ __launch_bounds__(kRotaryThreads) void rotary_kernel(const RotaryArgs
         Heads f;
 #pragma unroll
         for (int k = 0; k < kAhead; ++k) {
-          const uint8_t* xh = x + (int64_t)min(h + k, last - 1) * a.x_head;
+          if (h + k >= last) break;
+          const uint8_t* xh = x + (int64_t)(h + k) * a.x_head;
           if (whole) {
             f.r[k][0].load(xh + lo);
           } else {  // the last element of an odd rest
@@ -185,22 +177,16 @@ __global__ __launch_bounds__(kRotaryThreads) void rotary_kernel(const RotaryArgs
           }
 #pragma unroll
           for (int i = 0; i < kRuns; ++i) f.r[k][i].turn(u[i], turned);
-          const int64_t head = (int64_t)(h + k) * a.y_head;
-          if (kAligned && a.y_span != 0) {
-            const uint32_t off = (uint32_t)(local * (uint64_t)a.y_inner + head);
-            f.r[k][0].store(out, off + lo);
-            if constexpr (kRuns == 2) f.r[k][1].store(out, off + hi);
+          uint8_t* yh = y + (int64_t)(h + k) * a.y_head;
+          if (whole) {
+            f.r[k][0].store(yh + lo);
           } else {
-            if (whole) {
-              f.r[k][0].store(y + head + lo);
-            } else {
-              RotaryRun<DT, 1, false> one;
-              one.w[0] = f.r[k][0].w[0];
-              one.store(y + head + lo);
-            }
-            if constexpr (kRuns == 2)
-              if (both) f.r[k][1].store(y + head + hi);
+            RotaryRun<DT, 1, false> one;
+            one.w[0] = f.r[k][0].w[0];
+            one.store(yh + lo);
           }
+          if constexpr (kRuns == 2)
+            if (both) f.r[k][1].store(yh + hi);
         }
       }
     }
@@ -209,7 +195,6 @@ __global__ __launch_bounds__(kRotaryThreads) void rotary_kernel(const RotaryArgs
 
 template <int DT, int kP, bool kInterleaved, bool kAligned>
 void launch_rotary(RotaryArgs a, hipStream_t s) {
-  constexpr int kB = ChunkElt<DT>::kBytes;
   a.turned = a.half / kP;
   a.items = a.turned + (a.rest + 2 * kP - 1) / (2 * kP);
   const int lanes = a.items < kRotaryThreads ? a.items : kRotaryThreads;
@@ -220,13 +205,11 @@ void launch_rotary(RotaryArgs a, hipStream_t s) {
   int64_t groups = (want + threads - 1) / threads;
   groups = groups > a.heads ? a.heads : groups;
   a.per_thread = (int32_t)((a.heads + groups - 1) / groups);
-  // Tokens of y at one stride, a workgroup's within the range of 32-bit offsets: stores through a descriptor.
-  const int64_t span = (a.per_block - 1) * a.y_inner + (a.heads - 1) * a.y_head + (int64_t)(2 * a.half + a.rest) * kB;
-  const bool flat = a.tokens <= a.inner.d || a.y_outer == (int64_t)a.inner.d * a.y_inner;
-  a.y_span = kAligned && flat && span < (1ll << 31) ? (uint32_t)span : 0;
   const uint32_t need = (a.tokens + a.per_block - 1) / a.per_block, most = 1u << 22;
   const dim3 grid(need < most ? need : most, (unsigned)((a.heads + a.per_thread - 1) / a.per_thread));
-  rotary_kernel<DT, kP, kInterleaved, kAligned><<<grid, kRotaryThreads, 0, s>>>(a);
+  // Four heads ahead take registers that a thread of few heads has better use for (200000 x 1 of 128: 29 us, 36 so).
+  if (a.per_thread >= 4) rotary_kernel<DT, kP, kInterleaved, kAligned, 4><<<grid, kRotaryThreads, 0, s>>>(a);
+  else rotary_kernel<DT, kP, kInterleaved, kAligned, 1><<<grid, kRotaryThreads, 0, s>>>(a);
 }
 
 template <int DT, bool kInterleaved>
