@@ -143,3 +143,40 @@ def draws(seed, count, tensor, step, stream=0):
         k0, k1 = (k0 + 0x9E3779B9) & LOW, (k1 + 0xBB67AE85) & LOW
     words = torch.stack(c, 1)
     return torch.stack((words & 0xFFFF, words >> 16), -1).view(-1)[:count]
+
+
+# ---- a block with rotary positions -------------------------------------------------
+
+
+def swin_block_rotary(x, H, W, window, shift, heads, params, rate, dim, interleaved=False, amplitude=1.0, use_attn_mask=True):
+    """SequentialSwinTransformer.forward (models/transformer.py:138-298) with rotary
+    positions by a token's row and column in its window, in 64 bits; params as
+    swin_oracle.swin_block_attention's, those that need a gradient in the graph."""
+    from . import swin_oracle as so
+
+    B, _, C = x.shape
+    p = {k: v.double() for k, v in params.items() if v.is_floating_point()}
+    y = layer_norm(x, p["norm1.weight"], p["norm1.bias"])[0].view(B, H, W, C)
+    win = so.partition_frame(y, window, shift, shift)
+    at = torch.arange(window * window)
+    positions = torch.stack((at // window, at % window), -1)
+
+    def projected(name):
+        t = win @ p[f"attn.{name}_linear.weight"].T + p[f"attn.{name}_linear.bias"]
+        if name == "v":
+            return t
+        t = t.unflatten(-1, (heads, C // heads))
+        return rotary(t, positions, rate, dim, 2, interleaved, amplitude).flatten(-2)
+
+    mask = so.shift_mask(H, W, window, shift) if shift > 0 and use_attn_mask else None
+    o = so.window_attention_core(projected("q"), projected("k"), projected("v"), heads, (C // heads) ** -0.5,
+                                 p.get("attn.relative_position_bias_table"), (window, window), mask, compute_dtype=torch.float64)
+    o = o @ p["attn.proj.weight"].T + p["attn.proj.bias"]
+    return so.reverse_frame(o, B, H, W, window, shift, shift, residual=x.double()).view(B, H * W, C)
+
+
+def mlp(x, params):
+    """SequentialMlp.forward (models/mlp.py:152-172) in 64 bits, in the graph."""
+    p = {k: v.double() for k, v in params.items()}
+    h = layer_norm(x, p["norm2.weight"], p["norm2.bias"])[0] @ p["fc1.weight"].T + p["fc1.bias"]
+    return torch.nn.functional.gelu(h) @ p["fc2.weight"].T + p["fc2.bias"] + x

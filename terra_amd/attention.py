@@ -15,9 +15,10 @@ from typing import Callable, Optional, Sequence, Union
 
 import torch
 import torch.nn.functional as F
+from torch.autograd import forward_ad
 
 from . import autograd, kernels
-from .kernels import ShiftMask, WindowMask
+from .kernels import Norm, ShiftMask, WindowMask
 
 
 def run_with_seed(init_seed: Optional[int], fn: Callable):
@@ -61,6 +62,23 @@ def plain_norm(module: torch.nn.Module, channels: int) -> bool:
             and tuple(module.normalized_shape) == (channels,))
 
 
+def normed(module: torch.nn.Module, x: torch.Tensor) -> torch.Tensor:
+    """``module(x)``, by the HIP kernels where it is a :func:`plain_norm` over x's last
+    dimension: in the type that torch's would have (fp32 under autocast).  Calls that torch
+    traces or transforms, and tensors of other classes, are torch's."""
+    if (x.device.type != "cuda" or x.dtype not in (torch.float32, torch.bfloat16, torch.float16) or x.dim() < 1
+            or type(x) not in (torch.Tensor, torch.nn.Parameter) or not plain_norm(module, x.shape[-1])
+            or forward_ad._current_level >= 0 or torch.compiler.is_compiling()
+            or torch._C._functorch.peek_interpreter_stack() is not None):
+        return module(x)
+    autocast = torch.is_autocast_enabled("cuda")
+    params = [t for t in (module.weight, getattr(module, "bias", None)) if t is not None]
+    if (autocast and type(module) is not torch.nn.LayerNorm) or any(
+            t.device != x.device or t.dtype not in (torch.float32, x.dtype) for t in params):
+        return module(x)
+    return autograd.layer_norm(x, Norm.of(module), torch.float32 if autocast else None)
+
+
 def relative_position_index(window_size: Sequence[int]) -> torch.Tensor:
     """Swin relative-position index [Wh*Ww, Wh*Ww] (models/attention.py:205-214):
     idx[i, j] = (hi - hj + Wh - 1) * (2*Ww - 1) + (wi - wj + Ww - 1)."""
@@ -68,6 +86,12 @@ def relative_position_index(window_size: Sequence[int]) -> torch.Tensor:
     hi = torch.arange(wh).repeat_interleave(ww)
     wi = torch.arange(ww).repeat(wh)
     return (hi[:, None] - hi[None, :] + wh - 1) * (2 * ww - 1) + (wi[:, None] - wi[None, :] + ww - 1)
+
+
+def token_positions(window_size: Sequence[int]) -> torch.Tensor:
+    """Row and column of each token of a window, int32 [Wh*Ww, 2]."""
+    wh, ww = int(window_size[0]), int(window_size[1])
+    return torch.stack((torch.arange(wh).repeat_interleave(ww), torch.arange(ww).repeat(wh)), 1).to(torch.int32)
 
 
 class WindowAttention(torch.nn.Module):
@@ -78,11 +102,16 @@ class WindowAttention(torch.nn.Module):
     (the same mask in closed form), or a :class:`kernels.WindowMask` adding
     per-window land bits.  ``use_flash_attention`` is accepted for signature
     compatibility; the fused HIP core serves every case.
+
+    ``rotary`` (optional, build-defined): rotary positions of the query and key
+    heads by the token's row and column in its window, a :class:`kernels.Rotary` of
+    two axes or True for one over whole heads.  A block without the
+    bias table (the reference's windows of 32 x 32) knows no positions otherwise.
     """
 
     def __init__(self, embedding_dim, window_size, num_heads, qkv_bias=True, qk_scale=None,
                  use_attn_mask=True, use_relative_position_bias=True, use_flash_attention=False,
-                 init_seed_base=None):
+                 init_seed_base=None, rotary: Union[None, bool, kernels.Rotary] = None):
         super().__init__()
         self.use_attn_mask = use_attn_mask
         self.use_relative_position_bias = use_relative_position_bias
@@ -94,6 +123,12 @@ class WindowAttention(torch.nn.Module):
             raise AssertionError(f"dim {self.dim} must be divisible by num_heads {num_heads}")
         head_dim = self.dim // num_heads
         self.scale = qk_scale or head_dim ** -0.5
+        self.rotary = kernels.Rotary(head_dim, axes=2) if rotary is True else rotary or None
+        if self.rotary is not None:
+            if self.rotary.axes != 2 or self.rotary.dim > head_dim:
+                raise ValueError(f"rotary positions of a window have two axes and at most the {head_dim} elements of a head "
+                                 f"(got {self.rotary.axes} and {self.rotary.dim})")
+            self.register_buffer("token_positions", token_positions(self.window_size), persistent=False)
 
         if self.use_relative_position_bias:
             wh, ww = self.window_size
@@ -156,11 +191,21 @@ class WindowAttention(torch.nn.Module):
         return autograd.window_attention(q, k, v, self.num_heads, self.window_size, self.scale,
                                          bias_table=self._table(), mask=mask, n_real=n_real)
 
+    def __setstate__(self, state):
+        """A module pickled when this option was not there yet has it off."""
+        super().__setstate__(state)
+        if not hasattr(self, "rotary"):
+            self.rotary = None
+
     def attend(self, x: torch.Tensor, mask=None) -> torch.Tensor:
         """Everything of forward but the output projection: q/k/v and the
         fused core, O [B_, N, C] (models/attention.py:244-278).  In training
         the core's backward kernel also sums the q | k | v gradient's columns,
         which the projection's backward takes as its bias gradient."""
+        if self.rotary is not None:
+            return autograd.window_attention_qkv(self.qkv(x), self.num_heads, self.window_size, self.scale,
+                                                 bias_table=self._table(), mask=mask, rot=self.rotary,
+                                                 positions=self.token_positions)
         link = autograd.ColumnSumLink() if torch.is_grad_enabled() else None
         return autograd.window_attention_qkv(self.qkv(x, bias_sums=link), self.num_heads, self.window_size,
                                              self.scale, bias_table=self._table(), mask=mask, bias_sums=link)

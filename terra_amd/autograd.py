@@ -526,6 +526,50 @@ class _AttentionQKV(torch.autograd.Function):
         return dqkv, dtable, None, None, None, None, None, None, None
 
 
+class _RotaryAttentionQKV(torch.autograd.Function):
+    """:class:`_AttentionQKV` with rotary positions of the query and key heads: their
+    columns are turned into a buffer of their own in one launch, and the
+    backward turns their gradients back in place in the [B_, N, 3C] buffer."""
+
+    @staticmethod
+    def forward(ctx, qkv, table, num_heads, window_size, scale, mask, n_real, mask_value, rot, positions):
+        ctx.cfg = (num_heads, window_size, scale, mask, n_real, mask_value, rot)
+        qk = _turned_heads(qkv, num_heads, rot, positions)
+        ctx.save_for_backward(qk, qkv, table, positions)
+        C = qkv.shape[-1] // 3
+        return kernels.window_attention(qk[..., :C], qk[..., C:], qkv[..., 2 * C:], num_heads, window_size, scale,
+                                        bias_table=table, mask=mask, n_real=n_real, mask_value=mask_value)
+
+    @staticmethod
+    def backward(ctx, grad: torch.Tensor):
+        qk, qkv, table, positions = ctx.saved_tensors
+        num_heads, window_size, scale, mask, n_real, mask_value, rot = ctx.cfg
+        C = qkv.shape[-1] // 3
+        _check_backward(qk[..., :C], num_heads, window_size, n_real)
+        dqkv = torch.empty(qkv.shape, dtype=qkv.dtype, device=qkv.device)
+        dbias = None
+        if table is not None and ctx.needs_input_grad[1]:
+            dbias = torch.zeros(table.shape, dtype=torch.float32, device=table.device)
+        kernels.window_attention_backward(qk[..., :C], qk[..., C:], qkv[..., 2 * C:], grad.contiguous(), num_heads,
+                                          window_size, scale, bias_table=table, mask=mask, n_real=n_real,
+                                          mask_value=mask_value, dq=dqkv[..., :C], dk=dqkv[..., C:2 * C],
+                                          dv=dqkv[..., 2 * C:], dbias=dbias)
+        heads = _query_key_heads(dqkv, num_heads)
+        kernels.rotary(heads, rot, positions, inverse=True, out=heads)
+        dtable = None if dbias is None else dbias.to(table.dtype)
+        return dqkv, dtable, None, None, None, None, None, None, None, None
+
+
+def _query_key_heads(qkv: torch.Tensor, num_heads: int) -> torch.Tensor:
+    """The query and key columns of q | k | v [B_, N, 3C] as heads [B_, N, 2 num_heads, D]."""
+    C = qkv.shape[-1] // 3
+    return qkv[..., :2 * C].unflatten(-1, (2 * num_heads, C // num_heads))
+
+
+def _turned_heads(qkv: torch.Tensor, num_heads: int, rot: kernels.Rotary, positions: torch.Tensor) -> torch.Tensor:
+    return kernels.rotary(_query_key_heads(qkv, num_heads), rot, positions).flatten(-2)
+
+
 def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, num_heads: int,
                      window_size: Tuple[int, int], scale: float, bias_table: Optional[torch.Tensor] = None,
                      mask: MaskArg = None, n_real: Optional[int] = None,
@@ -541,11 +585,21 @@ def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, num_head
 def window_attention_qkv(qkv: torch.Tensor, num_heads: int, window_size: Tuple[int, int], scale: float,
                          bias_table: Optional[torch.Tensor] = None, mask: MaskArg = None,
                          n_real: Optional[int] = None, mask_value: float = kernels.MASK_VALUE,
-                         bias_sums: Optional[ColumnSumLink] = None) -> torch.Tensor:
+                         bias_sums: Optional[ColumnSumLink] = None, rot: Optional[kernels.Rotary] = None,
+                         positions: Optional[torch.Tensor] = None) -> torch.Tensor:
     """Attention over the column blocks q | k | v of one [B_, N, 3C] tensor,
     with gradients (see :class:`_AttentionQKV`).  ``bias_sums``: the
-    :class:`ColumnSumLink` of the :func:`linear` that produced ``qkv``."""
+    :class:`ColumnSumLink` of the :func:`linear` that produced ``qkv``.  ``rot``,
+    ``positions``: rotary positions of the query and key heads (:func:`kernels.rotary`); then
+    no sums are handed over."""
     C = qkv.shape[-1] // 3
+    if rot is not None:
+        if _needs_grad(qkv, bias_table):
+            return _RotaryAttentionQKV.apply(qkv.contiguous(), bias_table, num_heads, tuple(window_size), scale, mask, n_real,
+                                             mask_value, rot, positions)
+        qk = _turned_heads(qkv, num_heads, rot, positions)
+        return kernels.window_attention(qk[..., :C], qk[..., C:], qkv[..., 2 * C:], num_heads, window_size, scale,
+                                        bias_table=bias_table, mask=mask, n_real=n_real, mask_value=mask_value)
     if _needs_grad(qkv, bias_table):
         if not qkv.is_contiguous():
             qkv = qkv.contiguous()
@@ -779,8 +833,8 @@ def residual_norm(h: torch.Tensor, x: torch.Tensor, post_norm: Optional[Norm] = 
 
 
 def layer_norm(x: torch.Tensor, norm: Norm, out_dtype: Optional[torch.dtype] = None) -> torch.Tensor:
-    """:func:`kernels.layer_norm` with gradients for x and the norm's parameters.
-    An x whose rows the kernels cannot read in place is copied first.  The autograd
+    """:func:`kernels.layer_norm` with gradients of every order for x and the norm's
+    parameters; a pass that is to be differentiated itself (``create_graph``) runs in torch's operations.  An x whose rows the kernels cannot read in place is copied first.  The autograd
     node is a C++ one (csrc/training_binding.cpp); it keeps x, the parameters and two fp32 values a row."""
     try:
         call = kernels._norm_call(x, norm, out_dtype)

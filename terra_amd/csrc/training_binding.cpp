@@ -6,7 +6,6 @@
 // is done here.  Allocations are torch's; the arithmetic is the library's,
 // reached by the addresses that bind() is given.
 #include <torch/csrc/autograd/function.h>
-#include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/functions/utils.h>
 #include <torch/csrc/autograd/saved_variable.h>
 #include <torch/csrc/autograd/variable.h>
@@ -133,7 +132,20 @@ NormGradients norm_gradients(const NormCall& c, const Tensor& dy, const Tensor& 
   return g;
 }
 
-constexpr const char* kOnce = "layer_norm cannot be differentiated twice: its gradient has no gradient";
+// The same in torch's operations, in fp32 where the types are shorter, for a
+// backward pass that is to be differentiated itself.
+variable_list norm_gradients_in_operations(const NormCall& c, const Tensor& dy, const Tensor& x, const Tensor& weight,
+                                           const Tensor& bias) {
+  const Tensor xf = x.to(at::kFloat), d = dy.to(at::kFloat);
+  const Tensor centred = c.desc.norm == TERRA_NORM_LAYER ? xf - xf.mean(-1, true) : xf;
+  const Tensor r = (centred * centred).mean(-1, true).add(static_cast<double>(c.desc.eps)).rsqrt(), xh = centred * r;
+  const Tensor g = weight.defined() ? d * weight.to(at::kFloat) : d;
+  Tensor dx = g - xh * (g * xh).mean(-1, true);
+  if (c.desc.norm == TERRA_NORM_LAYER) dx = dx - g.mean(-1, true);
+  auto over_rows = [](const Tensor& t, const Tensor& like) { return t.reshape({-1, t.size(-1)}).sum(0).to(like.scalar_type()); };
+  return {(dx * r).to(x.scalar_type()), weight.defined() ? over_rows(d * xh, weight) : Tensor(),
+          bias.defined() ? over_rows(d, bias) : Tensor()};
+}
 
 struct LayerNormBackward : public torch::autograd::Node {
   std::shared_ptr<NormCall> call;
@@ -155,33 +167,20 @@ struct LayerNormBackward : public torch::autograd::Node {
     std::lock_guard<std::mutex> lock(mutex_);
     const Tensor dy = grads[0];
     if (!dy.defined()) return variable_list(3);
-    variable_list out;
-    {
-      at::AutoGradMode off(false);
-      Tensor xv = x.unpack(), wv, bv;
-      if (has_weight) wv = weight.unpack();
-      if (has_bias) bv = bias.unpack();
-      NormCall c = *call;
-      if (xv.strides() != at::IntArrayRef(x_strides)) {  // tensors saved by a hook may come back with others
-        xv = xv.contiguous();
-        c.desc.inner = 1;
-        c.desc.inner_stride = c.desc.outer_stride = c.desc.channels;
-      }
-      const auto g = norm_gradients(c, dy.to(scalar_type(c.desc.y_dtype)).contiguous(), xv, wv, bv, statistics.unpack(),
-                                    task_should_compute_output(0), has_weight && task_should_compute_output(1),
-                                    has_bias && task_should_compute_output(2));
-      out = {g.dx, g.dweight, g.dbias};
+    Tensor xv = x.unpack(), wv, bv;
+    if (has_weight) wv = weight.unpack();
+    if (has_bias) bv = bias.unpack();
+    if (at::GradMode::is_enabled()) return norm_gradients_in_operations(*call, dy, xv, wv, bv);  // create_graph
+    NormCall c = *call;
+    if (xv.strides() != at::IntArrayRef(x_strides)) {  // tensors saved by a hook may come back with others
+      xv = xv.contiguous();
+      c.desc.inner = 1;
+      c.desc.inner_stride = c.desc.outer_stride = c.desc.channels;
     }
-    if (!at::GradMode::is_enabled()) return out;
-    // Asked for with create_graph: gradients that refuse to be differentiated, tied
-    // to all they depend on, since a pass to one of those would leave them out otherwise.
-    torch::autograd::edge_list sources = next_edges();
-    sources.push_back(torch::autograd::impl::gradient_edge(dy));
-    const std::shared_ptr<torch::autograd::Node> refuse(new torch::autograd::Error(kOnce, std::move(sources)),
-                                                        torch::autograd::deleteNode);
-    for (auto& t : out)
-      if (t.defined()) torch::autograd::set_history(t, refuse);
-    return out;
+    const auto g = norm_gradients(c, dy.to(scalar_type(c.desc.y_dtype)).contiguous(), xv, wv, bv, statistics.unpack(),
+                                  task_should_compute_output(0), has_weight && task_should_compute_output(1),
+                                  has_bias && task_should_compute_output(2));
+    return {g.dx, g.dweight, g.dbias};
   }
 };
 

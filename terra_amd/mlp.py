@@ -18,8 +18,9 @@ A call that needs a gradient runs autograd.mlp: the LayerNorm forward and
 backward (residual gradient included) on the HIP LayerNorm kernels over the
 token rows, the GEMMs on the linear and weight-gradient kernels where they
 serve the shapes, else on hipBLASLt.  Other shapes and dtypes run the
-reference's own sequence of torch modules on the device (norm2, fc1, act,
-fc2, residual).
+reference's own sequence of torch modules on the device (fc1, act, fc2,
+residual) behind norm2, which a plain LayerNorm or RMSNorm of any width
+has on the kernels of ``autograd.layer_norm``.
 
 Optional and build-defined, for regularised training: ``hidden_dropout``
 (after the GELU, in one launch with it), and the half-block's end, y =
@@ -40,7 +41,7 @@ import torch
 import torch.nn.functional as F
 
 from . import autograd, config, kernels
-from .attention import make_linear_with_seed, plain, plain_norm, probability
+from .attention import make_linear_with_seed, normed as norm_of, plain, plain_norm, probability
 
 
 def _disable_parameters_if_mlp_off(module: torch.nn.Module) -> None:
@@ -233,7 +234,7 @@ class SequentialMlp(torch.nn.Module):
             xn = autograd.partition_ln(rows.view(1, -1, 1, C), kernels.rows_geometry(rows.shape[0], C), n.weight, n.bias,
                                        n.eps, out_dtype=autograd.linear_input_dtype(rows), link=link).view(-1, C)
         else:
-            xn = self.norm2(x).reshape(rows.shape)
+            xn = norm_of(self.norm2, x).reshape(rows.shape)
         fc1, fc2, bias_sums = self.fc1, self.fc2, None
         own = [plain(fc, torch.nn.Linear) for fc in (fc1, fc2)]
         gelu = plain(self.act, torch.nn.GELU) and self.act.approximate == "none"
@@ -273,6 +274,6 @@ class SequentialMlp(torch.nn.Module):
                                 self.fc2.bias, n.eps)
         shortcut = x
         if config.use_layernorm:
-            x = self.norm2(x)
+            x = norm_of(self.norm2, x)
         x = self.fc2(self.act(self.fc1(x)))
         return x + shortcut

@@ -1,0 +1,167 @@
+"""AdamW over all parameters in a few launches (the reference trains with AdamW:
+optimizer/utils.py:8, optimizer/distributed_adamw.py:8), on
+``kernels.gradient_norm`` and ``kernels.adamw_step``.
+"""
+from __future__ import annotations
+
+from itertools import chain
+from typing import Callable, Optional, Tuple, Union
+
+import torch
+
+from . import kernels
+from .kernels import Moments
+
+_MOMENTS = ("exp_avg", "exp_avg_sq", "scales")
+
+
+class AdamW(torch.optim.Optimizer):
+    """``torch.optim.AdamW`` with fp32 moments whatever the parameters' dtype, or moments in 8
+    bits, and with clipping to a norm over all groups in the step itself.
+
+    ``bits``: 32, or 8 for parameters of at least ``min_8bit_size`` elements (see
+    :func:`kernels.adamw_step`; smaller ones keep 32).  ``seed`` fixes their random rounding (None: from torch's generator).
+    ``max_grad_norm``: gradients are scaled by min(1, max_grad_norm / (norm + 1e-6)) as
+    they are read; ``param.grad`` stays as it is, and ``grad_norm`` holds the norm (on
+    the device) after a step.  ``skip_nonfinite``: a step whose norm is infinite or
+    NaN changes nothing and is not counted.  ``capturable``: the count is kept in device
+    memory, so that a step may be captured into a graph (run one before); an
+    ``lr`` of a group may then be a one-element fp32 tensor on the device.
+
+    State dicts of ``torch.optim.AdamW`` load (and those of 32-bit moments load there)."""
+
+    def __init__(self, params, lr: Union[float, torch.Tensor] = 1e-3, betas: Tuple[float, float] = (0.9, 0.999),
+                 eps: float = 1e-8, weight_decay: float = 1e-2, *, maximize: bool = False, bits: int = 32,
+                 min_8bit_size: int = 4096, max_grad_norm: Optional[float] = None, skip_nonfinite: bool = False,
+                 capturable: bool = False, seed: Optional[int] = None):
+        if bits not in (8, 32):
+            raise ValueError(f"moments are held in 32 bits or in 8 (got {bits})")
+        if not isinstance(lr, torch.Tensor) and not lr >= 0.0:
+            raise ValueError(f"lr must be >= 0 (got {lr})")
+        if not all(0.0 <= b < 1.0 for b in betas) or len(betas) != 2:
+            raise ValueError(f"betas must be two numbers in [0, 1) (got {betas})")
+        if not eps >= 0.0 or not weight_decay >= 0.0:
+            raise ValueError(f"eps and weight_decay must be >= 0 (got {eps}, {weight_decay})")
+        if max_grad_norm is not None and not max_grad_norm > 0.0:
+            raise ValueError(f"max_grad_norm must be positive (got {max_grad_norm})")
+        if seed is None:
+            seed = int(torch.randint(0, 1 << 62, (1,)).item()) if bits == 8 else 0
+        super().__init__(params, dict(lr=lr, betas=tuple(betas), eps=eps, weight_decay=weight_decay, maximize=maximize,
+                                      bits=bits, min_8bit_size=min_8bit_size, seed=int(seed)))
+        self.max_grad_norm, self.skip_nonfinite, self.capturable = max_grad_norm, bool(skip_nonfinite), bool(capturable)
+        self.grad_norm: Optional[torch.Tensor] = None
+        self._seeds = {}
+
+    def __setstate__(self, state):
+        super().__setstate__(state)
+        self._seeds = {}
+
+    def __getstate__(self):
+        own = {k: v for k, v in self.__dict__.items() if k in ("max_grad_norm", "skip_nonfinite", "capturable", "grad_norm")}
+        return {**super().__getstate__(), **own}
+
+    def _seed(self, seed: int, device: torch.device) -> torch.Tensor:
+        t = self._seeds.get((seed, device))
+        if t is None:
+            t = self._seeds[seed, device] = torch.tensor([seed], dtype=torch.int64, device=device)
+        return t
+
+    def _begin(self, p: torch.Tensor, group: dict, count) -> dict:
+        m = kernels.moments(p, 8 if group["bits"] == 8 and p.numel() >= group["min_8bit_size"] else 32)
+        state = self.state[p]
+        state["step"] = count
+        state.update((k, v) for k, v in zip(_MOMENTS, m) if v is not None)
+        return state
+
+    @torch.no_grad()
+    def step(self, closure: Optional[Callable] = None):
+        loss = None
+        if closure is not None:
+            with torch.enable_grad():
+                loss = closure()
+        active = [[p for p in group["params"] if p.grad is not None] for group in self.param_groups]
+        grads = [p.grad for ps in active for p in ps]
+        if not grads:
+            return loss
+        norm = None
+        if self.max_grad_norm is not None or self.skip_nonfinite:
+            norm = kernels.gradient_norm(grads, self.max_grad_norm)
+            self.grad_norm = norm.norm
+        on_device = self.capturable or self.skip_nonfinite
+        for index, (group, params) in enumerate(zip(self.param_groups, active)):
+            for params, count in self._counted(group, params, on_device, norm):
+                moments = [Moments(s["exp_avg"], s["exp_avg_sq"], s.get("scales")) for s in map(self.state.__getitem__, params)]
+                kernels.adamw_step(params, [p.grad for p in params], moments, count, lr=group["lr"], betas=group["betas"],
+                                   eps=group["eps"], weight_decay=group["weight_decay"], maximize=group["maximize"],
+                                   grad_factor=None if norm is None or self.max_grad_norm is None else norm.factor,
+                                   found_inf=norm.nonfinite if self.skip_nonfinite else None,
+                                   seed=self._seed(group["seed"], params[0].device) if group["bits"] == 8 else None,
+                                   stream=index)
+        return loss
+
+    def _counted(self, group, params, on_device, norm):
+        """[(parameters, their count with this step)]: those that have taken as many steps, on the host
+        by the number, on the device by the counter that they share."""
+        sets, fresh = {}, None
+        for p in params:
+            state = self.state[p]
+            if "exp_avg" not in state:
+                if fresh is None:
+                    fresh = torch.zeros(1, dtype=torch.int64, device=p.device) if on_device else 0
+                state = self._begin(p, group, fresh)
+            count = state["step"]
+            sets.setdefault(id(count) if on_device else count, (count, []))[1].append(p)
+        if on_device:  # a parameter that takes no part in this step leaves the others' counter
+            left = {}
+            taking = set(map(id, params))
+            for p in group["params"]:
+                count = self.state[p].get("step") if p in self.state and id(p) not in taking else None
+                if count is not None and id(count) in sets:
+                    left.setdefault(id(count), count.clone())
+                    self.state[p]["step"] = left[id(count)]
+        out = []
+        for count, members in sets.values():
+            if on_device:
+                count.add_(1 if not self.skip_nonfinite else norm.nonfinite.eq(0))
+            else:
+                count += 1
+                for p in members:
+                    self.state[p]["step"] = count
+            out.append((members, count))
+        return out
+
+    def load_state_dict(self, state_dict):
+        super().load_state_dict(state_dict)
+        # Moments keep their own types (the parent casts them to the parameters').
+        ids = chain.from_iterable(g["params"] for g in state_dict["param_groups"])
+        counters = {}
+        for at, p in zip(ids, chain.from_iterable(g["params"] for g in self.param_groups)):
+            saved = state_dict["state"].get(at)
+            if not saved:
+                continue
+            state = self.state[p]
+            for name in _MOMENTS:
+                t = saved.get(name)
+                if t is None:
+                    continue
+                if name == "scales":
+                    state[name] = t.detach().to(device=p.device, dtype=torch.float32, copy=True).contiguous()
+                    continue
+                held = torch.float8_e4m3fn if saved.get("scales") is not None else torch.float32
+                if held != torch.float32 and t.stride() != p.stride():
+                    raise ValueError("moments in 8 bits of a parameter that lay otherwise in memory")
+                state[name] = torch.empty_like(p, dtype=held)
+                state[name].copy_(t.to(held))
+            on_device = self.capturable or self.skip_nonfinite
+            group = next(i for i, g in enumerate(self.param_groups) if any(q is p for q in g["params"]))
+            count = int(saved["step"])
+            if on_device:
+                key = (group, count)
+                if key not in counters:
+                    counters[key] = torch.tensor([count], dtype=torch.int64, device=p.device)
+                count = counters[key]
+            state["step"] = count
+        for group in self.param_groups:  # of torch.optim.AdamW's groups
+            for name, value in self.defaults.items():
+                group.setdefault(name, value)
+            group["betas"] = tuple(group["betas"])

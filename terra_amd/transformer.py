@@ -35,16 +35,18 @@ with the window reverse and the roll in one launch each way
 tokens, which stand in window order [B_, N, C]), ``layer_scale`` (a gate per
 channel, its initial value), ``residual_scale`` and ``dropout`` (in training
 mode; the mask is drawn from torch's seed and never stored).  ``forward(x, next_norm=norm)`` also gives ``norm(y)`` from the same
-launch, for an MLP half that takes it (``SequentialMlp.forward(y, normed=z)``).
+launch, for an MLP half that takes it (``SequentialMlp.forward(y, normed=z)``);
+``rotary`` — rotary positions of the query and key heads in each window
+(``WindowAttention``), on the staged path.
 """
 from __future__ import annotations
 
-from typing import Optional, Tuple
+from typing import Optional, Tuple, Union
 
 import torch
 
 from . import autograd, config, kernels
-from .attention import WindowAttention, plain, plain_norm, probability
+from .attention import WindowAttention, normed, plain, plain_norm, probability
 from .kernels import ShiftMask, WindowGeometry, WindowMask
 from .utils import get_swin_attention_mask, land_window_bits
 
@@ -57,7 +59,7 @@ class SequentialSwinTransformer(torch.nn.Module):
                  pad: Tuple[int, int, int, int] = (0, 0, 0, 0), win_row_begin: int = 0,
                  win_rows: Optional[int] = None, valid_windows: Optional[Tuple[int, int]] = None,
                  post_norm: bool = False, layer_scale: Optional[float] = None, residual_scale: float = 1.0,
-                 dropout: float = 0.0):
+                 dropout: float = 0.0, rotary: Union[None, bool, kernels.Rotary] = None):
         super().__init__()
         self.layer_idx = layer_idx
         self.init_seed_base = None if init_seed_base is None else int(init_seed_base) + int(layer_idx) * 100
@@ -75,7 +77,8 @@ class SequentialSwinTransformer(torch.nn.Module):
         self.attn = WindowAttention(embedding_dim, window_size=(window_size, window_size), num_heads=num_heads,
                                     qkv_bias=True, qk_scale=None, use_attn_mask=use_attn_mask,
                                     use_relative_position_bias=use_relative_position_bias,
-                                    use_flash_attention=use_flash_attention, init_seed_base=self.init_seed_base)
+                                    use_flash_attention=use_flash_attention, init_seed_base=self.init_seed_base,
+                                    rotary=rotary)
         self.pad = tuple(int(p) for p in pad)
         self.win_row_begin = int(win_row_begin)
         self.win_rows = win_rows
@@ -195,6 +198,8 @@ class SequentialSwinTransformer(torch.nn.Module):
         attn = self.attn
         if not self.use_fused_block or not kernels.swin_block_supported(x, geom, attn.num_heads):
             return False
+        if getattr(attn, "rotary", None) is not None:
+            return False
         if config.use_layernorm and not self._fusable_norm(x.dtype):
             return False
         if torch.is_grad_enabled() and (x.requires_grad or any(p.requires_grad for p in self.parameters())):
@@ -218,7 +223,7 @@ class SequentialSwinTransformer(torch.nn.Module):
         attn = self.attn
         lins = (attn.q_linear, attn.k_linear, attn.v_linear, attn.proj)
         return (config.use_layernorm and self._fusable_norm(x.dtype) and x.numel() <= 1 << 24
-                and type(attn) is WindowAttention
+                and type(attn) is WindowAttention and attn.rotary is None
                 and autograd._needs_grad(x, self.norm1.weight, self.norm1.bias, *(l.weight for l in lins[:3]))
                 and all(type(l) is torch.nn.Linear for l in lins) and attn.proj.bias is not None
                 and len({l.weight.dtype for l in lins[:3]}) == 1
@@ -235,6 +240,8 @@ class SequentialSwinTransformer(torch.nn.Module):
         440 -> 320."""
         attn = self.attn
         if not self.use_fused_block or not kernels.swin_block_f32_supported(x, geom, attn.num_heads):
+            return None
+        if getattr(attn, "rotary", None) is not None:
             return None
         if not self._plain_attn(attn, "forward", "attend", "qkv", "core"):
             return None
@@ -309,7 +316,7 @@ class SequentialSwinTransformer(torch.nn.Module):
             windows = autograd.partition_ln(grid, geom, n.weight, n.bias, n.eps,
                                             out_dtype=autograd.linear_input_dtype(grid), link=link)
         else:
-            windows = self.norm1(x).contiguous().view(grid.shape) if config.use_layernorm else grid
+            windows = normed(self.norm1, x).contiguous().view(grid.shape) if config.use_layernorm else grid
             windows = autograd.partition(windows, geom)
         h, post = self.attn(windows, mask=self.window_mask(geom)).contiguous(), self.post_norm1
         if post is not None and not plain_norm(post, C):
@@ -374,7 +381,7 @@ class SequentialSwinTransformer(torch.nn.Module):
                                               out_dtype=autograd.linear_input_dtype(grid), link=link)
         else:
             if config.use_layernorm:  # a norm layer the gather does not fuse runs on its own
-                grid = self.norm1(grid.view(B, L, C)).contiguous().view(B, H, W, C)
+                grid = normed(self.norm1, grid.view(B, L, C)).contiguous().view(B, H, W, C)
             x_windows = autograd.partition(grid, geom)
         bias_sums = None
         if not training and self._proj_scatter(x_windows, shortcut, geom):

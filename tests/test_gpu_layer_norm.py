@@ -294,13 +294,25 @@ class TestAutograd:
             kernels.layer_norm(t, Norm())
         check_forward(autograd.layer_norm(t, Norm()), t, Norm())
 
-    def test_second_derivatives_are_refused(self, dev):
-        x = _x((4, 32), F32).to(dev).requires_grad_()
-        w = torch.ones(32, device=dev, requires_grad=True)
-        y = autograd.layer_norm(x, Norm(w))
-        g, = torch.autograd.grad(y.square().sum(), x, create_graph=True)
-        with pytest.raises(RuntimeError, match="differentiated twice"):
-            torch.autograd.grad(g.sum(), x)
+    @pytest.mark.parametrize("rms", [False, True])
+    def test_second_derivatives(self, dev, rms):
+        """Of a pass in fp32 operations of torch: each of the some ten operations between the leaves and the second
+        derivative is off by C / 8 + 24 roundings of its largest terms."""
+        x, norm = _rand((4, 32), F32, 1).to(dev).requires_grad_(), _norm(32, rms=rms, dev=dev)
+        norm = Norm(norm.weight.requires_grad_(), norm.bias.requires_grad_(), norm.eps, rms)
+        leaves = (x, norm.weight, norm.bias)
+        y = autograd.layer_norm(x, norm)
+        g = torch.autograd.grad(y.pow(3).sum(), leaves, create_graph=True)
+        h = torch.autograd.grad(sum(t.square().sum() for t in g), leaves)
+        ref = [t.detach().cpu().double().requires_grad_() for t in leaves]
+        yr = tr.layer_norm(ref[0], ref[1], ref[2], norm.eps, rms)[0]
+        gr = torch.autograd.grad(yr.pow(3).sum(), ref, create_graph=True)
+        hr = torch.autograd.grad(sum(t.square().sum() for t in gr), ref)
+        for a, b in zip(g, gr):
+            check = (a.detach().cpu().double() - b.detach()).abs().max()
+            assert check <= 10 * 28 * U * max(t.abs().max() for t in gr).detach()
+        for a, b in zip(h, hr):
+            assert (a.cpu().double() - b).abs().max() <= 20 * 28 * U * max(t.abs().max() for t in hr)
 
     def test_forward_mode_is_refused(self, dev):
         x = _x((4, 32), F32).to(dev)

@@ -1,0 +1,275 @@
+"""Rotary positions in the window attention and the half-block, against the
+64-bit oracle; the norms that the halves call by themselves.
+
+Tolerances, those of the halves' other tests: fp32 within 1e-5 of the oracle's largest value for outputs and
+gradients; bf16 within 2e-2 of the largest output and 3e-2 normwise for outputs' attention term and gradients."""
+import copy
+import io
+
+import pytest
+import torch
+
+from helpers import gain_block, rel_maxabs, rel_norm
+from oracle import swin_oracle as so
+from oracle import training as tr
+from terra_amd import autograd, workloads
+from terra_amd.attention import WindowAttention, normed
+from terra_amd.kernels import Rotary
+from terra_amd.mlp import SequentialMlp
+from terra_amd.transformer import SequentialSwinTransformer
+
+pytestmark = pytest.mark.gpu
+
+F32, BF16 = torch.float32, torch.bfloat16
+CASES = [  # layer (1: shifted), H, W, C, heads, window, rotary, dtype, bias
+    (0, 14, 21, 96, 3, 7, True, F32, True),
+    (1, 14, 21, 96, 3, 7, Rotary(16, axes=2, interleaved=True, amplitude=1.2), F32, True),
+    (1, 16, 24, 192, 6, 8, True, BF16, True),
+    (0, 16, 16, 256, 4, 8, Rotary(32, axes=2, base=100.0), BF16, False),
+    (1, 64, 64, 256, 4, 32, True, BF16, False),
+]
+
+
+def _block(layer, H, W, C, heads, window, rot, bias):
+    blk = SequentialSwinTransformer(layer, H, W, C, window_size=window, num_heads=heads, rotary=rot,
+                                    use_attn_mask=bias, use_relative_position_bias=bias, init_seed_base=11)
+    return gain_block(blk)
+
+
+def _oracle(blk, x, grads=None):
+    """y, or with grads the gradients of x and the parameters, by the oracle."""
+    rot, attn = blk.attn.rotary, blk.attn
+    params = {k: v.detach().float().cpu().requires_grad_(grads is not None) for k, v in blk.named_parameters()}
+    x = x.detach().float().cpu().requires_grad_(grads is not None)
+    y = tr.swin_block_rotary(x, *blk.input_resolution, blk.window_size, blk.shift_size, attn.num_heads, params, rot.rates,
+                             rot.dim, rot.interleaved, rot.amplitude, blk.use_attn_mask)
+    if grads is None:
+        return y.detach()
+    got = torch.autograd.grad(y, [x, *params.values()], grads.detach().double().cpu())
+    return dict(zip(["x", *params], got))
+
+
+def _rel(dtype):
+    return (rel_maxabs, 1e-5) if dtype == F32 else (rel_norm, 3e-2)
+
+
+@pytest.mark.parametrize("case", CASES)
+def test_forward(dev, case):
+    layer, H, W, C, heads, window, rot, dtype, bias = case
+    blk = _block(layer, H, W, C, heads, window, rot, bias).to(dev).to(dtype)
+    x = workloads.activations((2, H * W, C), 7, dtype)
+    with torch.no_grad():
+        y = blk(x.to(dev))
+    ref = _oracle(blk, x)
+    assert rel_maxabs(y, ref) <= (1e-5 if dtype == F32 else 2e-2)
+    norm, tol = _rel(dtype)
+    assert norm(y.double().cpu() - x.double(), ref - x.double()) <= tol
+    off = SequentialSwinTransformer(layer, H, W, C, window_size=window, num_heads=heads, use_attn_mask=bias,
+                                    use_relative_position_bias=bias).to(dev).to(dtype)
+    off.load_state_dict(blk.state_dict())  # the positions are no parameters
+    with torch.no_grad():
+        assert rel_maxabs(off(x.to(dev)), ref) > 0.05
+
+
+@pytest.mark.parametrize("case", CASES)
+def test_backward(dev, case):
+    layer, H, W, C, heads, window, rot, dtype, bias = case
+    blk = _block(layer, H, W, C, heads, window, rot, bias).to(dev).to(dtype)
+    x = workloads.activations((1, H * W, C), 7, dtype).to(dev).requires_grad_()
+    dy = workloads.activations((1, H * W, C), 8, dtype)
+    blk(x).backward(dy.to(dev))
+    ref = _oracle(blk, x, dy)
+    got = {"x": x.grad, **{k: p.grad for k, p in blk.named_parameters()}}
+    norm, tol = _rel(dtype)
+    for name, g in ref.items():
+        if name.endswith("k_linear.bias") and not bias:
+            pass  # not 0 here: a key's bias is turned with it
+        assert norm(got[name], g) <= tol, name
+
+
+def test_under_autocast(dev):
+    """fp32 parameters under bf16 autocast, the types that the block without positions has."""
+    blk = _block(1, 16, 24, 192, 6, 8, True, True).to(dev)
+    x = workloads.activations((1, 384, 192), 7, F32).to(dev).requires_grad_()
+    with torch.autocast("cuda", torch.bfloat16):
+        y = blk(x)
+    assert y.dtype == F32
+    y.backward(torch.ones_like(y))
+    ref = _oracle(blk, x)
+    assert rel_norm(y.detach().cpu() - x.detach().cpu(), ref - x.detach().double().cpu()) <= 3e-2
+    grads = _oracle(blk, x, torch.ones_like(y))
+    for name, p in blk.named_parameters():
+        assert p.grad.dtype == F32 and rel_norm(p.grad, grads[name]) <= 3e-2, name
+
+
+def test_with_the_regularised_tail(dev):
+    kw = dict(window_size=8, num_heads=6, rotary=True, post_norm=True, layer_scale=0.5, residual_scale=0.75)
+    blk = SequentialSwinTransformer(1, 16, 16, 192, **kw).to(dev)
+    x = workloads.activations((2, 256, 192), 7, F32).to(dev).requires_grad_()
+    y, z = blk(x, next_norm=torch.nn.LayerNorm(192, device=dev))
+    (y.sum() + z.square().sum()).backward()
+    assert all(p.grad is not None and p.grad.isfinite().all() for p in blk.parameters())
+
+
+def test_only_differences_of_positions_count(dev):
+    """All positions moved by the same rows and columns: the same attention, to what fp32 rounding makes of angles and logits."""
+    attn = WindowAttention(96, (7, 7), 3, rotary=True, use_relative_position_bias=False).to(dev)
+    with torch.no_grad():
+        for p in attn.parameters():
+            p.mul_(6.0)
+        x = workloads.activations((4, 49, 96), 3, F32).to(dev)
+        a = attn(x)
+        attn.token_positions += torch.tensor([1000, -77], device=dev, dtype=torch.int32)
+        assert rel_maxabs(attn(x), a) <= 1e-5
+
+
+def test_positions_of_a_module(dev):
+    attn = WindowAttention(64, (3, 5), 2, rotary=True)
+    assert attn.token_positions.tolist() == [[i, j] for i in range(3) for j in range(5)]
+    assert "token_positions" not in attn.state_dict()
+    assert WindowAttention(64, (3, 5), 2).rotary is None and WindowAttention(64, (3, 5), 2, rotary=False).rotary is None
+    for bad in (Rotary(32), Rotary(64, axes=2)):
+        with pytest.raises(ValueError, match="two axes"):
+            WindowAttention(64, (3, 5), 2, rotary=bad)
+    with pytest.raises(ValueError, match="positions of the tokens"):
+        WindowAttention(64, (8, 8), 2, rotary=True).to(dev)(torch.zeros(1, 49, 64, device=dev))
+
+
+def test_copies_and_pickles(dev):
+    blk = _block(1, 16, 24, 192, 6, 8, True, True).to(dev)
+    x = workloads.activations((1, 384, 192), 7, F32).to(dev)
+    with torch.no_grad():
+        y = blk(x)
+        f = io.BytesIO()
+        torch.save(blk, f)
+        f.seek(0)
+        for other in (copy.deepcopy(blk), torch.load(f, weights_only=False)):  # of a file that this test wrote
+            assert torch.equal(other(x), y)
+    old = SequentialSwinTransformer(1, 16, 24, 192, window_size=8, num_heads=6)
+    old.attn.__dict__.pop("rotary")  # as one of before would have been pickled
+    f = io.BytesIO()
+    torch.save(old, f)
+    f.seek(0)
+    assert torch.load(f, weights_only=False).attn.rotary is None
+
+
+def test_captured(dev):
+    blk = _block(0, 16, 24, 192, 6, 8, True, True).to(dev).to(BF16)
+    x = workloads.activations((1, 384, 192), 7, BF16).to(dev)
+    with torch.no_grad():
+        blk(x)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            y = blk(x)
+        for seed in range(3):
+            x.copy_(workloads.activations((1, 384, 192), seed, BF16))
+            graph.replay()
+            eager = blk(x)
+            torch.cuda.synchronize()
+            assert torch.equal(y, eager)
+
+
+# ---- the halves' own norms -------------------------------------------------------
+
+
+def _mlp(C, norm=None, act=torch.nn.GELU, seed=3):
+    m = SequentialMlp(C, 2 * C, act_layer=act, init_seed_base=seed)
+    if norm is not None:
+        m.norm2 = norm
+    with torch.no_grad():
+        for i, p in enumerate(m.parameters()):
+            p.copy_(workloads.activations(p.shape, 50 + i, F32) * (0.3 if p.dim() > 1 else 0.2) + (1.0 if p.dim() == 1 and i == 0 else 0.0))
+    return m
+
+
+@pytest.mark.parametrize("C", [100, 130, 1200])
+def test_mlp_of_other_widths(dev, C):
+    m = _mlp(C).to(dev)
+    x = workloads.activations((3, 40, C), 7, F32).to(dev).requires_grad_()
+    y = m(x)
+    assert type(y.grad_fn).__name__ != "LayerNormBackward"
+    params = {k: p.detach().cpu().requires_grad_() for k, p in m.named_parameters()}
+    xr = x.detach().cpu().requires_grad_()
+    ref = tr.mlp(xr.double(), params)
+    assert rel_maxabs(y, ref) <= 1e-5
+    dy = workloads.activations((3, 40, C), 8, F32)
+    y.backward(dy.to(dev))
+    grads = torch.autograd.grad(ref, [xr, *params.values()], dy.double())
+    for got, g in zip([x.grad, *(p.grad for p in m.parameters())], grads):
+        assert rel_maxabs(got, g) <= 1e-5
+
+
+class TestNormed:
+    """What the kernels serve, and what stays torch's."""
+
+    def _same(self, module, x, tol=1e-6):
+        y, ref = normed(module, x), module(x)
+        assert y.dtype == ref.dtype and y.shape == ref.shape
+        assert rel_maxabs(y, ref) <= tol
+        return y
+
+    def test_types(self, dev):
+        for C in (100, 1030, 4096):
+            ln, rms = torch.nn.LayerNorm(C, device=dev), torch.nn.RMSNorm(C, device=dev)
+            x = workloads.activations((5, C), 3, F32).to(dev)
+            for n in (ln, rms, torch.nn.LayerNorm(C, elementwise_affine=False), torch.nn.LayerNorm(C, bias=False, device=dev)):
+                assert normed(n, x.clone().requires_grad_()).grad_fn.name() == "LayerNormBackward"
+                self._same(n, x)
+            self._same(copy.deepcopy(ln).to(BF16), x.to(BF16), 2.0 ** -7)  # two roundings of bf16 apart at most
+            self._same(copy.deepcopy(rms).half(), x.half(), 2.0 ** -10)
+            with torch.autocast("cuda", BF16):
+                assert self._same(ln, x).dtype == F32
+                assert self._same(ln, x.to(BF16)).dtype == F32
+
+    def test_hooks_see_the_call(self, dev):
+        ln, seen = torch.nn.LayerNorm(100, device=dev), []
+        ln.register_forward_hook(lambda *a: seen.append(1))
+        normed(ln, torch.zeros(2, 100, device=dev))
+        assert seen == [1]
+
+    def test_other_norms_are_called(self, dev):
+        class Own(torch.nn.LayerNorm):
+            def forward(self, x):
+                return super().forward(x) + 1
+
+        x = torch.ones(2, 100, device=dev)
+        own = Own(100, device=dev)
+        assert torch.equal(normed(own, x), own(x)) and normed(own, x).grad_fn.name() == "AddBackward0"
+        assert normed(torch.nn.Identity(), x) is x
+        assert normed(torch.nn.LayerNorm(100, device=dev, dtype=torch.float64), x.double()).dtype == torch.float64
+
+    def test_transforms_are_torchs(self, dev):
+        ln, x = torch.nn.LayerNorm(100, device=dev), workloads.activations((5, 100), 3, F32).to(dev)
+        f = lambda t: normed(ln, t).pow(3).sum()  # noqa: E731
+        g = torch.func.grad(f)(x)
+        t = x.clone().requires_grad_()
+        assert rel_maxabs(g, torch.autograd.grad(f(t), t)[0]) <= 1e-5
+        tangent = torch.ones_like(x)
+        with torch.autograd.forward_ad.dual_level():
+            d = torch.autograd.forward_ad.unpack_dual(normed(ln, torch.autograd.forward_ad.make_dual(x, tangent)))
+            assert d.tangent is not None
+        assert torch.func.vmap(lambda t: normed(ln, t))(x).shape == x.shape
+
+    def test_second_derivatives(self, dev):
+        ln, x = torch.nn.LayerNorm(100, device=dev), workloads.activations((5, 100), 3, F32).to(dev).requires_grad_()
+        outs = []
+        for f in (lambda t: normed(ln, t), lambda t: ln(t)):
+            g, = torch.autograd.grad(f(x).pow(3).sum(), x, create_graph=True)
+            outs.append(torch.autograd.grad(g.square().sum(), x)[0])
+        assert rel_maxabs(*outs) <= 1e-5
+
+
+@pytest.mark.parametrize("norm_layer", [torch.nn.LayerNorm, torch.nn.RMSNorm])
+def test_attention_half_with_a_norm_of_its_own(dev, norm_layer):
+    """A norm that the gather does not take runs over the rows by the norm kernels."""
+    blk = SequentialSwinTransformer(1, 14, 14, 96, window_size=7, num_heads=3, norm_layer=norm_layer, init_seed_base=5).to(dev)
+    x = workloads.activations((2, 196, 96), 7, F32).to(dev)
+    if norm_layer is torch.nn.RMSNorm:
+        with torch.no_grad():
+            y = blk(x)
+            called = copy.deepcopy(blk)
+            called.norm1.register_forward_hook(lambda *a: None)
+            assert rel_maxabs(y, called(x)) <= 1e-6
+    t = x.clone().requires_grad_()
+    blk(t).sum().backward()
+    assert t.grad.isfinite().all() and blk.norm1.weight.grad is not None
