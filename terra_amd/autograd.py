@@ -847,8 +847,8 @@ def layer_norm(x: torch.Tensor, norm: Norm, out_dtype: Optional[torch.dtype] = N
 
 
 class _Rotary(torch.autograd.Function):
-    """kernels.rotary.  A linear map: a tangent is turned as the values are, a
-    gradient back, and that may be differentiated again."""
+    """kernels.rotary of a dual tensor.  A linear map: a tangent is turned as the
+    values are, a gradient back, and that may be differentiated again."""
 
     @staticmethod
     def forward(ctx, x, rot, positions, inverse):
@@ -869,15 +869,14 @@ class _Rotary(torch.autograd.Function):
 def rotary(x: torch.Tensor, rot: kernels.Rotary, positions: torch.Tensor, inverse: bool = False) -> torch.Tensor:
     """:func:`kernels.rotary` with derivatives of every order, backward and
     forward mode.  Heads that the kernel cannot read in place are copied first."""
-    if x.dim() >= 2 and x.stride(-1) != 1:
-        x = x.contiguous()
     positions = positions.contiguous()
     try:
-        kernels._rotary_call(x, rot, positions, inverse, None)
+        call = kernels._rotary_call(x, rot, positions, bool(inverse), None)
     except ValueError:
         if x.is_contiguous():
             raise
         x = x.contiguous()
-    if _needs_grad(x) or _has_tangent(x):
-        return _Rotary.apply(x, rot, positions, inverse)
-    return kernels.rotary(x, rot, positions, inverse)
+        call = kernels._rotary_call(x, rot, positions, bool(inverse), None)
+    if _has_tangent(x):
+        return _Rotary.apply(x, rot, positions, bool(inverse))
+    return _lib.load_training().rotary_with_gradient(call, x, positions, rot.turns(x.device))

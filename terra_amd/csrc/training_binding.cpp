@@ -280,7 +280,6 @@ std::shared_ptr<RotaryCall> make_rotary_call(const std::string& desc) {
 
 Tensor rotary(const std::shared_ptr<RotaryCall>& call, const Tensor& x, const Tensor& positions, const Tensor& turns,
               const std::optional<Tensor>& out) {
-  const pybind11::gil_scoped_release no_gil;
   const at::AutoGradMode off(false);
   const c10::DeviceGuard guard(x.device());
   Tensor y;
@@ -293,6 +292,51 @@ Tensor rotary(const std::shared_ptr<RotaryCall>& call, const Tensor& x, const Te
   if (call->desc.tokens > 0)
     check(rotary_entry(x.const_data_ptr(), y.data_ptr(), positions.const_data_ptr(),
                        static_cast<const double*>(turns.const_data_ptr()), &call->desc, current_stream(x)), "terra_swin_rotary");
+  return y;
+}
+
+// The gradient's call: the turn back, from a packed gradient into a packed one.
+std::shared_ptr<RotaryCall> backward_call(const RotaryCall& c) {
+  auto b = std::make_shared<RotaryCall>(c);
+  auto& d = b->desc;
+  d.inverse = !d.inverse;
+  d.x_head_stride = d.y_head_stride = d.head_dim;
+  d.x_inner_stride = d.y_inner_stride = static_cast<int64_t>(d.heads) * d.head_dim;
+  d.x_outer_stride = d.y_outer_stride = d.inner * d.x_inner_stride;
+  return b;
+}
+
+Tensor rotary_with_gradient(const std::shared_ptr<RotaryCall>& call, const Tensor& x, const Tensor& positions, const Tensor& turns);
+
+// A linear map: its gradient is turned back, and may be differentiated again.
+struct RotaryBackward : public torch::autograd::Node {
+  std::shared_ptr<RotaryCall> call;  // of the gradient
+  SavedVariable positions, turns;
+
+  std::string name() const override { return "RotaryBackward"; }
+
+  void release_variables() override {
+    std::lock_guard<std::mutex> lock(mutex_);
+    positions.reset_data();
+    turns.reset_data();
+  }
+
+  variable_list apply(variable_list&& grads) override {
+    std::lock_guard<std::mutex> lock(mutex_);
+    if (!grads[0].defined()) return variable_list(1);
+    return {rotary_with_gradient(call, grads[0].contiguous(), positions.unpack(), turns.unpack())};
+  }
+};
+
+Tensor rotary_with_gradient(const std::shared_ptr<RotaryCall>& call, const Tensor& x, const Tensor& positions, const Tensor& turns) {
+  Tensor y = rotary(call, x, positions, turns, std::nullopt);
+  if (!x.requires_grad() || !at::GradMode::is_enabled()) return y;
+  std::shared_ptr<RotaryBackward> node(new RotaryBackward(), torch::autograd::deleteNode);
+  node->set_next_edges({torch::autograd::impl::gradient_edge(x)});
+  node->call = backward_call(*call);
+  node->positions = SavedVariable(positions, false);
+  node->turns = SavedVariable(turns, false);
+  torch::autograd::set_history(y, node);
   return y;
 }
 
@@ -436,7 +480,9 @@ PYBIND11_MODULE(_training, m) {
   m.def("layer_norm", &layer_norm);
   m.def("layer_norm_forward", &layer_norm_forward);
   m.def("layer_norm_backward", &layer_norm_backward);
-  m.def("rotary", &rotary);
+  const auto no_gil = pybind11::call_guard<pybind11::gil_scoped_release>();  // a launch may wait for room in the queue
+  m.def("rotary", &rotary, no_gil);
+  m.def("rotary_with_gradient", &rotary_with_gradient, no_gil);
   m.def("gradient_norm", &gradient_norm);
   m.def("adamw_step", [](const std::vector<Tensor>& params, const std::vector<Tensor>& grads, const std::vector<Tensor>& firsts,
                          const std::vector<Tensor>& seconds, const std::vector<std::optional<Tensor>>& scales, double lr,
