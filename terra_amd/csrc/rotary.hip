@@ -35,22 +35,31 @@ struct RotaryArgs {
   float amplitude, sign;
 };
 
-// kN elements that lie side by side, one access where aligned (to all of them).
-template <int DT, int kN, bool kAligned>
+// kN elements that lie side by side, one access where aligned (to all of them).  kStream: past the
+// caches; lines that several accesses share stay there until the last of them.
+template <int DT, int kN, bool kAligned, bool kStream>
 struct RotaryRun {
   static constexpr int kB = ChunkElt<DT>::kBytes, kWords = (kN * kB + 3) / 4;
   typedef uint32_t Vec __attribute__((ext_vector_type(kWords)));
   uint32_t w[kWords];
 
+  template <typename V>
+  static __device__ __forceinline__ V read(const uint8_t* p) {
+    if constexpr (kStream) return __builtin_nontemporal_load(reinterpret_cast<const V*>(p));
+    else return *reinterpret_cast<const V*>(p);
+  }
+  template <typename V>
+  static __device__ __forceinline__ void write(V v, uint8_t* p) {
+    if constexpr (kStream) __builtin_nontemporal_store(v, reinterpret_cast<V*>(p));
+    else *reinterpret_cast<V*>(p) = v;
+  }
   __device__ __forceinline__ void load(const uint8_t* p) {
-    if constexpr (kAligned) {
-      if constexpr (kWords == 1) {
-        w[0] = __builtin_nontemporal_load(reinterpret_cast<const uint32_t*>(p));
-      } else {
-        const Vec v = __builtin_nontemporal_load(reinterpret_cast<const Vec*>(p));
+    if constexpr (kAligned && kWords == 1) {
+      w[0] = read<uint32_t>(p);
+    } else if constexpr (kAligned) {
+      const Vec v = read<Vec>(p);
 #pragma unroll
-        for (int i = 0; i < kWords; ++i) w[i] = v[i];
-      }
+      for (int i = 0; i < kWords; ++i) w[i] = v[i];
     } else if constexpr (kB == 4) {
 #pragma unroll
       for (int i = 0; i < kWords; ++i) w[i] = reinterpret_cast<const uint32_t*>(p)[i];
@@ -61,15 +70,13 @@ struct RotaryRun {
     }
   }
   __device__ __forceinline__ void store(uint8_t* p) const {
-    if constexpr (kAligned) {
-      if constexpr (kWords == 1) {
-        __builtin_nontemporal_store(w[0], reinterpret_cast<uint32_t*>(p));
-      } else {
-        Vec v;
+    if constexpr (kAligned && kWords == 1) {
+      write(w[0], p);
+    } else if constexpr (kAligned) {
+      Vec v;
 #pragma unroll
-        for (int i = 0; i < kWords; ++i) v[i] = w[i];
-        __builtin_nontemporal_store(v, reinterpret_cast<Vec*>(p));
-      }
+      for (int i = 0; i < kWords; ++i) v[i] = w[i];
+      write(v, p);
     } else if constexpr (kB == 4) {
 #pragma unroll
       for (int i = 0; i < kWords; ++i) reinterpret_cast<uint32_t*>(p)[i] = w[i];
@@ -102,10 +109,10 @@ constexpr int kRotaryThreads = 256;
 // of kP.  Behind the rotated items come those that are copied, 2 kP elements each, which go
 // through the same loop: a line that holds some of both is read and written at once.  kAhead: heads that a
 // thread reads at a time.
-template <int DT, int kP, bool kInterleaved, bool kAligned, int kAhead>
+template <int DT, int kP, bool kInterleaved, bool kAligned, bool kStream, int kAhead>
 __global__ __launch_bounds__(kRotaryThreads) void rotary_kernel(const RotaryArgs a) {
   constexpr int kB = ChunkElt<DT>::kBytes, kRun = kInterleaved ? 2 * kP : kP, kRuns = kInterleaved ? 1 : 2;
-  typedef RotaryRun<DT, kRun, kAligned> Run;
+  typedef RotaryRun<DT, kRun, kAligned, kStream> Run;
   const int first = blockIdx.y * a.per_thread, last = min(first + a.per_thread, a.heads);
   uint32_t local, lane;
   a.lanes.divmod(threadIdx.x, local, lane);
@@ -136,7 +143,7 @@ __global__ __launch_bounds__(kRotaryThreads) void rotary_kernel(const RotaryArgs
           if (whole) {
             f.r[k][0].load(xh + lo);
           } else {  // the last element of an odd rest
-            RotaryRun<DT, 1, false> one;
+            RotaryRun<DT, 1, false, false> one;
             one.load(xh + lo);
             f.r[k][0].w[0] = one.w[0];
           }
@@ -181,7 +188,7 @@ __global__ __launch_bounds__(kRotaryThreads) void rotary_kernel(const RotaryArgs
           if (whole) {
             f.r[k][0].store(yh + lo);
           } else {
-            RotaryRun<DT, 1, false> one;
+            RotaryRun<DT, 1, false, false> one;
             one.w[0] = f.r[k][0].w[0];
             one.store(yh + lo);
           }
@@ -207,9 +214,21 @@ void launch_rotary(RotaryArgs a, hipStream_t s) {
   a.per_thread = (int32_t)((a.heads + groups - 1) / groups);
   const uint32_t need = (a.tokens + a.per_block - 1) / a.per_block, most = 1u << 22;
   const dim3 grid(need < most ? need : most, (unsigned)((a.heads + a.per_thread - 1) / a.per_thread));
+  // Past the caches where what the lanes of a head read at once is whole lines of 128 bytes (156672 tokens of 16
+  // heads of 128 bf16, pairs 64 apart: 231 us, 254 through them; but 312500 of 6 heads of 32, whose lines
+  // hold four such pieces: 111 us, 61 through them; 46875 of 16 heads of 80: 100 and 59).
+  constexpr int kB = ChunkElt<DT>::kBytes;
+  const bool lines = kInterleaved ? (2 * a.half + a.rest) * kB % 128 == 0 : a.half * kB % 128 == 0 && a.rest * kB % 256 == 0;
   // Four heads ahead take registers that a thread of few heads has better use for (200000 x 1 of 128: 29 us, 36 so).
-  if (a.per_thread >= 4) rotary_kernel<DT, kP, kInterleaved, kAligned, 4><<<grid, kRotaryThreads, 0, s>>>(a);
-  else rotary_kernel<DT, kP, kInterleaved, kAligned, 1><<<grid, kRotaryThreads, 0, s>>>(a);
+  const bool many = a.per_thread >= 4;
+  if constexpr (kAligned)
+    if (lines) {
+      if (many) rotary_kernel<DT, kP, kInterleaved, true, true, 4><<<grid, kRotaryThreads, 0, s>>>(a);
+      else rotary_kernel<DT, kP, kInterleaved, true, true, 1><<<grid, kRotaryThreads, 0, s>>>(a);
+      return;
+    }
+  if (many) rotary_kernel<DT, kP, kInterleaved, kAligned, false, 4><<<grid, kRotaryThreads, 0, s>>>(a);
+  else rotary_kernel<DT, kP, kInterleaved, kAligned, false, 1><<<grid, kRotaryThreads, 0, s>>>(a);
 }
 
 template <int DT, bool kInterleaved>
