@@ -41,13 +41,61 @@ struct NormArgs {
   }
 };
 
-// Parameter c in fp32, `none` where the pointer is NULL.
-__device__ __forceinline__ float norm_param(const void* p, int dtype, float none, int c) {
-  if (p == nullptr) return none;
-  if (dtype == TERRA_DTYPE_F32) return reinterpret_cast<const float*>(p)[c];
-  const uint16_t v = reinterpret_cast<const uint16_t*>(p)[c];
-  return dtype == TERRA_DTYPE_BF16 ? bf16_bits_to_f32(v) : __half2float(__ushort_as_half(v));
+// Calls f(load), where load(c) is parameter c in fp32 (`none` where the pointer is NULL): the type is asked once, so that
+// the loads of f stand side by side.
+template <typename F>
+__device__ __forceinline__ void with_param(const void* p, int dtype, float none, F f) {
+  if (p == nullptr) f([&](int) { return none; });
+  else if (dtype == TERRA_DTYPE_F32) f([&](int c) { return reinterpret_cast<const float*>(p)[c]; });
+  else if (dtype == TERRA_DTYPE_BF16) f([&](int c) { return bf16_bits_to_f32(reinterpret_cast<const uint16_t*>(p)[c]); });
+  else f([&](int c) { return __half2float(__ushort_as_half(reinterpret_cast<const uint16_t*>(p)[c])); });
 }
+
+// A parameter of a row's lanes: in LDS where rows share a workgroup (kG <= 64; the caller adds the
+// barrier), else, each lane's columns being its own, in registers.  0 in absent columns.
+template <int kG, int kK, int kP>
+struct NormParam {
+  static constexpr bool kLds = kG <= 64;
+  static constexpr int kCols = kG * kK * kChunkCols, kThreads = tail_threads(kG);
+  struct Shared { __attribute__((aligned(16))) float v[kLds ? kCols : 4]; };
+  Shared* s;
+  float r[kLds ? 1 : kK][kChunkCols];
+
+  __device__ __forceinline__ explicit NormParam(Shared* shared) : s(shared) {}
+
+  template <bool kVec>
+  __device__ __forceinline__ void fill(const RowLanes<kG, kK, kP>& at, const void* p, int dtype, float none) {
+    const int C = at.C;
+    with_param(p, dtype, none, [&](auto load) {
+      if constexpr (kLds) {
+        for (int c = threadIdx.x; c < kCols; c += kThreads) s->v[c] = c < C ? load(c) : 0.f;
+      } else {
+#pragma unroll
+        for (int k = 0; k < kK; ++k)
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const int col = at.base(k, h);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {  // kVec: four at once
+              const bool has = at.template has<kVec>(k, 4 * h + j);
+              const float v = load(kVec ? (has ? col : 0) + j : (has ? col + j : 0));
+              r[k][4 * h + j] = has ? v : 0.f;
+            }
+          }
+      }
+    });
+  }
+  __device__ __forceinline__ void get(int k, const RowLanes<kG, kK, kP>& at, float (&f)[kChunkCols]) const {
+    if constexpr (kLds) {
+      const float4 lo = *reinterpret_cast<const float4*>(&s->v[at.base(k, 0)]);
+      const float4 hi = *reinterpret_cast<const float4*>(&s->v[at.base(k, 1)]);
+      f[0] = lo.x, f[1] = lo.y, f[2] = lo.z, f[3] = lo.w, f[4] = hi.x, f[5] = hi.y, f[6] = hi.z, f[7] = hi.w;
+    } else {
+#pragma unroll
+      for (int j = 0; j < kChunkCols; ++j) f[j] = r[k][j];
+    }
+  }
+};
 
 // The statistics of a row held as kK chunks a lane: v becomes xh (zero in
 // absent columns), r is returned.
@@ -86,6 +134,7 @@ __device__ __forceinline__ float norm_row(float (&v)[kK][kChunkCols], bool layer
 struct NormPlan {
   uint32_t parts;  // workgroups of the sums over rows
   bool held;       // rows are held in registers (else read again)
+  bool flat;       // and read by the aligned chunks of the packed tensor
   TailShape shape;
 };
 #define TERRA_NORM_TYPES(X) X(f32, f32) X(f32, bf16) X(f32, f16) X(bf16, bf16) X(bf16, f32) X(f16, f16) X(f16, f32)

@@ -11,8 +11,11 @@ constexpr int kNormMaxChannels = 1 << 24;
 struct NormAlignment {
   uintptr_t bits = 0;
   int C = 0;
+  bool packed = false;       // x's rows follow each other
+  uintptr_t pointers = 0;    // the bits of the addresses alone
   bool vec() const { return C % kChunkCols == 0 && bits % 16 == 0; }
   bool pairs() const { return C % 2 == 0 && bits % 4 == 0; }
+  bool flat() const { return !vec() && packed && pointers % 16 == 0; }
 };
 
 bool is_float(int dtype) { return dtype == TERRA_DTYPE_F32 || dtype == TERRA_DTYPE_BF16 || dtype == TERRA_DTYPE_F16; }
@@ -44,14 +47,16 @@ int norm_prepare(const terra_swin_layer_norm_desc* d, NormArgs* a, NormAlignment
   a->eps = d->eps;
   a->inv_c = 1.f / (float)d->channels;
   al->C = a->C;
+  al->packed = (d->rows <= 1 || (d->inner_stride == d->channels || d->inner == 1)) &&
+               (d->rows <= d->inner || d->outer_stride == d->inner * d->channels);
   al->bits = (d->rows > d->inner ? (uintptr_t)a->outer_bytes : 0) | (d->inner > 1 ? (uintptr_t)a->step_bytes : 0);
   return TERRA_OK;
 }
 
-int norm_pointer(const void* p, int dtype, const char* name, bool needed, uintptr_t* bits) {
+int norm_pointer(const void* p, int dtype, const char* name, bool needed, NormAlignment* al) {
   if (p == nullptr) return needed ? fail(TERRA_ERR_NULL, "%s is NULL", name) : TERRA_OK;
   if ((uintptr_t)p % (uintptr_t)dtype_size(dtype) != 0) return fail(TERRA_ERR_ALIGN, "%s is not aligned to its elements", name);
-  if (bits != nullptr) *bits |= (uintptr_t)p;
+  if (al != nullptr) al->bits |= (uintptr_t)p, al->pointers |= (uintptr_t)p;
   return TERRA_OK;
 }
 
@@ -67,33 +72,56 @@ bool norm_meet(const void* p, int64_t bytes, const void* q, int64_t more) {
   return p != nullptr && q != nullptr && bytes > 0 && more > 0 && a < b + (uintptr_t)more && b < a + (uintptr_t)bytes;
 }
 
-constexpr int kNormHeld = 8192;  // channels of rows that are held in registers
+constexpr int kNormHeld = 16384;  // channels of rows that are held in registers
 
 // How many lanes and chunks hold a row.  Waves rather than workgroups as far as the registers
 // go: what its lanes add up needs no barrier (39168 x 4096 bf16, forward: 118 us, as 512 lanes
 // of one chunk 135; 78336 x 2048: 108 and 143).  The backward, with two sums for each column
 // and two rows, goes so far as four chunks (78336 x 2048: 156 us, as 256 lanes 167; 39168 x 4096 as
 // 256 lanes of two 161, as waves of eight 175); rows that are not aligned or that have fp32 in them as far as two
-// where a few lanes hold them.  Eight lanes where a row has at most eight chunks: the heads of a packed q | k | v.
+// where a few lanes hold them.  As few lanes as chunks where a row has at most eight: the heads of a packed q | k | v.
 TailShape norm_shape(int C, bool pieces, bool vec, bool backward) {
   const int n = (C + kChunkCols - 1) / kChunkCols;
-  if (n <= 8) return {8, 1};
+  if (n <= 8) return {n <= 2 ? 2 : n <= 4 ? 4 : 8, 1};
+  if (n > 1024) return {1024, 2};
   if (n > 512) return {512, 2};
   if (n > 256) return backward ? TailShape{256, 2} : TailShape{64, 8};
   if (n > 128) return {64, 4};
   return tail_shape(C, pieces, backward && (pieces || !vec) ? 2 : 3);
 }
 
+// The same for rows that are read by the aligned chunks of the tensor, a chunk more than C takes where the
+// row begins in one.  Parameters stand in registers too: two chunks a lane, up to four where waves can hold the row so
+// (58252 x 1030 bf16: 70 and 82 us forward and backward, as waves of four chunks 84 and 141, as 256 lanes 99 and 163).
+TailShape flat_shape(int C, int chunk) {
+  const int n = (C + chunk - 1 + kChunkCols - 1) / kChunkCols;
+  if (n <= 16) return {n <= 8 ? 8 : 16, 1};
+  if (n <= 128) return {n <= 32 ? 16 : n <= 64 ? 32 : 64, 2};
+  if (n <= 256) return {64, n <= 192 ? 3 : 4};
+  return {n <= 512 ? 256 : n <= 1024 ? 512 : 1024, 2};
+}
+
+// Whether packed rows that are not whole chunks are read by the tensor's aligned chunks or by columns, 60 million elements
+// (flat, by columns; us): 1001 bf16 forward 68, 92, backward 76, 134; 1030 fp32 106, 121 and 134, 216; 4097 fp32
+// 96, 129 and 144, 199.  By pairs of 16-bit columns the forward is the faster one as far as a wave holds the row
+// (500: 67, 57; 2042: 73, 64; beyond, at 4090, the same), the backward is not (500: 73, 87).
+bool norm_flat(int C, bool pieces, bool backward) {
+  const int chunk = pieces ? 4 : kChunkCols;
+  return C + chunk - 1 <= kNormHeld && (backward || pieces || C % 2 != 0 || C > 2048);
+}
+
 // Workgroups of the sums over rows, at most what fits the 256 compute units at once (524288 x 192
 // bf16: 512 workgroups 84 us, 1024 93; with four chunks a lane one wave a SIMD does).
-NormPlan norm_plan(uint32_t rows, int C, bool pieces, bool vec, bool backward) {
+NormPlan norm_plan(uint32_t rows, int C, bool pieces, bool vec, bool flat, bool backward) {
   NormPlan p = {};
-  p.held = C <= kNormHeld;
-  if (p.held) {
-    p.shape = norm_shape(C, pieces, vec, backward);
+  p.flat = flat && norm_flat(C, pieces, backward);
+  p.held = !p.flat && C <= kNormHeld;
+  if (p.flat || p.held) {
+    p.shape = p.flat ? flat_shape(C, pieces ? 4 : kChunkCols) : norm_shape(C, pieces, vec, backward);
     const uint32_t groups = (uint32_t)(tail_threads(p.shape.lanes) / p.shape.lanes), useful = (rows + groups - 1) / groups;
-    const uint32_t most = p.shape.chunks >= 4 ? 256u : p.shape.lanes <= 16 && p.shape.chunks == 1 ? 1024u : 512u;
+    const uint32_t most = p.shape.chunks >= 4 || p.shape.lanes > 512 ? 256u : p.shape.lanes <= 16 && p.shape.chunks == 1 ? 1024u : 512u;
     p.parts = useful < most ? useful : most;
+    if (p.flat) p.parts = (p.parts + 7) / 8 * 8;  // rows of a group: a multiple of eight apart
     return p;
   }
   const uint32_t strips = (uint32_t)((C + 511) / 512), most = strips < 1024 ? 1024 / strips : 1, useful = (rows + 31) / 32;
@@ -172,8 +200,8 @@ extern "C" int terra_swin_layer_norm(const void* x, void* y, const terra_swin_la
   NormAlignment al;
   TERRA_TRY(norm_prepare(desc, &a, &al));
   if (a.rows == 0) return TERRA_OK;
-  TERRA_TRY(norm_pointer(x, desc->x_dtype, "x", true, &al.bits));
-  TERRA_TRY(norm_pointer(y, desc->y_dtype, "y", true, &al.bits));
+  TERRA_TRY(norm_pointer(x, desc->x_dtype, "x", true, &al));
+  TERRA_TRY(norm_pointer(y, desc->y_dtype, "y", true, &al));
   TERRA_TRY(norm_pointer(weight, desc->param_dtype, "the weight", false, nullptr));
   TERRA_TRY(norm_pointer(bias, desc->param_dtype, "the bias", false, nullptr));
   if (((uintptr_t)statistics & 7u) != 0) return fail(TERRA_ERR_ALIGN, "statistics must be 8-byte aligned");
@@ -187,7 +215,7 @@ extern "C" int terra_swin_layer_norm(const void* x, void* y, const terra_swin_la
   a.b = bias;
   a.statistics = (float2*)statistics;
   norm_launch(false, desc->x_dtype, desc->y_dtype, a,
-              norm_plan(a.rows, a.C, norm_by_pieces(desc), al.vec(), false), al, (hipStream_t)stream);
+              norm_plan(a.rows, a.C, norm_by_pieces(desc), al.vec(), al.flat(), false), al, (hipStream_t)stream);
   return norm_launched("terra_swin_layer_norm");
 }
 
@@ -198,10 +226,11 @@ extern "C" int terra_swin_layer_norm_workspace(const terra_swin_layer_norm_desc*
   TERRA_TRY(norm_prepare(desc, &a, &al));
   if (a.rows == 0) return 0;
   int most = 0;
-  for (const bool vec : {false, true}) {  // which, the call's addresses say
-    const int n = (int)norm_plan(a.rows, a.C, norm_by_pieces(desc), vec, true).parts * 2 * a.C;
-    most = n > most ? n : most;
-  }
+  for (const bool vec : {false, true})  // which, the call's addresses say
+    for (const bool flat : {false, true}) {
+      const int n = (int)norm_plan(a.rows, a.C, norm_by_pieces(desc), vec, flat && !vec, true).parts * 2 * a.C;
+      most = n > most ? n : most;
+    }
   return most;
 }
 
@@ -225,9 +254,9 @@ extern "C" int terra_swin_layer_norm_bwd(const void* dy, const void* x, const fl
     norm_finish_kernel<<<finish, kFinishThreads, 0, s>>>(f);
     return norm_launched("terra_swin_layer_norm_bwd");
   }
-  TERRA_TRY(norm_pointer(dy, yd, "dy", true, &al.bits));
-  TERRA_TRY(norm_pointer(x, xd, "x", true, &al.bits));
-  TERRA_TRY(norm_pointer(dx, xd, "dx", false, &al.bits));
+  TERRA_TRY(norm_pointer(dy, yd, "dy", true, &al));
+  TERRA_TRY(norm_pointer(x, xd, "x", true, &al));
+  TERRA_TRY(norm_pointer(dx, xd, "dx", false, &al));
   TERRA_TRY(norm_pointer(weight, desc->param_dtype, "the weight", false, nullptr));
   if (statistics == nullptr) return fail(TERRA_ERR_NULL, "statistics are NULL");
   if (((uintptr_t)statistics & 7u) != 0) return fail(TERRA_ERR_ALIGN, "statistics must be 8-byte aligned");
@@ -241,7 +270,7 @@ extern "C" int terra_swin_layer_norm_bwd(const void* dy, const void* x, const fl
   a.dx = (uint8_t*)dx;
   a.w = weight;
   a.statistics = (float2*)const_cast<float*>(statistics);
-  const NormPlan p = norm_plan(a.rows, a.C, norm_by_pieces(desc), al.vec(), true);
+  const NormPlan p = norm_plan(a.rows, a.C, norm_by_pieces(desc), al.vec(), al.flat(), true);
   a.parts = p.parts;
   a.partial = sums ? workspace : nullptr;
   norm_launch(true, xd, yd, a, p, al, s);

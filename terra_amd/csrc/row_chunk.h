@@ -141,10 +141,14 @@ __device__ __forceinline__ ChunkDraws half_draws(uint64_t seed, bool odd, uint32
 }
 
 // ---- sums over the lanes of a row ---------------------------------------------
-// Sum over the kL aligned lanes of a wave (kL = 8, 16, 32 or 64); every lane ends
+// Sum over the kL aligned lanes of a wave (kL = 2, 4, 8, 16, 32 or 64); every lane ends
 // with the same bits, since each step adds the same two values on both sides.
 template <int kL>
 __device__ __forceinline__ float lanes_sum(float v) {
+  if constexpr (kL < 8) {
+    v += dpp_move<0xb1>(v);
+    return kL == 2 ? v : v + dpp_move<0x4e>(v);
+  }
   if constexpr (kL == 8) return group8_sum(v);
   v = row16_sum(v);
   if constexpr (kL >= 32) {
@@ -199,7 +203,8 @@ struct RowSum {
     return a;
   }
   static __device__ __forceinline__ float waves_sum(float v) {
-    static_assert(kG <= 64 || kWaves == 4 || kWaves == 8, "waves of a row");
+    static_assert(kG <= 64 || kWaves == 4 || kWaves == 8 || kWaves == 16, "waves of a row");
+    if constexpr (kWaves == 16) return row16_sum(v);
     if constexpr (kWaves == 8) return group8_sum(v);
     v += dpp_move<0xb1>(v);
     return v + dpp_move<0x4e>(v);

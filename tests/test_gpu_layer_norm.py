@@ -92,7 +92,9 @@ def check_backward(grads, dy, x, norm):
 
 
 SHAPES = [(1, 1), (1, 8), (3, 7), (2, 5, 16), (9, 33), (5, 64), (67, 96), (130, 100), (33, 192), (7, 386), (21, 768),
-          (17, 1024), (5, 1030), (6, 2048), (4, 4096), (3, 4098), (2, 8192), (3, 8200), (2, 8201), (2, 20000), (1, 40001)]
+          (17, 1024), (5, 1030), (6, 2048), (4, 4096), (3, 4098), (2, 8192), (3, 8200), (2, 8201), (2, 20000), (1, 40001),
+          (2, 16), (70, 24), (5, 32), (1, 385), (200, 385), (77, 1001), (9, 1101), (5, 1601), (40, 2049), (9, 5001),
+          (3, 12000), (2, 16384), (3, 16383), (2, 16385)]
 
 
 @pytest.mark.parametrize("rms", [False, True])
@@ -110,7 +112,7 @@ def test_against_oracle(dev, xt, yt, shape, rms):
     check_backward(grads, dy, x, norm)
 
 
-@pytest.mark.parametrize("C", [24, 100, 130, 768, 9000])
+@pytest.mark.parametrize("C", [16, 24, 99, 100, 130, 385, 768, 1001, 9000, 9001])
 @pytest.mark.parametrize("rows", [40, 3001])
 def test_sums_over_many_rows(dev, rows, C):
     """Rows of many workgroups; the sums are the same in a second call."""
@@ -181,8 +183,8 @@ def _device_storage(x, dev):
 
 
 @pytest.mark.parametrize("offset", [0, 1, 3, 8])
-def test_addresses_off_any_alignment(dev, offset):
-    rows, C = 11, 64
+@pytest.mark.parametrize("rows,C", [(11, 64), (11, 63), (1, 17), (5, 1001), (3, 2051), (2, 9001)])
+def test_addresses_off_any_alignment(dev, offset, rows, C):
     buf = _x((rows * C + 8,), BF16).to(dev)
     x = buf[offset:offset + rows * C].view(rows, C)
     norm = _norm(C, dev=dev)
@@ -191,6 +193,11 @@ def test_addresses_off_any_alignment(dev, offset):
     assert kernels.layer_norm(x, norm, out=y).data_ptr() == y.data_ptr()
     check_forward(y, x, norm)
     assert bool((out[:offset] == 7).all()) and bool((out[offset + rows * C:] == 7).all())  # what stands beside it is left
+    _, st = kernels.layer_norm(x, norm, statistics=True)
+    dy = torch.zeros_like(out)
+    dy[offset:offset + rows * C] = _rand((rows * C,), BF16, 3).to(dev)
+    dy = dy[offset:offset + rows * C].view(rows, C)
+    check_backward(kernels.layer_norm_backward(dy, x, norm, st), dy, x, norm)
 
 
 @pytest.mark.parametrize("shape", [(0, 8), (4, 0, 8), (0, 9000)])
