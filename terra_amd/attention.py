@@ -65,16 +65,17 @@ def plain_norm(module: torch.nn.Module, channels: int) -> bool:
 def normed(module: torch.nn.Module, x: torch.Tensor) -> torch.Tensor:
     """``module(x)``, by the HIP kernels where it is a :func:`plain_norm` over x's last
     dimension: in the type that torch's would have (fp32 under autocast).  Calls that torch
-    traces or transforms, and tensors of other classes, are torch's."""
+    traces, transforms or watches, and tensors of other classes, are torch's."""
+    classes = (torch.Tensor, torch.nn.Parameter)
     if (x.device.type != "cuda" or x.dtype not in (torch.float32, torch.bfloat16, torch.float16) or x.dim() < 1
-            or type(x) not in (torch.Tensor, torch.nn.Parameter) or not plain_norm(module, x.shape[-1])
-            or forward_ad._current_level >= 0 or torch.compiler.is_compiling()
-            or torch._C._functorch.peek_interpreter_stack() is not None):
+            or type(x) not in classes or not plain_norm(module, x.shape[-1])
+            or forward_ad._current_level >= 0 or torch.compiler.is_compiling() or torch.jit.is_tracing()
+            or torch._C._len_torch_dispatch_stack() > 0 or torch._C._functorch.peek_interpreter_stack() is not None):
         return module(x)
     autocast = torch.is_autocast_enabled("cuda")
     params = [t for t in (module.weight, getattr(module, "bias", None)) if t is not None]
     if (autocast and type(module) is not torch.nn.LayerNorm) or any(
-            t.device != x.device or t.dtype not in (torch.float32, x.dtype) for t in params):
+            t.device != x.device or t.dtype not in (torch.float32, x.dtype) or type(t) not in classes for t in params):
         return module(x)
     return autograd.layer_norm(x, Norm.of(module), torch.float32 if autocast else None)
 

@@ -22,6 +22,7 @@ from typing import Optional, Tuple, Union
 
 import torch
 from torch.autograd import forward_ad
+from torch.autograd.function import once_differentiable
 
 from . import _lib, kernels
 from .kernels import Norm, ShiftMask, WindowGeometry, WindowMask
@@ -541,6 +542,7 @@ class _RotaryAttentionQKV(torch.autograd.Function):
                                         bias_table=table, mask=mask, n_real=n_real, mask_value=mask_value)
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, grad: torch.Tensor):
         qk, qkv, table, positions = ctx.saved_tensors
         num_heads, window_size, scale, mask, n_real, mask_value, rot = ctx.cfg

@@ -5,6 +5,7 @@
 // tensors by what each costs, so what a call does once its options are checked
 // is done here.  Allocations are torch's; the arithmetic is the library's,
 // reached by the addresses that bind() is given.
+#include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/function.h>
 #include <torch/csrc/autograd/functions/utils.h>
 #include <torch/csrc/autograd/saved_variable.h>
@@ -186,7 +187,6 @@ struct LayerNormBackward : public torch::autograd::Node {
 
 Tensor layer_norm(const std::shared_ptr<NormCall>& call, const Tensor& x, const std::optional<Tensor>& weight,
                   const std::optional<Tensor>& bias) {
-  const pybind11::gil_scoped_release no_gil;  // a launch may wait for room in the queue
   const Tensor w = weight.value_or(Tensor()), b = bias.value_or(Tensor());
   bool grad = x.requires_grad(), tangent = x._fw_grad(0).defined();
   for (const Tensor& t : {w, b})
@@ -477,12 +477,13 @@ PYBIND11_MODULE(_training, m) {
   pybind11::class_<NormCall, std::shared_ptr<NormCall>>(m, "NormCall").def(pybind11::init(&make_norm_call));
   pybind11::class_<RotaryCall, std::shared_ptr<RotaryCall>>(m, "RotaryCall").def(pybind11::init(&make_rotary_call));
   m.def("bind", &bind);
-  m.def("layer_norm", &layer_norm);
   m.def("layer_norm_forward", &layer_norm_forward);
   m.def("layer_norm_backward", &layer_norm_backward);
   const auto no_gil = pybind11::call_guard<pybind11::gil_scoped_release>();  // a launch may wait for room in the queue
   m.def("rotary", &rotary, no_gil);
-  m.def("rotary_with_gradient", &rotary_with_gradient, no_gil);
+  // What saves tensors may call hooks in Python: their exceptions pass as they are.
+  m.def("layer_norm", torch::wrap_pybind_function_no_gil(&layer_norm));
+  m.def("rotary_with_gradient", torch::wrap_pybind_function_no_gil(&rotary_with_gradient));
   m.def("gradient_norm", &gradient_norm);
   m.def("adamw_step", [](const std::vector<Tensor>& params, const std::vector<Tensor>& grads, const std::vector<Tensor>& firsts,
                          const std::vector<Tensor>& seconds, const std::vector<std::optional<Tensor>>& scales, double lr,

@@ -1777,7 +1777,8 @@ class Rotary:
         """The rates in whole turns a position (fp64) on ``device``, kept there."""
         t = self._turns.get(device)
         if t is None:
-            t = (self.rates / (2 * math.pi)).to(device)
+            with torch.inference_mode(False):  # a later graph may save them
+                t = (self.rates / (2 * math.pi)).to(device)
             self._turns[t.device] = t  # with its index, as the devices of tensors have it
         return t
 

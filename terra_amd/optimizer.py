@@ -134,7 +134,7 @@ class AdamW(torch.optim.Optimizer):
         super().load_state_dict(state_dict)
         # Moments keep their own types (the parent casts them to the parameters').
         ids = chain.from_iterable(g["params"] for g in state_dict["param_groups"])
-        counters = {}
+        counters, group_of = {}, {id(p): i for i, g in enumerate(self.param_groups) for p in g["params"]}
         for at, p in zip(ids, chain.from_iterable(g["params"] for g in self.param_groups)):
             saved = state_dict["state"].get(at)
             if not saved:
@@ -153,10 +153,9 @@ class AdamW(torch.optim.Optimizer):
                 state[name] = torch.empty_like(p, dtype=held)
                 state[name].copy_(t.to(held))
             on_device = self.capturable or self.skip_nonfinite
-            group = next(i for i, g in enumerate(self.param_groups) if any(q is p for q in g["params"]))
             count = int(saved["step"])
             if on_device:
-                key = (group, count)
+                key = (group_of[id(p)], count)
                 if key not in counters:
                     counters[key] = torch.tensor([count], dtype=torch.int64, device=p.device)
                 count = counters[key]

@@ -350,6 +350,23 @@ class TestAutograd:
         y.backward(dy)
         check_backward((big.grad[:, 1],), dy, big[:, 1], Norm())
 
+    def test_an_exception_of_a_hook_passes(self, dev):
+        def full(t):
+            raise KeyError("full")
+
+        x = _x((6, 64), F32).to(dev).requires_grad_()
+        with torch.autograd.graph.saved_tensors_hooks(full, lambda t: t):
+            with pytest.raises(KeyError, match="full"):
+                autograd.layer_norm(x, Norm())
+
+    @pytest.mark.parametrize("reentrant", [False, True])
+    def test_checkpointed(self, dev, reentrant):
+        from torch.utils.checkpoint import checkpoint
+
+        x, norm, dy = _x((6, 64), F32).to(dev).requires_grad_(), _norm(64, dev=dev), _rand((6, 64), F32, 3).to(dev)
+        checkpoint(lambda t: autograd.layer_norm(t, norm), x, use_reentrant=reentrant).backward(dy)
+        check_backward((x.grad,), dy, x, norm)
+
     def test_twice_over_a_retained_graph(self, dev):
         x = _x((4, 64), F32).to(dev).requires_grad_()
         y = autograd.layer_norm(x, Norm())

@@ -182,6 +182,22 @@ class TestAutograd:
         scale = 24 * x.detach().abs().max().item() ** 3 * x.detach().abs().max().item() ** 2
         assert (h.cpu().double() - hr).abs().max() <= 608 * U * scale
 
+    def test_first_used_in_inference_mode(self, dev):
+        rot, positions = Rotary(16), torch.arange(4, device=dev)
+        with torch.inference_mode():
+            kernels.rotary(torch.zeros(4, 2, 16, device=dev), rot, positions)
+        x, dy = _rand((4, 2, 16), F32).to(dev).requires_grad_(), _rand((4, 2, 16), F32, 2).to(dev)
+        autograd.rotary(x, rot, positions).backward(dy)
+        check(x.grad, dy, rot, positions, inverse=True)
+
+    def test_checkpointed(self, dev):
+        from torch.utils.checkpoint import checkpoint
+
+        rot, positions = Rotary(16), torch.arange(4, device=dev)
+        x, dy = _rand((4, 2, 16), F32).to(dev).requires_grad_(), _rand((4, 2, 16), F32, 2).to(dev)
+        checkpoint(lambda t: autograd.rotary(t, rot, positions), x, use_reentrant=False).backward(dy)
+        check(x.grad, dy, rot, positions, inverse=True)
+
     def test_heads_of_a_packed_row(self, dev):
         qkv = _rand((6, 9, 16), BF16).to(dev).requires_grad_()
         rot, positions, dy = Rotary(16), torch.arange(6, device=dev), _rand((6, 6, 16), BF16, 2).to(dev)

@@ -273,3 +273,40 @@ def test_attention_half_with_a_norm_of_its_own(dev, norm_layer):
     t = x.clone().requires_grad_()
     blk(t).sum().backward()
     assert t.grad.isfinite().all() and blk.norm1.weight.grad is not None
+
+
+def test_norms_that_torch_traces_or_watches(dev):
+    """normed leaves those to the module: a trace holds the norm, a mode sees it."""
+    from torch.utils._python_dispatch import TorchDispatchMode
+
+    class Seen(TorchDispatchMode):
+        ops = []
+
+        def __torch_dispatch__(self, func, types, args=(), kwargs=None):
+            self.ops.append(str(func))
+            return func(*args, **(kwargs or {}))
+
+    class Half(torch.nn.Module):
+        def __init__(self):
+            super().__init__()
+            self.norm = torch.nn.LayerNorm(33)
+
+        def forward(self, t):
+            return normed(self.norm, t)
+
+    half, x = Half().to(dev), torch.arange(66.0, device=dev).view(2, 33)
+    norm, traced = half.norm, torch.jit.trace(half, (x,))
+    other = x.flip(0) * 2 + 1
+    assert torch.equal(traced(other), norm(other))
+    with Seen():
+        normed(norm, x)
+    assert any("layer_norm" in name for name in Seen.ops)
+
+
+def test_only_one_derivative(dev):
+    """Of the core with rotary positions, as a second one would be wrong without a word."""
+    attn = WindowAttention(64, (4, 4), 2, rotary=True).to(dev)
+    x = workloads.activations((3, 16, 64), 7, F32).to(dev).requires_grad_()
+    g, = torch.autograd.grad(attn(x).square().sum(), x, create_graph=True)
+    with pytest.raises(RuntimeError, match="once_differentiable"):
+        g.sum().backward()
