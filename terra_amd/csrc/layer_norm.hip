@@ -102,12 +102,16 @@ TailShape flat_shape(int C, int chunk) {
 }
 
 // Whether packed rows that are not whole chunks are read by the tensor's aligned chunks or by columns, 60 million elements
-// (flat, by columns; us): 1001 bf16 forward 68, 92, backward 76, 134; 1030 fp32 106, 121 and 134, 216; 4097 fp32
+// (by chunks, by columns; us): 1001 bf16 forward 68, 92, backward 76, 134; 1030 fp32 106, 121 and 134, 216; 4097 fp32
 // 96, 129 and 144, 199.  By pairs of 16-bit columns the forward is the faster one as far as a wave holds the row
-// (500: 67, 57; 2042: 73, 64; beyond, at 4090, the same), the backward is not (500: 73, 87).
+// (500: 67, 57; 2042: 73, 64; beyond, at 4090, the same), the backward is not (500: 73, 87).  Narrow rows share their chunks
+// with too many neighbours: 17 bf16 128, 94 and 186, 185, 17 fp32 157, 101 and 244, 186; 33 bf16 88, 96 and 115, 186,
+// 33 fp32 137, 105 and 176, 192, 70 fp32 110, 128 and 151, 227.
 bool norm_flat(int C, bool pieces, bool backward) {
   const int chunk = pieces ? 4 : kChunkCols;
-  return C + chunk - 1 <= kNormHeld && (backward || pieces || C % 2 != 0 || C > 2048);
+  if (C + chunk - 1 > kNormHeld) return false;
+  if (backward) return C >= 32;
+  return pieces ? C >= 64 : C > 2048 || (C >= 32 && C % 2 != 0);
 }
 
 // Workgroups of the sums over rows, at most what fits the 256 compute units at once (524288 x 192

@@ -574,7 +574,7 @@ void launch_norm_bwd(const NormArgs& a, hipStream_t s) {
 
 template <int DTX, int DTY, int kG, int kK>
 void launch_norm_flat(const NormArgs& a, hipStream_t s) {
-  constexpr uint32_t kGroups = tail_threads(kG) / kG, kMost = kG > 64 ? 1024u : 2048u;
+  constexpr uint32_t kGroups = tail_threads(kG) / kG, kMost = kG > 64 ? 1024u : (kG > 16 ? 2048u : 8192u);
   const uint32_t need = ((a.rows + kGroups - 1) / kGroups + 7) / 8 * 8;
   norm_flat_kernel<DTX, DTY, kG, kK><<<need < kMost ? need : kMost, tail_threads(kG), 0, s>>>(a);
 }
