@@ -780,7 +780,8 @@ typedef struct terra_swin_adamw_tensor {
  *   param = param (1 - lr weight_decay) - lr / (1 - beta1^step) m / (sqrt(v / (1 - beta2^step)) + eps)
  * step, lr: from device memory where their pointers are not NULL (int64, fp32), so that a replayed graph
  * takes what is there then.  grad_factor (fp32, NULL: 1).  found_inf (fp32, NULL: 0): where it is not 0
- * nothing is written.  Moments in 8 bits: m is rounded to the nearest code; of
+ * nothing is written.  Moments in 8 bits: a block's scales are its largest |m| and sqrt(v) over 448, in 32 bits; m / scale
+ * is rounded to the nearest code; of
  * the two codes a <= sqrt(v) / scale < b the upper one is taken where
  *   v / scale^2 - a^2 > u (b^2 - a^2),   u = (draw + 1/2) / 65536,
  * so that the mean of the squares is v; draws as those of dropout with the counter (element >> 3,

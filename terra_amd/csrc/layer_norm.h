@@ -11,6 +11,10 @@
 // from fp64 sums.  Row r of x begins (r / inner) outer + (r % inner) step
 // elements into x, so the heads of a packed q|k|v are rows too; y, dy and dx are packed.
 //
+// Bound by memory: a row is read once and held in registers through its two sums, the next one on its
+// way meanwhile (39168 x 4096 bf16: forward 118 us, 5.4 TB/s, backward 161 us, 6.0; 524288 x 192 fp32 to bf16: 94 and
+// 167 us; a large copy moves 5.35).  One row of 1024 is a launch (3 us).
+//
 // Sums over rows: workgroups keep the sums of the rows that they take and write
 // them to a workspace, a second launch adds those up in fp64: no atomics, an
 // order that the sizes and alignments fix.

