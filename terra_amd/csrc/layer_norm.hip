@@ -91,27 +91,30 @@ TailShape norm_shape(int C, bool pieces, bool vec, bool backward) {
 }
 
 // The same for rows that are read by the aligned chunks of the tensor, a chunk more than C takes where the
-// row begins in one.  Parameters stand in registers too: two chunks a lane, up to four where waves can hold the row so
-// (58252 x 1030 bf16: 70 and 82 us forward and backward, as waves of four chunks 84 and 141, as 256 lanes 99 and 163).
+// row begins in one.  Parameters stand in registers too: one to three chunks a lane, up to four where waves can hold the
+// row so.  Three where two would leave many lanes idle (60 million elements, bf16 backward: 514 by 32 lanes of
+// three 83 us, by 64 of two 108; 1030 by 64 of three 82, by 64 of four 141, by 256 of one 163).
 TailShape flat_shape(int C, int chunk) {
   const int n = (C + chunk - 1 + kChunkCols - 1) / kChunkCols;
   if (n <= 16) return {n <= 8 ? 8 : 16, 1};
-  if (n <= 128) return {n <= 32 ? 16 : n <= 64 ? 32 : 64, 2};
-  if (n <= 256) return {64, n <= 192 ? 3 : 4};
+  for (int lanes = 8; lanes <= 32; lanes *= 2) {
+    if (n <= 2 * lanes) return {lanes, 2};
+    if (n <= 3 * lanes) return {lanes, 3};
+  }
+  if (n <= 256) return {64, n <= 128 ? 2 : n <= 192 ? 3 : 4};
   return {n <= 512 ? 256 : n <= 1024 ? 512 : 1024, 2};
 }
 
-// Whether packed rows that are not whole chunks are read by the tensor's aligned chunks or by columns, 60 million elements
-// (by chunks, by columns; us): 1001 bf16 forward 68, 92, backward 76, 134; 1030 fp32 106, 121 and 134, 216; 4097 fp32
-// 96, 129 and 144, 199.  By pairs of 16-bit columns the forward is the faster one as far as a wave holds the row
-// (500: 67, 57; 2042: 73, 64; beyond, at 4090, the same), the backward is not (500: 73, 87).  Narrow rows share their chunks
-// with too many neighbours: 17 bf16 128, 94 and 186, 185, 17 fp32 157, 101 and 244, 186; 33 bf16 88, 96 and 115, 186,
-// 33 fp32 137, 105 and 176, 192, 70 fp32 110, 128 and 151, 227.
+// Whether packed rows that are not whole chunks are read by the tensor's aligned chunks, or by columns (16-bit ones by pairs
+// where those stand aligned).  60 million elements, by chunks and by columns, us: 1001 bf16 forward 57, 92, backward
+// 76, 134; 1030 bf16 59, 73 and 82, 136; 1030 fp32 100, 119 and 135, 219; 4097 fp32 96, 129 and 144, 199.  Narrow
+// rows share their chunks with too many neighbours: 17 fp32 157, 101 and 244, 186; 50 bf16 forward 69, 64, 61 bf16
+// 84, 71, but 33 bf16 backward 115, 186.
 bool norm_flat(int C, bool pieces, bool backward) {
   const int chunk = pieces ? 4 : kChunkCols;
   if (C + chunk - 1 > kNormHeld) return false;
   if (backward) return C >= 32;
-  return pieces ? C >= 64 : C > 2048 || (C >= 32 && C % 2 != 0);
+  return C >= 64;
 }
 
 // Workgroups of the sums over rows, at most what fits the 256 compute units at once (524288 x 192

@@ -572,11 +572,21 @@ void launch_norm_bwd(const NormArgs& a, hipStream_t s) {
   norm_bwd_kernel<DTX, DTY, kG, kK, kVec, kPairs><<<a.parts, tail_threads(kG), 0, s>>>(a);
 }
 
+// Workgroups that the compute units hold at once, no more: each reads the parameters of its columns one by one first.
 template <int DTX, int DTY, int kG, int kK>
 void launch_norm_flat(const NormArgs& a, hipStream_t s) {
-  constexpr uint32_t kGroups = tail_threads(kG) / kG, kMost = kG > 64 ? 1024u : (kG > 16 ? 2048u : 8192u);
+  constexpr int kThreads = tail_threads(kG);
+  constexpr uint32_t kGroups = kThreads / kG;
+  static const uint32_t most = [] {
+    int n = 0;
+    if (hipOccupancyMaxActiveBlocksPerMultiprocessor(&n, norm_flat_kernel<DTX, DTY, kG, kK>, kThreads, 0) != hipSuccess || n < 1) {
+      (void)hipGetLastError();
+      n = 2;
+    }
+    return 256u * (uint32_t)n;
+  }();
   const uint32_t need = ((a.rows + kGroups - 1) / kGroups + 7) / 8 * 8;
-  norm_flat_kernel<DTX, DTY, kG, kK><<<need < kMost ? need : kMost, tail_threads(kG), 0, s>>>(a);
+  norm_flat_kernel<DTX, DTY, kG, kK><<<need < most ? need : most, kThreads, 0, s>>>(a);
 }
 
 template <int DTX, int DTY, int kG, int kK>
@@ -587,9 +597,12 @@ void launch_norm_flat_bwd(const NormArgs& a, hipStream_t s) {
 #define TERRA_NORM_FLAT_SHAPES(f, shape, ...)                                                \
   switch ((shape).lanes * 10 + (shape).chunks) {                                             \
     case 81: return f<DTX, DTY, 8, 1>(__VA_ARGS__);                                          \
+    case 83: return f<DTX, DTY, 8, 3>(__VA_ARGS__);                                          \
     case 161: return f<DTX, DTY, 16, 1>(__VA_ARGS__);                                        \
     case 162: return f<DTX, DTY, 16, 2>(__VA_ARGS__);                                        \
+    case 163: return f<DTX, DTY, 16, 3>(__VA_ARGS__);                                        \
     case 322: return f<DTX, DTY, 32, 2>(__VA_ARGS__);                                        \
+    case 323: return f<DTX, DTY, 32, 3>(__VA_ARGS__);                                        \
     case 642: return f<DTX, DTY, 64, 2>(__VA_ARGS__);                                        \
     case 643: return f<DTX, DTY, 64, 3>(__VA_ARGS__);                                        \
     case 644: return f<DTX, DTY, 64, 4>(__VA_ARGS__);                                        \

@@ -1932,7 +1932,7 @@ def adamw_step(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], mo
         param = param (1 - lr weight_decay) - lr / (1 - beta1^step) m / (sqrt(v / (1 - beta2^step)) + eps)
 
     params: fp32, bf16 or fp16, dense; grads of the same dtype or fp32 (for fp32 params any of the
-    three).  ``step`` counts from 1.  ``step`` (int64) and ``lr`` (fp32) may be one-element tensors on the device, which a
+    three).  A 16-bit param is rounded once, to nearest: of a step below half of its own, nothing is left.  ``step`` counts from 1.  ``step`` (int64) and ``lr`` (fp32) may be one-element tensors on the device, which a
     captured graph's replays read anew.  ``grad_factor``, ``found_inf``: fp32 scalars on the device, such as
     :func:`gradient_norm` gives: the gradients' factor, and where ``found_inf`` is not 0 nothing changes.
 

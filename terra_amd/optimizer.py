@@ -26,7 +26,7 @@ class AdamW(torch.optim.Optimizer):
     the device) after a step.  ``skip_nonfinite``: a step whose norm is infinite or
     NaN changes nothing and is not counted.  ``capturable``: the count is kept in device
     memory, so that a step may be captured into a graph (run one before); an
-    ``lr`` of a group may then be a one-element fp32 tensor on the device.
+    ``lr`` of a group may then be a one-element fp32 tensor on the device.  See :meth:`replayed`.
 
     State dicts of ``torch.optim.AdamW`` load (and those of 32-bit moments load there)."""
 
@@ -98,6 +98,12 @@ class AdamW(torch.optim.Optimizer):
                                    seed=self._seed(group["seed"], params[0].device) if group["bits"] == 8 else None,
                                    stream=index)
         return loss
+
+    def replayed(self) -> None:
+        """Counts the parameters as changed, which a replay of a captured step does not do by itself: what is derived from
+        them outside of the graph and kept until they change (the halves' packed weights in inference) is made anew."""
+        params = [p for g in self.param_groups for p in g["params"]]
+        torch.autograd.graph.increment_version(p for p in params if not p.is_inference())
 
     def _counted(self, group, params, on_device, norm):
         """[(parameters, their count with this step)]: those that have taken as many steps, on the host

@@ -365,3 +365,26 @@ def test_packed_weights_follow_the_step(dev):
         fresh = SequentialMlp(128, 512).to(dev).to(torch.bfloat16)
         fresh.load_state_dict(m.state_dict())
         assert torch.equal(after, fresh(x)) and not torch.equal(after, before)
+
+
+def test_packed_weights_follow_replays(dev):
+    """A replayed step changes no version: the halves are told."""
+    m = SequentialMlp(128, 512, init_seed_base=3).to(dev).to(torch.bfloat16)
+    x = workloads.activations((64, 128), 7, torch.bfloat16).to(dev)
+    for p in m.parameters():
+        p.grad = torch.ones_like(p)
+    opt = AdamW(m.parameters(), lr=0.1, capturable=True)
+    opt.step()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        opt.step()
+    for _ in range(3):
+        with torch.no_grad():
+            m(x)
+        graph.replay()
+        opt.replayed()
+        with torch.no_grad():
+            fresh = SequentialMlp(128, 512).to(dev).to(torch.bfloat16)
+            fresh.load_state_dict(m.state_dict())
+            assert torch.equal(m(x), fresh(x))
