@@ -198,6 +198,13 @@ class WindowAttention(torch.nn.Module):
         if not hasattr(self, "rotary"):
             self.rotary = None
 
+    def _load_from_state_dict(self, *args, **kwargs):
+        """The positions are in no state dict: a module that was built without memory has them from here on."""
+        super()._load_from_state_dict(*args, **kwargs)
+        if self.rotary is not None and not self.token_positions.is_meta:
+            with torch.no_grad():
+                self.token_positions.copy_(token_positions(self.window_size))
+
     def attend(self, x: torch.Tensor, mask=None) -> torch.Tensor:
         """Everything of forward but the output projection: q/k/v and the
         fused core, O [B_, N, C] (models/attention.py:244-278).  In training

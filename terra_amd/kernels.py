@@ -1755,7 +1755,7 @@ class Rotary:
         scale = 1.0
         if scaling == "ntk":
             base *= factor ** (pairs / (pairs - 1)) if pairs > 1 else 1.0
-        rates = base ** (-torch.arange(pairs, dtype=torch.float64) / pairs)
+        rates = base ** (-torch.arange(pairs, dtype=torch.float64, device="cpu") / pairs)
         if scaling == "linear":
             rates = rates / factor
         elif scaling == "yarn":

@@ -67,7 +67,8 @@ class AdamW(torch.optim.Optimizer):
         return t
 
     def _begin(self, p: torch.Tensor, group: dict, count) -> dict:
-        m = kernels.moments(p, 8 if group["bits"] == 8 and p.numel() >= group["min_8bit_size"] else 32)
+        bits = group["bits"]
+        m = kernels.moments(p, 32 if bits == 8 and p.numel() < group["min_8bit_size"] else bits)
         state = self.state[p]
         state["step"] = count
         state.update((k, v) for k, v in zip(_MOMENTS, m) if v is not None)

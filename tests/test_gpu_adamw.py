@@ -388,3 +388,17 @@ def test_packed_weights_follow_replays(dev):
             fresh = SequentialMlp(128, 512).to(dev).to(torch.bfloat16)
             fresh.load_state_dict(m.state_dict())
             assert torch.equal(m(x), fresh(x))
+
+
+def test_groups_of_different_bits(dev):
+    a, b = (torch.nn.Parameter(torch.ones(5000, device=dev)) for _ in range(2))
+    opt = AdamW([dict(params=[a], bits=8), dict(params=[b])], lr=0.1)
+    a.grad = b.grad = torch.full_like(a, 0.5)
+    opt.step()
+    assert opt.state[a]["exp_avg"].dtype == torch.float8_e4m3fn and opt.state[b]["exp_avg"].dtype == torch.float32
+    # The first step comes before the first rounding of a moment: some ten roundings of 0.1 and one of 0.9 apart on each side.
+    assert (a - b).abs().max().item() <= 2 * (10 * 0.1 + 1) * 2.0 ** -24
+    c = torch.nn.Parameter(torch.ones(8, device=dev))
+    c.grad = torch.ones_like(c)
+    with pytest.raises(ValueError, match="32 bits or in 8"):
+        AdamW([dict(params=[c], bits=16)]).step()

@@ -92,3 +92,16 @@ def test_draws_are_those_of_dropout():
     for p in (0.1, 0.5, 0.9):
         keep = rg.keep_mask(seed, 6, 77, p, 3)[5]
         assert torch.equal(d >= round(p * 65536), keep)
+
+
+def test_positions_of_a_module_built_without_memory():
+    from terra_amd.attention import WindowAttention
+
+    real = WindowAttention(32, (3, 5), 2, rotary=True)
+    with torch.device("meta"):
+        m = WindowAttention(32, (3, 5), 2, rotary=True)
+    m = m.to_empty(device="cpu")
+    m.token_positions.fill_(77)
+    m.load_state_dict(real.state_dict())
+    assert torch.equal(m.token_positions, real.token_positions)
+    assert torch.equal(m.rotary.rates, real.rotary.rates)
