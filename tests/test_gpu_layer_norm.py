@@ -247,6 +247,36 @@ def test_rows_past_32_bits_of_elements(dev):
     check_backward((g.dx[-4:], g.dweight, g.dbias), dy[-4:].clone(), x[-4:], norm)
 
 
+def test_odd_rows_past_32_bits_of_elements(dev):
+    rows, C = 2_200_001, 999
+    x = torch.empty(rows, C, dtype=BF16, device=dev)
+    x[:4], x[-4:] = _x((4, C), BF16).to(dev), _x((4, C), BF16, 2).to(dev)
+    x[4:-4] = 0
+    norm = _norm(C, dev=dev)
+    y, st = kernels.layer_norm(x, norm, statistics=True)
+    check_forward(y[-4:].clone(), x[-4:], norm)
+    check_forward(y[:4].clone(), x[:4], norm)
+    dy = y.zero_()
+    dy[-4:] = _rand((4, C), BF16, 3).to(dev)
+    g = kernels.layer_norm_backward(dy, x, norm, st)
+    check_backward((g.dx[-4:], g.dweight, g.dbias), dy[-4:].clone(), x[-4:], norm)
+
+
+@pytest.mark.parametrize("dt", [F32, BF16])
+@pytest.mark.parametrize("C", [33, 65, 99, 385, 1030, 2049, 5001, 9001])
+def test_nan_of_neighbours_that_share_a_chunk(dev, C, dt):
+    """Every other row is NaN: the rows between them are as they are by themselves, bit by bit."""
+    x, norm, dy = _x((40, C), dt).to(dev), _norm(C, dev=dev), _rand((40, C), dt, 3).to(dev)
+    y, st = kernels.layer_norm(x, norm, statistics=True)
+    dx = kernels.layer_norm_backward(dy, x, norm, st).dx
+    x[1::2], dy[::2] = float("nan"), float("nan")
+    z, _ = kernels.layer_norm(x, norm, statistics=True)
+    assert torch.equal(z[::2], y[::2]) and bool(z[1::2].isnan().all())
+    x = _x((40, C), dt).to(dev)
+    again = kernels.layer_norm_backward(dy, x, norm, st).dx
+    assert torch.equal(again[1::2], dx[1::2]) and bool(again[::2].isnan().all())
+
+
 class TestAutograd:
     def test_gradients(self, dev):
         x = _x((5, 7, 96), F32).to(dev).requires_grad_()
