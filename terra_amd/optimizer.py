@@ -109,7 +109,7 @@ class AdamW(torch.optim.Optimizer):
     def _counted(self, group, params, on_device, norm):
         """[(parameters, their count with this step)]: those that have taken as many steps, on the host
         by the number, on the device by the counter that they share."""
-        sets, fresh = {}, None
+        sets, made, fresh = {}, {}, None
         for p in params:
             state = self.state[p]
             if "exp_avg" not in state:
@@ -117,6 +117,12 @@ class AdamW(torch.optim.Optimizer):
                     fresh = torch.zeros(1, dtype=torch.int64, device=p.device) if on_device else 0
                 state = self._begin(p, group, fresh)
             count = state["step"]
+            if on_device and not isinstance(count, torch.Tensor):  # an option that was set after some steps
+                if count not in made:
+                    made[count] = torch.tensor([count], dtype=torch.int64, device=p.device)
+                count = state["step"] = made[count]
+            elif not on_device and isinstance(count, torch.Tensor):
+                count = state["step"] = int(count)
             sets.setdefault(id(count) if on_device else count, (count, []))[1].append(p)
         if on_device:  # a parameter that takes no part in this step leaves the others' counter
             left = {}

@@ -402,3 +402,16 @@ def test_groups_of_different_bits(dev):
     c.grad = torch.ones_like(c)
     with pytest.raises(ValueError, match="32 bits or in 8"):
         AdamW([dict(params=[c], bits=16)]).step()
+
+
+def test_options_set_between_steps(dev):
+    """The count moves to the device and back; the steps are those of an optimizer that counts on the host."""
+    a, b = ([torch.nn.Parameter(torch.linspace(-1, 1, n, device=dev)) for n in (33, 700)] for _ in range(2))
+    one, two = AdamW(a, lr=0.1), AdamW(b, lr=0.1)
+    for step in range(6):
+        one.capturable, one.skip_nonfinite = step in (2, 3), step == 3
+        for ps, opt in ((a, one), (b, two)):
+            for k, p in enumerate(ps):
+                p.grad = torch.full_like(p, 0.3 * (k + 1) - 0.1 * step)
+            opt.step()
+    assert all(torch.equal(p, q) for p, q in zip(a, b)) and one.state[a[0]]["step"] == two.state[b[0]]["step"] == 6
