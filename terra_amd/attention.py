@@ -188,7 +188,13 @@ class WindowAttention(torch.nn.Module):
     def core(self, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
              mask: Union[None, torch.Tensor, ShiftMask, WindowMask] = None,
              n_real: Optional[int] = None) -> torch.Tensor:
-        """Fused core on projected q/k/v [B_, N, C] (row strides may exceed C)."""
+        """Fused core on projected q/k/v [B_, N, C] (row strides may exceed C);
+        with rotary positions the query and key heads are turned first."""
+        if self.rotary is not None:
+            at = self.token_positions
+            if n_real is not None and n_real <= at.shape[0] < q.shape[-2]:  # rows of padding behind the window's tokens
+                at = F.pad(at, (0, 0, 0, q.shape[-2] - at.shape[0]))
+            q, k = (autograd.rotary(t.unflatten(-1, (self.num_heads, -1)), self.rotary, at).flatten(-2) for t in (q, k))
         return autograd.window_attention(q, k, v, self.num_heads, self.window_size, self.scale,
                                          bias_table=self._table(), mask=mask, n_real=n_real)
 
