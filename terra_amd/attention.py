@@ -90,9 +90,10 @@ def relative_position_index(window_size: Sequence[int]) -> torch.Tensor:
 
 
 def token_positions(window_size: Sequence[int]) -> torch.Tensor:
-    """Row and column of each token of a window, int32 [Wh*Ww, 2]."""
+    """Row and column of each token of a window, int32 [Wh*Ww, 2], on the CPU."""
     wh, ww = int(window_size[0]), int(window_size[1])
-    return torch.stack((torch.arange(wh).repeat_interleave(ww), torch.arange(ww).repeat(wh)), 1).to(torch.int32)
+    rows, columns = (torch.arange(n, dtype=torch.int32, device="cpu") for n in (wh, ww))
+    return torch.stack((rows.repeat_interleave(ww), columns.repeat(wh)), 1)
 
 
 class WindowAttention(torch.nn.Module):
@@ -108,6 +109,8 @@ class WindowAttention(torch.nn.Module):
     heads by the token's row and column in its window, a :class:`kernels.Rotary` of
     two axes or True for one over whole heads.  A block without the
     bias table (the reference's windows of 32 x 32) knows no positions otherwise.
+    Other positions than the rows and columns may be set (``token_positions``);
+    they are in no state dict, and loading one leaves them.
     """
 
     def __init__(self, embedding_dim, window_size, num_heads, qkv_bias=True, qk_scale=None,
@@ -129,7 +132,7 @@ class WindowAttention(torch.nn.Module):
             if self.rotary.axes != 2 or self.rotary.dim > head_dim:
                 raise ValueError(f"rotary positions of a window have two axes and at most the {head_dim} elements of a head "
                                  f"(got {self.rotary.axes} and {self.rotary.dim})")
-            self.register_buffer("token_positions", token_positions(self.window_size), persistent=False)
+        self._positions = None
 
         if self.use_relative_position_bias:
             wh, ww = self.window_size
@@ -145,6 +148,37 @@ class WindowAttention(torch.nn.Module):
         self.v_linear = make_linear_with_seed(self.dim, self.dim, bias=qkv_bias, init_seed=seed(3))
         self.proj = make_linear_with_seed(self.dim, self.dim, bias=True, init_seed=seed(4))
         self.softmax = torch.nn.Softmax(dim=-1)
+        self._unloaded = self.q_linear.weight.is_meta  # built without memory, no state dict loaded yet
+
+    @property
+    def token_positions(self) -> torch.Tensor:
+        """Row and column of each token of the window (int32 [Wh*Ww, 2], where the parameters are), or what was set."""
+        if self.rotary is None and self._positions is None:
+            raise AttributeError("a module without rotary positions")
+        return self._positions_on(self.q_linear.weight.device)
+
+    @token_positions.setter
+    def token_positions(self, positions: torch.Tensor) -> None:
+        self._positions, self._unloaded = positions, False
+
+    def _positions_on(self, device: torch.device) -> torch.Tensor:
+        """The positions on ``device``, kept there.  No buffer, which memory that is given anew
+        (``to_empty``, parameters assigned from a state dict) would leave without values: made where there are none."""
+        t = self._positions
+        if t is not None and t.device == device:
+            return t
+        with torch.inference_mode(False):  # a later graph may save them
+            made = (token_positions(self.window_size) if t is None or t.is_meta else t).to(device)
+        if not made.is_meta:
+            self._positions = made
+        return made
+
+    def _apply(self, fn, recurse=True):
+        """The positions move with the parameters, not in a first call, which may be captured."""
+        super()._apply(fn, recurse)
+        if self.rotary is not None:
+            self.token_positions
+        return self
 
     def _cached(self, name: str, tensors, build):
         """``build()`` cached under ``name`` until any of ``tensors`` changes
@@ -191,7 +225,7 @@ class WindowAttention(torch.nn.Module):
         """Fused core on projected q/k/v [B_, N, C] (row strides may exceed C);
         with rotary positions the query and key heads are turned first."""
         if self.rotary is not None:
-            at = self.token_positions
+            at = self._positions_on(q.device)
             if n_real is not None and n_real <= at.shape[0] < q.shape[-2]:  # rows of padding behind the window's tokens
                 at = F.pad(at, (0, 0, 0, q.shape[-2] - at.shape[0]))
             q, k = (autograd.rotary(t.unflatten(-1, (self.num_heads, -1)), self.rotary, at).flatten(-2) for t in (q, k))
@@ -199,17 +233,20 @@ class WindowAttention(torch.nn.Module):
                                          bias_table=self._table(), mask=mask, n_real=n_real)
 
     def __setstate__(self, state):
-        """A module pickled when this option was not there yet has it off."""
+        """A module pickled when this option was not there yet has it off; the
+        positions of one that held them as a buffer are taken out of it."""
         super().__setstate__(state)
         if not hasattr(self, "rotary"):
             self.rotary = None
+        if "_positions" not in self.__dict__:
+            self._positions, self._unloaded = self._buffers.pop("token_positions", None), False
+            self._non_persistent_buffers_set.discard("token_positions")
 
     def _load_from_state_dict(self, *args, **kwargs):
-        """The positions are in no state dict: a module that was built without memory has them from here on."""
+        """What a module that was built without memory had for positions before its first state dict is not theirs."""
         super()._load_from_state_dict(*args, **kwargs)
-        if self.rotary is not None and not self.token_positions.is_meta:
-            with torch.no_grad():
-                self.token_positions.copy_(token_positions(self.window_size))
+        if self._unloaded:
+            self._positions, self._unloaded = None, False
 
     def attend(self, x: torch.Tensor, mask=None) -> torch.Tensor:
         """Everything of forward but the output projection: q/k/v and the
@@ -219,7 +256,7 @@ class WindowAttention(torch.nn.Module):
         if self.rotary is not None:
             return autograd.window_attention_qkv(self.qkv(x), self.num_heads, self.window_size, self.scale,
                                                  bias_table=self._table(), mask=mask, rot=self.rotary,
-                                                 positions=self.token_positions)
+                                                 positions=self._positions_on(x.device))
         link = autograd.ColumnSumLink() if torch.is_grad_enabled() else None
         return autograd.window_attention_qkv(self.qkv(x, bias_sums=link), self.num_heads, self.window_size,
                                              self.scale, bias_table=self._table(), mask=mask, bias_sums=link)
