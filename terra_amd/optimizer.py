@@ -15,6 +15,15 @@ from .kernels import Moments
 _MOMENTS = ("exp_avg", "exp_avg_sq", "scales")
 
 
+def _refuse_other_updates(group: dict) -> None:
+    """Options of torch's groups that name an update which :meth:`AdamW.step` does not make."""
+    for name in ("amsgrad", "differentiable"):
+        if group.get(name, False):
+            raise ValueError(f"{name} is not available: a group with {name}=True would be stepped without it")
+    if not group.get("decoupled_weight_decay", True) and group.get("weight_decay", 0.0) != 0.0:
+        raise ValueError("a group with decoupled_weight_decay=False (torch.optim.Adam's) would be stepped with decoupled decay")
+
+
 class AdamW(torch.optim.Optimizer):
     """``torch.optim.AdamW`` with fp32 moments whatever the parameters' dtype, or moments in 8
     bits, and with clipping to a norm over all groups in the step itself.
@@ -28,7 +37,8 @@ class AdamW(torch.optim.Optimizer):
     memory, so that a step may be captured into a graph (run one before); an
     ``lr`` of a group may then be a one-element fp32 tensor on the device.  See :meth:`replayed`.
 
-    State dicts of ``torch.optim.AdamW`` load (and those of 32-bit moments load there)."""
+    State dicts of ``torch.optim.AdamW`` load (and those of 32-bit moments load there); one with
+    ``amsgrad`` or ``differentiable``, or of ``torch.optim.Adam`` with a weight decay, raises."""
 
     def __init__(self, params, lr: Union[float, torch.Tensor] = 1e-3, betas: Tuple[float, float] = (0.9, 0.999),
                  eps: float = 1e-8, weight_decay: float = 1e-2, *, maximize: bool = False, bits: int = 32,
@@ -59,6 +69,11 @@ class AdamW(torch.optim.Optimizer):
     def __getstate__(self):
         own = {k: v for k, v in self.__dict__.items() if k in ("max_grad_norm", "skip_nonfinite", "capturable", "grad_norm")}
         return {**super().__getstate__(), **own}
+
+    def add_param_group(self, param_group):
+        if isinstance(param_group, dict):
+            _refuse_other_updates({**self.defaults, **param_group})
+        super().add_param_group(param_group)
 
     def _seed(self, seed: int, device: torch.device) -> torch.Tensor:
         t = self._seeds.get((seed, device))
@@ -144,7 +159,15 @@ class AdamW(torch.optim.Optimizer):
         return out
 
     def load_state_dict(self, state_dict):
-        super().load_state_dict(state_dict)
+        def check(_, given):  # behind the other hooks, before anything is changed
+            for group in given["param_groups"]:
+                _refuse_other_updates(group)
+
+        hook = self.register_load_state_dict_pre_hook(check)
+        try:
+            super().load_state_dict(state_dict)
+        finally:
+            hook.remove()
         # Moments keep their own types (the parent casts them to the parameters').
         ids = chain.from_iterable(g["params"] for g in state_dict["param_groups"])
         counters, group_of = {}, {id(p): i for i, g in enumerate(self.param_groups) for p in g["params"]}
@@ -177,3 +200,5 @@ class AdamW(torch.optim.Optimizer):
             for name, value in self.defaults.items():
                 group.setdefault(name, value)
             group["betas"] = tuple(group["betas"])
+            if "decoupled_weight_decay" in group:
+                group["decoupled_weight_decay"] = True
