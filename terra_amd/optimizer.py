@@ -159,15 +159,19 @@ class AdamW(torch.optim.Optimizer):
         return out
 
     def load_state_dict(self, state_dict):
-        def check(_, given):  # behind the other hooks, before anything is changed
-            for group in given["param_groups"]:
+        given = []
+
+        def check(_, made):  # what the hooks before it made of the state dict, before anything is changed
+            for group in made["param_groups"]:
                 _refuse_other_updates(group)
+            given.append(made)
 
         hook = self.register_load_state_dict_pre_hook(check)
         try:
             super().load_state_dict(state_dict)
         finally:
             hook.remove()
+        state_dict = given[0]
         # Moments keep their own types (the parent casts them to the parameters').
         ids = chain.from_iterable(g["params"] for g in state_dict["param_groups"])
         counters, group_of = {}, {id(p): i for i, g in enumerate(self.param_groups) for p in g["params"]}

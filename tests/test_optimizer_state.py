@@ -81,3 +81,25 @@ def test_what_the_options_do_not_change_loads():
         assert group["maximize"] == theirs.param_groups[0]["maximize"]
         for p, q in zip(theirs.param_groups[0]["params"], group["params"]):
             assert ours.state[q]["step"] == 2 and torch.equal(ours.state[q]["exp_avg"], theirs.state[p]["exp_avg"])
+
+
+# ---- hooks -----------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("steps", [(1,), (1, 2)])
+def test_state_dicts_that_hooks_make(steps):
+    """What load_state_dict's hooks give is what is loaded, moments in their own types."""
+    theirs = _theirs()
+    saved = {"optimizer": copy.deepcopy(theirs.state_dict())}
+    ours = AdamW(_params(torch.bfloat16))
+    ours.register_load_state_dict_pre_hook(lambda _, d: d["optimizer"])
+    if 2 in steps:  # and one that changes it in place, a copy of the first level
+        def double(_, d):
+            d["state"] = {i: {**s, "exp_avg": 2 * s["exp_avg"]} for i, s in d["state"].items()}
+        ours.register_load_state_dict_pre_hook(double)
+    for _ in range(2):  # the hooks are those of before each time
+        ours.load_state_dict(copy.deepcopy(saved))  # the second hook writes into it
+        for p, q in zip(theirs.param_groups[0]["params"], ours.param_groups[0]["params"]):
+            a, b = theirs.state[p], ours.state[q]
+            assert b["exp_avg"].dtype == b["exp_avg_sq"].dtype == torch.float32 and b["step"] == 2
+            assert torch.equal(b["exp_avg"], steps[-1] * a["exp_avg"]) and torch.equal(b["exp_avg_sq"], a["exp_avg_sq"])
