@@ -159,7 +159,7 @@ class AdamW(torch.optim.Optimizer):
         return out
 
     def load_state_dict(self, state_dict):
-        given = []
+        own, given = self.param_groups, []
 
         def check(_, made):  # what the hooks before it made of the state dict, before anything is changed
             for group in made["param_groups"]:
@@ -200,9 +200,9 @@ class AdamW(torch.optim.Optimizer):
                     counters[key] = torch.tensor([count], dtype=torch.int64, device=p.device)
                 count = counters[key]
             state["step"] = count
-        for group in self.param_groups:  # of torch.optim.AdamW's groups
+        for group, before in zip(self.param_groups, own):  # torch.optim.AdamW's groups do not have all options
             for name, value in self.defaults.items():
-                group.setdefault(name, value)
+                group.setdefault(name, before.get(name, value))
             group["betas"] = tuple(group["betas"])
             if "decoupled_weight_decay" in group:
                 group["decoupled_weight_decay"] = True

@@ -103,3 +103,22 @@ def test_state_dicts_that_hooks_make(steps):
             a, b = theirs.state[p], ours.state[q]
             assert b["exp_avg"].dtype == b["exp_avg_sq"].dtype == torch.float32 and b["step"] == 2
             assert torch.equal(b["exp_avg"], steps[-1] * a["exp_avg"]) and torch.equal(b["exp_avg_sq"], a["exp_avg_sq"])
+
+
+# ---- options that torch's groups do not have -----------------------------------------
+
+
+def _groups(params, **first):
+    return [dict(params=params[:2], **first), dict(params=params[2:])]
+
+
+def test_options_of_ones_own_groups_stay():
+    """What a state dict does not say of a group is the group's own, not the optimizer's."""
+    theirs = torch.optim.AdamW(_groups(_params(), lr=0.3))
+    ours = AdamW(_groups(_params(), bits=8, min_8bit_size=100, seed=9), lr=1.0)
+    ours.load_state_dict(theirs.state_dict())
+    a, b = ours.param_groups
+    assert (a["bits"], a["min_8bit_size"], a["seed"], a["lr"]) == (8, 100, 9, 0.3)
+    assert (b["bits"], b["min_8bit_size"], b["lr"]) == (32, 4096, 1e-3)
+    ours.load_state_dict(AdamW(_groups(_params(), bits=8, min_8bit_size=7, seed=11)).state_dict())
+    assert (ours.param_groups[0]["min_8bit_size"], ours.param_groups[0]["seed"]) == (7, 11)  # said, so taken
