@@ -8,6 +8,7 @@ from itertools import chain
 from typing import Callable, Optional, Tuple, Union
 
 import torch
+import torch.nn.functional as F
 
 from . import kernels
 from .kernels import Moments
@@ -24,6 +25,22 @@ def _refuse_other_updates(group: dict) -> None:
         raise ValueError("a group with decoupled_weight_decay=False (torch.optim.Adam's) would be stepped with decoupled decay")
 
 
+def _in_8_bits(p: torch.Tensor, exp_avg: torch.Tensor, exp_avg_sq: torch.Tensor) -> Moments:
+    """fp32 moments of p in 8 bits: the nearest codes, of a root above 0 never that of 0."""
+    made, n = kernels.moments(p, 8), p.numel()
+    for i, values in enumerate((exp_avg, exp_avg_sq.sqrt())):
+        lain = torch.empty_like(p, dtype=torch.float32).copy_(values).as_strided((n,), (1,))  # in the order of memory
+        blocks = F.pad(lain, (0, -n % 256)).view(-1, 256)
+        top = blocks.abs().amax(1)
+        scale = torch.where(top.isfinite(), top / 448, torch.inf)  # infinite: the block is NaN when it is read
+        parts = torch.where(scale[:, None] > 0, blocks / scale[:, None], 0.0).clamp(-448.0, 448.0)
+        if i == 1:
+            parts = torch.where((blocks > 0) & scale.isfinite()[:, None], parts.clamp_min(2.0 ** -9), parts)
+        made.scales[i] = scale
+        made[i].as_strided((n,), (1,)).copy_(parts.view(-1)[:n])
+    return made
+
+
 class AdamW(torch.optim.Optimizer):
     """``torch.optim.AdamW`` with fp32 moments whatever the parameters' dtype, or moments in 8
     bits, and with clipping to a norm over all groups in the step itself.
@@ -37,7 +54,8 @@ class AdamW(torch.optim.Optimizer):
     memory, so that a step may be captured into a graph (run one before); an
     ``lr`` of a group may then be a one-element fp32 tensor on the device.  See :meth:`replayed`.
 
-    State dicts of ``torch.optim.AdamW`` load (and those of 32-bit moments load there); one with
+    State dicts of ``torch.optim.AdamW`` load (and those of 32-bit moments load there), their moments
+    in the bits that the group has; one with
     ``amsgrad`` or ``differentiable``, or of ``torch.optim.Adam`` with a weight decay, raises."""
 
     def __init__(self, params, lr: Union[float, torch.Tensor] = 1e-3, betas: Tuple[float, float] = (0.9, 0.999),
@@ -172,6 +190,12 @@ class AdamW(torch.optim.Optimizer):
         finally:
             hook.remove()
         state_dict = given[0]
+        for group, before in zip(self.param_groups, own):  # torch.optim.AdamW's groups do not have all options
+            for name, value in self.defaults.items():
+                group.setdefault(name, before.get(name, value))
+            group["betas"] = tuple(group["betas"])
+            if "decoupled_weight_decay" in group:
+                group["decoupled_weight_decay"] = True
         # Moments keep their own types (the parent casts them to the parameters').
         ids = chain.from_iterable(g["params"] for g in state_dict["param_groups"])
         counters, group_of = {}, {id(p): i for i, g in enumerate(self.param_groups) for p in g["params"]}
@@ -192,6 +216,9 @@ class AdamW(torch.optim.Optimizer):
                     raise ValueError("moments in 8 bits of a parameter that lay otherwise in memory")
                 state[name] = torch.empty_like(p, dtype=held)
                 state[name].copy_(t.to(held))
+            group = self.param_groups[group_of[id(p)]]
+            if group["bits"] == 8 and "exp_avg" in saved and saved.get("scales") is None and p.numel() >= group["min_8bit_size"]:
+                state.update(zip(_MOMENTS, _in_8_bits(p, state["exp_avg"], state["exp_avg_sq"])))
             on_device = self.capturable or self.skip_nonfinite
             count = int(saved["step"])
             if on_device:
@@ -200,9 +227,3 @@ class AdamW(torch.optim.Optimizer):
                     counters[key] = torch.tensor([count], dtype=torch.int64, device=p.device)
                 count = counters[key]
             state["step"] = count
-        for group, before in zip(self.param_groups, own):  # torch.optim.AdamW's groups do not have all options
-            for name, value in self.defaults.items():
-                group.setdefault(name, before.get(name, value))
-            group["betas"] = tuple(group["betas"])
-            if "decoupled_weight_decay" in group:
-                group["decoupled_weight_decay"] = True

@@ -1,0 +1,71 @@
+"""State dicts between terra_amd.optimizer.AdamW and torch's, groups and draws, on the device.
+
+Tolerances, with u = 2^-24, as in the other tests of the optimizer: n steps of fp32 parameters against 64 bits are off by 3 u of the
+parameter and 40 u of what a step takes off, at most 10 lr a step: n (3 u max|p| + 400 u lr)."""
+import copy
+
+import pytest
+import torch
+
+from terra_amd import kernels, workloads
+from terra_amd.optimizer import AdamW
+
+pytestmark = pytest.mark.gpu
+
+U = 2.0 ** -24
+SHAPES = [(70, 90), (90,), (5000,), (1,)]
+OPTS = dict(lr=1e-2, betas=(0.9, 0.99), eps=1e-6, weight_decay=0.1)
+
+
+def _params(dev, dtype=torch.float32):
+    return [torch.nn.Parameter(workloads.activations(s, 10 + i, torch.float32).to(dtype).to(dev)) for i, s in enumerate(SHAPES)]
+
+
+def _set_grads(params, step):
+    for i, p in enumerate(params):
+        p.grad = (workloads.activations(tuple(p.shape), 100 * step + i, torch.float32) * 0.3).to(p.dtype).to(p.device)
+
+
+def _steps(opt, steps):
+    params = [p for g in opt.param_groups for p in g["params"]]
+    for step in steps:
+        _set_grads(params, step)
+        opt.step()
+
+
+def _near(params, ref, n, lr=OPTS["lr"]):
+    for p, r in zip(params, ref):
+        e = (p.detach().double().cpu() - r.detach()).abs().max().item()
+        assert e <= n * (3 * U * r.detach().abs().max().item() + 400 * U * lr), e
+
+
+def test_moments_of_torchs_step_on_in_8_bits(dev):
+    """What was loaded is what the next step takes: its first moment is beta1 times the codes' value and the gradient's part.
+    The sum in 64 bits of two terms rounded to 32, 2 u of their magnitudes, and half a step of e4m3 at most, 2^-4 of
+    the value or half of the least step, 2^-10 of the scale."""
+    theirs = torch.optim.AdamW(_params(dev), **OPTS)
+    _steps(theirs, (1, 2))
+    params = [torch.nn.Parameter(p.detach().clone()) for p in theirs.param_groups[0]["params"]]
+    ours = AdamW(params, bits=8, min_8bit_size=100, seed=3)
+    ours.load_state_dict(copy.deepcopy(theirs.state_dict()))
+    read = {}
+    for p in params:
+        s = ours.state[p]
+        assert ("scales" in s) == (p.numel() >= 100) and s["step"] == 2
+        if "scales" in s:
+            read[p] = [t.double() for t in kernels.Moments(s["exp_avg"], s["exp_avg_sq"], s["scales"]).values()]
+    _steps(ours, (3,))
+    for p, (m, v) in read.items():
+        s = ours.state[p]
+        got = kernels.Moments(s["exp_avg"], s["exp_avg_sq"], s["scales"]).values()[0].double()
+        terms = 0.9 * m, 0.1 * p.grad.double()
+        least = 2.0 ** -10 * s["scales"][0].double().repeat_interleave(256)[:p.numel()].view(p.shape)
+        tol = 2 * U * (terms[0].abs() + terms[1].abs()) + torch.maximum(2.0 ** -4 * (terms[0] + terms[1]).abs() * (1 + 4 * U), least)
+        assert bool(((got - terms[0] - terms[1]).abs() <= tol * (1 + 8 * U)).all())
+        assert p.isfinite().all()
+    with_codes = ours.state_dict()
+    again = AdamW([torch.nn.Parameter(p.detach().clone()) for p in params], bits=8)
+    again.load_state_dict(copy.deepcopy(with_codes))
+    _steps(ours, (4,))
+    _steps(again, (4,))
+    assert all(torch.equal(p, q) for p, q in zip(params, again.param_groups[0]["params"]))

@@ -5,6 +5,7 @@ import io
 import pytest
 import torch
 
+from oracle import training as tr
 from terra_amd import kernels
 from terra_amd.optimizer import AdamW
 
@@ -122,3 +123,61 @@ def test_options_of_ones_own_groups_stay():
     assert (b["bits"], b["min_8bit_size"], b["lr"]) == (32, 4096, 1e-3)
     ours.load_state_dict(AdamW(_groups(_params(), bits=8, min_8bit_size=7, seed=11)).state_dict())
     assert (ours.param_groups[0]["min_8bit_size"], ours.param_groups[0]["seed"]) == (7, 11)  # said, so taken
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_moments_of_torchs_in_8_bits(dtype):
+    """A group of 8 bits has what it loads in 8 bits.  With u = 2^-24, a scale is off by a rounding and a quotient by another:
+    the nearest code is that of a value within 3 u of the quotient (the root: one more rounding), half a step of e4m3 at most, 2^-4 of
+    the value or half of its least step, from it."""
+    theirs = torch.optim.AdamW(_params(), **OPTS)
+    theirs.param_groups[0]["params"][0].data = theirs.param_groups[0]["params"][0].data.t().contiguous().t()
+    for step in (1, 2):
+        _set_grads(theirs.param_groups[0]["params"], step)
+        theirs.param_groups[0]["params"][2].grad[256:600] *= 10.0 ** torch.linspace(-9, 3, 344)
+        theirs.param_groups[0]["params"][2].grad[768:1024] = 0.0
+        theirs.step()
+    params = _params(dtype)
+    params[0].data = params[0].data.t().contiguous().t()
+    ours = AdamW(params, bits=8, min_8bit_size=100, seed=1)
+    ours.load_state_dict(copy.deepcopy(theirs.state_dict()))
+    for p, q in zip(theirs.param_groups[0]["params"], params):
+        a, b = theirs.state[p], ours.state[q]
+        assert b["step"] == 2 and ("scales" in b) == (q.numel() >= 100)
+        if "scales" not in b:
+            assert torch.equal(b["exp_avg"], a["exp_avg"]) and torch.equal(b["exp_avg_sq"], a["exp_avg_sq"])
+            continue
+        held = kernels.Moments(b["exp_avg"], b["exp_avg_sq"], b["scales"])
+        assert all(t.dtype == torch.float8_e4m3fn and t.shape == q.shape and t.stride() == q.stride() for t in held[:2])
+        for i, values in enumerate((a["exp_avg"].double(), a["exp_avg_sq"].double().sqrt())):
+            lain = torch.empty_like(q, dtype=torch.float64).copy_(values).as_strided((q.numel(),), (1,))
+            codes = held[i].as_strided((q.numel(),), (1,))
+            block = torch.arange(q.numel()) // 256
+            top = torch.zeros(held.scales.shape[1], dtype=torch.float64).scatter_reduce_(0, block, lain.abs(), "amax")
+            scales = held.scales[i].double()
+            assert bool(((scales - top / 448).abs() <= 2 * 2.0 ** -24 * top / 448).all())
+            per = scales[block]
+            e = (codes.double() * per - lain).abs()
+            low = 2.0 ** -10 * (1 if i == 0 else 2)  # a root below the least code is held as that
+            assert bool((e <= torch.maximum((2.0 ** -4 + 8 * 2.0 ** -24) * lain.abs(), low * per)).all())
+            assert i == 0 or torch.equal(lain > 0, codes.float() > 0)
+
+
+def test_nearest_codes_of_moments():
+    """Against the oracle's codes, away from the borders of two; infinities and NaN make a block NaN, as in a step."""
+    from terra_amd.optimizer import _in_8_bits
+
+    gen = torch.Generator().manual_seed(3)
+    m = torch.randn(1000, generator=gen) * 10.0 ** (torch.rand(1000, generator=gen) * 6 - 6)
+    v = torch.rand(1000, generator=gen) * 10.0 ** (torch.rand(1000, generator=gen) * 12 - 12)
+    m[600], v[900] = float("nan"), float("inf")
+    held = _in_8_bits(torch.zeros(1000), m, v)
+    block = torch.arange(1000) // 256
+    a, b = held.values()
+    assert a.isnan().nonzero().view(-1).tolist() == list(range(512, 768)) and b.isnan().nonzero().view(-1).tolist() == list(range(768, 1000))
+    ok = block != 2
+    code, near = tr.nearest_code((m.double() / held.scales[0].double()[block])[ok])
+    same = code == held.exp_avg.view(torch.uint8)[ok]
+    assert bool((same | (near < 8 * 2.0 ** -24) | ((code % 128 == 0) & (held.exp_avg.view(torch.uint8)[ok] % 128 == 0))).all())
+    empty = _in_8_bits(torch.zeros(3, 0), torch.zeros(3, 0), torch.zeros(3, 0))
+    assert empty.scales.shape == (2, 0) and empty.exp_avg.shape == (3, 0)
