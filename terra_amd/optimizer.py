@@ -179,9 +179,16 @@ class AdamW(torch.optim.Optimizer):
     def load_state_dict(self, state_dict):
         own, given = self.param_groups, []
 
+        def pairs(made):  # its numbers of the parameters, and those
+            return zip(*(chain.from_iterable(g["params"] for g in groups) for groups in (made["param_groups"], own)))
+
         def check(_, made):  # what the hooks before it made of the state dict, before anything is changed
             for group in made["param_groups"]:
                 _refuse_other_updates(group)
+            for at, p in pairs(made):
+                state = made["state"].get(at) or {}
+                if state.get("scales") is not None and any(state[k].stride() != p.stride() for k in _MOMENTS[:2]):
+                    raise ValueError("moments in 8 bits of a parameter that lay otherwise in memory")
             given.append(made)
 
         hook = self.register_load_state_dict_pre_hook(check)
@@ -197,9 +204,8 @@ class AdamW(torch.optim.Optimizer):
             if "decoupled_weight_decay" in group:
                 group["decoupled_weight_decay"] = True
         # Moments keep their own types (the parent casts them to the parameters').
-        ids = chain.from_iterable(g["params"] for g in state_dict["param_groups"])
         counters, group_of = {}, {id(p): i for i, g in enumerate(self.param_groups) for p in g["params"]}
-        for at, p in zip(ids, chain.from_iterable(g["params"] for g in self.param_groups)):
+        for at, p in pairs(state_dict):
             saved = state_dict["state"].get(at)
             if not saved:
                 continue
@@ -212,8 +218,6 @@ class AdamW(torch.optim.Optimizer):
                     state[name] = t.detach().to(device=p.device, dtype=torch.float32, copy=True).contiguous()
                     continue
                 held = torch.float8_e4m3fn if saved.get("scales") is not None else torch.float32
-                if held != torch.float32 and t.stride() != p.stride():
-                    raise ValueError("moments in 8 bits of a parameter that lay otherwise in memory")
                 state[name] = torch.empty_like(p, dtype=held)
                 state[name].copy_(t.to(held))
             group = self.param_groups[group_of[id(p)]]

@@ -181,3 +181,28 @@ def test_nearest_codes_of_moments():
     assert bool((same | (near < 8 * 2.0 ** -24) | ((code % 128 == 0) & (held.exp_avg.view(torch.uint8)[ok] % 128 == 0))).all())
     empty = _in_8_bits(torch.zeros(3, 0), torch.zeros(3, 0), torch.zeros(3, 0))
     assert empty.scales.shape == (2, 0) and empty.exp_avg.shape == (3, 0)
+
+
+def _in_8_bits(params):
+    """An optimizer with 8-bit moments after two steps of torch's."""
+    opt = AdamW(params, bits=8, min_8bit_size=100, seed=1)
+    opt.load_state_dict(_theirs().state_dict())
+    return opt
+
+
+def test_moments_in_8_bits_of_another_layout_are_refused_as_a_whole():
+    """Their scales go by blocks of memory.  What was there stays, all of it."""
+    theirs, params = _in_8_bits(_params()), _params()
+    params[0].data = params[0].data.t().contiguous().t()
+    ours = AdamW(params, lr=0.5)
+    ours.load_state_dict(_theirs(3).state_dict())
+    before = _snapshot(ours)
+    with pytest.raises(ValueError, match="lay otherwise in memory"):
+        ours.load_state_dict(theirs.state_dict())
+    after = _snapshot(ours)
+    assert after[0] == before[0]
+    assert all(after[1][i][k] is before[1][i][k] for i in before[1] for k in before[1][i])
+    with pytest.raises(ValueError, match="match the size"):
+        AdamW(_params()[:3]).load_state_dict(theirs.state_dict())
+    with pytest.raises(ValueError, match="number of parameter groups"):
+        AdamW(_groups(_params())).load_state_dict(theirs.state_dict())
