@@ -176,6 +176,25 @@ class AdamW(torch.optim.Optimizer):
             out.append((members, count))
         return out
 
+    def state_dict(self):
+        """As torch's, each parameter with its count as a number (in device memory parameters share a counter, to
+        which an optimizer that loads it would add once for each of them)."""
+        numbers = {}
+
+        def counted(_, made):  # before the other hooks
+            for at, state in made["state"].items():
+                count = state.get("step") if isinstance(state, dict) else None
+                if isinstance(count, torch.Tensor):
+                    if id(count) not in numbers:
+                        numbers[id(count)] = int(count)
+                    made["state"][at] = {**state, "step": numbers[id(count)]}
+
+        hook = self.register_state_dict_post_hook(counted, prepend=True)
+        try:
+            return super().state_dict()
+        finally:
+            hook.remove()
+
     def load_state_dict(self, state_dict):
         own, given = self.param_groups, []
 

@@ -69,3 +69,27 @@ def test_moments_of_torchs_step_on_in_8_bits(dev):
     _steps(ours, (4,))
     _steps(again, (4,))
     assert all(torch.equal(p, q) for p, q in zip(params, again.param_groups[0]["params"]))
+
+
+@pytest.mark.parametrize("kw", [dict(capturable=True), dict(skip_nonfinite=True), dict()])
+@pytest.mark.parametrize("form", [dict(foreach=False), dict(foreach=True), dict(capturable=True), dict(fused=True)])
+def test_counts_step_on_in_torchs(dev, kw, form):
+    """From counts in device memory to each form of torch's step and back, against 64 bits all the way."""
+    params = _params(dev)
+    ref = [torch.nn.Parameter(p.detach().double().cpu()) for p in params]
+    ref_opt = torch.optim.AdamW(ref, **OPTS)
+    ours = AdamW(params, **OPTS, **kw)
+    _steps(ours, (1, 2))
+    back = torch.optim.AdamW(params, **form)
+    made = copy.deepcopy(ours.state_dict())
+    made["param_groups"][0].update(form)  # torch takes its options from the state dict
+    back.load_state_dict(made)
+    _steps(back, (3, 4))
+    _steps(ref_opt, (1, 2, 3, 4))
+    assert [int(back.state[p]["step"]) for p in params] == [4] * len(params)
+    assert [int(ours.state[p]["step"]) for p in params] == [2] * len(params)
+    _near(params, ref, 4)
+    ours.load_state_dict(copy.deepcopy(back.state_dict()))
+    _steps(ours, (5,))
+    _steps(ref_opt, (5,))
+    _near(params, ref, 5)

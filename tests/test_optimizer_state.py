@@ -206,3 +206,54 @@ def test_moments_in_8_bits_of_another_layout_are_refused_as_a_whole():
         AdamW(_params()[:3]).load_state_dict(theirs.state_dict())
     with pytest.raises(ValueError, match="number of parameter groups"):
         AdamW(_groups(_params())).load_state_dict(theirs.state_dict())
+
+
+# ---- counts in device memory ---------------------------------------------------------
+
+
+@pytest.mark.parametrize("kw", [dict(capturable=True), dict(skip_nonfinite=True), dict()])
+@pytest.mark.parametrize("foreach", [False, True])
+@pytest.mark.parametrize("saved", [True, False])
+def test_counts_that_load_into_torchs(kw, foreach, saved):
+    """Each parameter's count is its own in torch's optimizer, and steps there leave this one's."""
+    theirs, ours = _theirs(), AdamW(_params(), **kw)
+    ours.load_state_dict(copy.deepcopy(theirs.state_dict()))
+    made = ours.state_dict()
+    assert all(type(s["step"]) is int for s in made["state"].values())
+    if saved:
+        f = io.BytesIO()
+        torch.save(made, f)
+        f.seek(0)
+        made = torch.load(f, weights_only=True)
+    back = torch.optim.AdamW([torch.nn.Parameter(p.detach().clone()) for p in theirs.param_groups[0]["params"]], foreach=foreach)
+    back.load_state_dict(made)
+    back.param_groups[0]["foreach"] = foreach
+    for step in (3, 4):
+        for opt in (theirs, back):
+            _set_grads(opt.param_groups[0]["params"], step)
+            opt.step()
+    for p, q in zip(theirs.param_groups[0]["params"], back.param_groups[0]["params"]):
+        assert int(back.state[q]["step"]) == int(theirs.state[p]["step"]) == 4
+        assert torch.allclose(p, q, rtol=1e-6, atol=1e-7)
+    assert all(int(ours.state[p]["step"]) == 2 for p in ours.param_groups[0]["params"])
+
+
+def test_parameters_share_their_counter_again():
+    theirs = _theirs()
+    ours, other = (AdamW(_params(), capturable=True) for _ in range(2))
+    ours.load_state_dict(theirs.state_dict())
+    other.load_state_dict(ours.state_dict())
+    for opt in (ours, other):
+        counts = [opt.state[p]["step"] for p in opt.param_groups[0]["params"]]
+        assert all(c is counts[0] for c in counts) and counts[0].dtype == torch.int64 and int(counts[0]) == 2
+    assert other.state[other.param_groups[0]["params"][0]]["step"] is not ours.state[ours.param_groups[0]["params"][0]]["step"]
+
+
+def test_hooks_see_the_counts_that_are_saved():
+    ours, seen = AdamW(_params(), capturable=True), []
+    ours.load_state_dict(_theirs().state_dict())
+    ours.register_state_dict_post_hook(lambda _, d: seen.append([s["step"] for s in d["state"].values()]) or {"optimizer": d})
+    for _ in range(2):
+        made = ours.state_dict()
+        assert list(made) == ["optimizer"] and [s["step"] for s in made["optimizer"]["state"].values()] == [2] * 4
+    assert seen == [[2] * 4] * 2 and all(type(n) is int for n in seen[0])
