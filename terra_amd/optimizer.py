@@ -46,7 +46,9 @@ class AdamW(torch.optim.Optimizer):
     bits, and with clipping to a norm over all groups in the step itself.
 
     ``bits``: 32, or 8 for parameters of at least ``min_8bit_size`` elements (see
-    :func:`kernels.adamw_step`; smaller ones keep 32).  ``seed`` fixes their random rounding (None: from torch's generator).
+    :func:`kernels.adamw_step`; smaller ones keep 32).  ``seed`` fixes their random rounding
+    (None: from torch's generator, one for all groups that have none of their own; processes that hold replicas of the
+    parameters need the same).
     ``max_grad_norm``: gradients are scaled by min(1, max_grad_norm / (norm + 1e-6)) as
     they are read; ``param.grad`` stays as it is, and ``grad_norm`` holds the norm (on
     the device) after a step.  ``skip_nonfinite``: a step whose norm is infinite or
@@ -72,10 +74,8 @@ class AdamW(torch.optim.Optimizer):
             raise ValueError(f"eps and weight_decay must be >= 0 (got {eps}, {weight_decay})")
         if max_grad_norm is not None and not max_grad_norm > 0.0:
             raise ValueError(f"max_grad_norm must be positive (got {max_grad_norm})")
-        if seed is None:
-            seed = int(torch.randint(0, 1 << 62, (1,)).item()) if bits == 8 else 0
         super().__init__(params, dict(lr=lr, betas=tuple(betas), eps=eps, weight_decay=weight_decay, maximize=maximize,
-                                      bits=bits, min_8bit_size=min_8bit_size, seed=int(seed)))
+                                      bits=bits, min_8bit_size=min_8bit_size, seed=None if seed is None else int(seed)))
         self.max_grad_norm, self.skip_nonfinite, self.capturable = max_grad_norm, bool(skip_nonfinite), bool(capturable)
         self.grad_norm: Optional[torch.Tensor] = None
         self._seeds = {}
@@ -91,9 +91,20 @@ class AdamW(torch.optim.Optimizer):
     def add_param_group(self, param_group):
         if isinstance(param_group, dict):
             _refuse_other_updates({**self.defaults, **param_group})
+            if param_group.get("bits", self.defaults["bits"]) == 8 and param_group.get("seed") is None:
+                param_group["seed"] = self._drawn_seed()
         super().add_param_group(param_group)
 
-    def _seed(self, seed: int, device: torch.device) -> torch.Tensor:
+    def _drawn_seed(self) -> int:
+        """The seed of groups that are given none, drawn when the first of them needs it."""
+        if self.defaults["seed"] is None:
+            self.defaults["seed"] = int(torch.randint(0, 1 << 62, (1,)).item())
+        return self.defaults["seed"]
+
+    def _seed(self, group: dict, device: torch.device) -> torch.Tensor:
+        if group["seed"] is None:  # its bits were set later
+            group["seed"] = self._drawn_seed()
+        seed = group["seed"]
         t = self._seeds.get((seed, device))
         if t is None:
             t = self._seeds[seed, device] = torch.tensor([seed], dtype=torch.int64, device=device)
@@ -129,7 +140,7 @@ class AdamW(torch.optim.Optimizer):
                                    eps=group["eps"], weight_decay=group["weight_decay"], maximize=group["maximize"],
                                    grad_factor=None if norm is None or self.max_grad_norm is None else norm.factor,
                                    found_inf=norm.nonfinite if self.skip_nonfinite else None,
-                                   seed=self._seed(group["seed"], params[0].device) if group["bits"] == 8 else None,
+                                   seed=self._seed(group, params[0].device) if group["bits"] == 8 else None,
                                    stream=index)
         return loss
 
@@ -219,6 +230,8 @@ class AdamW(torch.optim.Optimizer):
         for group, before in zip(self.param_groups, own):  # torch.optim.AdamW's groups do not have all options
             for name, value in self.defaults.items():
                 group.setdefault(name, before.get(name, value))
+            if group["seed"] is None:
+                group["seed"] = before.get("seed")
             group["betas"] = tuple(group["betas"])
             if "decoupled_weight_decay" in group:
                 group["decoupled_weight_decay"] = True

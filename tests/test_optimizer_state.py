@@ -257,3 +257,55 @@ def test_hooks_see_the_counts_that_are_saved():
         made = ours.state_dict()
         assert list(made) == ["optimizer"] and [s["step"] for s in made["optimizer"]["state"].values()] == [2] * 4
     assert seen == [[2] * 4] * 2 and all(type(n) is int for n in seen[0])
+
+
+# ---- seeds -------------------------------------------------------------------------
+
+
+def _drawn(n):
+    """The n seeds that torch's generator would give after seed 5."""
+    with torch.random.fork_rng(devices=[]):
+        torch.manual_seed(5)
+        return [int(torch.randint(0, 1 << 62, (1,)).item()) for _ in range(n)]
+
+
+def test_seeds_of_groups():
+    """A group of 8 bits has a seed of torch's generator wherever it said so; nothing is drawn without one."""
+    first, _ = _drawn(2)
+    with torch.random.fork_rng(devices=[]):
+        torch.manual_seed(5)
+        before = torch.get_rng_state()
+        AdamW(_params())
+        AdamW(_params(), bits=8, seed=3)
+        AdamW([dict(params=_params(), bits=8, seed=0)])
+        assert torch.equal(torch.get_rng_state(), before)
+        assert AdamW(_params(), bits=8).param_groups[0]["seed"] == first
+        torch.manual_seed(5)
+        opt = AdamW(_groups(_params(), bits=8))  # the group says 8 bits, the optimizer 32
+        assert opt.param_groups[0]["seed"] == first
+        opt.add_param_group(dict(params=_params(), bits=8))
+        opt.add_param_group(dict(params=_params(), bits=8, seed=0))
+        assert [g["seed"] for g in opt.param_groups[2:]] == [first, 0]
+    assert AdamW(_groups(_params(), bits=8), seed=12).param_groups[0]["seed"] == 12
+    assert [g["seed"] for g in AdamW(_groups(_params(), bits=8, seed=4), bits=8, seed=12).param_groups] == [4, 12]
+
+
+def test_a_group_whose_bits_are_set_later_has_a_seed():
+    first, = _drawn(1)
+    opt = AdamW(_params())
+    opt.param_groups[0]["bits"] = 8
+    with torch.random.fork_rng(devices=[]):
+        torch.manual_seed(5)
+        assert opt._seed(opt.param_groups[0], torch.device("cpu")).tolist() == [first]
+    assert opt._seed(opt.param_groups[0], torch.device("cpu")).tolist() == [first] == [opt.param_groups[0]["seed"]]
+    assert opt.state_dict()["param_groups"][0]["seed"] == first
+
+
+def test_seeds_go_with_state_dicts():
+    opt = AdamW(_groups(_params(), bits=8))
+    other = AdamW(_groups(_params(), bits=8))
+    other.load_state_dict(opt.state_dict())
+    assert other.param_groups[0]["seed"] == opt.param_groups[0]["seed"]
+    eight = AdamW(_params(), bits=8, seed=3)
+    eight.load_state_dict(AdamW(_params()).state_dict())  # of 32 bits: it names no seed
+    assert (eight.param_groups[0]["bits"], eight.param_groups[0]["seed"]) == (32, 3)
