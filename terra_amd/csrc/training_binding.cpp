@@ -392,14 +392,17 @@ struct AdamOptions {
   bool maximize;
 };
 
+// places: the tensors' numbers in the random numbers' counter, as many as there are tensors, or none: their places in the list.
 void adamw_step(const std::vector<Tensor>& params, const std::vector<Tensor>& grads, const std::vector<Tensor>& firsts,
-                const std::vector<Tensor>& seconds, const std::vector<std::optional<Tensor>>& scales, const AdamOptions& o) {
+                const std::vector<Tensor>& seconds, const std::vector<std::optional<Tensor>>& scales,
+                const std::vector<uint32_t>& places, const AdamOptions& o) {
   const pybind11::gil_scoped_release no_gil;
   const at::AutoGradMode off(false);
   if (params.empty()) return;
   const size_t n = params.size();
   TORCH_CHECK_VALUE(grads.size() == n && firsts.size() == n, "as many gradients and moments as parameters (got ", n, ", ",
                     grads.size(), " and ", firsts.size(), ")");
+  TORCH_CHECK_VALUE(places.empty() || places.size() == n, "as many places as parameters (got ", n, " and ", places.size(), ")");
   const c10::Device device = params[0].device();
   std::vector<terra_swin_adamw_tensor> list;
   list.reserve(n);
@@ -432,7 +435,7 @@ void adamw_step(const std::vector<Tensor>& params, const std::vector<Tensor>& gr
     list.push_back({const_cast<void*>(p.const_data_ptr()), g.const_data_ptr(), const_cast<void*>(m.const_data_ptr()),
                     const_cast<void*>(v.const_data_ptr()),
                     scaled ? static_cast<float*>(const_cast<void*>(scales[i]->const_data_ptr())) : nullptr, p.numel(),
-                    static_cast<uint32_t>(i), dtype_code(p.scalar_type()), dtype_code(g.scalar_type())});
+                    places.empty() ? static_cast<uint32_t>(i) : places[i], dtype_code(p.scalar_type()), dtype_code(g.scalar_type())});
   }
   TORCH_CHECK_VALUE(!scaled_any || o.seed.has_value(), "moments in 8 bits need a seed (see dropout_seed)");
   const c10::DeviceGuard guard(device);
@@ -486,12 +489,13 @@ PYBIND11_MODULE(_training, m) {
   m.def("rotary_with_gradient", torch::wrap_pybind_function_no_gil(&rotary_with_gradient));
   m.def("gradient_norm", &gradient_norm);
   m.def("adamw_step", [](const std::vector<Tensor>& params, const std::vector<Tensor>& grads, const std::vector<Tensor>& firsts,
-                         const std::vector<Tensor>& seconds, const std::vector<std::optional<Tensor>>& scales, double lr,
+                         const std::vector<Tensor>& seconds, const std::vector<std::optional<Tensor>>& scales,
+                         const std::vector<uint32_t>& places, double lr,
                          double beta1, double beta2, double eps, double weight_decay, int64_t step,
                          const std::optional<Tensor>& step_tensor, const std::optional<Tensor>& lr_tensor,
                          const std::optional<Tensor>& grad_factor, const std::optional<Tensor>& found_inf,
                          const std::optional<Tensor>& seed, uint32_t stream, bool maximize) {
-    adamw_step(params, grads, firsts, seconds, scales,
+    adamw_step(params, grads, firsts, seconds, scales, places,
                {lr, beta1, beta2, eps, weight_decay, step, step_tensor, lr_tensor, grad_factor, found_inf, seed, stream, maximize});
   });
 }

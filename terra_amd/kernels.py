@@ -1924,7 +1924,8 @@ def adamw_step(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], mo
                step: Union[int, torch.Tensor], lr: Union[float, torch.Tensor] = 1e-3,
                betas: Tuple[float, float] = (0.9, 0.999), eps: float = 1e-8, weight_decay: float = 1e-2,
                maximize: bool = False, grad_factor: Optional[torch.Tensor] = None,
-               found_inf: Optional[torch.Tensor] = None, seed: Optional[torch.Tensor] = None, stream: int = 0) -> None:
+               found_inf: Optional[torch.Tensor] = None, seed: Optional[torch.Tensor] = None, stream: int = 0,
+               places: Optional[Sequence[int]] = None) -> None:
     """An AdamW step (decoupled weight decay) over many tensors in a few launches, in place:
 
         g = grad * grad_factor
@@ -1938,8 +1939,9 @@ def adamw_step(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], mo
 
     Moments in 8 bits (see :class:`Moments`): the first is rounded to the nearest code; the second up or down at random, with the
     mean that it has (0.999 v lies far nearer to v's own code than to the next: rounded to nearest it would never move),
-    from ``seed`` (see :func:`dropout_seed`), ``stream``, the step, the tensor's place in
-    the list and the element.  A block of 256 with an infinity or a NaN is NaN as a whole from then on.
+    from ``seed`` (see :func:`dropout_seed`), ``stream``, the step, the tensor's number in
+    ``places`` (by default its place in the list) and the element: calls with the same seed, stream and step need other places each.
+    A block of 256 with an infinity or a NaN is NaN as a whole from then on.
 
     No two of the tensors may overlap, nor a gradient one that is written."""
     beta1, beta2 = betas
@@ -1947,8 +1949,11 @@ def adamw_step(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], mo
         raise ValueError(f"as many moments as parameters (got {len(moments)} and {len(params)})")
     if not 0 <= stream < 1 << 32:
         raise ValueError(f"stream must be in [0, 2^32) (got {stream})")
+    places = None if places is None else list(places)
+    if places is not None and (len(places) != len(params) or not all(0 <= place < 1 << 32 for place in places)):
+        raise ValueError(f"places must be one number in [0, 2^32) for each of the {len(params)} parameters (got {places})")
     step_at, lr_at = (t if isinstance(t, torch.Tensor) else None for t in (step, lr))
     _lib.load_training().adamw_step(
-        list(params), list(grads), [m[0] for m in moments], [m[1] for m in moments], [m[2] for m in moments],
+        list(params), list(grads), [m[0] for m in moments], [m[1] for m in moments], [m[2] for m in moments], places or [],
         0.0 if lr_at is not None else float(lr), float(beta1), float(beta2), float(eps), float(weight_decay),
         0 if step_at is not None else int(step), step_at, lr_at, grad_factor, found_inf, seed, stream, bool(maximize))

@@ -134,6 +134,8 @@ class AdamW(torch.optim.Optimizer):
             self.grad_norm = norm.norm
         on_device = self.capturable or self.skip_nonfinite
         for index, (group, params) in enumerate(zip(self.param_groups, active)):
+            # A tensor's draws go by its place in the group, whichever parameters step together.
+            place = {id(p): i for i, p in enumerate(group["params"])} if group["bits"] == 8 else None
             for params, count in self._counted(group, params, on_device, norm):
                 moments = [Moments(s["exp_avg"], s["exp_avg_sq"], s.get("scales")) for s in map(self.state.__getitem__, params)]
                 kernels.adamw_step(params, [p.grad for p in params], moments, count, lr=group["lr"], betas=group["betas"],
@@ -141,7 +143,7 @@ class AdamW(torch.optim.Optimizer):
                                    grad_factor=None if norm is None or self.max_grad_norm is None else norm.factor,
                                    found_inf=norm.nonfinite if self.skip_nonfinite else None,
                                    seed=self._seed(group, params[0].device) if group["bits"] == 8 else None,
-                                   stream=index)
+                                   stream=index, places=None if place is None else [place[id(p)] for p in params])
         return loss
 
     def replayed(self) -> None:

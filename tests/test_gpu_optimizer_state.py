@@ -93,3 +93,55 @@ def test_counts_step_on_in_torchs(dev, kw, form):
     _steps(ours, (5,))
     _steps(ref_opt, (5,))
     _near(params, ref, 5)
+
+
+def _codes(opt, p):
+    return opt.state[p]["exp_avg_sq"].view(torch.uint8)
+
+
+@pytest.mark.parametrize("capturable", [True, False])
+def test_draws_of_tensors_that_step_apart(dev, capturable):
+    """Two parameters of one group with the same gradients and as many steps, which each left out another step: their
+    codes are drawn apart."""
+    params = [torch.nn.Parameter(torch.zeros(5000, device=dev)) for _ in range(3)]
+    opt = AdamW(params, bits=8, min_8bit_size=100, seed=5, capturable=capturable)
+    for left in (0, 1, None, None):
+        for i, p in enumerate(params):
+            p.grad = None if i == left else torch.linspace(0.01, 1.0, 5000, device=dev)
+        opt.step()
+    assert [int(opt.state[p]["step"]) for p in params] == [3, 3, 4]
+    a, b, c = (_codes(opt, p) for p in params)
+    assert not torch.equal(a, b) and not torch.equal(a, c) and not torch.equal(b, c)
+
+
+def test_draws_do_not_go_by_what_else_steps(dev):
+    """The same parameter at the same place of its group: alone, or with others that step, or that have no gradient."""
+    def run(with_gradient):
+        params = [torch.nn.Parameter(torch.zeros(n, device=dev)) for n in (300, 5000)]
+        opt = AdamW(params, bits=8, min_8bit_size=100, seed=5)
+        for _ in range(3):
+            params[1].grad = torch.linspace(0.01, 1.0, 5000, device=dev)
+            params[0].grad = torch.ones(300, device=dev) if with_gradient else None
+            opt.step()
+        return _codes(opt, params[1])
+
+    assert torch.equal(run(True), run(False))
+
+
+def test_places(dev):
+    """A call's places are the tensors' numbers; without, their places in the list."""
+    def run(order, **kw):
+        params = [torch.zeros(1000, device=dev) for _ in range(3)]
+        moments = [kernels.moments(p, 8) for p in params]
+        grads = [torch.linspace(0.01, 1.0 + i, 1000, device=dev) for i in range(3)]
+        pick = lambda ts: [ts[i] for i in order]  # noqa: E731
+        kernels.adamw_step(pick(params), pick(grads), pick(moments), 1, seed=torch.tensor([9], device=dev), **kw)
+        return [m.exp_avg_sq.view(torch.uint8) for m in moments]
+
+    ref = run((0, 1, 2))
+    for got in (run((0, 1, 2), places=(0, 1, 2)), run((2, 0, 1), places=[2, 0, 1])):
+        assert all(torch.equal(a, b) for a, b in zip(got, ref))
+    assert all(not torch.equal(a, b) for a, b in zip(run((0, 1, 2), places=(5, (1 << 32) - 1, 7)), ref))
+    for bad in ((), (0, 1), (0, 1, 2, 3), (0, 1, -1), (0, 1, 1 << 32)):
+        with pytest.raises(ValueError, match="places"):
+            run((0, 1, 2), places=bad)
