@@ -80,7 +80,7 @@ constexpr int kNormHeld = 16384;  // channels of rows that are held in registers
 // and two rows, goes so far as four chunks (78336 x 2048: 156 us, as 256 lanes 167; 39168 x 4096 as
 // 256 lanes of two 161, as waves of eight 175); rows that are not aligned or that have fp32 in them as far as two
 // where a few lanes hold them.  As few lanes as chunks where a row has at most eight: the heads of a packed q | k | v.
-TailShape norm_shape(int C, bool pieces, bool vec, bool backward) {
+constexpr TailShape norm_shape(int C, bool pieces, bool vec, bool backward) {
   const int n = (C + kChunkCols - 1) / kChunkCols;
   if (n <= 8) return {n <= 2 ? 2 : n <= 4 ? 4 : 8, 1};
   if (n > 1024) return {1024, 2};
@@ -94,7 +94,7 @@ TailShape norm_shape(int C, bool pieces, bool vec, bool backward) {
 // row begins in one.  Parameters stand in registers too: one to three chunks a lane, up to four where waves can hold the
 // row so.  Three where two would leave many lanes idle (60 million elements, bf16 backward: 514 by 32 lanes of
 // three 83 us, by 64 of two 108; 1030 by 64 of three 82, by 64 of four 141, by 256 of one 163).
-TailShape flat_shape(int C, int chunk) {
+constexpr TailShape flat_shape(int C, int chunk) {
   const int n = (C + chunk - 1 + kChunkCols - 1) / kChunkCols;
   if (n <= 16) return {n <= 8 ? 8 : 16, 1};
   for (int lanes = 8; lanes <= 32; lanes *= 2) {
@@ -104,6 +104,44 @@ TailShape flat_shape(int C, int chunk) {
   if (n <= 256) return {64, n <= 128 ? 2 : n <= 192 ? 3 : 4};
   return {n <= 512 ? 256 : n <= 1024 ? 512 : 1024, 2};
 }
+
+// Every row that is held has a shape that holds it, among those that the launches know (layer_norm_kernels.h, where
+// eight lanes of three chunks have no kernel that accesses fp32 by pieces).
+constexpr bool norm_shape_known(TailShape s, bool pieces, bool backward) {
+  switch (s.lanes * 10 + s.chunks) {
+    case 21: case 41: case 81: case 161: case 162: case 163: case 322: case 323: case 642: case 644: case 5122: case 10242: return true;
+    case 83: return !pieces;
+    case 648: return !backward;
+    case 2562: return backward;
+    default: return false;
+  }
+}
+constexpr bool flat_shape_known(TailShape s) {
+  switch (s.lanes * 10 + s.chunks) {
+    case 81: case 83: case 161: case 162: case 163: case 322: case 323: case 642: case 643: case 644: case 2562: case 5122:
+    case 10242: return true;
+    default: return false;
+  }
+}
+constexpr bool norm_shapes_hold() {
+  for (int n = 1; n <= kNormHeld / kChunkCols; ++n)  // a shape goes by the chunks of a row
+    for (int options = 0; options < 8; ++options) {
+      const bool pieces = options & 1, backward = options & 4;
+      const TailShape s = norm_shape(n * kChunkCols, pieces, options & 2, backward);
+      if (s.lanes * s.chunks < n || !norm_shape_known(s, pieces, backward)) return false;
+    }
+  return true;
+}
+constexpr bool flat_shapes_hold() {
+  for (int n = 2; n <= kNormHeld / kChunkCols; ++n)
+    for (int chunk = 4; chunk <= kChunkCols; chunk += 4) {  // of the widest row that touches n chunks
+      const TailShape s = flat_shape(n * kChunkCols - chunk + 1, chunk);
+      if (s.lanes * s.chunks < n || !flat_shape_known(s)) return false;
+    }
+  return true;
+}
+static_assert(norm_shapes_hold(), "a row without a shape that holds it");
+static_assert(flat_shapes_hold(), "a packed row without a shape that holds it");
 
 // Whether packed rows that are not whole chunks are read by the tensor's aligned chunks, or by columns (16-bit ones by pairs
 // where those stand aligned).  60 million elements, by chunks and by columns, us: 1001 bf16 forward 57, 92, backward

@@ -629,6 +629,7 @@ void flat_bwd(const NormArgs& a, const NormPlan& p, hipStream_t s) {
     return f<DTX, DTY, g, k, false, false>(__VA_ARGS__);                                     \
   }
 // Calls f<DTX, DTY, lanes, chunks, kVec, kPairs>(...) for the shape of the call; wide: that of 2049 to 4096 channels.
+// 83 is no shape of fp32 pieces, which layer_norm.hip asserts of all widths.
 #define TERRA_NORM_SHAPES(f, shape, wide, ...)                                                   \
   switch ((shape).lanes * 10 + (shape).chunks) {                                             \
     case 21: TERRA_NORM_ROWS(f, 2, 1, __VA_ARGS__)                                           \

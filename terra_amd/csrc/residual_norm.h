@@ -243,7 +243,7 @@ struct RowLanes {
 // single columns take more (524288 x 190 bf16: 530 us, with three 1091).  Eight lanes a row only where
 // columns stand eight by eight: as 16-byte pieces of fp32 they would read a
 // 16-bit h in runs of 64 bytes.  From 129 chunks on a workgroup holds the row.
-inline TailShape tail_shape(int C, bool pieces, int most) {
+constexpr TailShape tail_shape(int C, bool pieces, int most) {
   const int n = (C + kChunkCols - 1) / kChunkCols;
   if (n > 512) return {512, 2};
   if (n > 256) return {512, 1};
