@@ -737,7 +737,7 @@ typedef struct terra_swin_rotary_desc {
 } terra_swin_rotary_desc;
 
 /* turns: fp64 [dim / 2 / axes].  y may be x itself, with x's strides; it must not
- * overlap it otherwise. */
+ * overlap it otherwise.  Each stride of y steps over all that the smaller ones reach, in any order of the three. */
 int terra_swin_rotary(const void* x, void* y, const void* positions, const double* turns,
                       const terra_swin_rotary_desc* desc, void* stream);
 

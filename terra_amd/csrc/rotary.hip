@@ -14,6 +14,7 @@
 // copy moves the same bytes in 250); by the sines and cosines where it has one (200000 of 128: 29 us, 3.6 TB/s).
 #include "row_chunk.h"
 
+#include <algorithm>
 #include <initializer_list>
 
 namespace terra {
@@ -258,6 +259,25 @@ int64_t rotary_span(int64_t tokens, int64_t inner, int64_t so, int64_t si, int64
   return (tokens - 1) / inner * so + (tokens < inner ? tokens - 1 : inner - 1) * si + (int64_t)(heads - 1) * sh + head_dim;
 }
 
+struct Level {
+  int64_t stride, size;
+};
+
+// Whether each level of a tensor steps over all that the finer ones reach, so that no two elements share a place.
+bool strides_nest(const Level (&levels)[4]) {
+  Level by_stride[4];
+  int count = 0;
+  for (const Level& l : levels)
+    if (l.size > 1) by_stride[count++] = l;
+  std::sort(by_stride, by_stride + count, [](const Level& a, const Level& b) { return a.stride < b.stride; });
+  __int128 reach = 1;
+  for (int i = 0; i < count; ++i) {
+    if (by_stride[i].stride < reach) return false;
+    reach += (__int128)(by_stride[i].size - 1) * by_stride[i].stride;
+  }
+  return true;
+}
+
 }  // namespace
 }  // namespace terra
 
@@ -294,6 +314,8 @@ extern "C" int terra_swin_rotary(const void* x, void* y, const void* positions, 
   const int64_t outer_tokens = (d->tokens - 1) / d->inner, inner_tokens = d->tokens < d->inner ? d->tokens : d->inner;
   if ((d->heads > 1 && d->y_head_stride == 0) || (inner_tokens > 1 && d->y_inner_stride == 0) || (outer_tokens > 0 && d->y_outer_stride == 0))
     return fail(TERRA_ERR_SHAPE, "elements of y share a place");
+  if (!strides_nest({{1, d->head_dim}, {d->y_head_stride, d->heads}, {d->y_inner_stride, inner_tokens}, {d->y_outer_stride, outer_tokens + 1}}))
+    return fail(TERRA_ERR_SHAPE, "y's strides do not nest: elements of it may share a place");
   const bool same = x == y && d->x_outer_stride == d->y_outer_stride && d->x_inner_stride == d->y_inner_stride &&
                     d->x_head_stride == d->y_head_stride;
   const uintptr_t p = (uintptr_t)x, q = (uintptr_t)y;

@@ -1861,7 +1861,8 @@ def rotary(x: torch.Tensor, rotary: Rotary, positions: torch.Tensor, inverse: bo
     last dimension) for each token of x's last dimensions before the heads, shared over those
     before them: [N] or [B, N] for x [B, N, heads, head_dim].  Angles are taken in 64 bits, the
     rotation in fp32, rounded once.  ``inverse``: by the negative angles, which is the backward.
-    The tokens may have two strides, the heads another.  ``out`` may be ``x``, whose unrotated elements are then not touched."""
+    The tokens may have two strides, the heads another.  ``out`` may be ``x``, whose unrotated elements are then not touched; no
+    two of its elements may share a place."""
     call = _rotary_call(x, rotary, positions, bool(inverse), out)
     return _lib.load_training().rotary(call, x, positions, rotary.turns(x.device), out)
 
