@@ -65,12 +65,15 @@ def plain_norm(module: torch.nn.Module, channels: int) -> bool:
 def normed(module: torch.nn.Module, x: torch.Tensor) -> torch.Tensor:
     """``module(x)``, by the HIP kernels where it is a :func:`plain_norm` over x's last
     dimension: in the type that torch's would have (fp32 under autocast).  Calls that torch
-    traces, transforms or watches, and tensors of other classes, are torch's."""
+    traces, transforms or watches, tensors of other classes, and sizes and eps that the kernels do not take are torch's."""
     classes = (torch.Tensor, torch.nn.Parameter)
     if (x.device.type != "cuda" or x.dtype not in (torch.float32, torch.bfloat16, torch.float16) or x.dim() < 1
             or type(x) not in classes or not plain_norm(module, x.shape[-1])
             or forward_ad._current_level >= 0 or torch.compiler.is_compiling() or torch.jit.is_tracing()
             or torch._C._len_torch_dispatch_stack() > 0 or torch._C._functorch.peek_interpreter_stack() is not None):
+        return module(x)
+    C = x.shape[-1]
+    if not 1 <= C <= 1 << 24 or x.numel() // C >= 1 << 31 or (module.eps is not None and not module.eps >= 0.0):
         return module(x)
     autocast = torch.is_autocast_enabled("cuda")
     params = [t for t in (module.weight, getattr(module, "bias", None)) if t is not None]
