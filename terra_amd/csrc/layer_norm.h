@@ -7,17 +7,19 @@
 //   dw = sum over rows of dy xh,  db = sum over rows of dy
 //
 // All of it in fp32, two-pass statistics, y and dx rounded once; the parameters
-// are read in their own type and their gradients written in it, rounded once
-// from fp64 sums.  Row r of x begins (r / inner) outer + (r % inner) step
+// are read in their own type and their gradients written in it.  Row r of x begins (r / inner) outer + (r % inner) step
 // elements into x, so the heads of a packed q|k|v are rows too; y, dy and dx are packed.
 //
-// Bound by memory: a row is read once and held in registers through its two sums, the next one on its
-// way meanwhile (39168 x 4096 bf16: forward 118 us, 5.4 TB/s, backward 161 us, 6.0; 524288 x 192 fp32 to bf16: 94 and
+// Bound by memory: a row is read once and held in registers through its two sums, in the forward with the next one on
+// its way meanwhile (39168 x 4096 bf16: forward 118 us, 5.4 TB/s, backward 161 us, 6.0; 524288 x 192 fp32 to bf16: 94 and
 // 167 us; a large copy moves 5.35).  One row of 1024 is a launch (3 us).
+// Rows above 16384 channels are read again for each sum by a workgroup a row: 3662 x 16384 bf16 51 and 93 us,
+// 1831 x 32768 253 and 294 (1.0 and 1.2 TB/s).
 //
-// Sums over rows: workgroups keep the sums of the rows that they take and write
-// them to a workspace, a second launch adds those up in fp64: no atomics, an
-// order that the sizes and alignments fix.
+// Sums over rows: workgroups keep the sums of the rows that they take in fp32 and write
+// them to a workspace, a second launch adds those up in fp64 and rounds once: no atomics, an
+// order that the sizes and alignments fix.  (fp64 from the first row on would
+// double the registers of the sums.)
 #pragma once
 
 #include "residual_norm.h"

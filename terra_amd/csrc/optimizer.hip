@@ -242,7 +242,8 @@ struct AdamStep {
     if (a.maximize) factor = -factor;
     step = (uint32_t)t;
   }
-  __device__ __forceinline__ float updated(float p, float m, float r) const {  // r: the second moment's root
+  // r: the second moment's root.  The quotient by the hardware's reciprocal, an ulp: what a step takes off is off by that.
+  __device__ __forceinline__ float updated(float p, float m, float r) const {
     return fmaf(-rate * m, __builtin_amdgcn_rcpf(fmaf(r, root, eps)), p * keep);
   }
 };
