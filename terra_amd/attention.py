@@ -227,13 +227,11 @@ class WindowAttention(torch.nn.Module):
              n_real: Optional[int] = None) -> torch.Tensor:
         """Fused core on projected q/k/v [B_, N, C] (row strides may exceed C);
         with rotary positions the query and key heads are turned first."""
-        if self.rotary is not None:
-            at = self._positions_on(q.device)
-            if n_real is not None and n_real <= at.shape[0] < q.shape[-2]:  # rows of padding behind the window's tokens
-                at = F.pad(at, (0, 0, 0, q.shape[-2] - at.shape[0]))
-            q, k = (autograd.rotary(t.unflatten(-1, (self.num_heads, -1)), self.rotary, at).flatten(-2) for t in (q, k))
-        return autograd.window_attention(q, k, v, self.num_heads, self.window_size, self.scale,
-                                         bias_table=self._table(), mask=mask, n_real=n_real)
+        at = None if self.rotary is None else self._positions_on(q.device)
+        if at is not None and n_real is not None and n_real <= at.shape[0] < q.shape[-2]:  # rows of padding behind the window's
+            at = F.pad(at, (0, 0, 0, q.shape[-2] - at.shape[0]))
+        return autograd.window_attention(q, k, v, self.num_heads, self.window_size, self.scale, bias_table=self._table(),
+                                         mask=mask, n_real=n_real, rot=self.rotary, positions=at)
 
     def __setstate__(self, state):
         """A module pickled when this option was not there yet has it off; the

@@ -562,6 +562,13 @@ class _RotaryAttentionQKV(torch.autograd.Function):
         return dqkv, dtable, None, None, None, None, None, None, None, None
 
 
+class _TurnedAttention(_Attention):
+    """:class:`_Attention` of query and key heads that were turned.  Their turn back has derivatives, so a second one
+    would pass through it without the core's terms: it is refused."""
+
+    backward = staticmethod(once_differentiable(_Attention.backward))
+
+
 def _query_key_heads(qkv: torch.Tensor, num_heads: int) -> torch.Tensor:
     """The query and key columns of q | k | v [B_, N, 3C] as heads [B_, N, 2 num_heads, D]."""
     C = qkv.shape[-1] // 3
@@ -575,11 +582,15 @@ def _turned_heads(qkv: torch.Tensor, num_heads: int, rot: kernels.Rotary, positi
 def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, num_heads: int,
                      window_size: Tuple[int, int], scale: float, bias_table: Optional[torch.Tensor] = None,
                      mask: MaskArg = None, n_real: Optional[int] = None,
-                     mask_value: float = kernels.MASK_VALUE) -> torch.Tensor:
+                     mask_value: float = kernels.MASK_VALUE, rot: Optional[kernels.Rotary] = None,
+                     positions: Optional[torch.Tensor] = None) -> torch.Tensor:
     """:func:`kernels.window_attention` with gradients for q, k, v and the bias
-    table."""
+    table.  ``rot``, ``positions``: rotary positions of the query and key heads (:func:`kernels.rotary`)."""
+    if rot is not None:
+        q, k = (rotary(t.unflatten(-1, (num_heads, -1)), rot, positions).flatten(-2) for t in (q, k))
     if _needs_grad(q, k, v, bias_table):
-        return _Attention.apply(q, k, v, bias_table, num_heads, tuple(window_size), scale, mask, n_real, mask_value)
+        function = _Attention if rot is None else _TurnedAttention
+        return function.apply(q, k, v, bias_table, num_heads, tuple(window_size), scale, mask, n_real, mask_value)
     return kernels.window_attention(q, k, v, num_heads, window_size, scale, bias_table=bias_table, mask=mask,
                                     n_real=n_real, mask_value=mask_value)
 

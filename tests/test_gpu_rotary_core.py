@@ -65,3 +65,12 @@ def test_windows_in_padded_rows(dev, dtype):
         assert rel_maxabs(got, attn.attend(x)) <= (1e-5 if dtype == F32 else 2e-2)
         with pytest.raises(ValueError, match="positions of the tokens"):
             attn.core(*padded)
+
+
+def test_only_one_derivative_of_the_core(dev):
+    """As attend's: a second one would leave terms out without a word."""
+    attn = _attn(dev, F32, True)
+    x = workloads.activations((4, 49, 96), 3, F32).to(dev).requires_grad_()
+    g, = torch.autograd.grad(attn.core(*attn.qkv(x).chunk(3, -1)).square().sum(), x, create_graph=True)
+    with pytest.raises(RuntimeError, match="once_differentiable"):
+        g.sum().backward()
